@@ -457,6 +457,90 @@ SMOE_API int smoe_decode_layer_status(const void* scratch, int64_t hidden, int64
                                       int* failed);
 SMOE_API int smoe_decode_layer_wait_test(int withhold);
 
+/* ---- 4-bit weights with a float16 scale and bias for each group of 32, 64 or 128 columns (the reference keeps
+ * its dense layers, shared experts and the draft head's experts in this form: `to_affine`, strata_mlx/gguf.py:182-276,
+ * `nn.QuantizedLinear` / `QuantizedSwitchLinear`, strata_mlx/load.py:235-256, strata_mlx/mtp.py:34-75):
+ *
+ *   w[r, c] = code[r, c] * scale[r, c / group] + bias[r, c / group],  code in 0 .. 15
+ *
+ * Codes come eight to a 32-bit word, weight 8 j + i in bits 4 i .. 4 i + 3 of word j. cols is a multiple of group. */
+
+/* codes [rows][cols / 8], scales and biases [rows][cols / group] float16 of float16 / float32 weights w [rows][cols]:
+ * scale = (max - min) / 15 and bias = min of the group, each rounded to float16, code = (w - bias) / scale rounded to
+ * even within 0 .. 15 (0 where the scale is 0), every step one float32 operation. */
+SMOE_API int smoe_q4_quantize(const void* w, int dtype, int64_t rows, int64_t cols, int group, uint32_t* codes,
+                              uint16_t* scales, uint16_t* biases, void* stream);
+
+/* out [rows][cols]: code * scale + bias in float32, rounded to out_dtype. */
+SMOE_API int smoe_q4_dequant(const uint32_t* codes, const uint16_t* scales, const uint16_t* biases, int64_t rows,
+                             int64_t cols, int group, void* out, int out_dtype, void* stream);
+
+/* The layout the products read (16-row strips of 128-column tiles, codes and scales together), made once from the
+ * three arrays of a stack (experts, rows, cols): smoe_q4_bytes() bytes, 16-byte aligned. smoe_q4_unpack gives the
+ * floats back: out [experts][rows][cols], the bits of smoe_q4_dequant. smoe_q4_bytes is 0 for shapes it cannot hold. */
+SMOE_API size_t smoe_q4_bytes(int64_t experts, int64_t rows, int64_t cols, int group);
+SMOE_API int smoe_q4_pack(const uint32_t* codes, const uint16_t* scales, const uint16_t* biases, int64_t experts,
+                          int64_t rows, int64_t cols, int group, uint8_t* packed, void* stream);
+SMOE_API int smoe_q4_unpack(const uint8_t* packed, int64_t experts, int64_t rows, int64_t cols, int group, void* out,
+                            int out_dtype, void* stream);
+
+/* Products on packed 4-bit weights, float32 sums, x and the outputs of `dtype`; either part may be empty:
+ *   dense:  dense_out[t, r] = W[r, :] . x[t, :] for t < dense_tokens, W a packed matrix (dense_rows, cols)
+ *   stack:  out[p, r] = W[idx[p]][r, :] . x[p / share, :] for p < pairs, W a packed stack (experts, rows, cols)
+ * With second matrices (dense2 / stack2, of the same shapes) a result is silu(W . x) * (W2 . x), times
+ * sigmoid(dense_gate[t]) (`dtype`) or weights[p] (float32) where given, rounded once. Both parts in one call are both
+ * of one kind. Pairs with idx[p] >= experts are left out (their rows of out stay as they were). Up to 2048 pairs and
+ * experts; x 16-byte aligned, its rows cols apart. The weights may be read while the launch before on the stream still
+ * runs: they must not be written by it (smoe_q4_pack excepted). */
+typedef struct SmoeQ4Product {
+    int dtype;
+    int group;
+    const void* x;
+    int64_t cols;
+    const uint8_t *dense, *dense2;
+    int64_t dense_rows, dense_tokens;
+    const void* dense_gate;
+    void* dense_out;
+    const uint8_t *stack, *stack2;
+    int64_t rows, experts;
+    const uint32_t* idx;
+    int64_t pairs, share;
+    const float* weights;
+    void* out;
+} SmoeQ4Product;
+SMOE_API int smoe_q4_product(const SmoeQ4Product* p, void* stream);
+
+/* smoe_q4_product's dense part alone: out[t, r] = W[r, :] . x[t, :] for t < tokens (`nn.QuantizedLinear`). */
+SMOE_API int smoe_q4_linear(const uint8_t* packed, int64_t rows, int64_t cols, int group, const void* x, int64_t tokens,
+                            void* out, int dtype, void* stream);
+
+/* A MoE block behind its route (smoe_route's idx, weights and gate_out) on packed 4-bit experts, for 1 to 64 tokens,
+ * in two launches (gate, up and SwiGLU of the routed and the shared expert; down and the combine):
+ *   out[t] = sum_j weights[t, j] down_e(silu(gate_e x) * up_e x) + sigmoid(shared_gate[t]) shared(x), e = idx[t, j]
+ * gate, up: (experts, ffn, hidden) with groups of `group` columns, down: (experts, hidden, ffn) with `down_group`; the
+ * shared expert's likewise with shared_ffn rows (0: none; shared_gate null: not gated). A choice idx >= experts adds
+ * nothing. Sums and SwiGLU are float32; between the launches the SwiGLU times its weight is kept in `dtype`. Workspace:
+ * smoe_q4_moe_workspace_size() bytes, one for each call in flight. Replaces `_Routed.__call__` behind its router
+ * (strata_mlx/fused.py:491-497). Weights as smoe_q4_product's. */
+typedef struct SmoeQ4Moe {
+    int dtype;
+    int group, down_group;
+    int64_t tokens, hidden, experts, k, ffn, shared_ffn;
+    const void* x;
+    const uint32_t* idx;
+    const float* weights;
+    const void* shared_gate;
+    const uint8_t *gate, *up, *down;
+    const uint8_t *sgate, *sup, *sdown;
+    void* out;
+} SmoeQ4Moe;
+SMOE_API size_t smoe_q4_moe_workspace_size(int dtype, int64_t tokens, int64_t k, int64_t ffn, int64_t shared_ffn);
+SMOE_API int smoe_q4_moe(const SmoeQ4Moe* m, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Whether a bounded wait of the 4-bit kernels gave up since the last clear (SMOE_ETIMEOUT; outputs since are not
+ * valid). Synchronizes the device. */
+SMOE_API int smoe_q4_status(int* status, int clear);
+
 #ifdef __cplusplus
 }
 #endif

@@ -4,4 +4,4 @@
 the kernels live in libstrata_moe.so (C ABI: include/strata_moe.h), built by `strata_mlx_b200._build`.
 """
 
-from . import blocks, fused  # noqa: F401
+from . import affine, blocks, fused  # noqa: F401

@@ -59,6 +59,24 @@ class SmoeHyper(ctypes.Structure):
                 ("eps", _c.c_float), ("dtype", _i)]
 
 
+class SmoeQ4Product(ctypes.Structure):
+    """`SmoeQ4Product` of include/strata_moe.h: products on packed 4-bit weights."""
+
+    _fields_ = [("dtype", _i), ("group", _i), ("x", _p), ("cols", _i64), ("dense", _p), ("dense2", _p),
+                ("dense_rows", _i64), ("dense_tokens", _i64), ("dense_gate", _p), ("dense_out", _p), ("stack", _p),
+                ("stack2", _p), ("rows", _i64), ("experts", _i64), ("idx", _p), ("pairs", _i64), ("share", _i64),
+                ("weights", _p), ("out", _p)]
+
+
+class SmoeQ4Moe(ctypes.Structure):
+    """`SmoeQ4Moe` of include/strata_moe.h: a MoE block on 4-bit experts."""
+
+    _fields_ = [("dtype", _i), ("group", _i), ("down_group", _i), ("tokens", _i64), ("hidden", _i64), ("experts", _i64),
+                ("k", _i64), ("ffn", _i64), ("shared_ffn", _i64), ("x", _p), ("idx", _p), ("weights", _p),
+                ("shared_gate", _p), ("gate", _p), ("up", _p), ("down", _p), ("sgate", _p), ("sup", _p), ("sdown", _p),
+                ("out", _p)]
+
+
 # name -> (restype, argtypes): the declarations of include/strata_moe.h
 SIGNATURES = {
     "smoe_last_error": (_c.c_char_p, []),
@@ -119,6 +137,16 @@ SIGNATURES = {
     "smoe_tile_matmul_pair": (_i, [_i, _p, _p, _i64, _i64, _i64, _p, _i64, _p, _p, _p, _p, _sz, _p]),
     "smoe_tile_matmul_pair_rows": (_i, [_i, _p, _p, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _p, _p, _p, _sz,
                                         _p]),
+    "smoe_q4_quantize": (_i, [_p, _i, _i64, _i64, _i, _p, _p, _p, _p]),
+    "smoe_q4_dequant": (_i, [_p, _p, _p, _i64, _i64, _i, _p, _i, _p]),
+    "smoe_q4_bytes": (_sz, [_i64, _i64, _i64, _i]),
+    "smoe_q4_pack": (_i, [_p, _p, _p, _i64, _i64, _i64, _i, _p, _p]),
+    "smoe_q4_unpack": (_i, [_p, _i64, _i64, _i64, _i, _p, _i, _p]),
+    "smoe_q4_linear": (_i, [_p, _i64, _i64, _i, _p, _i64, _p, _i, _p]),
+    "smoe_q4_product": (_i, [_c.POINTER(SmoeQ4Product), _p]),
+    "smoe_q4_moe_workspace_size": (_sz, [_i, _i64, _i64, _i64, _i64]),
+    "smoe_q4_moe": (_i, [_c.POINTER(SmoeQ4Moe), _p, _sz, _p]),
+    "smoe_q4_status": (_i, [_c.POINTER(_i), _i]),
 }
 
 _lib = None
@@ -128,7 +156,8 @@ KERNELS_PER_CALL = {"smoe_tiles_of": 2, "smoe_tiles_of_noalloc": 2, "smoe_tile_m
                     "smoe_tile_matmul_pair": 2, "smoe_tile_matmul_pair_rows": 2, "smoe_ep_dispatch": 2,
                     "smoe_ep_exchange_alloc": 0, "smoe_ep_exchange_open": 0, "smoe_ep_exchange_close": 0,
                     "smoe_ep_exchange_free": 0, "smoe_ep_exchange_status": 0, "smoe_decode_layer_status": 0, "smoe_decode_layer_wait_test": 0,
-                    "smoe_matvec_status": 0, "smoe_matvec_wait_test": 0, "smoe_hyper_connection": 3}
+                    "smoe_matvec_status": 0, "smoe_matvec_wait_test": 0, "smoe_hyper_connection": 3,
+                    "smoe_q4_moe": 2, "smoe_q4_status": 0}
 launches = 0
 
 

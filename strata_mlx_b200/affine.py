@@ -1,0 +1,355 @@
+"""Layers on 4-bit weights with a float16 scale and bias for each group of columns, on B200: MLX's affine form, which
+the reference holds its dense layers, its shared experts and its draft head's experts in (`to_affine`,
+strata_mlx/gguf.py:182-276; `nn.QuantizedLinear`, strata_mlx/load.py:235-256; `QuantizedSwitchLinear`,
+strata_mlx/mtp.py:34-75).
+
+    quantize, dequantize    floats to codes, scales and biases, and back
+    QuantizedLinear         one layer: x W^T for any number of tokens
+    QuantizedSwitchLinear   one projection of every expert, for (token, expert) pairs
+    QuantizedSwitchGLU      the routed experts' SwiGLU feed-forwards
+    QuantizedMLP            the shared expert
+    moe                     a MoE block behind its route, for which `fused.SparseMoeBlock` calls it
+
+A weight is code * scale + bias with a code of 4 bits, eight codes to a 32-bit word (weight 8 j + i in bits 4 i of
+word j), groups of 32, 64 or 128 columns. A layer lays its arrays out once for the kernels (libstrata_moe.so) and
+keeps that alone. Products are exact in each weight (codes are not rounded to floats first) with float32 sums.
+Activations are float16 or float32; tensors are torch CUDA tensors and there is no CPU path.
+"""
+
+import ctypes
+
+import torch
+
+from . import _lib
+from .blocks import _flat_idx
+
+BITS = 4
+GROUPS = (32, 64, 128)
+MAX_PAIRS = 2048  # (token, expert) pairs of one launch; a longer call goes in several
+MOE_TOKENS = 64  # tokens that `moe` takes at once; a longer call goes in several
+
+
+def _check_group(group_size: int, bits: int = BITS) -> None:
+    if bits != BITS:
+        raise ValueError(f"weights of {bits} bits are not supported (4 bits)")
+    if group_size not in GROUPS:
+        raise ValueError(f"groups of {group_size} columns are not supported (32, 64 or 128)")
+
+
+def _same_device(*tensors):
+    _lib.require_cuda(*tensors)
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) > 1:
+        raise ValueError(f"tensors on different devices: {sorted(map(str, devices))}")
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """t contiguous and on a 16-byte boundary (a view into another tensor may not be)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _check_parts(codes, scales, biases, group_size, bits=BITS):
+    _check_group(group_size, bits)
+    _same_device(codes, scales, biases)
+    if codes.dtype not in (torch.int32, torch.uint32):
+        raise ValueError(f"codes come as 32-bit words, not {codes.dtype}")
+    if scales.dtype != torch.float16 or biases.dtype != torch.float16:
+        raise ValueError("scales and biases are float16")
+    if codes.dim() < 2 or scales.shape != biases.shape or scales.shape[:-1] != codes.shape[:-1] or (
+            codes.shape[-1] * 8 != scales.shape[-1] * group_size):
+        raise ValueError(f"codes {tuple(codes.shape)}, scales {tuple(scales.shape)} and biases {tuple(biases.shape)} "
+                         f"are no matrix in groups of {group_size}")
+
+
+def quantize(w: torch.Tensor, group_size: int = 64, bits: int = BITS):
+    """Float weights (..., rows, cols) as (codes int32 (..., rows, cols / 8), scales, biases float16 (..., rows,
+    cols / group_size)). Of each group, bias is the least value and scale a fifteenth of the range, both rounded to
+    float16; a code is (w - bias) / scale rounded to even within 0 .. 15 (0 where the scale is 0). Values beyond
+    float16's range or not finite give groups that are not finite."""
+    _check_group(group_size, bits)
+    _lib.require_cuda(w)
+    if w.dim() < 1 or w.shape[-1] == 0 or w.shape[-1] % group_size:
+        raise ValueError(f"{tuple(w.shape)}: the columns are no whole number of groups of {group_size}")
+    code = _lib.dtype_code(w.dtype)
+    cols = w.shape[-1]
+    rows = w.numel() // cols
+    with torch.cuda.device(w.device):
+        w2 = _aligned(w)
+        codes = torch.empty((*w.shape[:-1], cols // 8), dtype=torch.int32, device=w.device)
+        scales = torch.empty((*w.shape[:-1], cols // group_size), dtype=torch.float16, device=w.device)
+        biases = torch.empty_like(scales)
+        if rows:
+            _lib.call("smoe_q4_quantize", _lib.ptr(w2), code, rows, cols, group_size, _lib.ptr(codes),
+                      _lib.ptr(scales), _lib.ptr(biases), _lib.stream())
+    return codes, scales, biases
+
+
+def dequantize(codes: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor, group_size: int = 64, bits: int = BITS,
+               dtype: torch.dtype = torch.float16) -> torch.Tensor:
+    """The floats (..., rows, cols) of `quantize`'s arrays: code * scale + bias in float32, rounded to `dtype`."""
+    _check_parts(codes, scales, biases, group_size, bits)
+    code = _lib.dtype_code(dtype)
+    cols = codes.shape[-1] * 8
+    with torch.cuda.device(codes.device):
+        out = torch.empty((*codes.shape[:-1], cols), dtype=dtype, device=codes.device)
+        if out.numel():
+            codes, scales, biases = codes.contiguous(), scales.contiguous(), biases.contiguous()
+            _lib.call("smoe_q4_dequant", _lib.ptr(codes), _lib.ptr(scales), _lib.ptr(biases), out.numel() // cols, cols,
+                      group_size, _lib.ptr(out), code, _lib.stream())
+    return out
+
+
+class _Packed:
+    """A stack (experts, rows, cols) of 4-bit weights in the kernels' layout."""
+
+    def __init__(self, codes, scales, biases, group_size):
+        _check_parts(codes, scales, biases, group_size)
+        if codes.numel() == 0:
+            raise ValueError("a layer without weights")
+        self.num_experts, self.output_dims = (1, codes.shape[0]) if codes.dim() == 2 else codes.shape[:2]
+        self.input_dims, self.group_size = codes.shape[-1] * 8, group_size
+        self.device = codes.device
+        nbytes = int(_lib.lib().smoe_q4_bytes(self.num_experts, self.output_dims, self.input_dims, group_size))
+        with torch.cuda.device(self.device):
+            self.packed = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+            codes, scales, biases = codes.contiguous(), scales.contiguous(), biases.contiguous()
+            _lib.call("smoe_q4_pack", _lib.ptr(codes), _lib.ptr(scales), _lib.ptr(biases), self.num_experts,
+                      self.output_dims, self.input_dims, group_size, _lib.ptr(self.packed), _lib.stream())
+        self.data_ptr = self.packed.data_ptr()
+
+    @property
+    def nbytes(self) -> int:
+        return self.packed.numel()
+
+    def _floats(self, shape, dtype):
+        code = _lib.dtype_code(dtype)
+        with torch.cuda.device(self.device):
+            out = torch.empty(shape, dtype=dtype, device=self.device)
+            _lib.call("smoe_q4_unpack", _lib.ptr(self.packed), self.num_experts, self.output_dims, self.input_dims,
+                      self.group_size, _lib.ptr(out), code, _lib.stream())
+        return out
+
+    def _rows(self, x: torch.Tensor) -> torch.Tensor:
+        """x (..., in) as aligned rows (n, in)."""
+        if x.dim() < 1 or x.shape[-1] != self.input_dims:
+            raise ValueError(f"activations {tuple(x.shape)} do not end in {self.input_dims}")
+        if x.device != self.device:
+            _lib.require_cuda(x)
+            raise ValueError(f"activations on {x.device}, weights on {self.device}")
+        return _aligned(x.reshape(-1, self.input_dims))
+
+
+class QuantizedLinear(_Packed):
+    """One linear layer on 4-bit weights, used like `nn.Linear` without a bias: codes (out, in / 8), scales and biases
+    (out, in / group_size). x (..., in) -> (..., out) in x's type; a token gets the same bits alone as in a window."""
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor, group_size: int = 64):
+        if codes.dim() != 2:
+            raise ValueError(f"a layer's codes are (out, in / 8), not {tuple(codes.shape)}")
+        super().__init__(codes, scales, biases, group_size)
+
+    @classmethod
+    def from_float(cls, w: torch.Tensor, group_size: int = 64) -> "QuantizedLinear":
+        return cls(*quantize(w, group_size), group_size=group_size)
+
+    def floats(self, dtype: torch.dtype = torch.float16) -> torch.Tensor:
+        """The weights (out, in), as `dequantize` gives them."""
+        return self._floats((self.output_dims, self.input_dims), dtype)
+
+    def __call__(self, x: torch.Tensor) -> torch.Tensor:
+        code = _lib.dtype_code(x.dtype)
+        x2 = self._rows(x)
+        if self.device.index != torch.cuda.current_device():
+            with torch.cuda.device(self.device):
+                return self(x)
+        tokens = x2.shape[0]
+        out = torch.empty((*x.shape[:-1], self.output_dims), dtype=x.dtype, device=self.device)
+        if tokens:
+            _lib.call("smoe_q4_linear", self.data_ptr, self.output_dims, self.input_dims, self.group_size,
+                      x2.data_ptr(), tokens, out.data_ptr(), code, torch.cuda.current_stream().cuda_stream)
+        return out
+
+
+def _pair_chunks(pairs: int, share: int):
+    """Ranges of pairs, whole rows of `share`, that one launch takes."""
+    step = max(1, MAX_PAIRS // share) * share
+    return [(p, min(p + step, pairs)) for p in range(0, pairs, step)]
+
+
+def _check_pairs(indices, k):
+    _lib.require_cuda(indices)
+    if not 1 <= k <= MAX_PAIRS:
+        raise ValueError(f"{k} experts a row")
+
+
+class QuantizedSwitchLinear(_Packed):
+    """One projection of every expert on 4-bit weights: codes (experts, out, in / 8), scales and biases (experts, out,
+    in / group_size); its call takes what `BlockSwitchLinear`'s takes."""
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor, group_size: int = 64):
+        if codes.dim() != 3:
+            raise ValueError(f"a stack's codes are (experts, out, in / 8), not {tuple(codes.shape)}")
+        if codes.shape[0] > 2048:
+            raise ValueError(f"{codes.shape[0]} experts: a stack holds up to 2048")
+        super().__init__(codes, scales, biases, group_size)
+
+    @classmethod
+    def from_float(cls, w: torch.Tensor, group_size: int = 64) -> "QuantizedSwitchLinear":
+        return cls(*quantize(w, group_size), group_size=group_size)
+
+    @property
+    def shape(self):
+        return (self.num_experts, self.output_dims, self.input_dims)
+
+    def floats(self, dtype: torch.dtype = torch.float16) -> torch.Tensor:
+        return self._floats(self.shape, dtype)
+
+    def __call__(self, x: torch.Tensor, indices: torch.Tensor, sorted_indices: bool = False) -> torch.Tensor:
+        """Each (token, expert) pair of `indices` times its activation row; x (..., 1, in), one row per entry of
+        `indices` or one that the entries along its last axis share. Returns (*indices.shape, 1, out). An index at or
+        past the expert count names a pair that is left out (its row is not written)."""
+        ishape = tuple(indices.shape)
+        if x.dim() < 2 or x.shape[-2] != 1:
+            raise ValueError(f"activations {tuple(x.shape)} are not (..., 1, in)")
+        batch = tuple(x.shape[:-2])
+        k = ishape[-1] if indices.dim() else 1
+        if batch == ishape:
+            share = 1
+        elif indices.dim() and batch == (*ishape[:-1], 1):
+            share = k
+        else:
+            x, share = x.expand(*ishape, 1, self.input_dims), 1
+        out = _pairs_product(self, None, self._rows(x), indices, share)
+        return out.reshape(*ishape, 1, self.output_dims)
+
+
+def _pairs_product(lin, lin2, x2, indices, share, weights=None):
+    """(pairs, out): rows x2[p // share] through expert indices[p] of `lin`, or through gate `lin` and up `lin2`."""
+    code = _lib.dtype_code(x2.dtype)
+    if indices.device != lin.device:
+        _lib.require_cuda(indices)
+        raise ValueError(f"indices on {indices.device}, weights on {lin.device}")
+    with torch.cuda.device(lin.device):
+        idx = _flat_idx(indices)
+        pairs = idx.numel()
+        out = torch.empty((pairs, lin.output_dims), dtype=x2.dtype, device=lin.device)
+        if pairs:
+            _check_pairs(idx, share)
+            if x2.shape[0] * share != pairs:
+                raise ValueError("indices must hold the same number of experts for every row of x")
+        for p0, p1 in _pair_chunks(pairs, share):
+            spec = _lib.SmoeQ4Product(dtype=code, group=lin.group_size, x=x2[p0 // share].data_ptr(), cols=lin.input_dims,
+                                      stack=lin.data_ptr, stack2=lin2.data_ptr if lin2 is not None else None,
+                                      rows=lin.output_dims, experts=lin.num_experts, idx=idx[p0:].data_ptr(),
+                                      pairs=p1 - p0, share=share, out=out[p0:].data_ptr())
+            _lib.call("smoe_q4_product", ctypes.byref(spec), _lib.stream())
+    return out
+
+
+def _alike(a, b) -> bool:
+    return (a.num_experts, a.output_dims, a.input_dims, a.group_size, a.device) == (
+        b.num_experts, b.output_dims, b.input_dims, b.group_size, b.device)
+
+
+def _check_glu(gate, up, down):
+    if not _alike(gate, up):
+        raise ValueError("gate and up must have one shape, group size and device")
+    if (down.num_experts, down.input_dims, down.output_dims) != (gate.num_experts, gate.output_dims, gate.input_dims):
+        raise ValueError("down must take gate's outputs to its inputs")
+    if down.device != gate.device:
+        raise ValueError(f"down on {down.device}, gate on {gate.device}")
+
+
+class QuantizedSwitchGLU:
+    """The routed experts of one layer on 4-bit weights: x (..., in) and indices (..., k) -> (..., k, out), each
+    down(silu(gate x) * up x); gate and up in one launch that forms the SwiGLU."""
+
+    def __init__(self, gate: QuantizedSwitchLinear, up: QuantizedSwitchLinear, down: QuantizedSwitchLinear):
+        _check_glu(gate, up, down)
+        self.gate_proj, self.up_proj, self.down_proj = gate, up, down
+
+    def __call__(self, x: torch.Tensor, indices: torch.Tensor) -> torch.Tensor:
+        if indices.dim() < 1:
+            raise ValueError("indices must hold k experts for every token of x")
+        h = _pairs_product(self.gate_proj, self.up_proj, self.gate_proj._rows(x), indices, indices.shape[-1])
+        out = _pairs_product(self.down_proj, None, h, indices, 1)
+        return out.reshape(*indices.shape, self.down_proj.output_dims)
+
+
+class QuantizedMLP:
+    """The shared expert on 4-bit weights: down(silu(gate x) * up x)."""
+
+    def __init__(self, gate: QuantizedLinear, up: QuantizedLinear, down: QuantizedLinear):
+        _check_glu(gate, up, down)
+        self.gate_proj, self.up_proj, self.down_proj = gate, up, down
+
+    def __call__(self, x: torch.Tensor) -> torch.Tensor:
+        code = _lib.dtype_code(x.dtype)
+        gate, up = self.gate_proj, self.up_proj
+        x2 = gate._rows(x)
+        with torch.cuda.device(gate.device):
+            h = torch.empty((x2.shape[0], gate.output_dims), dtype=x.dtype, device=gate.device)
+            if x2.shape[0]:
+                spec = _lib.SmoeQ4Product(dtype=code, group=gate.group_size, x=x2.data_ptr(), cols=gate.input_dims,
+                                          dense=gate.data_ptr, dense2=up.data_ptr, dense_rows=gate.output_dims,
+                                          dense_tokens=x2.shape[0], dense_out=h.data_ptr())
+                _lib.call("smoe_q4_product", ctypes.byref(spec), _lib.stream())
+            out = self.down_proj(h)
+        return out.reshape(*x.shape[:-1], self.down_proj.output_dims)
+
+
+def moe_takes(switch_mlp, shared) -> bool:
+    """Whether `moe` runs these experts in its two launches: 4-bit, of one hidden size, group sizes alike in gate / up
+    and in down."""
+    if not isinstance(switch_mlp, QuantizedSwitchGLU) or not isinstance(shared, QuantizedMLP):
+        return False
+    g, d, sg, sd = switch_mlp.gate_proj, switch_mlp.down_proj, shared.gate_proj, shared.down_proj
+    return (g.input_dims == sg.input_dims and g.group_size == sg.group_size and d.group_size == sd.group_size
+            and g.device == sg.device)
+
+
+def moe(switch_mlp: QuantizedSwitchGLU, shared: QuantizedMLP, x: torch.Tensor, indices: torch.Tensor, w: torch.Tensor,
+        g: torch.Tensor) -> torch.Tensor:
+    """sum_j w_j switch_mlp(x, indices)_j + sigmoid(g) shared(x) in two launches: x (..., hidden), indices and w (...,
+    k) with w float32, g (..., 1) in x's type. Sums are float32 and rounded to x's type once (SwiGLU times its weight is
+    rounded to it between the launches). An index at or past the expert count adds nothing."""
+    if not moe_takes(switch_mlp, shared):
+        raise ValueError("moe takes 4-bit experts of one hidden size, with one group size in gate / up and one in down")
+    gate, down = switch_mlp.gate_proj, switch_mlp.down_proj
+    sgate, sdown = shared.gate_proj, shared.down_proj
+    code = _lib.dtype_code(x.dtype)
+    x2 = gate._rows(x)
+    _same_device(x, indices, w, g)
+    tokens, k = x2.shape[0], indices.shape[-1] if indices.dim() else 0
+    if indices.numel() != tokens * k or w.numel() != tokens * k or g.numel() != tokens or not 1 <= k <= 32:
+        raise ValueError("moe takes 1 to 32 experts and weights and one gate value for every token")
+    if w.dtype != torch.float32 or g.dtype != x.dtype:
+        raise ValueError("weights are float32 and gate values of the activations' type")
+    with torch.cuda.device(gate.device):
+        idx, w, g = _flat_idx(indices), w.contiguous(), g.contiguous()
+        out = torch.empty((tokens, gate.input_dims), dtype=x.dtype, device=gate.device)
+        for t0 in range(0, tokens, MOE_TOKENS):
+            n = min(MOE_TOKENS, tokens - t0)
+            nbytes = int(_lib.lib().smoe_q4_moe_workspace_size(code, n, k, gate.output_dims, sgate.output_dims))
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=gate.device)
+            spec = _lib.SmoeQ4Moe(
+                dtype=code, group=gate.group_size, down_group=down.group_size, tokens=n, hidden=gate.input_dims,
+                experts=gate.num_experts, k=k, ffn=gate.output_dims, shared_ffn=sgate.output_dims, x=x2[t0:].data_ptr(),
+                idx=idx[t0 * k:].data_ptr(), weights=w.data_ptr() + 4 * t0 * k,
+                shared_gate=g.data_ptr() + g.element_size() * t0, gate=gate.data_ptr, up=switch_mlp.up_proj.data_ptr,
+                down=down.data_ptr, sgate=sgate.data_ptr, sup=shared.up_proj.data_ptr, sdown=sdown.data_ptr,
+                out=out[t0:].data_ptr())
+            _lib.call("smoe_q4_moe", ctypes.byref(spec), _lib.ptr(ws), nbytes, _lib.stream())
+    return out.reshape(x.shape)
+
+
+def failed(clear: bool = False) -> bool:
+    """Whether a bounded wait of the 4-bit kernels gave up (outputs since are then not valid). Synchronizes."""
+    status = ctypes.c_int(0)
+    _lib.call("smoe_q4_status", ctypes.byref(status), int(clear))
+    return status.value != 0
+
+
+__all__ = ["BITS", "GROUPS", "QuantizedLinear", "QuantizedMLP", "QuantizedSwitchGLU", "QuantizedSwitchLinear", "dequantize",
+           "failed", "moe", "moe_takes", "quantize"]

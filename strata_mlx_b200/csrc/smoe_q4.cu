@@ -1,0 +1,454 @@
+// 4-bit weights with group scales: floats to codes and back, the layout of the kernels, and the entry points of the
+// products and of a MoE block on them.
+//
+// The conversions are one pass over memory each: a thread holds eight columns (one code word), so a warp reads 512
+// bytes of float16 or 1 KB of float32 in 16-byte pieces and writes 128 bytes of codes; a group's extremes come from
+// the 4, 8 or 16 lanes that hold it by shuffles. Bound by HBM.
+#include <algorithm>
+#include <string>
+
+#include "q4_launch.cuh"
+
+namespace smoe {
+namespace q4 {
+
+constexpr int kConvThreads = 256;
+
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+__device__ __forceinline__ void load8(const __half* p, float (&f)[8]) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 q = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        f[2 * i] = q.x;
+        f[2 * i + 1] = q.y;
+    }
+}
+__device__ __forceinline__ void load8(const float* p, float (&f)[8]) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+}
+__device__ __forceinline__ void store8(__half* p, const float (&f)[8]) {
+    uint4 v;
+    v.x = tc::pack_half2(f[0], f[1]);
+    v.y = tc::pack_half2(f[2], f[3]);
+    v.z = tc::pack_half2(f[4], f[5]);
+    v.w = tc::pack_half2(f[6], f[7]);
+    *reinterpret_cast<uint4*>(p) = v;
+}
+__device__ __forceinline__ void store8(float* p, const float (&f)[8]) {
+    *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
+}
+
+// words = rows cols / 8. The arithmetic of each value is a chain of single IEEE float32 operations (difference,
+// quotient, rounding to even), so the codes are the formula's exactly.
+template <typename T, int G>
+__global__ void __launch_bounds__(kConvThreads) q4_quantize_kernel(const T* __restrict__ w, int64_t words,
+                                                                   uint32_t* __restrict__ codes,
+                                                                   __half* __restrict__ scales,
+                                                                   __half* __restrict__ biases) {
+    const int64_t i = int64_t(blockIdx.x) * kConvThreads + threadIdx.x;
+    const bool in = i < words;
+    float f[8] = {};
+    if (in) load8(w + 8 * i, f);
+    float lo = f[0], hi = f[0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) {
+        lo = min_nan(lo, f[j]);
+        hi = max_nan(hi, f[j]);
+    }
+    // (a group's lanes are all in or all out: words is a multiple of G / 8)
+#pragma unroll
+    for (int o = 1; o < G / 8; o <<= 1) {
+        lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+    if (!in) return;
+    const __half sh = __float2half_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.0f)), bh = __float2half_rn(lo);
+    const float s = __half2float(sh), b = __half2float(bh);
+    uint32_t word = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        float q = s > 0.0f ? rintf(__fdiv_rn(__fsub_rn(f[j], b), s)) : 0.0f;
+        q = fminf(fmaxf(q, 0.0f), 15.0f);  // (a NaN becomes code 0; its group's scale or bias is not finite either)
+        word |= static_cast<uint32_t>(q) << (4 * j);
+    }
+    codes[i] = word;
+    if (i % (G / 8) == 0) {
+        scales[i / (G / 8)] = sh;
+        biases[i / (G / 8)] = bh;
+    }
+}
+
+// w = code * scale + bias in float32 (two roundings), then to T. With `packed`, from the kernels' layout: word i of
+// the matrix's rows x cols / 8.
+template <typename T>
+__global__ void __launch_bounds__(kConvThreads) q4_dequant_kernel(const uint32_t* __restrict__ codes,
+                                                                  const __half* __restrict__ scales,
+                                                                  const __half* __restrict__ biases,
+                                                                  const uint8_t* __restrict__ packed, int64_t words,
+                                                                  int64_t rows, int64_t cols, int group,
+                                                                  T* __restrict__ out) {
+    const int64_t i = int64_t(blockIdx.x) * kConvThreads + threadIdx.x;
+    if (i >= words) return;
+    uint32_t word;
+    float s, b;
+    if (packed == nullptr) {
+        word = codes[i];
+        const int64_t at = i / (group / 8);
+        s = __half2float(scales[at]);
+        b = __half2float(biases[at]);
+    } else {
+        const int64_t per_row = cols / 8, all = i / per_row;
+        const int c = static_cast<int>(i - all * per_row) * 8;
+        const int64_t e = all / rows, r = all - e * rows;
+        const uint8_t* tile = packed + ((e * strips_of_rows(rows) + r / kRows) * tiles_of_cols(cols) + c / kCols) *
+                                           tile_bytes_of(group);
+        const int row = static_cast<int>(r % kRows), j = (c % kCols) / 32, t = (c % 32) / 8;
+        word = *reinterpret_cast<const uint32_t*>(tile + row * 64 + (4 * t + j) * 4);
+        const __half2 p = *reinterpret_cast<const __half2*>(tile + kCodeBytes + (row * (kCols / group) + (c % kCols) / group) * 4);
+        s = __low2float(p);
+        b = __high2float(p);
+    }
+    float f[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = __fadd_rn(__fmul_rn(static_cast<float>((word >> (4 * j)) & 15u), s), b);
+    store8(out + 8 * i, f);
+}
+
+// One 32-bit word of the layout a thread: codes, or a (scale, bias) pair.
+__global__ void __launch_bounds__(kConvThreads) q4_pack_kernel(const uint32_t* __restrict__ codes,
+                                                               const __half* __restrict__ scales,
+                                                               const __half* __restrict__ biases, int64_t experts,
+                                                               int64_t rows, int64_t cols, int group,
+                                                               uint32_t* __restrict__ out, int64_t total) {
+    const int64_t i = int64_t(blockIdx.x) * kConvThreads + threadIdx.x;
+    if (i >= total) return;
+    const int per_tile = tile_bytes_of(group) / 4, groups = kCols / group;
+    const int64_t tile = i / per_tile;
+    const int at = static_cast<int>(i - tile * per_tile);
+    const int64_t tiles = tiles_of_cols(cols), strips = strips_of_rows(rows);
+    const int64_t strip = tile / tiles, e = strip / strips;
+    const int64_t c0 = (tile - strip * tiles) * kCols;
+    uint32_t v = 0;
+    if (at < kCodeBytes / 4) {
+        const int64_t r = (strip - e * strips) * kRows + at / 16, c = c0 + 32 * (at & 3) + 8 * ((at >> 2) & 3);
+        if (r < rows && c < cols) v = codes[(e * rows + r) * (cols / 8) + c / 8];
+    } else {
+        const int k = at - kCodeBytes / 4;
+        const int64_t r = (strip - e * strips) * kRows + k / groups, c = c0 + int64_t(k % groups) * group;
+        if (r < rows && c < cols) {
+            const int64_t from = (e * rows + r) * (cols / group) + c / group;
+            v = uint32_t(__half_as_ushort(scales[from])) | (uint32_t(__half_as_ushort(biases[from])) << 16);
+        }
+    }
+    out[i] = v;
+}
+
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+static bool group_ok(int g) { return g == 32 || g == 64 || g == 128; }
+static size_t stack_bytes(int64_t experts, int64_t rows, int64_t cols, int group) {
+    return size_t(experts) * strips_of_rows(rows) * tiles_of_cols(cols) * tile_bytes_of(group);
+}
+constexpr int64_t kMost = int64_t(1) << 30;  // rows, columns and tokens of a matrix
+
+}  // namespace q4
+}  // namespace smoe
+
+using namespace smoe;
+using namespace smoe::q4;
+
+#define Q4_TRY try {
+#define Q4_CATCH(what)                                           \
+    }                                                            \
+    catch (...) {                                                \
+        return fail(SMOE_EARG, what ": the host is out of memory"); \
+    }
+
+static int conv_grid(int64_t n, unsigned* grid) {
+    const int64_t g = (n + kConvThreads - 1) / kConvThreads;
+    SMOE_REQUIRE(g <= 0x7fffffff, SMOE_ESHAPE, "too many weights for one call");
+    *grid = static_cast<unsigned>(g);
+    return SMOE_OK;
+}
+
+static int check_matrix(int64_t rows, int64_t cols, int group) {
+    SMOE_REQUIRE(group_ok(group), SMOE_ESHAPE, "groups have 32, 64 or 128 columns, not " + std::to_string(group));
+    SMOE_REQUIRE(rows > 0 && rows <= kMost && cols > 0 && cols <= kMost, SMOE_ESHAPE,
+                 "a 4-bit matrix of " + std::to_string(rows) + " x " + std::to_string(cols));
+    SMOE_REQUIRE(cols % group == 0, SMOE_ESHAPE,
+                 std::to_string(cols) + " columns are no whole number of groups of " + std::to_string(group));
+    return SMOE_OK;
+}
+
+extern "C" size_t smoe_q4_bytes(int64_t experts, int64_t rows, int64_t cols, int group) {
+    if (!group_ok(group) || experts < 0 || rows <= 0 || cols <= 0 || cols % group != 0) return 0;
+    return stack_bytes(experts, rows, cols, group);
+}
+
+extern "C" int smoe_q4_quantize(const void* w, int dtype, int64_t rows, int64_t cols, int group, uint32_t* codes,
+                                uint16_t* scales, uint16_t* biases, void* stream) {
+    Q4_TRY
+    if (rows == 0) return SMOE_OK;
+    if (int s = check_matrix(rows, cols, group)) return s;
+    SMOE_REQUIRE(w && codes && scales && biases && aligned16(w), SMOE_EARG, "q4_quantize: null or misaligned pointer");
+    const int64_t words = rows * (cols / 8);
+    unsigned grid;
+    if (int s = conv_grid(words, &grid)) return s;
+    cudaStream_t st = as_stream(stream);
+    __half* sp = reinterpret_cast<__half*>(scales);
+    __half* bp = reinterpret_cast<__half*>(biases);
+    auto go = [&](auto xt) {
+        using XT = decltype(xt);
+        const XT* p = static_cast<const XT*>(w);
+        if (group == 32) q4_quantize_kernel<XT, 32><<<grid, kConvThreads, 0, st>>>(p, words, codes, sp, bp);
+        else if (group == 64) q4_quantize_kernel<XT, 64><<<grid, kConvThreads, 0, st>>>(p, words, codes, sp, bp);
+        else q4_quantize_kernel<XT, 128><<<grid, kConvThreads, 0, st>>>(p, words, codes, sp, bp);
+    };
+    if (dtype == SMOE_F16) go(__half{});
+    else if (dtype == SMOE_F32) go(float{});
+    else return fail(SMOE_EDTYPE, "q4_quantize takes float16 or float32 weights");
+    return launch_status("q4_quantize");
+    Q4_CATCH("q4_quantize")
+}
+
+static int dequant(const uint32_t* codes, const uint16_t* scales, const uint16_t* biases, const uint8_t* packed,
+                   int64_t experts, int64_t rows, int64_t cols, int group, void* out, int out_dtype, void* stream) {
+    if (experts == 0 || rows == 0) return SMOE_OK;
+    if (int s = check_matrix(rows, cols, group)) return s;
+    SMOE_REQUIRE(experts > 0, SMOE_ESHAPE, "q4_dequant: a negative number of matrices");
+    SMOE_REQUIRE((packed ? aligned16(packed) : codes && scales && biases) && out && aligned16(out), SMOE_EARG,
+                 "q4_dequant: null or misaligned pointer");
+    const int64_t words = experts * rows * (cols / 8);
+    unsigned grid;
+    if (int s = conv_grid(words, &grid)) return s;
+    cudaStream_t st = as_stream(stream);
+    const __half* sp = reinterpret_cast<const __half*>(scales);
+    const __half* bp = reinterpret_cast<const __half*>(biases);
+    if (out_dtype == SMOE_F16)
+        q4_dequant_kernel<__half><<<grid, kConvThreads, 0, st>>>(codes, sp, bp, packed, words, rows, cols, group,
+                                                               static_cast<__half*>(out));
+    else if (out_dtype == SMOE_F32)
+        q4_dequant_kernel<float><<<grid, kConvThreads, 0, st>>>(codes, sp, bp, packed, words, rows, cols, group,
+                                                              static_cast<float*>(out));
+    else
+        return fail(SMOE_EDTYPE, "q4_dequant gives float16 or float32");
+    return launch_status("q4_dequant");
+}
+
+extern "C" int smoe_q4_dequant(const uint32_t* codes, const uint16_t* scales, const uint16_t* biases, int64_t rows,
+                               int64_t cols, int group, void* out, int out_dtype, void* stream) {
+    Q4_TRY
+    return dequant(codes, scales, biases, nullptr, 1, rows, cols, group, out, out_dtype, stream);
+    Q4_CATCH("q4_dequant")
+}
+
+extern "C" int smoe_q4_unpack(const uint8_t* packed, int64_t experts, int64_t rows, int64_t cols, int group, void* out,
+                              int out_dtype, void* stream) {
+    Q4_TRY
+    SMOE_REQUIRE(packed || experts == 0 || rows == 0, SMOE_EARG, "q4_unpack: null pointer");
+    return dequant(nullptr, nullptr, nullptr, packed, experts, rows, cols, group, out, out_dtype, stream);
+    Q4_CATCH("q4_unpack")
+}
+
+extern "C" int smoe_q4_pack(const uint32_t* codes, const uint16_t* scales, const uint16_t* biases, int64_t experts,
+                            int64_t rows, int64_t cols, int group, uint8_t* packed, void* stream) {
+    Q4_TRY
+    if (experts == 0) return SMOE_OK;
+    if (int s = check_matrix(rows, cols, group)) return s;
+    SMOE_REQUIRE(experts > 0, SMOE_ESHAPE, "q4_pack: a negative number of matrices");
+    SMOE_REQUIRE(codes && scales && biases && packed && aligned16(packed), SMOE_EARG,
+                 "q4_pack: null or misaligned pointer");
+    const size_t bytes = stack_bytes(experts, rows, cols, group);
+    unsigned grid;
+    if (int s = conv_grid(static_cast<int64_t>(bytes / 4), &grid)) return s;
+    cudaStream_t st = as_stream(stream);
+    q4_pack_kernel<<<grid, kConvThreads, 0, st>>>(codes, reinterpret_cast<const __half*>(scales),
+                                                 reinterpret_cast<const __half*>(biases), experts, rows, cols, group,
+                                                 reinterpret_cast<uint32_t*>(packed), static_cast<int64_t>(bytes / 4));
+    pdl_note(st, Writes().add(packed, bytes));  // (a product right behind it must not read ahead)
+    return launch_status("q4_pack");
+    Q4_CATCH("q4_pack")
+}
+
+extern "C" int smoe_q4_product(const SmoeQ4Product* p, void* stream) {
+    Q4_TRY
+    SMOE_REQUIRE(p, SMOE_EARG, "q4_product: null pointer");
+    SMOE_REQUIRE(p->dtype == SMOE_F16 || p->dtype == SMOE_F32, SMOE_EDTYPE,
+                 "q4_product takes float16 or float32 activations");
+    SMOE_REQUIRE(p->dense_tokens >= 0 && p->pairs >= 0, SMOE_EARG, "q4_product: a negative count");
+    if (p->dense_tokens == 0 && p->pairs == 0) return SMOE_OK;
+    const size_t item = p->dtype == SMOE_F16 ? 2 : 4;
+    ProductArgs a = {};
+    Writes w;
+    cudaStream_t st = as_stream(stream);
+    a.early = true;
+    a.hint = p->pairs > 0;
+    SMOE_REQUIRE(p->x && aligned16(p->x), SMOE_EARG, "q4_product: activations must be 16-byte aligned");
+    a.x = p->x;
+    a.cols = p->cols;
+    a.share = 1;
+    const bool glu = (p->dense_tokens > 0 ? p->dense2 : p->stack2) != nullptr;
+    if (p->dense_tokens > 0) {
+        if (int s = check_matrix(p->dense_rows, p->cols, p->group)) return s;
+        SMOE_REQUIRE(p->dense && p->dense_out && aligned16(p->dense) && aligned16(p->dense2), SMOE_EARG,
+                     "q4_product: null or misaligned pointer");
+        SMOE_REQUIRE(p->dense_gate == nullptr || glu, SMOE_EARG, "q4_product: a gate needs gate and up matrices");
+        SMOE_REQUIRE(p->dense_tokens <= kMost && strips_of_rows(p->dense_rows) * ((p->dense_tokens + 7) / 8) <= kMost,
+                     SMOE_ESHAPE, "too many tokens for one q4_product call");
+        a.dw[0] = p->dense;
+        a.dw[1] = p->dense2;
+        a.d_out = p->dense_out;
+        a.d_rows = p->dense_rows;
+        a.d_tokens = p->dense_tokens;
+        a.d_gate = p->dense_gate;
+        w.add(p->dense_out, size_t(p->dense_tokens) * p->dense_rows * item);
+        const size_t bytes = stack_bytes(1, p->dense_rows, p->cols, p->group);
+        a.early = a.early && pdl_early(st, p->dense, bytes) && (!p->dense2 || pdl_early(st, p->dense2, bytes));
+    }
+    if (p->pairs > 0) {
+        if (int s = check_matrix(p->rows, p->cols, p->group)) return s;
+        SMOE_REQUIRE(p->stack && p->out && p->idx && aligned16(p->stack) && aligned16(p->stack2), SMOE_EARG,
+                     "q4_product: null or misaligned pointer");
+        SMOE_REQUIRE(p->share > 0 && p->pairs % p->share == 0, SMOE_EARG, "pairs must be a multiple of share");
+        SMOE_REQUIRE(p->experts > 0 && p->experts <= 2048, SMOE_ESHAPE, "q4_product takes 1 to 2048 experts");
+        SMOE_REQUIRE(p->pairs <= kMaxPairs, SMOE_ESHAPE,
+                     "q4_product takes up to " + std::to_string(kMaxPairs) + " pairs a call");
+        SMOE_REQUIRE(strips_of_rows(p->rows) * p->pairs <= kMost, SMOE_ESHAPE, "too many rows for one q4_product call");
+        SMOE_REQUIRE(p->dense_tokens == 0 || (p->stack2 != nullptr) == glu, SMOE_EARG,
+                     "q4_product: the dense and the stack part are both products or both gated");
+        SMOE_REQUIRE(p->weights == nullptr || glu, SMOE_EARG, "q4_product: weights need gate and up stacks");
+        a.rw[0] = p->stack;
+        a.rw[1] = p->stack2;
+        a.r_out = p->out;
+        a.r_rows = p->rows;
+        a.experts = p->experts;
+        a.pairs = p->pairs;
+        a.share = p->share;
+        a.idx = p->idx;
+        a.weights = p->weights;
+        w.add(p->out, size_t(p->pairs) * p->rows * item);
+        const size_t bytes = stack_bytes(p->experts, p->rows, p->cols, p->group);
+        a.early = a.early && pdl_early(st, p->stack, bytes) && (!p->stack2 || pdl_early(st, p->stack2, bytes));
+    }
+    return p->dtype == SMOE_F16 ? product_f16(a, p->group, w, st) : product_f32(a, p->group, w, st);
+    Q4_CATCH("q4_product")
+}
+
+extern "C" int smoe_q4_linear(const uint8_t* packed, int64_t rows, int64_t cols, int group, const void* x,
+                              int64_t tokens, void* out, int dtype, void* stream) {
+    SmoeQ4Product p = {};
+    p.dtype = dtype;
+    p.group = group;
+    p.x = x;
+    p.cols = cols;
+    p.dense = packed;
+    p.dense_rows = rows;
+    p.dense_tokens = tokens;
+    p.dense_out = out;
+    return smoe_q4_product(&p, stream);
+}
+
+static size_t moe_h_bytes(int dtype, int64_t rows, int64_t ffn) {
+    return (size_t(rows) * ffn * (dtype == SMOE_F16 ? 2 : 4) + 255) & ~size_t(255);
+}
+
+extern "C" size_t smoe_q4_moe_workspace_size(int dtype, int64_t tokens, int64_t k, int64_t ffn, int64_t shared_ffn) {
+    if (tokens <= 0 || k <= 0 || ffn <= 0 || shared_ffn < 0) return 0;
+    return moe_h_bytes(dtype, tokens * k, ffn) + moe_h_bytes(dtype, tokens, shared_ffn);
+}
+
+extern "C" int smoe_q4_moe(const SmoeQ4Moe* m, void* workspace, size_t workspace_bytes, void* stream) {
+    Q4_TRY
+    SMOE_REQUIRE(m, SMOE_EARG, "q4_moe: null pointer");
+    SMOE_REQUIRE(m->dtype == SMOE_F16 || m->dtype == SMOE_F32, SMOE_EDTYPE, "q4_moe takes float16 or float32 activations");
+    SMOE_REQUIRE(m->tokens >= 0, SMOE_EARG, "q4_moe: a negative count");
+    if (m->tokens == 0) return SMOE_OK;
+    SMOE_REQUIRE(m->tokens <= 64, SMOE_ESHAPE, "q4_moe takes up to 64 tokens a call");
+    SMOE_REQUIRE(m->experts > 0 && m->experts <= 2048, SMOE_ESHAPE, "q4_moe takes 1 to 2048 experts");
+    SMOE_REQUIRE(m->k >= 1 && m->k <= 32, SMOE_ESHAPE, "q4_moe takes 1 to 32 experts a token");
+    if (int s = check_matrix(m->ffn, m->hidden, m->group)) return s;
+    if (int s = check_matrix(m->hidden, m->ffn, m->down_group)) return s;
+    SMOE_REQUIRE(m->shared_ffn >= 0, SMOE_ESHAPE, "q4_moe: a negative width");
+    if (m->shared_ffn > 0) {
+        if (int s = check_matrix(m->shared_ffn, m->hidden, m->group)) return s;
+        if (int s = check_matrix(m->hidden, m->shared_ffn, m->down_group)) return s;
+        SMOE_REQUIRE(m->sgate && m->sup && m->sdown, SMOE_EARG, "q4_moe: a shared expert needs its three matrices");
+    }
+    SMOE_REQUIRE(m->x && m->idx && m->weights && m->gate && m->up && m->down && m->out && aligned16(m->down) &&
+                     aligned16(m->sdown),
+                 SMOE_EARG, "q4_moe: null or misaligned pointer");
+    SMOE_REQUIRE(workspace && aligned16(workspace) &&
+                     workspace_bytes >= smoe_q4_moe_workspace_size(m->dtype, m->tokens, m->k, m->ffn, m->shared_ffn),
+                 SMOE_EWORKSPACE, "q4_moe: workspace missing, misaligned or too small");
+    cudaStream_t st = as_stream(stream);
+    void* h = workspace;
+    void* hs = static_cast<uint8_t*>(workspace) + moe_h_bytes(m->dtype, m->tokens * m->k, m->ffn);
+    SmoeQ4Product p = {};
+    p.dtype = m->dtype;
+    p.group = m->group;
+    p.x = m->x;
+    p.cols = m->hidden;
+    if (m->shared_ffn > 0) {
+        p.dense = m->sgate;
+        p.dense2 = m->sup;
+        p.dense_rows = m->shared_ffn;
+        p.dense_tokens = m->tokens;
+        p.dense_gate = m->shared_gate;
+        p.dense_out = hs;
+    }
+    p.stack = m->gate;
+    p.stack2 = m->up;
+    p.rows = m->ffn;
+    p.experts = m->experts;
+    p.idx = m->idx;
+    p.pairs = m->tokens * m->k;
+    p.share = m->k;
+    p.weights = m->weights;
+    p.out = h;
+    if (int s = smoe_q4_product(&p, stream)) return s;
+    DownArgs d = {};
+    d.h = h;
+    d.hs = m->shared_ffn > 0 ? hs : nullptr;
+    d.w = m->down;
+    d.sw = m->sdown;
+    d.ffn = m->ffn;
+    d.sffn = m->shared_ffn;
+    d.rows = m->hidden;
+    d.experts = m->experts;
+    d.tokens = m->tokens;
+    d.k = m->k;
+    d.idx = m->idx;
+    d.out = m->out;
+    // (the launch before is the product above, which writes h and hs alone and has waited for everything before it)
+    d.early = true;
+    Writes w;
+    w.add(m->out, size_t(m->tokens) * m->hidden * (m->dtype == SMOE_F16 ? 2 : 4));
+    return m->dtype == SMOE_F16 ? down_f16(d, m->down_group, w, st) : down_f32(d, m->down_group, w, st);
+    Q4_CATCH("q4_moe")
+}
+
+extern "C" int smoe_q4_status(int* status, int clear) {
+    SMOE_REQUIRE(status, SMOE_EARG, "q4_status: null pointer");
+    *status = 0;
+    cudaError_t e = cudaDeviceSynchronize();
+    for (auto read : {product_status_f16, product_status_f32, down_status_f16, down_status_f32}) {
+        int v = 0;
+        if (e == cudaSuccess) e = read(&v, clear != 0);
+        if (v != 0) *status = v;
+    }
+    if (e != cudaSuccess) return fail(-static_cast<int>(e), std::string("q4_status: ") + cudaGetErrorString(e));
+    return SMOE_OK;
+}

@@ -14,7 +14,7 @@ import ctypes
 
 import torch
 
-from . import _lib
+from . import _lib, affine
 from .blocks import BlockMLP, BlockSwitchGLU, decode_products
 
 ROUTER_TOPK = True  # strata_mlx/fused.py:420 (the kernel is the only top-k here; kept for engines that set it)
@@ -85,6 +85,27 @@ def top_k_softmax(logits: torch.Tensor, k: int):
 
 
 _COUNTERS = {}
+_COUNTER_POOL = {}  # device -> [zeroed words, words given to captured calls]
+
+
+def _route_counters(nbytes: int, defer: bool, device) -> torch.Tensor:
+    """The zeroed counters of one route call; the kernels leave them zero. Eager calls of one stream run one after
+    another and share theirs; a captured call gets words of its own, because two graphs that hold one may run at once."""
+    words = nbytes // 4
+    if device not in _COUNTER_POOL and not torch.cuda.is_current_stream_capturing():
+        _COUNTER_POOL[device] = [torch.zeros(1 << 18, dtype=torch.int32, device=device), 0]
+    if torch.cuda.is_current_stream_capturing():
+        pool = _COUNTER_POOL.get(device)
+        if pool is None or pool[1] + words > pool[0].numel():
+            return torch.zeros(words, dtype=torch.int32, device=device)  # (a memset in the graph)
+        at, pool[1] = pool[1], pool[1] + (words + 15) // 16 * 16
+        return pool[0][at : at + words]
+    key = (str(device), nbytes, defer, torch.cuda.current_stream(device).cuda_stream)
+    counters = _COUNTERS.get(key)
+    if counters is None:
+        counters = _COUNTERS[key] = torch.zeros(words, dtype=torch.int32, device=device)
+    return counters
+
 
 FUSED_ROUTE = False  # decode: the route in the gate / up launch (smoe_route_matvec_batch; measured slower)
 LAYER_KERNEL = False  # one launch per one-token step (smoe_decode_layer) where the types and shapes allow it
@@ -172,10 +193,7 @@ def route(gate: "WindowLinear", shared_gate, x: torch.Tensor, k: int, local=None
     w = torch.empty((tokens, k), dtype=torch.float32, device=dev)
     g = torch.empty((tokens,), dtype=x.dtype, device=dev) if shared_gate is not None else None
     nbytes = int(_lib.lib().smoe_route_step_counters(tokens) if defer else _lib.lib().smoe_route_counters(tokens))
-    key = (str(dev), nbytes, defer)
-    counters = _COUNTERS.get(key)
-    if counters is None:
-        counters = _COUNTERS[key] = torch.zeros(nbytes // 4, dtype=torch.int32, device=dev)
+    counters = _route_counters(nbytes, defer, dev)
     lidx = torch.empty((tokens, k), dtype=torch.uint32, device=dev) if local is not None else None
     lead = x.shape[:-1]
     if defer:
@@ -233,9 +251,10 @@ class SparseMoeBlock:
         y = switch_mlp(x, idx); g = shared_expert_gate(x); s = shared_expert(x); out = moe_combine(y, w, g, s)
 
     gate: WindowLinear or float16 weight (experts, hidden); switch_mlp: BlockSwitchGLU; shared_expert:
-    BlockMLP; shared_expert_gate: float16 weight (1, hidden)."""
+    BlockMLP; shared_expert_gate: float16 weight (1, hidden). With the 4-bit experts of `affine` (QuantizedSwitchGLU,
+    QuantizedMLP) everything behind the route is two launches (`affine.moe`), its sums float32 to the end."""
 
-    def __init__(self, gate, switch_mlp: BlockSwitchGLU, shared_expert: BlockMLP, shared_expert_gate, top_k: int):
+    def __init__(self, gate, switch_mlp, shared_expert, shared_expert_gate, top_k: int):
         self.gate = gate if isinstance(gate, WindowLinear) else WindowLinear(gate)
         self.switch_mlp, self.shared_expert = switch_mlp, shared_expert
         self.shared_expert_gate = shared_expert_gate if isinstance(shared_expert_gate, WindowLinear) else WindowLinear(
@@ -258,6 +277,10 @@ class SparseMoeBlock:
             idx, w = top_k_softmax(logits, self.top_k)
             g = self.shared_expert_gate(x).to(x.dtype)
         ys = None
+        if affine.moe_takes(self.switch_mlp, self.shared_expert):
+            if step is not None:
+                launch_route(step)
+            return affine.moe(self.switch_mlp, self.shared_expert, x, idx, w, g)
         if isinstance(self.switch_mlp, BlockSwitchGLU) and isinstance(self.shared_expert, BlockMLP):
             ys = decode_products(self.switch_mlp, self.shared_expert, x, idx, w, g, route_step=step)
         if ys is None and step is not None:
