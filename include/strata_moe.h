@@ -534,7 +534,8 @@ typedef struct SmoeQ4Moe {
     const uint8_t *sgate, *sup, *sdown;
     void* out;
 } SmoeQ4Moe;
-SMOE_API size_t smoe_q4_moe_workspace_size(int dtype, int64_t tokens, int64_t k, int64_t ffn, int64_t shared_ffn);
+SMOE_API size_t smoe_q4_moe_workspace_size(int dtype, int64_t tokens, int64_t k, int64_t hidden, int64_t ffn,
+                                             int64_t shared_ffn);
 SMOE_API int smoe_q4_moe(const SmoeQ4Moe* m, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Whether a bounded wait of the 4-bit kernels gave up since the last clear (SMOE_ETIMEOUT; outputs since are not

@@ -144,7 +144,7 @@ SIGNATURES = {
     "smoe_q4_unpack": (_i, [_p, _i64, _i64, _i64, _i, _p, _i, _p]),
     "smoe_q4_linear": (_i, [_p, _i64, _i64, _i, _p, _i64, _p, _i, _p]),
     "smoe_q4_product": (_i, [_c.POINTER(SmoeQ4Product), _p]),
-    "smoe_q4_moe_workspace_size": (_sz, [_i, _i64, _i64, _i64, _i64]),
+    "smoe_q4_moe_workspace_size": (_sz, [_i, _i64, _i64, _i64, _i64, _i64]),
     "smoe_q4_moe": (_i, [_c.POINTER(SmoeQ4Moe), _p, _sz, _p]),
     "smoe_q4_status": (_i, [_c.POINTER(_i), _i]),
 }
@@ -192,8 +192,13 @@ def ptr(t):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
 
 
+def raw_stream(device: int) -> int:
+    """The handle of `device`'s current stream (no Stream object is made: 0.1 us against 3 us)."""
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
 def stream():
-    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    return ctypes.c_void_p(raw_stream(torch.cuda.current_device()))
 
 
 def dtype_code(dt) -> int:

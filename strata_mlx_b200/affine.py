@@ -36,11 +36,9 @@ def _check_group(group_size: int, bits: int = BITS) -> None:
         raise ValueError(f"groups of {group_size} columns are not supported (32, 64 or 128)")
 
 
-def _same_device(*tensors):
-    _lib.require_cuda(*tensors)
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) > 1:
-        raise ValueError(f"tensors on different devices: {sorted(map(str, devices))}")
+def _elsewhere(device) -> bool:
+    """Whether `device` is not the current one (the kernels launch on the current device)."""
+    return device.index != torch.cuda.current_device()
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
@@ -51,15 +49,17 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
 
 def _check_parts(codes, scales, biases, group_size, bits=BITS):
     _check_group(group_size, bits)
-    _same_device(codes, scales, biases)
+    _lib.require_cuda(codes, scales, biases)
+    if not codes.device == scales.device == biases.device:
+        raise ValueError(f"codes, scales and biases on {codes.device}, {scales.device} and {biases.device}")
     if codes.dtype not in (torch.int32, torch.uint32):
         raise ValueError(f"codes come as 32-bit words, not {codes.dtype}")
     if scales.dtype != torch.float16 or biases.dtype != torch.float16:
         raise ValueError("scales and biases are float16")
-    if codes.dim() < 2 or scales.shape != biases.shape or scales.shape[:-1] != codes.shape[:-1] or (
-            codes.shape[-1] * 8 != scales.shape[-1] * group_size):
-        raise ValueError(f"codes {tuple(codes.shape)}, scales {tuple(scales.shape)} and biases {tuple(biases.shape)} "
-                         f"are no matrix in groups of {group_size}")
+    cs, ss = codes.shape, scales.shape
+    if len(cs) < 2 or ss != biases.shape or ss[:-1] != cs[:-1] or cs[-1] * 8 != ss[-1] * group_size:
+        raise ValueError(f"codes {tuple(cs)}, scales {tuple(ss)} and biases {tuple(biases.shape)} are no matrix in groups "
+                         f"of {group_size}")
 
 
 def quantize(w: torch.Tensor, group_size: int = 64, bits: int = BITS):
@@ -72,16 +72,19 @@ def quantize(w: torch.Tensor, group_size: int = 64, bits: int = BITS):
     if w.dim() < 1 or w.shape[-1] == 0 or w.shape[-1] % group_size:
         raise ValueError(f"{tuple(w.shape)}: the columns are no whole number of groups of {group_size}")
     code = _lib.dtype_code(w.dtype)
+    if _elsewhere(w.device):
+        with torch.cuda.device(w.device):
+            return quantize(w, group_size, bits)
     cols = w.shape[-1]
     rows = w.numel() // cols
-    with torch.cuda.device(w.device):
-        w2 = _aligned(w)
-        codes = torch.empty((*w.shape[:-1], cols // 8), dtype=torch.int32, device=w.device)
-        scales = torch.empty((*w.shape[:-1], cols // group_size), dtype=torch.float16, device=w.device)
-        biases = torch.empty_like(scales)
-        if rows:
-            _lib.call("smoe_q4_quantize", _lib.ptr(w2), code, rows, cols, group_size, _lib.ptr(codes),
-                      _lib.ptr(scales), _lib.ptr(biases), _lib.stream())
+    w2 = _aligned(w)
+    lead = w.shape[:-1]
+    codes = w.new_empty((*lead, cols // 8), dtype=torch.int32)
+    scales = w.new_empty((*lead, cols // group_size), dtype=torch.float16)
+    biases = torch.empty_like(scales)
+    if rows:
+        _lib.call("smoe_q4_quantize", w2.data_ptr(), code, rows, cols, group_size, codes.data_ptr(), scales.data_ptr(),
+                  biases.data_ptr(), _lib.raw_stream(w.device.index))
     return codes, scales, biases
 
 
@@ -90,13 +93,16 @@ def dequantize(codes: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor, 
     """The floats (..., rows, cols) of `quantize`'s arrays: code * scale + bias in float32, rounded to `dtype`."""
     _check_parts(codes, scales, biases, group_size, bits)
     code = _lib.dtype_code(dtype)
+    if _elsewhere(codes.device):
+        with torch.cuda.device(codes.device):
+            return dequantize(codes, scales, biases, group_size, bits, dtype)
     cols = codes.shape[-1] * 8
-    with torch.cuda.device(codes.device):
-        out = torch.empty((*codes.shape[:-1], cols), dtype=dtype, device=codes.device)
-        if out.numel():
-            codes, scales, biases = codes.contiguous(), scales.contiguous(), biases.contiguous()
-            _lib.call("smoe_q4_dequant", _lib.ptr(codes), _lib.ptr(scales), _lib.ptr(biases), out.numel() // cols, cols,
-                      group_size, _lib.ptr(out), code, _lib.stream())
+    out = codes.new_empty((*codes.shape[:-1], cols), dtype=dtype)
+    n = out.numel()
+    if n:
+        codes, scales, biases = codes.contiguous(), scales.contiguous(), biases.contiguous()
+        _lib.call("smoe_q4_dequant", codes.data_ptr(), scales.data_ptr(), biases.data_ptr(), n // cols, cols, group_size,
+                  out.data_ptr(), code, _lib.raw_stream(codes.device.index))
     return out
 
 
@@ -131,13 +137,13 @@ class _Packed:
         return out
 
     def _rows(self, x: torch.Tensor) -> torch.Tensor:
-        """x (..., in) as aligned rows (n, in)."""
+        """x (..., in) as rows one after the other, on a 16-byte boundary."""
         if x.dim() < 1 or x.shape[-1] != self.input_dims:
             raise ValueError(f"activations {tuple(x.shape)} do not end in {self.input_dims}")
         if x.device != self.device:
             _lib.require_cuda(x)
             raise ValueError(f"activations on {x.device}, weights on {self.device}")
-        return _aligned(x.reshape(-1, self.input_dims))
+        return _aligned(x)
 
 
 class QuantizedLinear(_Packed):
@@ -160,14 +166,14 @@ class QuantizedLinear(_Packed):
     def __call__(self, x: torch.Tensor) -> torch.Tensor:
         code = _lib.dtype_code(x.dtype)
         x2 = self._rows(x)
-        if self.device.index != torch.cuda.current_device():
+        if _elsewhere(self.device):
             with torch.cuda.device(self.device):
                 return self(x)
-        tokens = x2.shape[0]
-        out = torch.empty((*x.shape[:-1], self.output_dims), dtype=x.dtype, device=self.device)
+        out = x.new_empty((*x.shape[:-1], self.output_dims))
+        tokens = x2.numel() // self.input_dims
         if tokens:
             _lib.call("smoe_q4_linear", self.data_ptr, self.output_dims, self.input_dims, self.group_size,
-                      x2.data_ptr(), tokens, out.data_ptr(), code, torch.cuda.current_stream().cuda_stream)
+                      x2.data_ptr(), tokens, out.data_ptr(), code, _lib.raw_stream(self.device.index))
         return out
 
 
@@ -220,7 +226,7 @@ class QuantizedSwitchLinear(_Packed):
             share = k
         else:
             x, share = x.expand(*ishape, 1, self.input_dims), 1
-        out = _pairs_product(self, None, self._rows(x), indices, share)
+        out = _pairs_product(self, None, self._rows(x).reshape(-1, self.input_dims), indices, share)
         return out.reshape(*ishape, 1, self.output_dims)
 
 
@@ -272,7 +278,8 @@ class QuantizedSwitchGLU:
     def __call__(self, x: torch.Tensor, indices: torch.Tensor) -> torch.Tensor:
         if indices.dim() < 1:
             raise ValueError("indices must hold k experts for every token of x")
-        h = _pairs_product(self.gate_proj, self.up_proj, self.gate_proj._rows(x), indices, indices.shape[-1])
+        h = _pairs_product(self.gate_proj, self.up_proj, self.gate_proj._rows(x).reshape(-1, x.shape[-1]), indices,
+                           indices.shape[-1])
         out = _pairs_product(self.down_proj, None, h, indices, 1)
         return out.reshape(*indices.shape, self.down_proj.output_dims)
 
@@ -287,7 +294,7 @@ class QuantizedMLP:
     def __call__(self, x: torch.Tensor) -> torch.Tensor:
         code = _lib.dtype_code(x.dtype)
         gate, up = self.gate_proj, self.up_proj
-        x2 = gate._rows(x)
+        x2 = gate._rows(x).reshape(-1, gate.input_dims)
         with torch.cuda.device(gate.device):
             h = torch.empty((x2.shape[0], gate.output_dims), dtype=x.dtype, device=gate.device)
             if x2.shape[0]:
@@ -319,8 +326,10 @@ def moe(switch_mlp: QuantizedSwitchGLU, shared: QuantizedMLP, x: torch.Tensor, i
     gate, down = switch_mlp.gate_proj, switch_mlp.down_proj
     sgate, sdown = shared.gate_proj, shared.down_proj
     code = _lib.dtype_code(x.dtype)
-    x2 = gate._rows(x)
-    _same_device(x, indices, w, g)
+    x2 = gate._rows(x).reshape(-1, gate.input_dims)
+    _lib.require_cuda(indices, w, g)
+    if any(t.device != gate.device for t in (indices, w, g)):
+        raise ValueError(f"weights on {gate.device}, a choice on another device")
     tokens, k = x2.shape[0], indices.shape[-1] if indices.dim() else 0
     if indices.numel() != tokens * k or w.numel() != tokens * k or g.numel() != tokens or not 1 <= k <= 32:
         raise ValueError("moe takes 1 to 32 experts and weights and one gate value for every token")
@@ -331,7 +340,8 @@ def moe(switch_mlp: QuantizedSwitchGLU, shared: QuantizedMLP, x: torch.Tensor, i
         out = torch.empty((tokens, gate.input_dims), dtype=x.dtype, device=gate.device)
         for t0 in range(0, tokens, MOE_TOKENS):
             n = min(MOE_TOKENS, tokens - t0)
-            nbytes = int(_lib.lib().smoe_q4_moe_workspace_size(code, n, k, gate.output_dims, sgate.output_dims))
+            nbytes = int(_lib.lib().smoe_q4_moe_workspace_size(code, n, k, gate.input_dims, gate.output_dims,
+                                                                sgate.output_dims))
             ws = torch.empty(nbytes, dtype=torch.uint8, device=gate.device)
             spec = _lib.SmoeQ4Moe(
                 dtype=code, group=gate.group_size, down_group=down.group_size, tokens=n, hidden=gate.input_dims,

@@ -1,5 +1,5 @@
 // 4-bit weights with a float16 scale and bias for each group of 32, 64 or 128 columns: the layout the kernels
-// read, and one tile of it times up to 8 NT activation rows on the tensor cores.
+// read, and a tile of two strips of it times 8 activation rows on the tensor cores.
 //
 //   w[r, c] = code[r, c] * scale[r, c / G] + bias[r, c / G],   code in 0 .. 15
 //
@@ -17,14 +17,16 @@
 // columns inside an MMA is free as long as A and B agree, so lane (g, t)'s word goes in as it lies: nibbles 0, 4
 // and 2, 6 to one MMA, 1, 5 and 3, 7 to the other. With float16 activations a nibble needs no conversion at all:
 // (word & 0x000f000f) is a pair of float16 subnormals q * 2^-24, exact in the tensor core, and (word & 0x00f000f0)
-// a pair of 16 q * 2^-24; the two MMAs keep sums of their own, joined as lo + hi / 16 and scaled by 2^24 scale at
-// the end of the group. Products are exact and sums are float32: the result is the formula's but for float32
-// rounding. The bias takes sum x over the group, from the same B operands times a matrix of ones.
+// a pair of 16 q * 2^-24; the two MMAs keep sums of their own, joined as lo + hi / 16 at the end of the group, and
+// the 2^24 comes at the end of the row. Products are exact and sums are float32: the result is the formula's but for float32
+// rounding. The bias takes sum x over the group, from the same B operands times a matrix of 2^-24.
 // Float32 activations are three bfloat16 pieces (8 + 8 + 8 bits: the whole float32), each through the same MMAs;
 // codes become bfloat16 by (q | 0x4300) - 128, exact too.
 #pragma once
 
 #include <cuda_bf16.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 #include "tc05.cuh"
@@ -60,18 +62,34 @@ __device__ __forceinline__ void bulk_load_hint(uint32_t dst, const void* src, ui
         : "memory");
 }
 
+// d (+)= a b: m16n8k16, float32 sums; with FIRST, d = a b
+template <bool FIRST>
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    if constexpr (FIRST)
+        asm(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+    else
+        asm(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+template <bool FIRST>
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    if constexpr (FIRST)
+        asm(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+    else
+        asm(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 // ---- A operands of one 32-column run from row g's word `u` and row g + 8's word `v`
@@ -93,7 +111,7 @@ struct Codes<__half> {
         lo[3] = v & 0x000f000fu;
         hi[3] = v & 0x00f000f0u;
     }
-    static constexpr uint32_t kOne = 0x3c003c00u;
+    static constexpr uint32_t kOne = 0x00010001u;  // 2^-24, as the codes
 };
 
 template <>
@@ -137,21 +155,25 @@ struct Acts<float> {
     }
 };
 
-// One run of up to MATS matrices times one block of 8 activation rows: sums of the group so far in lo / hi (float16:
-// hi holds 16 times its sum) and, of the activations alone, in on.
-template <int MATS>
-__device__ __forceinline__ void run_mma(const Codes<__half> (&a)[MATS], const Acts<__half>& x, float (&lo)[MATS][4],
-                                        float (&hi)[MATS][4], float (&on)[4]) {
+// The sums of one group of columns of MT strips times a block of 8 activation rows: codes in lo and hi (float16: hi
+// holds 16 times its sum, both 2^-24 times theirs; float32: lo alone), the activations alone in on (times 2^-24 too).
+template <typename T, int MT>
+struct Sums {
+    float lo[MT][4], hi[MT][4], on[4];
+};
+
+template <bool FIRST, int MT>
+__device__ __forceinline__ void run_mma(const Codes<__half> (&a)[MT], const Acts<__half>& x, Sums<__half, MT>& s) {
     const uint32_t b0 = __byte_perm(x.v.x, x.v.z, 0x5410), b1 = __byte_perm(x.v.y, x.v.w, 0x5410);
     const uint32_t c0 = __byte_perm(x.v.x, x.v.z, 0x7632), c1 = __byte_perm(x.v.y, x.v.w, 0x7632);
     constexpr uint32_t one = Codes<__half>::kOne;
 #pragma unroll
-    for (int m = 0; m < MATS; ++m) {
-        mma_f16(lo[m], a[m].lo[0], a[m].lo[1], a[m].lo[2], a[m].lo[3], b0, b1);
-        mma_f16(hi[m], a[m].hi[0], a[m].hi[1], a[m].hi[2], a[m].hi[3], c0, c1);
+    for (int m = 0; m < MT; ++m) {
+        mma_f16<FIRST>(s.lo[m], a[m].lo[0], a[m].lo[1], a[m].lo[2], a[m].lo[3], b0, b1);
+        mma_f16<FIRST>(s.hi[m], a[m].hi[0], a[m].hi[1], a[m].hi[2], a[m].hi[3], c0, c1);
     }
-    mma_f16(on, one, one, one, one, b0, b1);
-    mma_f16(on, one, one, one, one, c0, c1);
+    mma_f16<FIRST>(s.on, one, one, one, one, b0, b1);
+    mma_f16<false>(s.on, one, one, one, one, c0, c1);
 }
 
 __device__ __forceinline__ uint32_t bf16_pair(float& a, float& b) {
@@ -163,103 +185,110 @@ __device__ __forceinline__ uint32_t bf16_pair(float& a, float& b) {
     return r;
 }
 
-template <int MATS>
-__device__ __forceinline__ void run_mma(const Codes<float> (&a)[MATS], const Acts<float>& x, float (&lo)[MATS][4],
-                                        float (&hi)[MATS][4], float (&on)[4]) {
+template <bool FIRST, int MT>
+__device__ __forceinline__ void run_mma(const Codes<float> (&a)[MT], const Acts<float>& x, Sums<float, MT>& s) {
     float f[8] = {__uint_as_float(x.v.x), __uint_as_float(x.v.y), __uint_as_float(x.v.z), __uint_as_float(x.v.w),
                   __uint_as_float(x.w.x), __uint_as_float(x.w.y), __uint_as_float(x.w.z), __uint_as_float(x.w.w)};
     constexpr uint32_t one = Codes<float>::kOne;
-#pragma unroll
-    for (int piece = 0; piece < 3; ++piece) {
+    auto piece = [&](auto first) {
+        constexpr bool kFirst = decltype(first)::value;
         const uint32_t b0 = bf16_pair(f[0], f[4]), b1 = bf16_pair(f[2], f[6]);
         const uint32_t c0 = bf16_pair(f[1], f[5]), c1 = bf16_pair(f[3], f[7]);
 #pragma unroll
-        for (int m = 0; m < MATS; ++m) {
-            mma_bf16(lo[m], a[m].lo[0], a[m].lo[1], a[m].lo[2], a[m].lo[3], b0, b1);
-            mma_bf16(hi[m], a[m].hi[0], a[m].hi[1], a[m].hi[2], a[m].hi[3], c0, c1);
+        for (int m = 0; m < MT; ++m) {
+            mma_bf16<kFirst>(s.lo[m], a[m].lo[0], a[m].lo[1], a[m].lo[2], a[m].lo[3], b0, b1);
+            mma_bf16<false>(s.lo[m], a[m].hi[0], a[m].hi[1], a[m].hi[2], a[m].hi[3], c0, c1);
         }
-        mma_bf16(on, one, one, one, one, b0, b1);
-        mma_bf16(on, one, one, one, one, c0, c1);
-    }
+        mma_bf16<kFirst>(s.on, one, one, one, one, b0, b1);
+        mma_bf16<false>(s.on, one, one, one, one, c0, c1);
+    };
+    piece(std::integral_constant<bool, FIRST>{});
+    piece(std::false_type{});
+    piece(std::false_type{});
 }
+
+// What a row's sum is to be multiplied by in the end (the codes' 2^-24)
+template <typename T>
+__host__ __device__ constexpr float unit() { return sizeof(T) == 2 ? 16777216.0f : 1.0f; }
 
 // The end of a group: acc += scale (lo + hi) + bias on, rows g (values 0, 1) and g + 8 (values 2, 3).
-template <typename T>
-__device__ __forceinline__ void group_end(float (&acc)[4], const float (&lo)[4], const float (&hi)[4],
-                                          const float (&on)[4], uint32_t sb0, uint32_t sb1) {
+template <typename T, int MT>
+__device__ __forceinline__ void group_end(float (&acc)[4], const Sums<T, MT>& s, int m, uint32_t sb0, uint32_t sb1) {
     const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&sb0));
     const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&sb1));
-    constexpr bool kHalf = sizeof(T) == 2;
-    const float s0 = kHalf ? p.x * 16777216.0f : p.x, s1 = kHalf ? r.x * 16777216.0f : r.x;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float q = kHalf ? fmaf(hi[i], 0.0625f, lo[i]) : lo[i] + hi[i];
-        acc[i] = fmaf(q, i < 2 ? s0 : s1, fmaf(on[i], i < 2 ? p.y : r.y, acc[i]));
+        const float q = sizeof(T) == 2 ? fmaf(s.hi[m][i], 0.0625f, s.lo[m][i]) : s.lo[m][i];
+        acc[i] = fmaf(q, i < 2 ? p.x : r.x, fmaf(s.on[i], i < 2 ? p.y : r.y, acc[i]));
     }
 }
 
-// The (scale, bias) pairs of row `row` of a tile in shared memory
-template <int G>
-struct Pairs {
-    uint32_t v[kCols / G];
-    __device__ __forceinline__ explicit Pairs(const uint8_t* tile, int row) {
-        const uint8_t* p = tile + kCodeBytes + row * (kCols / G) * 4;
-        if constexpr (G == 32) {
-            const uint4 q = *reinterpret_cast<const uint4*>(p);
-            v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
-        } else if constexpr (G == 64) {
-            const uint2 q = *reinterpret_cast<const uint2*>(p);
-            v[0] = q.x, v[1] = q.y;
+// This lane's activations of a tile (row g, columns 8 t .. of each run): float16 all four runs at once, ahead of the
+// weights; float32 run by run as they are used (twice the registers). p: the lane's place in the row at the tile's first
+// column; runs: the row's runs from there on (four but for a last tile).
+template <typename T> struct TileActs;
+
+template <>
+struct TileActs<__half> {
+    Acts<__half> x[4];
+    __device__ __forceinline__ TileActs(const __half* p, int runs) {
+        if (runs >= 4) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j].load(p + 32 * j);
         } else {
-            v[0] = *reinterpret_cast<const uint32_t*>(p);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                x[j].zero();
+                if (j < runs) x[j].load(p + 32 * j);
+            }
         }
+    }
+    __device__ __forceinline__ Acts<__half> run(int j) const { return x[j]; }
+};
+
+template <>
+struct TileActs<float> {
+    const float* p;
+    int runs;
+    __device__ __forceinline__ TileActs(const float* at, int n) : p(at), runs(n) {}
+    __device__ __forceinline__ Acts<float> run(int j) const {
+        Acts<float> x;
+        if (j < runs) x.load(p + 32 * j);
+        else x.zero();
+        return x;
     }
 };
 
-// A tile of MATS matrices (shared memory, `mat_stride` bytes apart) times NT blocks of 8 activation rows.
-// load(nt, j, x): this lane's eight activations of run j and row 8 nt + g. on(nt): whether the block has rows at all
-// (the same for the whole warp).
-template <typename T, int G, int NT, int MATS, class Load, class On>
-__device__ __forceinline__ void tile_mma(const uint8_t* tile, int mat_stride, int lane, float (&acc)[MATS][NT][4],
-                                         Load load, On on_block) {
-    const int g = lane >> 2;
-    uint32_t wa[MATS][4], wb[MATS][4];
-    uint32_t pa[MATS][kCols / G], pb[MATS][kCols / G];
+// One tile of two strips (shared memory, `stride` bytes apart) times a block of 8 activation rows.
+template <typename T, int G>
+__device__ __forceinline__ void tile_mma(const uint8_t* tile, int stride, int lane, const TileActs<T>& x,
+                                         float (&acc)[2][4]) {
+    constexpr int kRuns = G / 32, kPairs = kCols / G;
+    uint32_t wa[2][4], wb[2][4];
 #pragma unroll
-    for (int m = 0; m < MATS; ++m) {
-        const uint8_t* p = tile + m * mat_stride;
-        const uint4 u = *reinterpret_cast<const uint4*>(p + 16 * lane);
-        const uint4 v = *reinterpret_cast<const uint4*>(p + 512 + 16 * lane);
+    for (int m = 0; m < 2; ++m) {
+        const uint8_t* p = tile + m * stride + 16 * lane;
+        const uint4 u = *reinterpret_cast<const uint4*>(p);
+        const uint4 v = *reinterpret_cast<const uint4*>(p + 512);
         wa[m][0] = u.x, wa[m][1] = u.y, wa[m][2] = u.z, wa[m][3] = u.w;
         wb[m][0] = v.x, wb[m][1] = v.y, wb[m][2] = v.z, wb[m][3] = v.w;
-        const Pairs<G> q0(p, g), q1(p, g + 8);
-#pragma unroll
-        for (int i = 0; i < kCols / G; ++i) pa[m][i] = q0.v[i], pb[m][i] = q1.v[i];
     }
-    constexpr int kRuns = G / 32;
+    const uint8_t* pairs = tile + kCodeBytes + (lane >> 2) * kPairs * 4;
 #pragma unroll
-    for (int gi = 0; gi < kCols / G; ++gi) {
+    for (int gi = 0; gi < kPairs; ++gi) {
+        Sums<T, 2> s;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            if (NT > 2 && !on_block(nt)) continue;
-            float lo[MATS][4] = {}, hi[MATS][4] = {}, on[4] = {};
+        for (int r = 0; r < kRuns; ++r) {
+            const int j = gi * kRuns + r;
+            const Codes<T> a[2] = {Codes<T>(wa[0][j], wb[0][j]), Codes<T>(wa[1][j], wb[1][j])};
+            if (r == 0) run_mma<true, 2>(a, x.run(j), s);
+            else run_mma<false, 2>(a, x.run(j), s);
+        }
 #pragma unroll
-            for (int r = 0; r < kRuns; ++r) {
-                const int j = gi * kRuns + r;
-                Acts<T> x;
-                load(nt, j, x);
-                // (with several blocks the codes are expanded again for each: five instructions a word, held registers
-                // would cost more)
-                if constexpr (MATS == 1) {
-                    const Codes<T> a[1] = {Codes<T>(wa[0][j], wb[0][j])};
-                    run_mma<1>(a, x, lo, hi, on);
-                } else {
-                    const Codes<T> a[2] = {Codes<T>(wa[0][j], wb[0][j]), Codes<T>(wa[MATS - 1][j], wb[MATS - 1][j])};
-                    run_mma<2>(a, x, lo, hi, on);
-                }
-            }
-#pragma unroll
-            for (int m = 0; m < MATS; ++m) group_end<T>(acc[m][nt], lo[m], hi[m], on, pa[m][gi], pb[m][gi]);
+        for (int m = 0; m < 2; ++m) {
+            const uint8_t* q = pairs + m * stride + 4 * gi;
+            group_end<T, 2>(acc[m], s, m, *reinterpret_cast<const uint32_t*>(q),
+                            *reinterpret_cast<const uint32_t*>(q + 8 * kPairs * 4));
         }
     }
 }

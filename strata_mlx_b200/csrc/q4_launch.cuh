@@ -10,7 +10,8 @@ namespace smoe {
 namespace q4 {
 
 constexpr int kSms = 148;
-constexpr int kCtasPerSm = 5;
+constexpr int kCtasPerSm = 2;
+constexpr int kDownCtas = kSms * kCtasPerSm;
 
 int product_f16(const ProductArgs& a, int group, const Writes& w, cudaStream_t st);
 int product_f32(const ProductArgs& a, int group, const Writes& w, cudaStream_t st);
@@ -30,30 +31,6 @@ inline cudaError_t read_status(int* v, bool clear) {
     return e;
 }
 
-// launch_pdl with a cluster of `csize` CTAs along x
-template <typename Args>
-inline cudaError_t launch_cluster(const Writes& writes, void (*kernel)(Args), unsigned ctas, int csize, size_t smem,
-                                  cudaStream_t st, const Args& args) {
-    const int status = max_smem(kernel, static_cast<int>(smem));
-    if (status != 0) return static_cast<cudaError_t>(-status);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = static_cast<unsigned>(csize);
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = csize > 1 ? 2 : 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args);
-    pdl_note(st, writes);
-    return e;
-}
-
 inline int status_of(cudaError_t e, const char* what) {
     if (e == cudaSuccess) return launch_status(what);
     cudaGetLastError();
@@ -61,64 +38,63 @@ inline int status_of(cudaError_t e, const char* what) {
     return -static_cast<int>(e);
 }
 
-// CTAs that share a job's columns: as many as keep every SM's slots taken, while each warp has a tile of its own
-inline int cluster_for(int64_t jobs, int64_t tiles) {
-    int c = 1;
-    while (c < 8 && jobs * 2 * c <= kSms * kCtasPerSm && tiles >= 2 * c * kWarps) c *= 2;
-    return c;
+// Warps that share a job's columns: the count with the least work for the busiest warp, a job's end taken as the work of
+// two tiles.
+inline int team_for(int64_t jobs, int64_t tiles) {
+    int best = 1;
+    int64_t least = 0;
+    for (int w = 1; w <= kWarps; w *= 2) {
+        const int64_t teams = int64_t(kSms) * kCtasPerSm * kWarps / w;
+        const int64_t work = (jobs + teams - 1) / teams * ((tiles + w - 1) / w + 2);
+        if (w == 1 || work < least) {
+            best = w;
+            least = work;
+        }
+    }
+    return best;
 }
 
-template <typename T, int G, int NT, int MATS>
+template <typename T, int G, bool GLU>
 inline int launch_product(const ProductArgs& args, const Writes& w, cudaStream_t st) {
     ProductArgs a = args;
-    const int64_t most = 8 * NT;
-    const int64_t jobs = strips_of_rows(a.d_rows) * ((a.d_tokens + most - 1) / most) +
-                         strips_of_rows(a.r_rows) * std::min(a.pairs, a.experts + a.pairs / most);
-    // (by the shapes alone: a token's sums are split alike alone and in a window)
-    const int csize = cluster_for(strips_of_rows(a.d_rows) + strips_of_rows(a.r_rows) * a.share, tiles_of_cols(a.cols));
-    a.stages = 4;
-    const size_t smem = product_smem<G, NT, MATS>(a.stages, a.pairs, a.experts);
-    const int64_t clusters = std::min<int64_t>(jobs, kSms * kCtasPerSm / csize);
-    return status_of(launch_cluster(w, q4_product_kernel<T, G, NT, MATS>, static_cast<unsigned>(clusters * csize), csize,
-                                    smem, st, a), "q4_product");
+    const int64_t wide = GLU ? 1 : 2;
+    const int64_t d_wide = (strips_of_rows(a.d_rows) + wide - 1) / wide, r_wide = (strips_of_rows(a.r_rows) + wide - 1) / wide;
+    const int64_t jobs = d_wide * ((a.d_tokens + kM - 1) / kM) + r_wide * std::min(a.pairs, a.experts + a.pairs / kM);
+    // (a dense matrix's by its shape alone: a token's sums are split alike alone and in a window)
+    a.team = team_for(a.pairs > 0 ? jobs : d_wide, tiles_of_cols(a.cols));
+    const size_t smem = product_smem<G>(a.pairs, a.experts);
+    if (int e = max_smem(q4_product_kernel<T, G, GLU>, static_cast<int>(smem))) return status_of(static_cast<cudaError_t>(-e), "q4_product");
+    const int64_t ctas = std::min<int64_t>((jobs * a.team + kWarps - 1) / kWarps, kSms * kCtasPerSm);
+    // (few jobs: a team on an SM of its own before two on one)
+    const int64_t spread = std::max<int64_t>(ctas, std::min<int64_t>(jobs, kSms));
+    return status_of(launch_pdl(w, q4_product_kernel<T, G, GLU>, dim3(static_cast<unsigned>(spread)), dim3(kThreads), smem,
+                                st, a), "q4_product");
 }
 
 template <typename T>
 inline int product(const ProductArgs& a, int group, const Writes& w, cudaStream_t st) {
-    const int64_t rows = std::max(a.d_tokens, a.pairs > 0 ? a.pairs / a.share : 0);
-    const bool two = rows > 8;
     const bool glu = a.dw[1] != nullptr || a.rw[1] != nullptr;
     auto go = [&](auto g) {
         constexpr int G = decltype(g)::value;
-        if (glu) return two ? launch_product<T, G, 2, 2>(a, w, st) : launch_product<T, G, 1, 2>(a, w, st);
-        return two ? launch_product<T, G, 2, 1>(a, w, st) : launch_product<T, G, 1, 1>(a, w, st);
+        return glu ? launch_product<T, G, true>(a, w, st) : launch_product<T, G, false>(a, w, st);
     };
     if (group == 32) return go(std::integral_constant<int, 32>{});
     if (group == 64) return go(std::integral_constant<int, 64>{});
     return go(std::integral_constant<int, 128>{});
 }
 
-template <typename T, int G, int NT>
-inline int launch_down(const DownArgs& args, const Writes& w, cudaStream_t st) {
-    DownArgs a = args;
-    const int64_t strips = strips_of_rows(a.rows);
-    // (at least one choice a token: a strip's tiles are the shared expert's and k experts' or more)
-    const int64_t tiles = tiles_of_cols(a.sffn) + a.k * tiles_of_cols(a.ffn);
-    const int csize = cluster_for(strips, tiles);
-    a.stages = 8;
-    const size_t smem = down_smem<G, NT>(a.stages, a.tokens * a.k, a.experts);
-    return status_of(launch_cluster(w, q4_down_kernel<T, G, NT>, static_cast<unsigned>(strips * csize), csize, smem, st, a),
-                     "q4_moe");
+template <typename T, int G>
+inline int launch_down(const DownArgs& a, const Writes& w, cudaStream_t st) {
+    const size_t smem = down_smem<G>(a.tokens, a.tokens * a.k, a.experts);
+    if (int e = max_smem(q4_down_kernel<T, G>, static_cast<int>(smem))) return status_of(static_cast<cudaError_t>(-e), "q4_moe");
+    return status_of(launch_pdl(w, q4_down_kernel<T, G>, dim3(kDownCtas), dim3(kThreads), smem, st, a), "q4_moe");
 }
 
 template <typename T>
 inline int down(const DownArgs& a, int group, const Writes& w, cudaStream_t st) {
     auto go = [&](auto g) {
         constexpr int G = decltype(g)::value;
-        if (a.tokens <= 8) return launch_down<T, G, 1>(a, w, st);
-        if (a.tokens <= 16) return launch_down<T, G, 2>(a, w, st);
-        if (a.tokens <= 32) return launch_down<T, G, 4>(a, w, st);
-        return launch_down<T, G, 8>(a, w, st);
+        return launch_down<T, G>(a, w, st);
     };
     if (group == 32) return go(std::integral_constant<int, 32>{});
     if (group == 64) return go(std::integral_constant<int, 64>{});

@@ -1,5 +1,5 @@
-// The two streaming kernels on 4-bit weights (layout and arithmetic: q4.cuh), instantiated by smoe_q4_f16.cu and
-// smoe_q4_f32.cu.
+// The two streaming kernels on 4-bit weights (layout and arithmetic: q4.cuh), instantiated by smoe_q4_product_*.cu and
+// smoe_q4_down_*.cu.
 //
 //   q4_product_kernel  out[p, r] = W[e_p][r, :] . x[p / share, :] for a dense matrix (every token through expert 0) and
 //                      / or a stack's (token, expert) pairs; with two stacks (gate, up) out = SwiGLU of the two sums,
@@ -8,24 +8,23 @@
 //                      block's down products and its combine, the pairs' weights already in h
 //
 // What bounds them: a weight is 4.5 bits (groups of 64) of HBM traffic and is used for at most a few rows, so the
-// floor is the weights' bytes. Everything here serves the stream of weights: a CTA is four warps, each with a ring
-// of bulk copies of its own that runs ahead of the arithmetic across the ends of jobs, and five CTAs share an SM,
-// so that 150 KB a SM are in flight (6.5 TB/s x 1 us of latency over 148 SMs asks for 44 KB). No barrier is on that
-// path: a warp waits only for its own copies, and the four meet once a job to add their sums.
+// floor is the weights' bytes; next to it stands the instruction issue (a tile of 16 x 128 weights is about 100 warp
+// instructions and 1152 bytes: 62 cycles of an SM at full bandwidth). So two strips of rows share each activation
+// operand, and nothing but a warp's own copies is waited for inside a job: every warp has a ring of bulk copies of its
+// own that runs ahead of the arithmetic across the ends of jobs, 16 warps a SM, 75 to 150 KB of a SM in flight (6.5
+// TB/s x 1 us of latency over 148 SMs asks for 44 KB).
 //
-// A job of the product kernel is a strip of 16 rows times one block of up to 8 NT activation rows of one expert; its
-// columns are split over the warps of a cluster of 1 to 8 CTAs (a fixed split, the partial sums added in its order:
-// the same bits every run). Several tokens of one expert read its rows once.
+// A job of the product kernel is two strips of 16 rows (gate's and up's, or two neighbours) times one block of up to 8
+// activation rows of one expert; its columns are split over a team of 1 to 8 warps of a CTA, the partial sums added in
+// the order of the columns: the same bits every run. Several tokens of one expert read its rows once.
 #pragma once
-
-#include <cooperative_groups.h>
 
 #include "q4.cuh"
 
 namespace smoe {
 namespace q4 {
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kMaxPairs = 2048;
 constexpr uint32_t kWaitLimit = 1u << 22;
@@ -48,9 +47,11 @@ struct ProductArgs {
     int64_t r_rows, experts, pairs, share;
     const uint32_t* idx;
     const float* weights;  // GLU: the pair's result times this, or null
-    int stages;            // slots of a warp's ring
-    bool early;            // the weights may be read before pdl_wait()
-    bool hint;             // weights evict-first in L2
+    uint32_t* zero;  // words to clear for the launch after (its counters)
+    int n_zero;
+    int team;    // warps that share a job's columns
+    bool early;  // the weights may be read before pdl_wait()
+    bool hint;   // weights evict-first in L2
 };
 
 struct DownArgs {
@@ -60,9 +61,10 @@ struct DownArgs {
     const uint8_t* sw;
     int64_t ffn, sffn, rows, experts, tokens, k;
     const uint32_t* idx;
-    void* out;  // (tokens, rows)
-    int stages;
-    bool early;  // idx and the weights may be read before pdl_wait()
+    void* out;           // (tokens, rows)
+    float* partial;      // [CTAs][2][tokens][32]
+    uint32_t* counters;  // one a job, zero
+    bool early;          // idx and the weights may be read before pdl_wait()
 };
 
 // ---- a warp's ring of bulk copies
@@ -165,6 +167,32 @@ __device__ __forceinline__ PairBlocks pair_blocks(uint8_t* mem, const uint32_t* 
     b.start = b.expert + pairs;
     b.count = b.start + pairs;
     const int tid = threadIdx.x;
+    if (pairs <= 32) {
+        // (a decode step's few pairs: one warp, one barrier)
+        if (tid < 32) {
+            const uint32_t e = tid < pairs ? idx[tid] : 0xffffffffu;
+            const bool in = e < uint32_t(experts);
+            const uint32_t same = __match_any_sync(0xffffffffu, e);
+            const int before = __popc(same & ((1u << tid) - 1)), within = before % most;
+            const bool lead = in && within == 0;
+            const uint32_t leads = __ballot_sync(0xffffffffu, lead);
+            const int members = lead ? min(most, __popc(same) - before) : 0;
+            const int first = warp_incl_sum(members, tid) - members;
+            const int leader = before < most ? __ffs(same) - 1 : static_cast<int>(__fns(same, 0, before - within + 1));
+            const int at = __shfl_sync(0xffffffffu, first, leader) + within;
+            if (lead) {
+                const int i = __popc(leads & ((1u << tid) - 1));
+                b.expert[i] = uint16_t(e);
+                b.start[i] = uint16_t(first);
+                b.count[i] = uint16_t(members);
+            }
+            if (in) b.list[at] = uint16_t(tid);
+            if (tid == 0) warp_sums[0] = __popc(leads);
+        }
+        __syncthreads();
+        b.n = warp_sums[0];
+        return b;
+    }
     for (int e = tid; e < experts; e += kThreads) seen[e] = 0;
     __syncthreads();
     if (tid < 32) {
@@ -213,430 +241,402 @@ __device__ __forceinline__ PairBlocks pair_blocks(uint8_t* mem, const uint32_t* 
     return b;
 }
 
-struct ProductJob {
-    const uint8_t* w[2];  // the strip's first tile
-    int strip, expert_block, tokens0, count;
-    bool dense;
-};
+constexpr int kMt = 2;      // strips whose tiles are multiplied together: gate and up, or two neighbours of one matrix
+constexpr int kStep = 2;    // tiles of a stage
+constexpr int kStages = 2;  // slots of a warp's ring
+constexpr int kM = 8;       // rows of activations in a block
+template <int G>
+__host__ __device__ constexpr int slot_bytes() {
+    return kMt * kStep * tile_bytes<G>();
+}
+constexpr int kRedFloats = kMt * kRows * kM;  // a warp's sums of one job
 
-template <int G, int MATS>
-__host__ __device__ constexpr int product_stage_tiles() {
-    return MATS == 2 ? 1 : 2;  // a stage is a tile of gate and of up, or two tiles of one matrix
-}
-template <int G, int MATS>
-__host__ __device__ constexpr int product_slot_bytes() {
-    return 2 * tile_bytes<G>();
-}
-// Shared memory: [ring slots, 4 warps][partial sums][pair blocks][barriers]
-template <int G, int NT, int MATS>
-__host__ __device__ constexpr size_t product_smem(int stages, int64_t pairs, int64_t experts) {
-    return size_t(kWarps) * stages * product_slot_bytes<G, MATS>() + size_t(kWarps) * MATS * kRows * 8 * NT * 4 +
-           pair_blocks_bytes(pairs, experts) + size_t(kWarps) * stages * 8;
+// Shared memory: [ring slots, 8 warps][two jobs' partial sums, 8 warps][pair blocks][barriers]
+template <int G>
+__host__ __device__ constexpr size_t product_smem(int64_t pairs, int64_t experts) {
+    return size_t(kWarps) * kStages * slot_bytes<G>() + size_t(kWarps) * 2 * kRedFloats * 4 +
+           pair_blocks_bytes(pairs, experts) + size_t(kWarps) * kStages * 8;
 }
 
 __device__ __forceinline__ float sigmoid_f(float g) { return 1.0f / (1.0f + expf(-g)); }
 
-template <typename T, int G, int NT, int MATS>
-__global__ void __launch_bounds__(kThreads) q4_product_kernel(const ProductArgs a) {
-    namespace cg = cooperative_groups;
+// GLU: the two strips of a job are gate's and up's, else two neighbours.
+template <typename T, int G, bool GLU>
+__global__ void __launch_bounds__(kThreads, 2) q4_product_kernel(const ProductArgs a) {
     constexpr int kTile = tile_bytes<G>();
-    constexpr int kStep = product_stage_tiles<G, MATS>();
-    constexpr int kSlot = product_slot_bytes<G, MATS>();
-    constexpr int kM = 8 * NT;
+    constexpr int kSlot = slot_bytes<G>();
+    constexpr int kWide = GLU ? 1 : 2;  // strips of the result in a job
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int warp_sums[kWarps];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    cg::cluster_group cluster = cg::this_cluster();
-    const int csize = static_cast<int>(cluster.num_blocks()), crank = static_cast<int>(cluster.block_rank());
-    const int cluster_id = blockIdx.x / csize, clusters = gridDim.x / csize;
+    const int team = warp / a.team, member = warp - team * a.team;
+    // (teams of one CTA are far apart in the jobs' order: a few jobs spread over the SMs)
+    const int team_id = team * gridDim.x + blockIdx.x, teams = kWarps / a.team * gridDim.x;
 
-    float* red = reinterpret_cast<float*>(smem + size_t(kWarps) * a.stages * kSlot);  // [warp][mat][row][member]
-    uint8_t* table = reinterpret_cast<uint8_t*>(red + kWarps * MATS * kRows * kM);
+    float* red = reinterpret_cast<float*>(smem + size_t(kWarps) * kStages * kSlot);
+    uint8_t* table = reinterpret_cast<uint8_t*>(red + kWarps * 2 * kRedFloats);
     uint64_t* bars = reinterpret_cast<uint64_t*>(table + pair_blocks_bytes(a.pairs, a.experts));
+    red += team * a.team * 2 * kRedFloats;  // [job's parity][member][strip][row][column]
     Ring ring;
-    ring.init(smem + size_t(warp) * a.stages * kSlot, bars + warp * a.stages, a.stages, kSlot, lane);
+    ring.init(smem + size_t(warp) * kStages * kSlot, bars + warp * kStages, kStages, kSlot, lane);
     const uint64_t policy = tc::policy_evict_first();
 
     const int ntiles = static_cast<int>(tiles_of_cols(a.cols));
-    const int ways = kWarps * csize, way = crank * kWarps + warp;
-    const int tile0 = static_cast<int>(int64_t(way) * ntiles / ways), tile1 = static_cast<int>(int64_t(way + 1) * ntiles / ways);
+    const int tile0 = member * ntiles / a.team, tile1 = (member + 1) * ntiles / a.team;
     const int steps = (tile1 - tile0 + kStep - 1) / kStep;
     const int64_t strip_bytes = int64_t(ntiles) * kTile;
     const int d_strips = static_cast<int>(strips_of_rows(a.d_rows)), r_strips = static_cast<int>(strips_of_rows(a.r_rows));
+    const int d_wide = (d_strips + kWide - 1) / kWide, r_wide = (r_strips + kWide - 1) / kWide;
     const int d_blocks = static_cast<int>((a.d_tokens + kM - 1) / kM);
-    const int d_jobs = d_strips * d_blocks;
+    const int d_jobs = d_wide * d_blocks;
     PairBlocks blocks{nullptr, nullptr, nullptr, nullptr, 0};
     int jobs = d_jobs;  // jobs known so far
 
-    auto job_of = [&](int j) {
-        ProductJob o;
-        o.dense = j < d_jobs;
-        if (o.dense) {
-            // (a strip's blocks of tokens are neighbours in time: the second reads the strip from L2)
-            o.strip = j / d_blocks;
-            o.tokens0 = (j - o.strip * d_blocks) * kM;
-            o.count = static_cast<int>(min(int64_t(kM), a.d_tokens - o.tokens0));
-            o.expert_block = 0;
-#pragma unroll
-            for (int m = 0; m < MATS; ++m) o.w[m] = a.dw[m] + o.strip * strip_bytes;
-        } else {
-            const int i = j - d_jobs;
-            o.strip = i / blocks.n;
-            o.expert_block = i - o.strip * blocks.n;
-            o.tokens0 = blocks.start[o.expert_block];
-            o.count = blocks.count[o.expert_block];
-#pragma unroll
-            for (int m = 0; m < MATS; ++m)
-                o.w[m] = a.rw[m] + (int64_t(blocks.expert[o.expert_block]) * r_strips + o.strip) * strip_bytes;
-        }
-        return o;
+    // job -> strips (from kWide times the first) and block of rows; a strip's blocks are neighbours in time, so that the
+    // second reads the strip from L2
+    auto place = [&](int j, int& strip, int& block) {
+        const int n = j < d_jobs ? d_blocks : blocks.n;
+        j = j < d_jobs ? j : j - d_jobs;
+        strip = j / n;
+        block = j - strip * n;
     };
 
     // the copies' cursor: the next stage to fetch
-    int fetch_job = cluster_id, fetch_step = 0;
-    const uint8_t* fetch_w[2] = {nullptr, nullptr};
-    auto fetch = [&]() {
-        while (ring.ok && !ring.full() && fetch_job < jobs && steps > 0) {
-            if (fetch_step == 0) {
-                const ProductJob o = job_of(fetch_job);
+    int fetch_job = team_id, fetch_step = 0;
+    const uint8_t* fetch_w[kMt] = {};
+    auto fetch = [&]() {  // (a slot is free)
+        if (fetch_job >= jobs || steps == 0 || !ring.ok) return;
+        if (fetch_step == 0) {
+            int strip, block;
+            place(fetch_job, strip, block);
+            const bool dense = fetch_job < d_jobs;
+            const int64_t first = dense ? 0 : int64_t(blocks.expert[block]) * r_strips;
 #pragma unroll
-                for (int m = 0; m < MATS; ++m) fetch_w[m] = o.w[m];
+            for (int m = 0; m < kMt; ++m) {
+                const uint8_t* w = dense ? a.dw[GLU ? m : 0] : a.rw[GLU ? m : 0];
+                // (the last job of an odd number of strips takes its one strip twice)
+                const int s = GLU ? strip : min(2 * strip + m, (dense ? d_strips : r_strips) - 1);
+                fetch_w[m] = w + (first + s) * strip_bytes + int64_t(tile0) * kTile;
             }
-            const int tile = tile0 + fetch_step * kStep;
-            const uint32_t bytes = static_cast<uint32_t>(min(kStep, tile1 - tile)) * kTile;
-            if (lane == 0) {
-                uint64_t* bar = &ring.bars[ring.head];
-                tc::mbar_arrive_expect_tx(bar, bytes * MATS);
+        }
+        const uint32_t bytes = fetch_step + 1 < steps ? kStep * kTile : (tile1 - tile0 - fetch_step * kStep) * kTile;
+        if (lane == 0) {
+            uint64_t* bar = &ring.bars[ring.head];
+            tc::mbar_arrive_expect_tx(bar, bytes * kMt);
 #pragma unroll
-                for (int m = 0; m < MATS; ++m) {
-                    const uint32_t dst = ring.base + ring.head * kSlot + m * kTile;
-                    if (a.hint) bulk_load_hint(dst, fetch_w[m] + int64_t(tile) * kTile, bytes, bar, policy);
-                    else bulk_load(dst, fetch_w[m] + int64_t(tile) * kTile, bytes, bar);
-                }
+            for (int m = 0; m < kMt; ++m) {
+                const uint32_t dst = ring.base + ring.head * kSlot + m * kStep * kTile;
+                if (a.hint) bulk_load_hint(dst, fetch_w[m], bytes, bar, policy);
+                else bulk_load(dst, fetch_w[m], bytes, bar);
             }
-            ring.push();
-            if (++fetch_step == steps) {
-                fetch_step = 0;
-                fetch_job += clusters;
-            }
+        }
+        ring.push();
+#pragma unroll
+        for (int m = 0; m < kMt; ++m) fetch_w[m] += bytes;
+        if (++fetch_step == steps) {
+            fetch_step = 0;
+            fetch_job += teams;
         }
     };
     if (!a.early) pdl_wait();
-    fetch();  // the dense part's weights, while the launch before still runs
+    // the dense part's weights, while the launch before still runs
+    for (int i = 0; i < kStages; ++i) fetch();
     pdl_wait();
     if (a.pairs > 0) {
         blocks = pair_blocks(table, a.idx, static_cast<int>(a.pairs), static_cast<int>(a.experts), kM, warp_sums);
-        jobs = d_jobs + blocks.n * r_strips;
-        fetch();
+        jobs = d_jobs + blocks.n * r_wide;
+        while (!ring.full() && fetch_job < jobs && steps > 0) fetch();
+        if (blockIdx.x == 0)
+            for (int i = tid; i < a.n_zero; i += kThreads) a.zero[i] = 0;
     }
 
     const T* x = static_cast<const T*>(a.x);
     const int col_runs = static_cast<int>(a.cols / 32);
-    for (int job = cluster_id; job < jobs; job += clusters) {
-        const ProductJob o = job_of(job);
-        const T* xp[NT];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int n = 8 * nt + g;
-            xp[nt] = nullptr;
-            if (n < o.count) {
-                const int64_t row = o.dense ? o.tokens0 + n : blocks.list[o.tokens0 + n] / a.share;
-                xp[nt] = x + row * a.cols + 8 * t;
-            }
-        }
-        float acc[MATS][NT][4] = {};
+    int parity = 0;
+    for (int job = team_id; job < jobs; job += teams, parity ^= 1) {
+        const bool dense = job < d_jobs;
+        int strip, block;
+        place(job, strip, block);
+        const int start = dense ? block * kM : blocks.start[block];
+        const int count = dense ? static_cast<int>(min(int64_t(kM), a.d_tokens - start)) : blocks.count[block];
+        // (columns past the count repeat the first row; their results are not written)
+        const int at = g < count ? start + g : start;
+        const T* xp = x + (dense ? int64_t(at) : int64_t(blocks.list[at]) / a.share) * a.cols + 8 * t;
+        float acc[kMt][4] = {};
         for (int s = 0; s < steps; ++s) {
-            // (the activations first: their latency passes while the weights' copies land)
-            Acts<T> xs[kStep][NT][4];
-#pragma unroll
-            for (int i = 0; i < kStep; ++i) {
-                const int tile = tile0 + s * kStep + i;
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if (xp[nt] != nullptr && tile < tile1 && tile * 4 + j < col_runs)
-                            xs[i][nt][j].load(xp[nt] + tile * kCols + 32 * j);
-                        else xs[i][nt][j].zero();
-                    }
-            }
+            const int tile = tile0 + s * kStep;
+            // (a tile's activations before its weights are waited for: both latencies pass together)
+            const TileActs<T> x0(xp + tile * kCols, col_runs - 4 * tile);
             const uint8_t* slot = ring.wait(lane);
-#pragma unroll
-            for (int i = 0; i < kStep; ++i) {
-                if (kStep > 1 && tile0 + s * kStep + i >= tile1) break;
-                auto load = [&](int nt, int j, Acts<T>& v) { v = xs[i][nt][j]; };
-                auto on = [&](int nt) { return true; };
-                tile_mma<T, G, NT, MATS>(slot + i * kTile, kTile, lane, acc, load, on);
-            }
+            const bool more = tile + 1 < tile1;
+            const TileActs<T> x1(xp + (tile + 1) * kCols, more ? col_runs - 4 * (tile + 1) : 0);
+            tile_mma<T, G>(slot, kStep * kTile, lane, x0, acc);
+            if (more) tile_mma<T, G>(slot + kTile, kStep * kTile, lane, x1, acc);
             __syncwarp();
             ring.pop();
             fetch();
         }
-        // the warps' sums, then the cluster's: partial sums in the order of the column ranges
+        // the team's sums, in the order of the column ranges (one barrier a job: the next job's sums have another place)
+        float* sums = red + parity * a.team * kRedFloats;
 #pragma unroll
-        for (int m = 0; m < MATS; ++m)
+        for (int m = 0; m < kMt; ++m)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    red[((warp * MATS + m) * kRows + g + 8 * (i >> 1)) * kM + 8 * nt + 2 * t + (i & 1)] = acc[m][nt][i];
-        if (csize > 1) cluster.sync();
-        else __syncthreads();
-        const int rows = static_cast<int>(o.dense ? a.d_rows : a.r_rows);
-        for (int i = crank * kThreads + tid; i < kRows * kM; i += csize * kThreads) {
-            const int r = i & (kRows - 1), n = i / kRows;
-            const int row = o.strip * kRows + r;
-            if (n >= o.count || row >= rows) continue;
-            float sum[MATS] = {};
-            for (int c = 0; c < csize; ++c) {
-                const float* from = csize > 1 ? cluster.map_shared_rank(red, c) : red;
-#pragma unroll
-                for (int w = 0; w < kWarps; ++w)
-#pragma unroll
-                    for (int m = 0; m < MATS; ++m) sum[m] += from[((w * MATS + m) * kRows + r) * kM + n];
+            for (int i = 0; i < 4; ++i)
+                sums[((member * kMt + m) * kRows + g + 8 * (i >> 1)) * kM + 2 * t + (i & 1)] = acc[m][i];
+        if (a.team == 1) __syncwarp();
+        else tc::named_barrier(1 + team, 32 * a.team);
+        const int rows = static_cast<int>(dense ? a.d_rows : a.r_rows);
+        for (int i = member * 32 + lane; i < kWide * kRows * count; i += 32 * a.team) {
+            const int r = i & (kWide * kRows - 1), n = i / (kWide * kRows);
+            const int row = strip * kWide * kRows + r;
+            if (row >= rows) continue;
+            float v = 0.0f, u = 0.0f;
+            for (int w = 0; w < a.team; ++w) {
+                v += sums[(w * kMt * kRows + r) * kM + n];
+                if constexpr (GLU) u += sums[((w * kMt + 1) * kRows + r) * kM + n];
             }
-            const int64_t to = o.dense ? o.tokens0 + n : blocks.list[o.tokens0 + n];
-            float v = sum[0];
-            if constexpr (MATS == 2) {
+            const int64_t to = dense ? start + n : blocks.list[start + n];
+            v *= unit<T>();
+            if constexpr (GLU) {
                 // silu(gate) up, times the row's share of the block's output: float32 up to the one rounding
-                v = sum[0] * sigmoid_f(sum[0]) * sum[MATS - 1];
-                if (o.dense) {
+                v = v * sigmoid_f(v) * (u * unit<T>());
+                if (dense) {
                     if (a.d_gate != nullptr) v *= sigmoid_f(to_f32(static_cast<const T*>(a.d_gate)[to]));
                 } else if (a.weights != nullptr) {
                     v *= a.weights[to];
                 }
             }
-            T* out = static_cast<T*>(o.dense ? a.d_out : a.r_out);
+            T* out = static_cast<T*>(dense ? a.d_out : a.r_out);
             out[to * rows + row] = from_f32<T>(v);
         }
-        if (csize > 1) cluster.sync();
-        else __syncthreads();
     }
     pdl_release();
     ring.drain(lane);
 }
 
-// ---- down products and the combine of a MoE block, at most 8 NT tokens
+// ---- down products and the combine of a MoE block, at most 64 tokens
+//
+// A job is two strips of the output. Its columns are one long sum: the shared expert's hidden values, then each chosen
+// expert's, in blocks of at most 8 rows of h (the pairs of one expert). There are few jobs (a hidden size of 2560: 80),
+// so all jobs' tiles in a row are cut into one even range for each CTA, and a CTA's range of a job into one for each
+// warp. A warp adds a block's sums into its own copy of the result in shared memory when the block ends, each row of h to
+// its token; a CTA adds its warps' in order, and the last CTA of a job to come adds the CTAs' in order.
 
-// The chosen experts, each with the tokens that chose it (a bit a token), in the order of the experts; a token's
-// second choice of the same expert is a group of its own, after them.
-constexpr uint16_t kNone = 0xffff, kAgain = 0x8000;
-struct Groups {
-    uint64_t* tokens;  // [experts]
-    uint16_t* key;     // [pairs]: the pair's expert; kNone: no expert, kAgain | expert: not the first time
-    uint16_t* group;   // [n]: the expert; kAgain | pair
-    int n;
-    __device__ __forceinline__ int expert(int i) const {
-        return group[i] & kAgain ? key[group[i] & ~kAgain] & ~kAgain : group[i];
-    }
-};
-__host__ __device__ constexpr size_t groups_bytes(int64_t pairs, int64_t experts) {
-    return (size_t(experts) * 8 + size_t(pairs) * 4 + 15) & ~size_t(15);
-}
-__device__ __forceinline__ Groups expert_groups(uint8_t* mem, const uint32_t* __restrict__ idx, int pairs, int k,
-                                                int experts, int* warp_sums) {
-    Groups r;
-    r.tokens = reinterpret_cast<uint64_t*>(mem);
-    r.key = reinterpret_cast<uint16_t*>(r.tokens + experts);
-    r.group = r.key + pairs;
-    const int tid = threadIdx.x;
-    for (int e = tid; e < experts; e += kThreads) r.tokens[e] = 0;
-    __syncthreads();
-    int again_any = 0;
-    for (int p = tid; p < pairs; p += kThreads) {
-        const uint32_t e = idx[p];
-        uint16_t key = kNone;
-        if (e < uint32_t(experts)) {
-            const int tok = p / k;
-            bool again = false;
-            for (int q = tok * k; q < p; ++q) again |= idx[q] == e;
-            key = uint16_t(e | (again ? kAgain : 0));
-            if (!again) atomicOr(reinterpret_cast<unsigned long long*>(&r.tokens[e]), 1ull << tok);
-            again_any |= again;
-        }
-        r.key[p] = key;
-    }
-    again_any = __syncthreads_or(again_any);
-    const int per = (experts + kThreads - 1) / kThreads;
-    const int e0 = min(experts, tid * per), e1 = min(experts, e0 + per);
-    int mine = 0;
-    for (int e = e0; e < e1; ++e) mine += r.tokens[e] != 0;
-    int i = block_excl_sum(mine, warp_sums, r.n);
-    for (int e = e0; e < e1; ++e)
-        if (r.tokens[e] != 0) r.group[i++] = uint16_t(e);
-    if (again_any) {
-        if (tid < 32) {
-            int n = r.n;
-            for (int p0 = 0; p0 < pairs; p0 += 32) {
-                const int p = p0 + tid;
-                const bool again = p < pairs && r.key[p] != kNone && (r.key[p] & kAgain);
-                const uint32_t m = __ballot_sync(0xffffffffu, again);
-                if (again) r.group[n + __popc(m & ((1u << tid) - 1))] = uint16_t(kAgain | p);
-                n += __popc(m);
-            }
-            if (tid == 0) warp_sums[0] = n;
-        }
-        __syncthreads();
-        r.n = warp_sums[0];
-    }
-    __syncthreads();
-    return r;
-}
+constexpr int kTokenStride = kMt * kRows + 4;  // floats of a token's sums: rows 0, 8, .. of four tokens on 32 banks
 
 template <int G>
-__host__ __device__ constexpr int down_slot_bytes() {
-    return tile_bytes<G>();
-}
-template <int G, int NT>
-__host__ __device__ constexpr size_t down_smem(int stages, int64_t pairs, int64_t experts) {
-    return size_t(kWarps) * stages * down_slot_bytes<G>() + size_t(kWarps) * kRows * 8 * NT * 4 + groups_bytes(pairs, experts) +
-           size_t(kWarps) * stages * 8;
+__host__ __device__ constexpr size_t down_smem(int64_t tokens, int64_t pairs, int64_t experts) {
+    return size_t(kWarps) * kStages * slot_bytes<G>() + size_t(kWarps) * tokens * kTokenStride * 4 +
+           pair_blocks_bytes(pairs, experts) + size_t(kWarps) * kStages * 8;
 }
 
-template <typename T, int G, int NT>
-__global__ void __launch_bounds__(kThreads) q4_down_kernel(const DownArgs a) {
-    namespace cg = cooperative_groups;
+template <typename T, int G>
+__global__ void __launch_bounds__(kThreads, 2) q4_down_kernel(const DownArgs a) {
     constexpr int kTile = tile_bytes<G>();
-    constexpr int kM = 8 * NT;
+    constexpr int kSlot = slot_bytes<G>();
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int warp_sums[kWarps];
+    __shared__ uint32_t arrived;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    cg::cluster_group cluster = cg::this_cluster();
-    const int csize = static_cast<int>(cluster.num_blocks()), crank = static_cast<int>(cluster.block_rank());
-    const int strip = blockIdx.x / csize;
+    const int strips = static_cast<int>(strips_of_rows(a.rows));
+    const int jobs = (strips + kMt - 1) / kMt;
+    const int tokens = static_cast<int>(a.tokens), k = static_cast<int>(a.k), pairs = tokens * k;
 
-    float* red = reinterpret_cast<float*>(smem + size_t(kWarps) * a.stages * kTile);  // [warp][row][token]
-    uint8_t* table = reinterpret_cast<uint8_t*>(red + kWarps * kRows * kM);
-    uint64_t* bars = reinterpret_cast<uint64_t*>(table + groups_bytes(a.tokens * a.k, a.experts));
+    float* red = reinterpret_cast<float*>(smem + size_t(kWarps) * kStages * kSlot);  // [warp][token][row]
+    uint8_t* table = reinterpret_cast<uint8_t*>(red + kWarps * tokens * kTokenStride);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(table + pair_blocks_bytes(pairs, a.experts));
     Ring ring;
-    ring.init(smem + size_t(warp) * a.stages * kTile, bars + warp * a.stages, a.stages, kTile, lane);
+    ring.init(smem + size_t(warp) * kStages * kSlot, bars + warp * kStages, kStages, kSlot, lane);
     const uint64_t policy = tc::policy_evict_first();
+    float* mine = red + warp * tokens * kTokenStride;
 
     if (!a.early) pdl_wait();
-    const Groups gr = expert_groups(table, a.idx, static_cast<int>(a.tokens * a.k), static_cast<int>(a.k),
-                                    static_cast<int>(a.experts), warp_sums);
-    // the strip's tiles: the shared expert's, then each chosen expert's; a way takes a range of them
+    const PairBlocks blocks = pair_blocks(table, a.idx, pairs, static_cast<int>(a.experts), kM, warp_sums);
+    // segments of a job: the shared expert's blocks of tokens, then the pairs' blocks
     const int stiles = static_cast<int>(tiles_of_cols(a.sffn)), ftiles = static_cast<int>(tiles_of_cols(a.ffn));
-    const int64_t strips = strips_of_rows(a.rows);
-    const int total = stiles + gr.n * ftiles;
-    const int ways = kWarps * csize, way = crank * kWarps + warp;
-    const int item0 = static_cast<int>(int64_t(way) * total / ways), item1 = static_cast<int>(int64_t(way + 1) * total / ways);
+    const int sblocks = stiles > 0 ? (tokens + kM - 1) / kM : 0;
+    const int shared_items = sblocks * stiles;
+    const int items = max(1, shared_items + blocks.n * ftiles);  // (a job without any tile still writes its zeros)
+    const bool any = shared_items + blocks.n > 0;
+    // a CTA's tiles of all jobs': an even share, at least a tile a warp (32 bits hold them: the host checks)
+    const int all = jobs * items;
+    const int share = max(min(kWarps, all), (all + int(gridDim.x) - 1) / int(gridDim.x));
+    const int begin = min(all, int(blockIdx.x) * share), end = min(all, begin + share);
+    const int job_first = begin / items, job_last = begin < end ? (end + items - 1) / items : job_first;
 
+    // a warp's tiles of a job
+    auto range_of = [&](int job, int& i0, int& i1) {
+        const int at = job * items;
+        const int p0 = max(begin, at) - at, n = min(end, at + items) - at - p0;
+        i0 = p0 + warp * n / kWarps;
+        i1 = p0 + (warp + 1) * n / kWarps;
+        if (!any) i0 = i1 = 0;
+    };
     struct Cursor {
-        int seg, tile, tiles;  // seg -1: the shared expert
+        int item, last, seg, tile;
     };
-    auto place = [&](int item) {
-        if (item < stiles) return Cursor{-1, item, stiles};
-        const int seg = (item - stiles) / ftiles;
-        return Cursor{seg, item - stiles - seg * ftiles, ftiles};
+    auto cursor_of = [&](int job) {
+        Cursor c;
+        range_of(job, c.item, c.last);
+        if (c.item < shared_items) {
+            c.seg = c.item / stiles;
+            c.tile = c.item - c.seg * stiles;
+        } else {
+            const int i = c.item - shared_items;
+            c.seg = i / ftiles;
+            c.tile = i - c.seg * ftiles;
+            c.seg += sblocks;
+        }
+        return c;
     };
-    auto step = [&](Cursor& c) {
-        if (++c.tile == c.tiles) {
-            ++c.seg;
+    auto tiles_in = [&](int seg) { return seg < sblocks ? stiles : ftiles; };
+    auto stage_of = [&](const Cursor& c) { return min(min(kStep, tiles_in(c.seg) - c.tile), c.last - c.item); };
+    auto advance = [&](Cursor& c, int n) {
+        c.item += n;
+        c.tile += n;
+        if (c.tile == tiles_in(c.seg)) {
             c.tile = 0;
-            c.tiles = ftiles;
+            ++c.seg;
         }
     };
-    auto strip_of = [&](const Cursor& c) {
-        return c.seg < 0 ? a.sw + int64_t(strip) * stiles * kTile
-                         : a.w + (int64_t(gr.expert(c.seg)) * strips + strip) * ftiles * kTile;
-    };
-    int next = item0;
-    Cursor fc = place(item0);
-    const uint8_t* fw = nullptr;
-    int fseg = -2;
-    auto fetch = [&]() {
-        while (ring.ok && !ring.full() && next < item1) {
-            if (fc.seg != fseg) {
-                fw = strip_of(fc);
-                fseg = fc.seg;
-            }
-            if (lane == 0) {
-                uint64_t* bar = &ring.bars[ring.head];
-                tc::mbar_arrive_expect_tx(bar, kTile);
-                bulk_load_hint(ring.base + ring.head * kTile, fw + int64_t(fc.tile) * kTile, kTile, bar, policy);
-            }
-            ring.push();
-            ++next;
-            step(fc);
+
+    int fetch_job = job_first, fetch_seg = -1;
+    Cursor fc = job_first < job_last ? cursor_of(fetch_job) : Cursor{0, 0, 0, 0};
+    const uint8_t* fetch_w[kMt] = {};
+    auto fetch = [&]() {  // (a slot is free)
+        if (!ring.ok) return;
+        while (fc.item >= fc.last) {
+            if (fetch_job + 1 >= job_last) return;
+            fc = cursor_of(++fetch_job);
+            fetch_seg = -1;
         }
+        if (fc.seg != fetch_seg) {
+            fetch_seg = fc.seg;
+            const bool shared = fc.seg < sblocks;
+            const int64_t strip_bytes = int64_t(shared ? stiles : ftiles) * kTile;
+            const uint8_t* w = shared ? a.sw : a.w + int64_t(blocks.expert[fc.seg - sblocks]) * strips * strip_bytes;
+            w += int64_t(fc.tile) * kTile;
+            fetch_w[0] = w + (fetch_job * kMt) * strip_bytes;
+            fetch_w[1] = w + min(fetch_job * kMt + 1, strips - 1) * strip_bytes;
+        }
+        const int n = stage_of(fc);
+        const uint32_t bytes = n * kTile;
+        if (lane == 0) {
+            uint64_t* bar = &ring.bars[ring.head];
+            tc::mbar_arrive_expect_tx(bar, bytes * kMt);
+#pragma unroll
+            for (int m = 0; m < kMt; ++m)
+                bulk_load_hint(ring.base + ring.head * kSlot + m * kStep * kTile, fetch_w[m], bytes, bar, policy);
+        }
+        ring.push();
+#pragma unroll
+        for (int m = 0; m < kMt; ++m) fetch_w[m] += bytes;
+        advance(fc, n);
     };
-    fetch();
+    for (int i = 0; i < kStages; ++i) fetch();
     pdl_wait();
 
-    float acc[1][NT][4] = {};
-    const T* xp[NT];
-    uint64_t mask = 0;
-    int seg = -2;
-    Cursor c = place(item0);
-    for (int item = item0; item < item1; ++item, step(c)) {
-        if (c.seg != seg) {
-            // this lane's row of each block of 8 tokens: the pair of token 8 nt + g that chose this expert
-            seg = c.seg;
-            const uint16_t group = seg < 0 ? 0 : gr.group[seg];
-            mask = seg < 0 ? ~0ull : group & kAgain ? 1ull << ((group & ~kAgain) / static_cast<int>(a.k)) : gr.tokens[group];
+    for (int job = job_first; job < job_last; ++job) {
+        for (int i = lane; i < tokens * kTokenStride; i += 32) mine[i] = 0.0f;
+        __syncwarp();
+        float acc[kMt][4] = {};
+        const T* xp = nullptr;
+        int count = 0, start = 0, runs = 0, seg = -1;
+        bool shared = false;
+        Cursor c = cursor_of(job);
+        while (c.item < c.last) {
+            if (c.seg != seg) {
+                seg = c.seg;
+                shared = seg < sblocks;
+                start = shared ? seg * kM : blocks.start[seg - sblocks];
+                count = shared ? min(kM, tokens - start) : blocks.count[seg - sblocks];
+                runs = static_cast<int>((shared ? a.sffn : a.ffn) / 32);
+                const int at = g < count ? start + g : start;
+                xp = shared ? static_cast<const T*>(a.hs) + at * a.sffn + 8 * t
+                            : static_cast<const T*>(a.h) + blocks.list[at] * a.ffn + 8 * t;
+            }
+            const int n = stage_of(c);
+            const TileActs<T> x0(xp + c.tile * kCols, runs - 4 * c.tile);
+            const uint8_t* slot = ring.wait(lane);
+            const TileActs<T> x1(xp + (c.tile + 1) * kCols, n > 1 ? runs - 4 * (c.tile + 1) : 0);
+            tile_mma<T, G>(slot, kStep * kTile, lane, x0, acc);
+            if (n > 1) tile_mma<T, G>(slot + kTile, kStep * kTile, lane, x1, acc);
+            __syncwarp();
+            ring.pop();
+            fetch();
+            advance(c, n);
+            if (c.seg != seg || c.item == c.last) {
+                // the block's end: each column's sums to its token, this lane's columns 2 t and 2 t + 1. A token that
+                // names an expert twice has two columns here, neighbours: column by column then.
+                auto add = [&](int h) {
+                    const int col = 2 * t + h;
+                    float* to = mine + (shared ? start + col : blocks.list[start + col] / k) * kTokenStride + g;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                const int tok = 8 * nt + g;
-                xp[nt] = nullptr;
-                if (tok >= a.tokens || !((mask >> tok) & 1)) continue;
-                if (seg < 0) {
-                    xp[nt] = static_cast<const T*>(a.hs) + tok * a.sffn + 8 * t;
+                    for (int m = 0; m < kMt; ++m) {
+                        to[m * kRows] += acc[m][h];
+                        to[m * kRows + 8] += acc[m][2 + h];
+                    }
+                };
+                const bool again = !shared && lane + 1 < count &&
+                                   blocks.list[start + lane] / k == blocks.list[start + lane + 1] / k;
+                if (__any_sync(0xffffffffu, again)) {
+                    for (int col = 0; col < count; ++col) {
+                        if (col == 2 * t) add(0);
+                        if (col == 2 * t + 1) add(1);
+                        __syncwarp();
+                    }
                 } else {
-                    int p = tok * static_cast<int>(a.k);
-                    if (group & kAgain) p = group & ~kAgain;
-                    else while (gr.key[p] != group) ++p;
-                    xp[nt] = static_cast<const T*>(a.h) + p * a.ffn + 8 * t;
+                    if (2 * t < count) add(0);
+                    if (2 * t + 1 < count) add(1);
+                }
+                __syncwarp();
+#pragma unroll
+                for (int m = 0; m < kMt; ++m)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[m][i] = 0.0f;
+            }
+        }
+        __syncthreads();
+        const int at = job * items;
+        const bool whole = begin <= at && end >= at + items;
+        const int values = kMt * kRows * tokens;
+        auto write = [&](int i, float sum) {
+            const int64_t row = int64_t(job) * kMt * kRows + (i & (kMt * kRows - 1));
+            if (row < a.rows) static_cast<T*>(a.out)[i / (kMt * kRows) * a.rows + row] = from_f32<T>(sum * unit<T>());
+        };
+        // (a job that a CTA shares is the first or the last of its range)
+        float* part = a.partial + (int64_t(blockIdx.x) * 2 + (job == job_first ? 0 : 1)) * values;
+        for (int i = tid; i < values; i += kThreads) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w)
+                sum += red[(w * tokens + i / (kMt * kRows)) * kTokenStride + (i & (kMt * kRows - 1))];
+            if (whole) write(i, sum);
+            else part[i] = sum;
+        }
+        if (!whole) {
+            // the CTAs of this job: those whose ranges meet it
+            const int c0 = at / share, c1 = (at + items - 1) / share;
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) arrived = atomicAdd(&a.counters[job], 1u);
+            __syncthreads();
+            if (arrived == uint32_t(c1 - c0)) {
+                __threadfence();
+                for (int i = tid; i < values; i += kThreads) {
+                    float sum = 0.0f;
+                    for (int cta = c0; cta <= c1; ++cta) {
+                        const int slot = cta * share >= at ? 0 : 1;  // (its range begins in this job, or before)
+                        sum += __ldcg(a.partial + (int64_t(cta) * 2 + slot) * values + i);
+                    }
+                    write(i, sum);
                 }
             }
         }
-        const int runs = static_cast<int>((seg < 0 ? a.sffn : a.ffn) / 32);
-        auto get = [&](int nt, int j, Acts<T>& v) {
-            if (xp[nt] != nullptr && c.tile * 4 + j < runs) v.load(xp[nt] + c.tile * kCols + 32 * j);
-            else v.zero();
-        };
-        // (up to 16 tokens: the activations before the wait; more would not fit the registers)
-        constexpr bool kAhead = NT <= 2;
-        Acts<T> xs[kAhead ? NT : 1][4];
-        if constexpr (kAhead) {
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) get(nt, j, xs[nt][j]);
-        }
-        const uint8_t* slot = ring.wait(lane);
-        auto load = [&](int nt, int j, Acts<T>& v) {
-            if constexpr (kAhead) v = xs[nt][j];
-            else get(nt, j, v);
-        };
-        auto on = [&](int nt) { return ((mask >> (8 * nt)) & 255) != 0 && 8 * nt < a.tokens; };
-        tile_mma<T, G, NT, 1>(slot, kTile, lane, acc, load, on);
-        __syncwarp();
-        ring.pop();
-        fetch();
+        __syncthreads();
     }
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            red[(warp * kRows + g + 8 * (i >> 1)) * kM + 8 * nt + 2 * t + (i & 1)] = acc[0][nt][i];
     pdl_release();
-    if (csize > 1) cluster.sync();
-    else __syncthreads();
-    for (int i = crank * kThreads + tid; i < kRows * kM; i += csize * kThreads) {
-        const int r = i & (kRows - 1), n = i / kRows;
-        const int64_t row = int64_t(strip) * kRows + r;
-        if (n >= a.tokens || row >= a.rows) continue;
-        float sum = 0.0f;
-        for (int cr = 0; cr < csize; ++cr) {
-            const float* from = csize > 1 ? cluster.map_shared_rank(red, cr) : red;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) sum += from[(w * kRows + r) * kM + n];
-        }
-        static_cast<T*>(a.out)[n * a.rows + row] = from_f32<T>(sum);
-    }
     ring.drain(lane);
-    if (csize > 1) cluster.sync();  // a CTA's sums are read by the others until here
 }
 
 }  // namespace q4

@@ -283,8 +283,8 @@ extern "C" int smoe_q4_pack(const uint32_t* codes, const uint16_t* scales, const
     Q4_CATCH("q4_pack")
 }
 
-extern "C" int smoe_q4_product(const SmoeQ4Product* p, void* stream) {
-    Q4_TRY
+// `zero`: words that the launch clears besides (for the launch after it)
+static int q4_product(const SmoeQ4Product* p, uint32_t* zero, int n_zero, void* stream) {
     SMOE_REQUIRE(p, SMOE_EARG, "q4_product: null pointer");
     SMOE_REQUIRE(p->dtype == SMOE_F16 || p->dtype == SMOE_F32, SMOE_EDTYPE,
                  "q4_product takes float16 or float32 activations");
@@ -343,12 +343,21 @@ extern "C" int smoe_q4_product(const SmoeQ4Product* p, void* stream) {
         const size_t bytes = stack_bytes(p->experts, p->rows, p->cols, p->group);
         a.early = a.early && pdl_early(st, p->stack, bytes) && (!p->stack2 || pdl_early(st, p->stack2, bytes));
     }
+    a.zero = zero;
+    a.n_zero = n_zero;
+    w.add(zero, size_t(n_zero) * 4);
     return p->dtype == SMOE_F16 ? product_f16(a, p->group, w, st) : product_f32(a, p->group, w, st);
+}
+
+extern "C" int smoe_q4_product(const SmoeQ4Product* p, void* stream) {
+    Q4_TRY
+    return q4_product(p, nullptr, 0, stream);
     Q4_CATCH("q4_product")
 }
 
 extern "C" int smoe_q4_linear(const uint8_t* packed, int64_t rows, int64_t cols, int group, const void* x,
                               int64_t tokens, void* out, int dtype, void* stream) {
+    Q4_TRY
     SmoeQ4Product p = {};
     p.dtype = dtype;
     p.group = group;
@@ -358,16 +367,35 @@ extern "C" int smoe_q4_linear(const uint8_t* packed, int64_t rows, int64_t cols,
     p.dense_rows = rows;
     p.dense_tokens = tokens;
     p.dense_out = out;
-    return smoe_q4_product(&p, stream);
+    return q4_product(&p, nullptr, 0, stream);
+    Q4_CATCH("q4_linear")
 }
 
-static size_t moe_h_bytes(int dtype, int64_t rows, int64_t ffn) {
-    return (size_t(rows) * ffn * (dtype == SMOE_F16 ? 2 : 4) + 255) & ~size_t(255);
-}
+// A call's workspace: the SwiGLU of the pairs and of the shared expert, the partial sums and the counters of the down
+// products' jobs.
+struct MoeSpace {
+    size_t h, hs, partial, counters, bytes;
+    MoeSpace(int dtype, int64_t tokens, int64_t k, int64_t hidden, int64_t ffn, int64_t shared_ffn) {
+        const size_t item = dtype == SMOE_F16 ? 2 : 4;
+        size_t at = 0;
+        auto take = [&](size_t n) {
+            const size_t from = at;
+            at += (n + 255) & ~size_t(255);
+            return from;
+        };
+        h = take(size_t(tokens) * k * ffn * item);
+        hs = take(size_t(tokens) * shared_ffn * item);
+        partial = take(size_t(kDownCtas) * 2 * tokens * kMt * kRows * 4);
+        counters = take(n_counters(hidden) * 4);
+        bytes = at;
+    }
+    static size_t n_counters(int64_t hidden) { return static_cast<size_t>((strips_of_rows(hidden) + kMt - 1) / kMt); }
+};
 
-extern "C" size_t smoe_q4_moe_workspace_size(int dtype, int64_t tokens, int64_t k, int64_t ffn, int64_t shared_ffn) {
-    if (tokens <= 0 || k <= 0 || ffn <= 0 || shared_ffn < 0) return 0;
-    return moe_h_bytes(dtype, tokens * k, ffn) + moe_h_bytes(dtype, tokens, shared_ffn);
+extern "C" size_t smoe_q4_moe_workspace_size(int dtype, int64_t tokens, int64_t k, int64_t hidden, int64_t ffn,
+                                             int64_t shared_ffn) {
+    if (tokens <= 0 || k <= 0 || hidden <= 0 || ffn <= 0 || shared_ffn < 0) return 0;
+    return MoeSpace(dtype, tokens, k, hidden, ffn, shared_ffn).bytes;
 }
 
 extern "C" int smoe_q4_moe(const SmoeQ4Moe* m, void* workspace, size_t workspace_bytes, void* stream) {
@@ -387,15 +415,22 @@ extern "C" int smoe_q4_moe(const SmoeQ4Moe* m, void* workspace, size_t workspace
         if (int s = check_matrix(m->hidden, m->shared_ffn, m->down_group)) return s;
         SMOE_REQUIRE(m->sgate && m->sup && m->sdown, SMOE_EARG, "q4_moe: a shared expert needs its three matrices");
     }
+    // (tiles of all the down products of a call, counted in 32 bits)
+    SMOE_REQUIRE(int64_t(MoeSpace::n_counters(m->hidden)) *
+                         (m->tokens * tiles_of_cols(m->shared_ffn) + m->tokens * m->k * tiles_of_cols(m->ffn)) < kMost,
+                 SMOE_ESHAPE, "q4_moe: the layer is too large for " + std::to_string(m->tokens) + " tokens a call");
     SMOE_REQUIRE(m->x && m->idx && m->weights && m->gate && m->up && m->down && m->out && aligned16(m->down) &&
                      aligned16(m->sdown),
                  SMOE_EARG, "q4_moe: null or misaligned pointer");
     SMOE_REQUIRE(workspace && aligned16(workspace) &&
-                     workspace_bytes >= smoe_q4_moe_workspace_size(m->dtype, m->tokens, m->k, m->ffn, m->shared_ffn),
+                     workspace_bytes >= smoe_q4_moe_workspace_size(m->dtype, m->tokens, m->k, m->hidden, m->ffn, m->shared_ffn),
                  SMOE_EWORKSPACE, "q4_moe: workspace missing, misaligned or too small");
     cudaStream_t st = as_stream(stream);
-    void* h = workspace;
-    void* hs = static_cast<uint8_t*>(workspace) + moe_h_bytes(m->dtype, m->tokens * m->k, m->ffn);
+    const MoeSpace space(m->dtype, m->tokens, m->k, m->hidden, m->ffn, m->shared_ffn);
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    void* h = ws + space.h;
+    void* hs = ws + space.hs;
+    uint32_t* counters = reinterpret_cast<uint32_t*>(ws + space.counters);
     SmoeQ4Product p = {};
     p.dtype = m->dtype;
     p.group = m->group;
@@ -418,7 +453,7 @@ extern "C" int smoe_q4_moe(const SmoeQ4Moe* m, void* workspace, size_t workspace
     p.share = m->k;
     p.weights = m->weights;
     p.out = h;
-    if (int s = smoe_q4_product(&p, stream)) return s;
+    if (int s = q4_product(&p, counters, static_cast<int>(MoeSpace::n_counters(m->hidden)), stream)) return s;
     DownArgs d = {};
     d.h = h;
     d.hs = m->shared_ffn > 0 ? hs : nullptr;
@@ -432,9 +467,12 @@ extern "C" int smoe_q4_moe(const SmoeQ4Moe* m, void* workspace, size_t workspace
     d.k = m->k;
     d.idx = m->idx;
     d.out = m->out;
-    // (the launch before is the product above, which writes h and hs alone and has waited for everything before it)
+    d.partial = reinterpret_cast<float*>(ws + space.partial);
+    d.counters = counters;
+    // (the launch before is the product above, which writes h, hs and the counters alone and has waited for everything before it)
     d.early = true;
     Writes w;
+    w.add(d.partial, space.counters - space.partial).add(counters, space.bytes - space.counters);
     w.add(m->out, size_t(m->tokens) * m->hidden * (m->dtype == SMOE_F16 ? 2 : 4));
     return m->dtype == SMOE_F16 ? down_f16(d, m->down_group, w, st) : down_f32(d, m->down_group, w, st);
     Q4_CATCH("q4_moe")
