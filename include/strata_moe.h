@@ -519,7 +519,8 @@ SMOE_API int smoe_q4_linear(const uint8_t* packed, int64_t rows, int64_t cols, i
  *   out[t] = sum_j weights[t, j] down_e(silu(gate_e x) * up_e x) + sigmoid(shared_gate[t]) shared(x), e = idx[t, j]
  * gate, up: (experts, ffn, hidden) with groups of `group` columns, down: (experts, hidden, ffn) with `down_group`; the
  * shared expert's likewise with shared_ffn rows (0: none; shared_gate null: not gated). A choice idx >= experts adds
- * nothing. Sums and SwiGLU are float32; between the launches the SwiGLU times its weight is kept in `dtype`. Workspace:
+ * nothing. Sums and SwiGLU are float32; between the launches the SwiGLU times its weight is kept in 22 bits or
+ * more. Workspace:
  * smoe_q4_moe_workspace_size() bytes, one for each call in flight. Replaces `_Routed.__call__` behind its router
  * (strata_mlx/fused.py:491-497). Weights as smoe_q4_product's. */
 typedef struct SmoeQ4Moe {
@@ -534,7 +535,7 @@ typedef struct SmoeQ4Moe {
     const uint8_t *sgate, *sup, *sdown;
     void* out;
 } SmoeQ4Moe;
-SMOE_API size_t smoe_q4_moe_workspace_size(int dtype, int64_t tokens, int64_t k, int64_t hidden, int64_t ffn,
+SMOE_API size_t smoe_q4_moe_workspace_size(int64_t tokens, int64_t k, int64_t hidden, int64_t ffn,
                                              int64_t shared_ffn);
 SMOE_API int smoe_q4_moe(const SmoeQ4Moe* m, void* workspace, size_t workspace_bytes, void* stream);
 

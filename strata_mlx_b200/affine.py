@@ -319,8 +319,8 @@ def moe_takes(switch_mlp, shared) -> bool:
 def moe(switch_mlp: QuantizedSwitchGLU, shared: QuantizedMLP, x: torch.Tensor, indices: torch.Tensor, w: torch.Tensor,
         g: torch.Tensor) -> torch.Tensor:
     """sum_j w_j switch_mlp(x, indices)_j + sigmoid(g) shared(x) in two launches: x (..., hidden), indices and w (...,
-    k) with w float32, g (..., 1) in x's type. Sums are float32 and rounded to x's type once (SwiGLU times its weight is
-    rounded to it between the launches). An index at or past the expert count adds nothing."""
+    k) with w float32, g (..., 1) in x's type. Sums are float32 and rounded to x's type once (the SwiGLU keeps 22 bits
+    or more between the launches). An index at or past the expert count adds nothing."""
     if not moe_takes(switch_mlp, shared):
         raise ValueError("moe takes 4-bit experts of one hidden size, with one group size in gate / up and one in down")
     gate, down = switch_mlp.gate_proj, switch_mlp.down_proj
@@ -340,7 +340,7 @@ def moe(switch_mlp: QuantizedSwitchGLU, shared: QuantizedMLP, x: torch.Tensor, i
         out = torch.empty((tokens, gate.input_dims), dtype=x.dtype, device=gate.device)
         for t0 in range(0, tokens, MOE_TOKENS):
             n = min(MOE_TOKENS, tokens - t0)
-            nbytes = int(_lib.lib().smoe_q4_moe_workspace_size(code, n, k, gate.input_dims, gate.output_dims,
+            nbytes = int(_lib.lib().smoe_q4_moe_workspace_size(n, k, gate.input_dims, gate.output_dims,
                                                                 sgate.output_dims))
             ws = torch.empty(nbytes, dtype=torch.uint8, device=gate.device)
             spec = _lib.SmoeQ4Moe(

@@ -9,17 +9,21 @@
 //   [strip][tile][ 16 rows x 64 B codes ][ 16 rows x 128 / G x (scale, bias) ]
 //
 // so a strip is one run of memory that bulk copies fetch in any pieces, every piece a multiple of 16 bytes. Rows
-// past the last and columns past the last are zero codes with zero scales and biases. Within a row's 16 code
-// words, word 4 t + j holds the eight codes of columns 32 j + 8 t .. + 7 of the tile: lane (g, t) of a warp (g =
-// lane / 4, t = lane % 4) reads 16 bytes at 64 g + 16 t and has its columns of all four 32-column runs.
+// past the last and columns past the last are zero codes with zero scales and biases.
+//
+// A row's 16 code words of a tile: word j of chunk t (four chunks of 16 bytes) holds the codes of columns 32 j + 8 t ..
+// + 7, so that lane (g, t) of a warp (g = lane / 4, t = lane % 4) has its columns of all four 32-column runs in one
+// 16-byte read. Chunk t of row r lies at place t ^ (r / 2 % 4): eight rows' chunks t are on eight different bank groups
+// (a thread a row reads so in the prompt's product). In a word, columns 0 .. 7 lie in nibbles 0, 4, 1, 5, 2, 6, 3, 7: the
+// nibbles under one mask, 16 bits apart, are neighbouring columns.
 //
 // Arithmetic. A run of 32 columns is two m16n8k16 MMAs, rows the M side, activation rows the N side. The order of
-// columns inside an MMA is free as long as A and B agree, so lane (g, t)'s word goes in as it lies: nibbles 0, 4
-// and 2, 6 to one MMA, 1, 5 and 3, 7 to the other. With float16 activations a nibble needs no conversion at all:
-// (word & 0x000f000f) is a pair of float16 subnormals q * 2^-24, exact in the tensor core, and (word & 0x00f000f0)
-// a pair of 16 q * 2^-24; the two MMAs keep sums of their own, joined as lo + hi / 16 at the end of the group, and
-// the 2^24 comes at the end of the row. Products are exact and sums are float32: the result is the formula's but for float32
-// rounding. The bias takes sum x over the group, from the same B operands times a matrix of 2^-24.
+// columns inside an MMA is free as long as A and B agree, so lane (g, t)'s word goes in as it lies: columns 0, 1 and 4,
+// 5 to one MMA, 2, 3 and 6, 7 to the other. With float16 activations a nibble needs no conversion at all: (word &
+// 0x000f000f) is a pair of float16 subnormals q * 2^-24, exact in the tensor core, and (word & 0x00f000f0) a pair of 16
+// q * 2^-24; the two MMAs keep sums of their own, joined as lo + hi / 16 at the end of the group, and the 2^24 comes at
+// the end of the row. Products are exact and sums are float32: the result is the formula's but for float32 rounding.
+// The bias takes sum x over the group, from the same B operands times a matrix of 2^-24.
 // Float32 activations are three bfloat16 pieces (8 + 8 + 8 bits: the whole float32), each through the same MMAs;
 // codes become bfloat16 by (q | 0x4300) - 128, exact too.
 #pragma once
@@ -45,6 +49,41 @@ __host__ __device__ constexpr int tile_bytes() {
 __host__ __device__ constexpr int tile_bytes_of(int g) { return kCodeBytes + kRows * (kCols / g) * 4; }
 __host__ __device__ constexpr int64_t tiles_of_cols(int64_t cols) { return (cols + kCols - 1) / kCols; }
 __host__ __device__ constexpr int64_t strips_of_rows(int64_t rows) { return (rows + kRows - 1) / kRows; }
+
+constexpr uint32_t kWaitLimit = 1u << 22;
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity) { return tc::mbar_wait(bar, parity, kWaitLimit); }
+
+// Where a row's chunk t lies in a tile, in bytes; lane (g, t)'s chunk of row g (that of row g + 8 lies 512 further)
+__host__ __device__ constexpr int chunk_at(int row, int t) { return row * 64 + ((t ^ ((row >> 1) & 3)) << 4); }
+__device__ __forceinline__ int lane_chunk(int lane) { return chunk_at(lane >> 2, lane & 3); }
+// A word of eight codes, weight i in bits 4 i, in the layout's order of nibbles, and back
+__device__ __forceinline__ uint32_t nibbles_in(uint32_t w) {
+    uint32_t r = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r |= ((w >> (4 * i)) & 15u) << (4 * ((i >> 1) + 4 * (i & 1)));
+    return r;
+}
+__device__ __forceinline__ uint32_t nibbles_out(uint32_t w) {
+    uint32_t r = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r |= ((w >> (4 * ((i >> 1) + 4 * (i & 1)))) & 15u) << (4 * i);
+    return r;
+}
+
+// The (scale, bias) pairs of row `row` of a tile in shared memory
+template <int G>
+__device__ __forceinline__ void load_pairs(const uint8_t* tile, int row, uint32_t (&v)[kCols / G]) {
+    const uint8_t* p = tile + kCodeBytes + row * (kCols / G) * 4;
+    if constexpr (G == 32) {
+        const uint4 q = *reinterpret_cast<const uint4*>(p);
+        v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
+    } else if constexpr (G == 64) {
+        const uint2 q = *reinterpret_cast<const uint2*>(p);
+        v[0] = q.x, v[1] = q.y;
+    } else {
+        v[0] = *reinterpret_cast<const uint32_t*>(p);
+    }
+}
 
 // Bulk copy of `bytes` (a multiple of 16, both addresses 16-byte aligned) of this GPU's memory into this CTA's
 // shared memory, completing on `bar`.
@@ -164,8 +203,7 @@ struct Sums {
 
 template <bool FIRST, int MT>
 __device__ __forceinline__ void run_mma(const Codes<__half> (&a)[MT], const Acts<__half>& x, Sums<__half, MT>& s) {
-    const uint32_t b0 = __byte_perm(x.v.x, x.v.z, 0x5410), b1 = __byte_perm(x.v.y, x.v.w, 0x5410);
-    const uint32_t c0 = __byte_perm(x.v.x, x.v.z, 0x7632), c1 = __byte_perm(x.v.y, x.v.w, 0x7632);
+    const uint32_t b0 = x.v.x, b1 = x.v.z, c0 = x.v.y, c1 = x.v.w;
     constexpr uint32_t one = Codes<__half>::kOne;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
@@ -192,8 +230,8 @@ __device__ __forceinline__ void run_mma(const Codes<float> (&a)[MT], const Acts<
     constexpr uint32_t one = Codes<float>::kOne;
     auto piece = [&](auto first) {
         constexpr bool kFirst = decltype(first)::value;
-        const uint32_t b0 = bf16_pair(f[0], f[4]), b1 = bf16_pair(f[2], f[6]);
-        const uint32_t c0 = bf16_pair(f[1], f[5]), c1 = bf16_pair(f[3], f[7]);
+        const uint32_t b0 = bf16_pair(f[0], f[1]), b1 = bf16_pair(f[4], f[5]);
+        const uint32_t c0 = bf16_pair(f[2], f[3]), c1 = bf16_pair(f[6], f[7]);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
             mma_bf16<kFirst>(s.lo[m], a[m].lo[0], a[m].lo[1], a[m].lo[2], a[m].lo[3], b0, b1);
@@ -267,7 +305,7 @@ __device__ __forceinline__ void tile_mma(const uint8_t* tile, int stride, int la
     uint32_t wa[2][4], wb[2][4];
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-        const uint8_t* p = tile + m * stride + 16 * lane;
+        const uint8_t* p = tile + m * stride + lane_chunk(lane);
         const uint4 u = *reinterpret_cast<const uint4*>(p);
         const uint4 v = *reinterpret_cast<const uint4*>(p + 512);
         wa[m][0] = u.x, wa[m][1] = u.y, wa[m][2] = u.z, wa[m][3] = u.w;

@@ -17,6 +17,10 @@ int product_f16(const ProductArgs& a, int group, const Writes& w, cudaStream_t s
 int product_f32(const ProductArgs& a, int group, const Writes& w, cudaStream_t st);
 int down_f16(const DownArgs& a, int group, const Writes& w, cudaStream_t st);
 int down_f32(const DownArgs& a, int group, const Writes& w, cudaStream_t st);
+// the dense part of `a` on the prompt's kernel (float16), and whether that is the faster one
+bool matmul_better(int64_t tokens, int64_t rows, int64_t cols);
+int matmul_f16(const ProductArgs& a, int group, const Writes& w, cudaStream_t st);
+cudaError_t matmul_status(int* v, bool clear);
 cudaError_t product_status_f16(int* v, bool clear);
 cudaError_t product_status_f32(int* v, bool clear);
 cudaError_t down_status_f16(int* v, bool clear);

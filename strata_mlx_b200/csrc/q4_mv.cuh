@@ -27,7 +27,6 @@ namespace q4 {
 constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kMaxPairs = 2048;
-constexpr uint32_t kWaitLimit = 1u << 22;
 
 // A wait that gave up (never seen; a copy that cannot complete) leaves SMOE_ETIMEOUT here, the launch's outputs are
 // then not valid. smoe_q4_status reads and clears it. One per translation unit.
@@ -47,6 +46,7 @@ struct ProductArgs {
     int64_t r_rows, experts, pairs, share;
     const uint32_t* idx;
     const float* weights;  // GLU: the pair's result times this, or null
+    bool pieces;     // GLU, float16: a result as two rows, its float16 and what that leaves (rows 2 p and 2 p + 1 of out)
     uint32_t* zero;  // words to clear for the launch after (its counters)
     int n_zero;
     int team;    // warps that share a job's columns
@@ -55,8 +55,8 @@ struct ProductArgs {
 };
 
 struct DownArgs {
-    const void* h;  // (pairs, ffn)
-    const void* hs; // (tokens, sffn), or null with sffn = 0
+    const void* h;   // (pairs, ffn); float16: (2 pairs, ffn), in pieces
+    const void* hs;  // (tokens, sffn) likewise, or null with sffn = 0
     const uint8_t* w;
     const uint8_t* sw;
     int64_t ffn, sffn, rows, experts, tokens, k;
@@ -95,7 +95,7 @@ struct Ring {
     // the slot at the tail, once its copies have landed
     __device__ __forceinline__ uint8_t* wait(int lane) {
         if (ok) {
-            ok = __all_sync(0xffffffffu, tc::mbar_wait(&bars[tail], phase, kWaitLimit));
+            ok = __all_sync(0xffffffffu, wait_for(&bars[tail], phase));
             if (!ok && lane == 0) atomicExch(&g_q4_status, SMOE_ETIMEOUT);
         }
         return ptr + tail * slot_bytes;
@@ -114,7 +114,7 @@ struct Ring {
     __device__ __forceinline__ void drain(int lane) {
         ok = true;
         while (in_flight > 0) {
-            if (!tc::mbar_wait(&bars[tail], phase, kWaitLimit) && lane == 0) atomicExch(&g_q4_status, SMOE_ETIMEOUT);
+            if (!wait_for(&bars[tail], phase) && lane == 0) atomicExch(&g_q4_status, SMOE_ETIMEOUT);
             pop();
         }
     }
@@ -407,7 +407,13 @@ __global__ void __launch_bounds__(kThreads, 2) q4_product_kernel(const ProductAr
                 }
             }
             T* out = static_cast<T*>(dense ? a.d_out : a.r_out);
-            out[to * rows + row] = from_f32<T>(v);
+            const T first = from_f32<T>(v);
+            if (GLU && sizeof(T) == 2 && a.pieces) {
+                out[2 * to * rows + row] = first;
+                out[(2 * to + 1) * rows + row] = from_f32<T>(v - to_f32(first));
+            } else {
+                out[to * rows + row] = first;
+            }
         }
     }
     pdl_release();
@@ -421,6 +427,13 @@ __global__ void __launch_bounds__(kThreads, 2) q4_product_kernel(const ProductAr
 // so all jobs' tiles in a row are cut into one even range for each CTA, and a CTA's range of a job into one for each
 // warp. A warp adds a block's sums into its own copy of the result in shared memory when the block ends, each row of h to
 // its token; a CTA adds its warps' in order, and the last CTA of a job to come adds the CTAs' in order.
+//
+// float16: h lies in two pieces of float16 (11 + 11 bits), because rounding it once would leave the block's result with
+// 1.4 times the error of its own rounding. A block is then four rows of h, their first pieces in columns 0 .. 3 of the
+// MMAs and their second in 4 .. 7: no more instructions than eight rows.
+
+template <typename T>
+__host__ __device__ constexpr int down_rows() { return sizeof(T) == 2 ? kM / 2 : kM; }
 
 constexpr int kTokenStride = kMt * kRows + 4;  // floats of a token's sums: rows 0, 8, .. of four tokens on 32 banks
 
@@ -434,6 +447,7 @@ template <typename T, int G>
 __global__ void __launch_bounds__(kThreads, 2) q4_down_kernel(const DownArgs a) {
     constexpr int kTile = tile_bytes<G>();
     constexpr int kSlot = slot_bytes<G>();
+    constexpr int kRowsIn = down_rows<T>(), kPieces = kM / kRowsIn;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int warp_sums[kWarps];
     __shared__ uint32_t arrived;
@@ -451,10 +465,10 @@ __global__ void __launch_bounds__(kThreads, 2) q4_down_kernel(const DownArgs a) 
     float* mine = red + warp * tokens * kTokenStride;
 
     if (!a.early) pdl_wait();
-    const PairBlocks blocks = pair_blocks(table, a.idx, pairs, static_cast<int>(a.experts), kM, warp_sums);
+    const PairBlocks blocks = pair_blocks(table, a.idx, pairs, static_cast<int>(a.experts), kRowsIn, warp_sums);
     // segments of a job: the shared expert's blocks of tokens, then the pairs' blocks
     const int stiles = static_cast<int>(tiles_of_cols(a.sffn)), ftiles = static_cast<int>(tiles_of_cols(a.ffn));
-    const int sblocks = stiles > 0 ? (tokens + kM - 1) / kM : 0;
+    const int sblocks = stiles > 0 ? (tokens + kRowsIn - 1) / kRowsIn : 0;
     const int shared_items = sblocks * stiles;
     const int items = max(1, shared_items + blocks.n * ftiles);  // (a job without any tile still writes its zeros)
     const bool any = shared_items + blocks.n > 0;
@@ -548,12 +562,12 @@ __global__ void __launch_bounds__(kThreads, 2) q4_down_kernel(const DownArgs a) 
             if (c.seg != seg) {
                 seg = c.seg;
                 shared = seg < sblocks;
-                start = shared ? seg * kM : blocks.start[seg - sblocks];
-                count = shared ? min(kM, tokens - start) : blocks.count[seg - sblocks];
+                start = shared ? seg * kRowsIn : blocks.start[seg - sblocks];
+                count = shared ? min(kRowsIn, tokens - start) : blocks.count[seg - sblocks];
                 runs = static_cast<int>((shared ? a.sffn : a.ffn) / 32);
-                const int at = g < count ? start + g : start;
-                xp = shared ? static_cast<const T*>(a.hs) + at * a.sffn + 8 * t
-                            : static_cast<const T*>(a.h) + blocks.list[at] * a.ffn + 8 * t;
+                const int n = g % kRowsIn, at = n < count ? start + n : start;
+                xp = shared ? static_cast<const T*>(a.hs) + (at * kPieces + g / kRowsIn) * a.sffn + 8 * t
+                            : static_cast<const T*>(a.h) + (blocks.list[at] * kPieces + g / kRowsIn) * a.ffn + 8 * t;
             }
             const int n = stage_of(c);
             const TileActs<T> x0(xp + c.tile * kCols, runs - 4 * c.tile);
@@ -566,8 +580,15 @@ __global__ void __launch_bounds__(kThreads, 2) q4_down_kernel(const DownArgs a) 
             fetch();
             advance(c, n);
             if (c.seg != seg || c.item == c.last) {
-                // the block's end: each column's sums to its token, this lane's columns 2 t and 2 t + 1. A token that
+                // the block's end: each column's sums to its token, this lane's columns 2 t and 2 t + 1 (with pieces,
+                // those of columns 2 t + 4 and 2 t + 5 added). A token that
                 // names an expert twice has two columns here, neighbours: column by column then.
+                if constexpr (kPieces == 2) {
+#pragma unroll
+                    for (int m = 0; m < kMt; ++m)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[m][i] += __shfl_xor_sync(0xffffffffu, acc[m][i], 2);
+                }
                 auto add = [&](int h) {
                     const int col = 2 * t + h;
                     float* to = mine + (shared ? start + col : blocks.list[start + col] / k) * kTokenStride + g;

@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(kConvThreads) q4_dequant_kernel(const uint32_t
         const uint8_t* tile = packed + ((e * strips_of_rows(rows) + r / kRows) * tiles_of_cols(cols) + c / kCols) *
                                            tile_bytes_of(group);
         const int row = static_cast<int>(r % kRows), j = (c % kCols) / 32, t = (c % 32) / 8;
-        word = *reinterpret_cast<const uint32_t*>(tile + row * 64 + (4 * t + j) * 4);
+        word = nibbles_out(*reinterpret_cast<const uint32_t*>(tile + chunk_at(row, t) + 4 * j));
         const __half2 p = *reinterpret_cast<const __half2*>(tile + kCodeBytes + (row * (kCols / group) + (c % kCols) / group) * 4);
         s = __low2float(p);
         b = __high2float(p);
@@ -144,8 +144,9 @@ __global__ void __launch_bounds__(kConvThreads) q4_pack_kernel(const uint32_t* _
     const int64_t c0 = (tile - strip * tiles) * kCols;
     uint32_t v = 0;
     if (at < kCodeBytes / 4) {
-        const int64_t r = (strip - e * strips) * kRows + at / 16, c = c0 + 32 * (at & 3) + 8 * ((at >> 2) & 3);
-        if (r < rows && c < cols) v = codes[(e * rows + r) * (cols / 8) + c / 8];
+        const int row = at / 16, t = ((at >> 2) & 3) ^ ((row >> 1) & 3);
+        const int64_t r = (strip - e * strips) * kRows + row, c = c0 + 32 * (at & 3) + 8 * t;
+        if (r < rows && c < cols) v = nibbles_in(codes[(e * rows + r) * (cols / 8) + c / 8]);
     } else {
         const int k = at - kCodeBytes / 4;
         const int64_t r = (strip - e * strips) * kRows + k / groups, c = c0 + int64_t(k % groups) * group;
@@ -283,8 +284,9 @@ extern "C" int smoe_q4_pack(const uint32_t* codes, const uint16_t* scales, const
     Q4_CATCH("q4_pack")
 }
 
-// `zero`: words that the launch clears besides (for the launch after it)
-static int q4_product(const SmoeQ4Product* p, uint32_t* zero, int n_zero, void* stream) {
+// pieces: results as two rows of float16 each (q4_mv.cuh); `zero`: words that the launch clears besides, for the launch
+// after it
+static int q4_product(const SmoeQ4Product* p, bool pieces, uint32_t* zero, int n_zero, void* stream) {
     SMOE_REQUIRE(p, SMOE_EARG, "q4_product: null pointer");
     SMOE_REQUIRE(p->dtype == SMOE_F16 || p->dtype == SMOE_F32, SMOE_EDTYPE,
                  "q4_product takes float16 or float32 activations");
@@ -314,7 +316,7 @@ static int q4_product(const SmoeQ4Product* p, uint32_t* zero, int n_zero, void* 
         a.d_rows = p->dense_rows;
         a.d_tokens = p->dense_tokens;
         a.d_gate = p->dense_gate;
-        w.add(p->dense_out, size_t(p->dense_tokens) * p->dense_rows * item);
+        w.add(p->dense_out, size_t(p->dense_tokens) * p->dense_rows * item * (pieces ? 2 : 1));
         const size_t bytes = stack_bytes(1, p->dense_rows, p->cols, p->group);
         a.early = a.early && pdl_early(st, p->dense, bytes) && (!p->dense2 || pdl_early(st, p->dense2, bytes));
     }
@@ -339,10 +341,13 @@ static int q4_product(const SmoeQ4Product* p, uint32_t* zero, int n_zero, void* 
         a.share = p->share;
         a.idx = p->idx;
         a.weights = p->weights;
-        w.add(p->out, size_t(p->pairs) * p->rows * item);
+        w.add(p->out, size_t(p->pairs) * p->rows * item * (pieces ? 2 : 1));
         const size_t bytes = stack_bytes(p->experts, p->rows, p->cols, p->group);
         a.early = a.early && pdl_early(st, p->stack, bytes) && (!p->stack2 || pdl_early(st, p->stack2, bytes));
     }
+    if (p->dtype == SMOE_F16 && p->pairs == 0 && !glu && matmul_better(p->dense_tokens, p->dense_rows, p->cols))
+        return matmul_f16(a, p->group, w, st);
+    a.pieces = pieces;
     a.zero = zero;
     a.n_zero = n_zero;
     w.add(zero, size_t(n_zero) * 4);
@@ -351,7 +356,7 @@ static int q4_product(const SmoeQ4Product* p, uint32_t* zero, int n_zero, void* 
 
 extern "C" int smoe_q4_product(const SmoeQ4Product* p, void* stream) {
     Q4_TRY
-    return q4_product(p, nullptr, 0, stream);
+    return q4_product(p, false, nullptr, 0, stream);
     Q4_CATCH("q4_product")
 }
 
@@ -367,7 +372,7 @@ extern "C" int smoe_q4_linear(const uint8_t* packed, int64_t rows, int64_t cols,
     p.dense_rows = rows;
     p.dense_tokens = tokens;
     p.dense_out = out;
-    return q4_product(&p, nullptr, 0, stream);
+    return q4_product(&p, false, nullptr, 0, stream);
     Q4_CATCH("q4_linear")
 }
 
@@ -375,16 +380,16 @@ extern "C" int smoe_q4_linear(const uint8_t* packed, int64_t rows, int64_t cols,
 // products' jobs.
 struct MoeSpace {
     size_t h, hs, partial, counters, bytes;
-    MoeSpace(int dtype, int64_t tokens, int64_t k, int64_t hidden, int64_t ffn, int64_t shared_ffn) {
-        const size_t item = dtype == SMOE_F16 ? 2 : 4;
+    MoeSpace(int64_t tokens, int64_t k, int64_t hidden, int64_t ffn, int64_t shared_ffn) {
         size_t at = 0;
         auto take = [&](size_t n) {
             const size_t from = at;
             at += (n + 255) & ~size_t(255);
             return from;
         };
-        h = take(size_t(tokens) * k * ffn * item);
-        hs = take(size_t(tokens) * shared_ffn * item);
+        // (four bytes a value: a float32, or its two float16 pieces)
+        h = take(size_t(tokens) * k * ffn * 4);
+        hs = take(size_t(tokens) * shared_ffn * 4);
         partial = take(size_t(kDownCtas) * 2 * tokens * kMt * kRows * 4);
         counters = take(n_counters(hidden) * 4);
         bytes = at;
@@ -392,10 +397,10 @@ struct MoeSpace {
     static size_t n_counters(int64_t hidden) { return static_cast<size_t>((strips_of_rows(hidden) + kMt - 1) / kMt); }
 };
 
-extern "C" size_t smoe_q4_moe_workspace_size(int dtype, int64_t tokens, int64_t k, int64_t hidden, int64_t ffn,
+extern "C" size_t smoe_q4_moe_workspace_size(int64_t tokens, int64_t k, int64_t hidden, int64_t ffn,
                                              int64_t shared_ffn) {
     if (tokens <= 0 || k <= 0 || hidden <= 0 || ffn <= 0 || shared_ffn < 0) return 0;
-    return MoeSpace(dtype, tokens, k, hidden, ffn, shared_ffn).bytes;
+    return MoeSpace(tokens, k, hidden, ffn, shared_ffn).bytes;
 }
 
 extern "C" int smoe_q4_moe(const SmoeQ4Moe* m, void* workspace, size_t workspace_bytes, void* stream) {
@@ -423,10 +428,10 @@ extern "C" int smoe_q4_moe(const SmoeQ4Moe* m, void* workspace, size_t workspace
                      aligned16(m->sdown),
                  SMOE_EARG, "q4_moe: null or misaligned pointer");
     SMOE_REQUIRE(workspace && aligned16(workspace) &&
-                     workspace_bytes >= smoe_q4_moe_workspace_size(m->dtype, m->tokens, m->k, m->hidden, m->ffn, m->shared_ffn),
+                     workspace_bytes >= smoe_q4_moe_workspace_size(m->tokens, m->k, m->hidden, m->ffn, m->shared_ffn),
                  SMOE_EWORKSPACE, "q4_moe: workspace missing, misaligned or too small");
     cudaStream_t st = as_stream(stream);
-    const MoeSpace space(m->dtype, m->tokens, m->k, m->hidden, m->ffn, m->shared_ffn);
+    const MoeSpace space(m->tokens, m->k, m->hidden, m->ffn, m->shared_ffn);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     void* h = ws + space.h;
     void* hs = ws + space.hs;
@@ -453,7 +458,7 @@ extern "C" int smoe_q4_moe(const SmoeQ4Moe* m, void* workspace, size_t workspace
     p.share = m->k;
     p.weights = m->weights;
     p.out = h;
-    if (int s = q4_product(&p, counters, static_cast<int>(MoeSpace::n_counters(m->hidden)), stream)) return s;
+    if (int s = q4_product(&p, p.dtype == SMOE_F16, counters, static_cast<int>(MoeSpace::n_counters(m->hidden)), stream)) return s;
     DownArgs d = {};
     d.h = h;
     d.hs = m->shared_ffn > 0 ? hs : nullptr;
@@ -482,7 +487,7 @@ extern "C" int smoe_q4_status(int* status, int clear) {
     SMOE_REQUIRE(status, SMOE_EARG, "q4_status: null pointer");
     *status = 0;
     cudaError_t e = cudaDeviceSynchronize();
-    for (auto read : {product_status_f16, product_status_f32, down_status_f16, down_status_f32}) {
+    for (auto read : {matmul_status, product_status_f16, product_status_f32, down_status_f16, down_status_f32}) {
         int v = 0;
         if (e == cudaSuccess) e = read(&v, clear != 0);
         if (v != 0) *status = v;

@@ -1,0 +1,436 @@
+// A prompt's product on 4-bit weights with group scales, on the 5th-generation tensor cores (layout: q4.cuh).
+//
+// out[t, r] = sum_c w[r, c] x[t, c], the weights w = code scale + bias rounded once to float16 (the activations' type)
+// and float32 sums. 128 weight rows are the M side of a tcgen05 MMA (8 strips), up to 256 tokens the N side, so a row is
+// decoded once for that many tokens. What bounds it: the tensor pipe (2 rows cols tokens flops at 4,096 multiply-adds a
+// cycle of an SM) and beside it the decoding's issue, 17 instructions for 8 weights: a stage of 128 x 128 weights takes
+// 272 issue slots a scheduler, its MMAs 4 cycles a token. From about 70 tokens a job on the tensor pipe is the longer.
+//
+// Per CTA (persistent over jobs = (block of tokens, 128 rows)), warp-specialized, every hand-off an mbarrier:
+//   warp 17   weights: a stage is one tile of each of the 8 strips, one TMA box (a copy a strip took the warp 120 cycles
+//             each to issue, more than the stage's work) into a ring of up to 10 slots
+//   warp 18   activations: the tokens' 128 columns by TMA (boxes of 128 / 64 / 32 / 16 rows x 64 columns, 128-byte
+//             swizzle) into a ring of its own
+//   warps 0-15 decoders, two groups on every other stage: a thread reads half of its row's 128 columns, (q | 0x6400) - 1024 makes a pair of codes
+//             float16 exactly, one fused multiply-add with the group's scale and bias rounds it to the weight; stored to
+//             its TMEM lane of an A slot
+//   warp 16   MMA: A from TMEM, B from shared memory, 8 MMAs of K = 16 a stage; commits free the slots.
+//   warps 19-22 read a job's sums back and write them out while the next job runs (jobs of up to 160 tokens have two
+//             accumulators); a CTA's last job is the decoders'
+// Every wait is bounded; one that gives up leaves SMOE_ETIMEOUT in the status and ends the CTA's work.
+#include <cuda.h>
+
+#include <algorithm>
+#include <mutex>
+
+#include "q4_launch.cuh"
+
+namespace smoe {
+namespace q4 {
+
+constexpr int kGDecoders = 16;   // two groups of 8 warps, every other stage each
+constexpr int kGGroup = 8;
+constexpr int kGEnders = 4;      // warps that write a job out while the next one runs
+constexpr int kGThreads = 32 * (kGDecoders + 3 + kGEnders);
+constexpr int kGM = 128;
+constexpr int kGStrips = kGM / kRows;
+constexpr int kGMaxN = 256;
+constexpr int kGASlots = 3;
+constexpr uint32_t kGAColumn = 320;  // of TMEM: A slots from here, 64 columns each; accumulators before
+constexpr int kGMaxRaw = 10;
+constexpr int kGMaxB = 6;
+constexpr int kGSmemLimit = 227 * 1024;
+
+static __device__ int g_q4_gemm_status = 0;
+
+struct GemmArgs {
+    const uint8_t* w;
+    __half* out;
+    int64_t rows, cols, tokens;
+    int n;        // tokens of a job, a multiple of 16
+    int nblocks;  // jobs' blocks of tokens
+    int mblocks;
+    int nb, nr;   // activation and raw slots
+    bool early;
+};
+
+struct alignas(64) GemmMaps {
+    CUtensorMap w;     // strips of the matrix as rows of 8-byte words, in boxes of a tile of 8 strips
+    CUtensorMap a[4];  // boxes of 16, 32, 64, 128 rows x 64 columns
+};
+
+struct GemmSmem {
+    uint64_t rawfull[kGMaxRaw], rawfree[kGMaxRaw], bfull[kGMaxB], bfree[kGMaxB];
+    uint64_t afull[kGASlots], afree[kGASlots], dfull[2], dfree[2];
+    uint32_t tmem_base;
+};
+
+template <int G>
+__host__ __device__ constexpr int raw_slot_bytes() { return kGStrips * tile_bytes<G>(); }
+__host__ __device__ constexpr int b_slot_bytes(int n) { return 2 * n * 128; }  // two atoms of 64 columns
+// [activation slots, 1024-aligned][raw slots][barriers]
+template <int G>
+__host__ __device__ constexpr size_t gemm_smem(int n, int nb, int nr) {
+    return size_t(nb) * b_slot_bytes(n) + size_t(nr) * raw_slot_bytes<G>() + sizeof(GemmSmem);
+}
+
+__device__ __forceinline__ bool elect_one() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(e));
+    return e != 0;
+}
+
+struct Phase {
+    int slot = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ void next(int n) {
+        if (++slot == n) {
+            slot = 0;
+            phase ^= 1;
+        }
+    }
+};
+
+// Eight codes of the layout's word as weights: w[i] = columns 2 i, 2 i + 1
+__device__ __forceinline__ void decode8(uint32_t word, __half2 s, __half2 b, uint32_t* out) {
+    const __half2 base = __half2half2(__ushort_as_half(0x6400));  // 1024
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t v = ((word >> (4 * i)) & 0x000f000fu) | 0x64006400u;
+        const __half2 w = __hfma2(__hsub2(*reinterpret_cast<const __half2*>(&v), base), s, b);
+        out[i] = *reinterpret_cast<const uint32_t*>(&w);
+    }
+}
+
+template <int G>
+__global__ void __launch_bounds__(kGThreads, 1) q4_matmul_kernel(const GemmArgs g, const __grid_constant__ GemmMaps maps) {
+    constexpr int kTile = tile_bytes<G>();
+    constexpr int kRaw = raw_slot_bytes<G>();
+    extern __shared__ __align__(1024) uint8_t gsmem[];
+    uint8_t* smem = gsmem;
+    const int bslot = b_slot_bytes(g.n);
+    uint8_t* raw = smem + size_t(g.nb) * bslot;
+    GemmSmem& S = *reinterpret_cast<GemmSmem*>(raw + g.nr * kRaw);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int jobs = g.nblocks * g.mblocks;
+    const int nk = static_cast<int>(tiles_of_cols(g.cols));
+    const int nd = 2 * g.n <= int(kGAColumn) ? 2 : 1;
+    if (smem_addr(smem) & 1023u) {  // the swizzled layout needs it
+        if (threadIdx.x == 0) atomicExch(&g_q4_gemm_status, SMOE_EARG);
+        return;
+    }
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < g.nr; ++i) {
+            tc::mbar_init(&S.rawfull[i], 1);
+            tc::mbar_init(&S.rawfree[i], kGGroup);
+        }
+        for (int i = 0; i < g.nb; ++i) {
+            tc::mbar_init(&S.bfull[i], 1);
+            tc::mbar_init(&S.bfree[i], 1);
+        }
+        for (int i = 0; i < kGASlots; ++i) {
+            tc::mbar_init(&S.afull[i], kGGroup);
+            tc::mbar_init(&S.afree[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            tc::mbar_init(&S.dfull[i], 1);
+            tc::mbar_init(&S.dfree[i], kGEnders);
+        }
+        tc::fence_barrier_init();
+    }
+    if (warp == kGDecoders) {
+        tc::tmem_alloc(&S.tmem_base, 512);
+        tc::tmem_relinquish();
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const uint32_t tmem = S.tmem_base;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        return __all_sync(0xffffffffu, wait_for(bar, parity));
+    };
+    // columns c0, c0 + step, .. (eight tokens each) of a job's accumulator, this warp's 32 rows
+    auto write_out = [&](int job, int slot, int c0, int step) {
+        tc::fence_after_sync();
+        const int64_t r = int64_t(job % g.mblocks) * kGM + 32 * (warp & 3) + lane, tok0 = int64_t(job / g.mblocks) * g.n;
+        const uint32_t from = tmem + (uint32_t(32 * (warp & 3)) << 16) + uint32_t(g.n * slot);
+        const int valid = static_cast<int>(min(int64_t(g.n), g.tokens - tok0));
+        __half* out = g.out + (tok0 + c0) * g.rows + r;
+        for (int c = c0; c < valid; c += step, out += step * g.rows) {
+            uint32_t v[8];
+            tc::tmem_ld8(from + c, v);
+            tc::tmem_wait_ld();
+            if (r < g.rows) {
+                __half* to = out;
+#pragma unroll
+                for (int j = 0; j < 8; ++j, to += g.rows)
+                    if (c + j < valid) *to = __float2half_rn(__uint_as_float(v[j]));
+            }
+            __syncwarp();
+        }
+        tc::fence_before_sync();
+        __syncwarp();
+    };
+    bool ok = true;
+
+    if (warp > kGDecoders + 2) {
+        // ---------------- the ends of all jobs but the last
+        pdl_wait();
+        Phase dp;
+        for (int job = blockIdx.x; job + int(gridDim.x) < jobs && ok; job += gridDim.x, dp.next(nd)) {
+            if (!(ok = wait(&S.dfull[dp.slot], dp.phase))) break;
+            write_out(job, dp.slot, 0, 8);
+            if (lane == 0) tc::mbar_arrive(&S.dfree[dp.slot]);
+        }
+    } else if (warp == kGDecoders + 1) {
+        // ---------------- the weights' producer
+        if (!g.early) pdl_wait();
+        Phase rp;
+        int stage = 0;
+        for (int job = blockIdx.x; job < jobs && ok; job += gridDim.x) {
+            const int mb = job % g.mblocks;
+            for (int s = 0; s < nk; ++s, ++stage, rp.next(g.nr)) {
+                if (stage >= g.nr && !(ok = wait(&S.rawfree[rp.slot], rp.phase ^ 1))) break;
+                if (lane == 0) {
+                    // (strips past the last read as zeros: weights of zero)
+                    tc::mbar_arrive_expect_tx(&S.rawfull[rp.slot], kRaw);
+                    tc::tma_load_2d(smem_addr(raw) + rp.slot * kRaw, &maps.w, s * (kTile / 8), mb * kGStrips,
+                                    &S.rawfull[rp.slot]);
+                }
+                __syncwarp();
+            }
+        }
+        // no copy may still be writing this CTA's shared memory when it leaves
+        for (int i = 0; i < g.nr && i < stage; ++i) {
+            const int st = stage - 1 - i;
+            wait_for(&S.rawfull[st % g.nr], (st / g.nr) & 1);
+        }
+    } else if (warp == kGDecoders + 2) {
+        // ---------------- the activations' producer (they are the launch before's)
+        pdl_wait();
+        Phase bp;
+        int stage = 0;
+        for (int job = blockIdx.x; job < jobs && ok; job += gridDim.x) {
+            const int tok0 = job / g.mblocks * g.n;
+            for (int s = 0; s < nk; ++s, ++stage, bp.next(g.nb)) {
+                if (stage >= g.nb && !(ok = wait(&S.bfree[bp.slot], bp.phase ^ 1))) break;
+                if (lane == 0) {
+                    const uint32_t dst = smem_addr(smem) + bp.slot * bslot;
+                    tc::mbar_arrive_expect_tx(&S.bfull[bp.slot], static_cast<uint32_t>(bslot));
+                    int done = 0;
+                    for (int left = g.n; left > 0;) {
+                        const int b = left >= 128 ? 3 : left >= 64 ? 2 : left >= 32 ? 1 : 0;
+                        for (int h = 0; h < 2; ++h)
+                            tc::tma_load_2d(dst + h * g.n * 128 + done * 128, &maps.a[b], s * kCols + 64 * h, tok0 + done,
+                                            &S.bfull[bp.slot]);
+                        done += 16 << b;
+                        left -= 16 << b;
+                    }
+                }
+                __syncwarp();
+            }
+        }
+        for (int i = 0; i < g.nb && i < stage; ++i) {
+            const int st = stage - 1 - i;
+            wait_for(&S.bfull[st % g.nb], (st / g.nb) & 1);
+        }
+    } else if (warp == kGDecoders) {
+        // ---------------- MMA (the converged warp issues, one elected lane)
+        const uint32_t idesc = tc::idesc_f16_f32(kGM, g.n);
+        Phase ap, bp, dp;
+        int count = 0;
+        for (int job = blockIdx.x; job < jobs && ok; job += gridDim.x, ++count, dp.next(nd)) {
+            if (count >= nd && !(ok = wait(&S.dfree[dp.slot], dp.phase ^ 1))) break;
+            tc::fence_after_sync();
+            const uint32_t d = tmem + uint32_t(g.n * dp.slot);
+            for (int s = 0; s < nk; ++s, ap.next(kGASlots), bp.next(g.nb)) {
+                if (!(ok = wait(&S.afull[ap.slot], ap.phase)) || !(ok = wait(&S.bfull[bp.slot], bp.phase))) break;
+                tc::fence_after_sync();
+                const uint64_t bd = tc::smem_desc_sw128(smem_addr(smem) + bp.slot * bslot);
+                if (elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < kCols / 16; ++k)
+                        tc::mma_f16_ts(d, tmem + kGAColumn + 64u * ap.slot + 8u * k,
+                                       bd + uint64_t(((k >> 2) * g.n * 128 + (k & 3) * 32) >> 4), idesc,
+                                       (s > 0 || k > 0) ? 1u : 0u);
+                    tc::mma_commit(&S.afree[ap.slot]);
+                    tc::mma_commit(&S.bfree[bp.slot]);
+                    if (s == nk - 1) tc::mma_commit(&S.dfull[dp.slot]);
+                }
+                __syncwarp();
+            }
+        }
+    } else {
+        // ---------------- decoders and the end of a job: thread L of the four lane quarters is weight row L. A group of
+        // eight warps takes every other stage, the two warps of a quarter two of the four chunks of the row's tile each
+        // (conflict-free 16-byte reads, 16 columns of each run).
+        const int L = 32 * (warp & 3) + lane, group = warp / kGGroup, pair = (warp >> 2) & 1;
+        const int row = L % kRows;
+        const uint32_t lanes = tmem + (uint32_t(32 * (warp & 3)) << 16);
+        const uint8_t* mine = raw + (L / kRows) * kTile;
+        const uint8_t *at0 = mine + chunk_at(row, 2 * pair), *at1 = mine + chunk_at(row, 2 * pair + 1);
+        Phase rp, ap, dp, last;
+        int stage = 0;
+        for (int job = blockIdx.x; job < jobs && ok; job += gridDim.x, dp.next(nd)) {
+            for (int s = 0; s < nk; ++s, ++stage, rp.next(g.nr), ap.next(kGASlots)) {
+                if ((stage & 1) != group) continue;
+                if (!(ok = wait(&S.rawfull[rp.slot], rp.phase))) break;
+                const int slot = rp.slot * kRaw;
+                const uint4 c0 = *reinterpret_cast<const uint4*>(at0 + slot), c1 = *reinterpret_cast<const uint4*>(at1 + slot);
+                uint32_t p[kCols / G];
+                load_pairs<G>(mine + slot, row, p);
+                const uint32_t w0[4] = {c0.x, c0.y, c0.z, c0.w}, w1[4] = {c1.x, c1.y, c1.z, c1.w};
+                // (the group waited for stage - 5's release two stages ago, so stage - 6's, this slot's one before, is past)
+                if (stage >= kGASlots && !(ok = wait(&S.afree[ap.slot], ap.phase ^ 1))) break;
+                tc::fence_after_sync();
+                const uint32_t to = lanes + kGAColumn + 64u * ap.slot + 8u * pair;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const __half2 sb = *reinterpret_cast<const __half2*>(&p[32 * j / G]);
+                    uint32_t v[8];
+                    decode8(w0[j], __low2half2(sb), __high2half2(sb), v);
+                    decode8(w1[j], __low2half2(sb), __high2half2(sb), v + 4);
+                    tc::tmem_st8(to + 16u * j, v);
+                }
+                tc::tmem_wait_st();
+                tc::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) {
+                    tc::mbar_arrive(&S.afull[ap.slot]);
+                    tc::mbar_arrive(&S.rawfree[rp.slot]);
+                }
+            }
+            // (a CTA's last job is written out by its decoders, who have nothing else left. They see every job's sums
+            // complete, one job late, which costs nothing: a wait two phases behind its barrier would return at once)
+            if (ok && job != int(blockIdx.x)) ok = wait(&S.dfull[last.slot], last.phase);
+            last = dp;
+            if (!ok || job + int(gridDim.x) < jobs) continue;
+            if (!(ok = wait(&S.dfull[dp.slot], dp.phase))) break;
+            pdl_wait();  // before an output
+            write_out(job, dp.slot, 8 * (warp >> 2), 8 * (kGDecoders / 4));
+        }
+    }
+    if (!ok && lane == 0) atomicExch(&g_q4_gemm_status, SMOE_ETIMEOUT);
+    pdl_wait();
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    pdl_release();
+    if (warp == kGDecoders) tc::tmem_dealloc(tmem, 512);
+}
+
+// ---- host
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// cuTensorMapEncodeTiled through the runtime's driver entry point (no link against libcuda)
+static EncodeTiledFn encoder() {
+    static std::once_flag once;
+    static EncodeTiledFn encode = nullptr;
+    std::call_once(once, [] {
+        void* fn = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            encode = reinterpret_cast<EncodeTiledFn>(fn);
+    });
+    return encode;
+}
+
+// Microseconds of the prompt's kernel with jobs of n tokens, as measured: a start, and for every round of jobs over the SMs
+// a stage's 0.45 us (its hand-offs and decoding) or 4.5 ns a token (its MMAs), whichever is longer, and 1 us at its ends.
+// (64007 x 2560: 48 us at 33 tokens; 4096 x 4096: 17 us at 33, 40 us at 1180; 1024 x 1024: 6.5 us at 33.)
+static double time_of(int64_t tokens, int64_t rows, int64_t cols, int n) {
+    const int64_t jobs = (tokens + n - 1) / n * ((rows + kGM - 1) / kGM);
+    const double stage = std::max(0.45, 0.0045 * n);
+    return 4.0 + double((jobs + kSms - 1) / kSms) * (double(tiles_of_cols(cols)) * stage + 1.0);
+}
+
+static int tokens_of_job(int64_t tokens, int64_t rows, int64_t cols) {
+    int best = 16;
+    for (int n = 32; n <= kGMaxN; n += 16)
+        if (time_of(tokens, rows, cols, n) < time_of(tokens, rows, cols, best)) best = n;
+    return best;
+}
+
+// The streaming kernel takes 3 us, and for every 8 tokens 0.3 us and 0.125 ps a weight (64007 x 2560: 27 us at 8 tokens, 48
+// at 16, 67 at 24; 4096 x 4096: 6, 8 and 13; 1024 x 1024: 18 at 256); up to 16 tokens are always its (a verify window's token then has the bits it has
+// alone).
+bool matmul_better(int64_t tokens, int64_t rows, int64_t cols) {
+    if (tokens <= 16) return false;
+    const double stream = 3.0 + double((tokens + 7) / 8) * (0.3 + double(rows) * double(cols) * 1.25e-7);
+    return time_of(tokens, rows, cols, tokens_of_job(tokens, rows, cols)) < stream;
+}
+
+template <int G>
+static int launch_gemm(GemmArgs a, const GemmMaps& maps, const Writes& w, cudaStream_t st) {
+    // (the copies' latency is what the rings hide: a stage of weights is 9 KB and some 0.2 us of work, so as many as fit
+    // beside three stages of activations, then more of those)
+    a.nr = kGMaxRaw;
+    a.nb = 3;
+    while (a.nb > 2 && gemm_smem<G>(a.n, a.nb, 4) > kGSmemLimit) --a.nb;
+    // (an even number: the two groups of decoders then wait for slots of their own, every phase in turn)
+    while (a.nr > 4 && gemm_smem<G>(a.n, a.nb, a.nr) > kGSmemLimit) a.nr -= 2;
+    while (a.nb < kGMaxB && gemm_smem<G>(a.n, a.nb + 1, a.nr) <= kGSmemLimit) ++a.nb;
+    const size_t smem = gemm_smem<G>(a.n, a.nb, a.nr);
+    if (int e = max_smem(q4_matmul_kernel<G>, static_cast<int>(smem))) return status_of(static_cast<cudaError_t>(-e), "q4_matmul");
+    const int64_t jobs = int64_t(a.nblocks) * a.mblocks;
+    return status_of(launch_pdl(w, q4_matmul_kernel<G>, dim3(static_cast<unsigned>(std::min<int64_t>(jobs, kSms))),
+                                dim3(kGThreads), smem, st, a, maps), "q4_matmul");
+}
+
+int matmul_f16(const ProductArgs& p, int group, const Writes& w, cudaStream_t st) {
+    GemmArgs a = {};
+    a.w = p.dw[0];
+    a.out = static_cast<__half*>(p.d_out);
+    a.rows = p.d_rows;
+    a.cols = p.cols;
+    a.tokens = p.d_tokens;
+    a.early = p.early;
+    a.mblocks = static_cast<int>((p.d_rows + kGM - 1) / kGM);
+    a.n = tokens_of_job(p.d_tokens, p.d_rows, p.cols);
+    a.nblocks = static_cast<int>((p.d_tokens + a.n - 1) / a.n);
+    EncodeTiledFn encode = encoder();
+    if (!encode) return fail(SMOE_EARG, "q4_product: cuTensorMapEncodeTiled is not available");
+    GemmMaps maps;
+    const cuuint32_t one[2] = {1, 1};
+    {
+        const int64_t tile = tile_bytes_of(group), strip_bytes = tiles_of_cols(p.cols) * tile;
+        const cuuint64_t dims[2] = {static_cast<cuuint64_t>(strip_bytes / 8), static_cast<cuuint64_t>(strips_of_rows(p.d_rows))};
+        const cuuint64_t strides[1] = {static_cast<cuuint64_t>(strip_bytes)};
+        const cuuint32_t box[2] = {static_cast<cuuint32_t>(tile / 8), kGStrips};
+        const CUresult r = encode(&maps.w, CU_TENSOR_MAP_DATA_TYPE_INT64, 2, const_cast<uint8_t*>(p.dw[0]), dims, strides, box,
+                                  one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (r != CUDA_SUCCESS)
+            return fail(SMOE_EARG, "q4_product: weight tensor map rejected (" + std::to_string(int(r)) + ")");
+    }
+    for (int b = 0; b < 4; ++b) {
+        // (rows past the tokens and columns past the last read as zeros)
+        const cuuint64_t dims[2] = {static_cast<cuuint64_t>(p.cols), static_cast<cuuint64_t>(p.d_tokens)};
+        const cuuint64_t strides[1] = {static_cast<cuuint64_t>(p.cols) * 2};
+        const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(16 << b)};
+        const CUresult r = encode(&maps.a[b], CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(p.x), dims, strides, box,
+                                  one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (r != CUDA_SUCCESS)
+            return fail(SMOE_EARG, "q4_product: activation tensor map rejected (" + std::to_string(int(r)) + ")");
+    }
+    if (group == 32) return launch_gemm<32>(a, maps, w, st);
+    if (group == 64) return launch_gemm<64>(a, maps, w, st);
+    return launch_gemm<128>(a, maps, w, st);
+}
+
+cudaError_t matmul_status(int* v, bool clear) {
+    cudaError_t e = cudaMemcpyFromSymbol(v, g_q4_gemm_status, sizeof(int));
+    if (e == cudaSuccess && clear) {
+        const int zero = 0;
+        e = cudaMemcpyToSymbol(g_q4_gemm_status, &zero, sizeof(int));
+    }
+    return e;
+}
+
+}  // namespace q4
+}  // namespace smoe

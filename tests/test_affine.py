@@ -101,12 +101,12 @@ def test_the_moe_block_checks_its_arguments(lib, kw, code):
 
 
 def test_the_moe_block_checks_its_workspace(lib):
-    need = lib.smoe_q4_moe_workspace_size(1, 2, 2, 128, 64, 64)
+    need = lib.smoe_q4_moe_workspace_size(2, 2, 128, 64, 64)
     assert need >= (4 + 2) * 64 * 2
     assert lib.smoe_q4_moe(_moe(), None, need, None) == EWORKSPACE
     assert lib.smoe_q4_moe(_moe(), A, need - 1, None) == EWORKSPACE
     assert lib.smoe_q4_moe(_moe(), A + 4, need, None) == EWORKSPACE
-    assert lib.smoe_q4_moe_workspace_size(1, 0, 2, 128, 64, 64) == 0
+    assert lib.smoe_q4_moe_workspace_size(0, 2, 128, 64, 64) == 0
 
 
 def test_there_is_no_cpu_path():
