@@ -14,12 +14,12 @@
 // A row's 16 code words of a tile: word j of chunk t (four chunks of 16 bytes) holds the codes of columns 32 j + 8 t ..
 // + 7, so that lane (g, t) of a warp (g = lane / 4, t = lane % 4) has its columns of all four 32-column runs in one
 // 16-byte read. Chunk t of row r lies at place t ^ (r / 2 % 4): eight rows' chunks t are on eight different bank groups
-// (a thread a row reads so in the prompt's product). In a word, columns 0 .. 7 lie in nibbles 0, 4, 1, 5, 2, 6, 3, 7: the
+// (a thread a row reads so in the prompt's product). In a word, columns 0 .. 7 lie in nibbles 0, 4, 2, 6, 1, 5, 3, 7: the
 // nibbles under one mask, 16 bits apart, are neighbouring columns.
 //
 // Arithmetic. A run of 32 columns is two m16n8k16 MMAs, rows the M side, activation rows the N side. The order of
-// columns inside an MMA is free as long as A and B agree, so lane (g, t)'s word goes in as it lies: columns 0, 1 and 4,
-// 5 to one MMA, 2, 3 and 6, 7 to the other. With float16 activations a nibble needs no conversion at all: (word &
+// columns inside an MMA is free as long as A and B agree, so lane (g, t)'s word goes in as it lies: columns 0 .. 3 to
+// one MMA, 4 .. 7 to the other (so that B's register pairs are halves of a 16-byte load). With float16 activations a nibble needs no conversion at all: (word &
 // 0x000f000f) is a pair of float16 subnormals q * 2^-24, exact in the tensor core, and (word & 0x00f000f0) a pair of 16
 // q * 2^-24; the two MMAs keep sums of their own, joined as lo + hi / 16 at the end of the group, and the 2^24 comes at
 // the end of the row. Products are exact and sums are float32: the result is the formula's but for float32 rounding.
@@ -56,17 +56,19 @@ __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity) { retur
 // Where a row's chunk t lies in a tile, in bytes; lane (g, t)'s chunk of row g (that of row g + 8 lies 512 further)
 __host__ __device__ constexpr int chunk_at(int row, int t) { return row * 64 + ((t ^ ((row >> 1) & 3)) << 4); }
 __device__ __forceinline__ int lane_chunk(int lane) { return chunk_at(lane >> 2, lane & 3); }
+// The nibble of a word that holds its column i
+__host__ __device__ constexpr int nibble_of(int i) { return (i >> 2) + 2 * ((i >> 1) & 1) + 4 * (i & 1); }
 // A word of eight codes, weight i in bits 4 i, in the layout's order of nibbles, and back
 __device__ __forceinline__ uint32_t nibbles_in(uint32_t w) {
     uint32_t r = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r |= ((w >> (4 * i)) & 15u) << (4 * ((i >> 1) + 4 * (i & 1)));
+    for (int i = 0; i < 8; ++i) r |= ((w >> (4 * i)) & 15u) << (4 * nibble_of(i));
     return r;
 }
 __device__ __forceinline__ uint32_t nibbles_out(uint32_t w) {
     uint32_t r = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r |= ((w >> (4 * ((i >> 1) + 4 * (i & 1)))) & 15u) << (4 * i);
+    for (int i = 0; i < 8; ++i) r |= ((w >> (4 * nibble_of(i))) & 15u) << (4 * i);
     return r;
 }
 
@@ -194,24 +196,35 @@ struct Acts<float> {
     }
 };
 
+// The matrix of ones (times 2^-24 for float16) as an A operand. Made by volatile moves: a constant would be moved into the
+// operand's four registers again for every MMA.
+template <typename T>
+struct Ones {
+    uint32_t v[4];
+    __device__ __forceinline__ Ones() {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) asm volatile("mov.b32 %0, %1;" : "=r"(v[i]) : "n"(Codes<T>::kOne));
+    }
+};
+
 // The sums of one group of columns of MT strips times a block of 8 activation rows: codes in lo and hi (float16: hi
 // holds 16 times its sum, both 2^-24 times theirs; float32: lo alone), the activations alone in on (times 2^-24 too).
 template <typename T, int MT>
 struct Sums {
-    float lo[MT][4], hi[MT][4], on[4];
+    float lo[MT][4], hi[MT][4], on[4], on2[4];  // (on2: half of the activations, to halve the chain of MMAs)
 };
 
 template <bool FIRST, int MT>
-__device__ __forceinline__ void run_mma(const Codes<__half> (&a)[MT], const Acts<__half>& x, Sums<__half, MT>& s) {
-    const uint32_t b0 = x.v.x, b1 = x.v.z, c0 = x.v.y, c1 = x.v.w;
-    constexpr uint32_t one = Codes<__half>::kOne;
+__device__ __forceinline__ void run_mma(const Codes<__half> (&a)[MT], const Acts<__half>& x, Sums<__half, MT>& s,
+                                        const Ones<__half>& one) {
+    const uint32_t b0 = x.v.x, b1 = x.v.y, c0 = x.v.z, c1 = x.v.w;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
         mma_f16<FIRST>(s.lo[m], a[m].lo[0], a[m].lo[1], a[m].lo[2], a[m].lo[3], b0, b1);
         mma_f16<FIRST>(s.hi[m], a[m].hi[0], a[m].hi[1], a[m].hi[2], a[m].hi[3], c0, c1);
     }
-    mma_f16<FIRST>(s.on, one, one, one, one, b0, b1);
-    mma_f16<false>(s.on, one, one, one, one, c0, c1);
+    mma_f16<FIRST>(s.on, one.v[0], one.v[1], one.v[2], one.v[3], b0, b1);
+    mma_f16<FIRST>(s.on2, one.v[0], one.v[1], one.v[2], one.v[3], c0, c1);
 }
 
 __device__ __forceinline__ uint32_t bf16_pair(float& a, float& b) {
@@ -224,21 +237,21 @@ __device__ __forceinline__ uint32_t bf16_pair(float& a, float& b) {
 }
 
 template <bool FIRST, int MT>
-__device__ __forceinline__ void run_mma(const Codes<float> (&a)[MT], const Acts<float>& x, Sums<float, MT>& s) {
+__device__ __forceinline__ void run_mma(const Codes<float> (&a)[MT], const Acts<float>& x, Sums<float, MT>& s,
+                                        const Ones<float>& one) {
     float f[8] = {__uint_as_float(x.v.x), __uint_as_float(x.v.y), __uint_as_float(x.v.z), __uint_as_float(x.v.w),
                   __uint_as_float(x.w.x), __uint_as_float(x.w.y), __uint_as_float(x.w.z), __uint_as_float(x.w.w)};
-    constexpr uint32_t one = Codes<float>::kOne;
     auto piece = [&](auto first) {
         constexpr bool kFirst = decltype(first)::value;
-        const uint32_t b0 = bf16_pair(f[0], f[1]), b1 = bf16_pair(f[4], f[5]);
-        const uint32_t c0 = bf16_pair(f[2], f[3]), c1 = bf16_pair(f[6], f[7]);
+        const uint32_t b0 = bf16_pair(f[0], f[1]), b1 = bf16_pair(f[2], f[3]);
+        const uint32_t c0 = bf16_pair(f[4], f[5]), c1 = bf16_pair(f[6], f[7]);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
             mma_bf16<kFirst>(s.lo[m], a[m].lo[0], a[m].lo[1], a[m].lo[2], a[m].lo[3], b0, b1);
             mma_bf16<false>(s.lo[m], a[m].hi[0], a[m].hi[1], a[m].hi[2], a[m].hi[3], c0, c1);
         }
-        mma_bf16<kFirst>(s.on, one, one, one, one, b0, b1);
-        mma_bf16<false>(s.on, one, one, one, one, c0, c1);
+        mma_bf16<kFirst>(s.on, one.v[0], one.v[1], one.v[2], one.v[3], b0, b1);
+        mma_bf16<kFirst>(s.on2, one.v[0], one.v[1], one.v[2], one.v[3], c0, c1);
     };
     piece(std::integral_constant<bool, FIRST>{});
     piece(std::false_type{});
@@ -254,10 +267,11 @@ template <typename T, int MT>
 __device__ __forceinline__ void group_end(float (&acc)[4], const Sums<T, MT>& s, int m, uint32_t sb0, uint32_t sb1) {
     const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&sb0));
     const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&sb1));
+    const float on[2] = {s.on[0] + s.on2[0], s.on[1] + s.on2[1]};  // (the same for both rows)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float q = sizeof(T) == 2 ? fmaf(s.hi[m][i], 0.0625f, s.lo[m][i]) : s.lo[m][i];
-        acc[i] = fmaf(q, i < 2 ? p.x : r.x, fmaf(s.on[i], i < 2 ? p.y : r.y, acc[i]));
+        acc[i] = fmaf(q, i < 2 ? p.x : r.x, fmaf(on[i & 1], i < 2 ? p.y : r.y, acc[i]));
     }
 }
 
@@ -300,7 +314,7 @@ struct TileActs<float> {
 // One tile of two strips (shared memory, `stride` bytes apart) times a block of 8 activation rows.
 template <typename T, int G>
 __device__ __forceinline__ void tile_mma(const uint8_t* tile, int stride, int lane, const TileActs<T>& x,
-                                         float (&acc)[2][4]) {
+                                         float (&acc)[2][4], const Ones<T>& one) {
     constexpr int kRuns = G / 32, kPairs = kCols / G;
     uint32_t wa[2][4], wb[2][4];
 #pragma unroll
@@ -319,8 +333,8 @@ __device__ __forceinline__ void tile_mma(const uint8_t* tile, int stride, int la
         for (int r = 0; r < kRuns; ++r) {
             const int j = gi * kRuns + r;
             const Codes<T> a[2] = {Codes<T>(wa[0][j], wb[0][j]), Codes<T>(wa[1][j], wb[1][j])};
-            if (r == 0) run_mma<true, 2>(a, x.run(j), s);
-            else run_mma<false, 2>(a, x.run(j), s);
+            if (r == 0) run_mma<true, 2>(a, x.run(j), s, one);
+            else run_mma<false, 2>(a, x.run(j), s, one);
         }
 #pragma unroll
         for (int m = 0; m < 2; ++m) {

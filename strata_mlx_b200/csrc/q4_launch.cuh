@@ -10,7 +10,7 @@ namespace smoe {
 namespace q4 {
 
 constexpr int kSms = 148;
-constexpr int kCtasPerSm = 2;
+constexpr int kCtasPerSm = QCTAS;
 constexpr int kDownCtas = kSms * kCtasPerSm;
 
 int product_f16(const ProductArgs& a, int group, const Writes& w, cudaStream_t st);

@@ -242,8 +242,13 @@ __device__ __forceinline__ PairBlocks pair_blocks(uint8_t* mem, const uint32_t* 
 }
 
 constexpr int kMt = 2;      // strips whose tiles are multiplied together: gate and up, or two neighbours of one matrix
-constexpr int kStep = 2;    // tiles of a stage
-constexpr int kStages = 2;  // slots of a warp's ring
+#ifndef QSTEP
+#define QSTEP 2
+#define QSTAGES 2
+#define QCTAS 2
+#endif
+constexpr int kStep = QSTEP;    // tiles of a stage
+constexpr int kStages = QSTAGES;  // slots of a warp's ring
 constexpr int kM = 8;       // rows of activations in a block
 template <int G>
 __host__ __device__ constexpr int slot_bytes() {
@@ -262,7 +267,7 @@ __device__ __forceinline__ float sigmoid_f(float g) { return 1.0f / (1.0f + expf
 
 // GLU: the two strips of a job are gate's and up's, else two neighbours.
 template <typename T, int G, bool GLU>
-__global__ void __launch_bounds__(kThreads, 2) q4_product_kernel(const ProductArgs a) {
+__global__ void __launch_bounds__(kThreads, QCTAS) q4_product_kernel(const ProductArgs a) {
     constexpr int kTile = tile_bytes<G>();
     constexpr int kSlot = slot_bytes<G>();
     constexpr int kWide = GLU ? 1 : 2;  // strips of the result in a job
@@ -350,6 +355,7 @@ __global__ void __launch_bounds__(kThreads, 2) q4_product_kernel(const ProductAr
             for (int i = tid; i < a.n_zero; i += kThreads) a.zero[i] = 0;
     }
 
+    const Ones<T> one;
     const T* x = static_cast<const T*>(a.x);
     const int col_runs = static_cast<int>(a.cols / 32);
     int parity = 0;
@@ -368,10 +374,14 @@ __global__ void __launch_bounds__(kThreads, 2) q4_product_kernel(const ProductAr
             // (a tile's activations before its weights are waited for: both latencies pass together)
             const TileActs<T> x0(xp + tile * kCols, col_runs - 4 * tile);
             const uint8_t* slot = ring.wait(lane);
-            const bool more = tile + 1 < tile1;
-            const TileActs<T> x1(xp + (tile + 1) * kCols, more ? col_runs - 4 * (tile + 1) : 0);
-            tile_mma<T, G>(slot, kStep * kTile, lane, x0, acc);
-            if (more) tile_mma<T, G>(slot + kTile, kStep * kTile, lane, x1, acc);
+            const bool more = kStep > 1 && tile + 1 < tile1;
+            if constexpr (kStep > 1) {
+                const TileActs<T> x1(xp + (tile + 1) * kCols, more ? col_runs - 4 * (tile + 1) : 0);
+                tile_mma<T, G>(slot, kStep * kTile, lane, x0, acc, one);
+                if (more) tile_mma<T, G>(slot + kTile, kStep * kTile, lane, x1, acc, one);
+            } else {
+                tile_mma<T, G>(slot, kStep * kTile, lane, x0, acc, one);
+            }
             __syncwarp();
             ring.pop();
             fetch();
@@ -444,7 +454,7 @@ __host__ __device__ constexpr size_t down_smem(int64_t tokens, int64_t pairs, in
 }
 
 template <typename T, int G>
-__global__ void __launch_bounds__(kThreads, 2) q4_down_kernel(const DownArgs a) {
+__global__ void __launch_bounds__(kThreads, QCTAS) q4_down_kernel(const DownArgs a) {
     constexpr int kTile = tile_bytes<G>();
     constexpr int kSlot = slot_bytes<G>();
     constexpr int kRowsIn = down_rows<T>(), kPieces = kM / kRowsIn;
@@ -550,6 +560,7 @@ __global__ void __launch_bounds__(kThreads, 2) q4_down_kernel(const DownArgs a) 
     for (int i = 0; i < kStages; ++i) fetch();
     pdl_wait();
 
+    const Ones<T> one;
     for (int job = job_first; job < job_last; ++job) {
         for (int i = lane; i < tokens * kTokenStride; i += 32) mine[i] = 0.0f;
         __syncwarp();
@@ -572,9 +583,13 @@ __global__ void __launch_bounds__(kThreads, 2) q4_down_kernel(const DownArgs a) 
             const int n = stage_of(c);
             const TileActs<T> x0(xp + c.tile * kCols, runs - 4 * c.tile);
             const uint8_t* slot = ring.wait(lane);
-            const TileActs<T> x1(xp + (c.tile + 1) * kCols, n > 1 ? runs - 4 * (c.tile + 1) : 0);
-            tile_mma<T, G>(slot, kStep * kTile, lane, x0, acc);
-            if (n > 1) tile_mma<T, G>(slot + kTile, kStep * kTile, lane, x1, acc);
+            if constexpr (kStep > 1) {
+                const TileActs<T> x1(xp + (c.tile + 1) * kCols, n > 1 ? runs - 4 * (c.tile + 1) : 0);
+                tile_mma<T, G>(slot, kStep * kTile, lane, x0, acc, one);
+                if (n > 1) tile_mma<T, G>(slot + kTile, kStep * kTile, lane, x1, acc, one);
+            } else {
+                tile_mma<T, G>(slot, kStep * kTile, lane, x0, acc, one);
+            }
             __syncwarp();
             ring.pop();
             fetch();

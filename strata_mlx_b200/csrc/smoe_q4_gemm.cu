@@ -98,7 +98,7 @@ __device__ __forceinline__ void decode8(uint32_t word, __half2 s, __half2 b, uin
     for (int i = 0; i < 4; ++i) {
         const uint32_t v = ((word >> (4 * i)) & 0x000f000fu) | 0x64006400u;
         const __half2 w = __hfma2(__hsub2(*reinterpret_cast<const __half2*>(&v), base), s, b);
-        out[i] = *reinterpret_cast<const uint32_t*>(&w);
+        out[(i >> 1) + 2 * (i & 1)] = *reinterpret_cast<const uint32_t*>(&w);  // nibbles i and i + 4 of the word
     }
 }
 
