@@ -87,6 +87,14 @@ __device__ __forceinline__ void load_pairs(const uint8_t* tile, int row, uint32_
     }
 }
 
+// One lane of a converged warp (a branch on it costs less than one on a lane's number: the copies and MMAs behind it take
+// their operands from the uniform datapath)
+__device__ __forceinline__ bool elect_one() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(e));
+    return e != 0;
+}
+
 // Bulk copy of `bytes` (a multiple of 16, both addresses 16-byte aligned) of this GPU's memory into this CTA's
 // shared memory, completing on `bar`.
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -283,7 +291,8 @@ template <typename T> struct TileActs;
 template <>
 struct TileActs<__half> {
     Acts<__half> x[4];
-    __device__ __forceinline__ TileActs(const __half* p, int runs) {
+    __device__ __forceinline__ TileActs(const __half* p, int runs) { load(p, runs); }
+    __device__ __forceinline__ void load(const __half* p, int runs) {
         if (runs >= 4) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) x[j].load(p + 32 * j);
@@ -303,6 +312,7 @@ struct TileActs<float> {
     const float* p;
     int runs;
     __device__ __forceinline__ TileActs(const float* at, int n) : p(at), runs(n) {}
+    __device__ __forceinline__ void load(const float* at, int n) { p = at, runs = n; }
     __device__ __forceinline__ Acts<float> run(int j) const {
         Acts<float> x;
         if (j < runs) x.load(p + 32 * j);

@@ -10,8 +10,7 @@ namespace smoe {
 namespace q4 {
 
 constexpr int kSms = 148;
-constexpr int kCtasPerSm = QCTAS;
-constexpr int kDownCtas = kSms * kCtasPerSm;
+constexpr int kDownCtas = kSms * kCtas;
 
 int product_f16(const ProductArgs& a, int group, const Writes& w, cudaStream_t st);
 int product_f32(const ProductArgs& a, int group, const Writes& w, cudaStream_t st);
@@ -48,7 +47,7 @@ inline int team_for(int64_t jobs, int64_t tiles) {
     int best = 1;
     int64_t least = 0;
     for (int w = 1; w <= kWarps; w *= 2) {
-        const int64_t teams = int64_t(kSms) * kCtasPerSm * kWarps / w;
+        const int64_t teams = int64_t(kSms) * kCtas * kWarps / w;
         const int64_t work = (jobs + teams - 1) / teams * ((tiles + w - 1) / w + 2);
         if (w == 1 || work < least) {
             best = w;
@@ -68,10 +67,9 @@ inline int launch_product(const ProductArgs& args, const Writes& w, cudaStream_t
     a.team = team_for(a.pairs > 0 ? jobs : d_wide, tiles_of_cols(a.cols));
     const size_t smem = product_smem<G>(a.pairs, a.experts);
     if (int e = max_smem(q4_product_kernel<T, G, GLU>, static_cast<int>(smem))) return status_of(static_cast<cudaError_t>(-e), "q4_product");
-    const int64_t ctas = std::min<int64_t>((jobs * a.team + kWarps - 1) / kWarps, kSms * kCtasPerSm);
-    // (few jobs: a team on an SM of its own before two on one)
-    const int64_t spread = std::max<int64_t>(ctas, std::min<int64_t>(jobs, kSms));
-    return status_of(launch_pdl(w, q4_product_kernel<T, G, GLU>, dim3(static_cast<unsigned>(spread)), dim3(kThreads), smem,
+    // (a team's CTA of its own while there are slots for it: the teams spread evenly over the SMs)
+    const int64_t ctas = std::min<int64_t>(jobs, kSms * kCtas);
+    return status_of(launch_pdl(w, q4_product_kernel<T, G, GLU>, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), smem,
                                 st, a), "q4_product");
 }
 

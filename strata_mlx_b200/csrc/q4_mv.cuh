@@ -242,13 +242,9 @@ __device__ __forceinline__ PairBlocks pair_blocks(uint8_t* mem, const uint32_t* 
 }
 
 constexpr int kMt = 2;      // strips whose tiles are multiplied together: gate and up, or two neighbours of one matrix
-#ifndef QSTEP
-#define QSTEP 2
-#define QSTAGES 2
-#define QCTAS 2
-#endif
-constexpr int kStep = QSTEP;    // tiles of a stage
-constexpr int kStages = QSTAGES;  // slots of a warp's ring
+constexpr int kStep = 2;    // tiles of a stage
+constexpr int kStages = 2;  // slots of a warp's ring
+constexpr int kCtas = 2;    // CTAs of an SM
 constexpr int kM = 8;       // rows of activations in a block
 template <int G>
 __host__ __device__ constexpr int slot_bytes() {
@@ -267,7 +263,7 @@ __device__ __forceinline__ float sigmoid_f(float g) { return 1.0f / (1.0f + expf
 
 // GLU: the two strips of a job are gate's and up's, else two neighbours.
 template <typename T, int G, bool GLU>
-__global__ void __launch_bounds__(kThreads, QCTAS) q4_product_kernel(const ProductArgs a) {
+__global__ void __launch_bounds__(kThreads, kCtas) q4_product_kernel(const ProductArgs a) {
     constexpr int kTile = tile_bytes<G>();
     constexpr int kSlot = slot_bytes<G>();
     constexpr int kWide = GLU ? 1 : 2;  // strips of the result in a job
@@ -325,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, QCTAS) q4_product_kernel(const Produ
             }
         }
         const uint32_t bytes = fetch_step + 1 < steps ? kStep * kTile : (tile1 - tile0 - fetch_step * kStep) * kTile;
-        if (lane == 0) {
+        if (elect_one()) {
             uint64_t* bar = &ring.bars[ring.head];
             tc::mbar_arrive_expect_tx(bar, bytes * kMt);
 #pragma unroll
@@ -369,18 +365,16 @@ __global__ void __launch_bounds__(kThreads, QCTAS) q4_product_kernel(const Produ
         const int at = g < count ? start + g : start;
         const T* xp = x + (dense ? int64_t(at) : int64_t(blocks.list[at]) / a.share) * a.cols + 8 * t;
         float acc[kMt][4] = {};
-        for (int s = 0; s < steps; ++s) {
-            const int tile = tile0 + s * kStep;
-            // (a tile's activations before its weights are waited for: both latencies pass together)
-            const TileActs<T> x0(xp + tile * kCols, col_runs - 4 * tile);
+        // (a tile's activations are loaded a tile ahead: their latency passes during the one before)
+        TileActs<T> x0(xp + tile0 * kCols, steps > 0 ? col_runs - 4 * tile0 : 0);
+        for (int tile = tile0; tile < tile1; tile += kStep) {
             const uint8_t* slot = ring.wait(lane);
-            const bool more = kStep > 1 && tile + 1 < tile1;
-            if constexpr (kStep > 1) {
-                const TileActs<T> x1(xp + (tile + 1) * kCols, more ? col_runs - 4 * (tile + 1) : 0);
-                tile_mma<T, G>(slot, kStep * kTile, lane, x0, acc, one);
-                if (more) tile_mma<T, G>(slot + kTile, kStep * kTile, lane, x1, acc, one);
-            } else {
-                tile_mma<T, G>(slot, kStep * kTile, lane, x0, acc, one);
+            const bool more = tile + 1 < tile1;
+            const TileActs<T> x1(xp + (tile + 1) * kCols, more ? col_runs - 4 * (tile + 1) : 0);
+            tile_mma<T, G>(slot, kStep * kTile, lane, x0, acc, one);
+            if (more) {
+                x0.load(xp + (tile + 2) * kCols, tile + 2 < tile1 ? col_runs - 4 * (tile + 2) : 0);
+                tile_mma<T, G>(slot + kTile, kStep * kTile, lane, x1, acc, one);
             }
             __syncwarp();
             ring.pop();
@@ -454,7 +448,7 @@ __host__ __device__ constexpr size_t down_smem(int64_t tokens, int64_t pairs, in
 }
 
 template <typename T, int G>
-__global__ void __launch_bounds__(kThreads, QCTAS) q4_down_kernel(const DownArgs a) {
+__global__ void __launch_bounds__(kThreads, kCtas) q4_down_kernel(const DownArgs a) {
     constexpr int kTile = tile_bytes<G>();
     constexpr int kSlot = slot_bytes<G>();
     constexpr int kRowsIn = down_rows<T>(), kPieces = kM / kRowsIn;
@@ -545,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, QCTAS) q4_down_kernel(const DownArgs
         }
         const int n = stage_of(fc);
         const uint32_t bytes = n * kTile;
-        if (lane == 0) {
+        if (elect_one()) {
             uint64_t* bar = &ring.bars[ring.head];
             tc::mbar_arrive_expect_tx(bar, bytes * kMt);
 #pragma unroll
@@ -583,13 +577,9 @@ __global__ void __launch_bounds__(kThreads, QCTAS) q4_down_kernel(const DownArgs
             const int n = stage_of(c);
             const TileActs<T> x0(xp + c.tile * kCols, runs - 4 * c.tile);
             const uint8_t* slot = ring.wait(lane);
-            if constexpr (kStep > 1) {
-                const TileActs<T> x1(xp + (c.tile + 1) * kCols, n > 1 ? runs - 4 * (c.tile + 1) : 0);
-                tile_mma<T, G>(slot, kStep * kTile, lane, x0, acc, one);
-                if (n > 1) tile_mma<T, G>(slot + kTile, kStep * kTile, lane, x1, acc, one);
-            } else {
-                tile_mma<T, G>(slot, kStep * kTile, lane, x0, acc, one);
-            }
+            const TileActs<T> x1(xp + (c.tile + 1) * kCols, n > 1 ? runs - 4 * (c.tile + 1) : 0);
+            tile_mma<T, G>(slot, kStep * kTile, lane, x0, acc, one);
+            if (n > 1) tile_mma<T, G>(slot + kTile, kStep * kTile, lane, x1, acc, one);
             __syncwarp();
             ring.pop();
             fetch();

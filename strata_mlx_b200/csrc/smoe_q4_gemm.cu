@@ -74,12 +74,6 @@ __host__ __device__ constexpr size_t gemm_smem(int n, int nb, int nr) {
     return size_t(nb) * b_slot_bytes(n) + size_t(nr) * raw_slot_bytes<G>() + sizeof(GemmSmem);
 }
 
-__device__ __forceinline__ bool elect_one() {
-    uint32_t e;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(e));
-    return e != 0;
-}
-
 struct Phase {
     int slot = 0;
     uint32_t phase = 0;
