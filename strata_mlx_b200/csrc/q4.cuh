@@ -95,15 +95,15 @@ __device__ __forceinline__ bool elect_one() {
     return e != 0;
 }
 
-// Bulk copy of `bytes` (a multiple of 16, both addresses 16-byte aligned) of this GPU's memory into this CTA's
-// shared memory, completing on `bar`.
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(dst),
-                 "l"(src), "r"(bytes), "r"(smem_addr(bar))
-                 : "memory");
+__device__ __forceinline__ uint64_t policy_evict_normal() {
+    uint64_t p;
+    asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(p));
+    return p;
 }
-__device__ __forceinline__ void bulk_load_hint(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar,
-                                               uint64_t policy) {
+
+// Bulk copy of `bytes` (a multiple of 16, both addresses 16-byte aligned) of this GPU's memory into this CTA's
+// shared memory, completing on `bar`, with an L2 cache policy.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar, uint64_t policy) {
     asm volatile(
         "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;\n" ::"r"(
             dst),

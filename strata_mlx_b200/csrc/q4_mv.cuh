@@ -67,56 +67,67 @@ struct DownArgs {
     bool early;          // idx and the weights may be read before pdl_wait()
 };
 
-// ---- a warp's ring of bulk copies
+// ---- a warp's ring of bulk copies: two slots, the copies' and the reader's counts say which
+
+constexpr int kStages = 2;  // slots
 
 struct Ring {
-    uint32_t base;    // shared address of slot 0
-    uint8_t* ptr;
+    uint8_t* slots;
     uint64_t* bars;
-    int slots, slot_bytes;
-    int head = 0, tail = 0;  // next slot to fill / to read
-    uint32_t phase = 0;
-    int in_flight = 0;
-    bool ok = true;
+    int slot_bytes;
+    uint32_t fetched = 0, taken = 0;
+    bool dead = false;  // a wait gave up: what follows is read as it lies, nothing more is fetched
 
-    __device__ __forceinline__ void init(uint8_t* p, uint64_t* b, int n, int bytes, int lane) {
-        ptr = p;
-        base = smem_addr(p);
+    __device__ __forceinline__ void init(uint8_t* p, uint64_t* b, int bytes, int lane) {
+        slots = p;
         bars = b;
-        slots = n;
         slot_bytes = bytes;
         if (lane == 0) {
-            for (int i = 0; i < n; ++i) tc::mbar_init(&bars[i], 1);
+            for (int i = 0; i < kStages; ++i) tc::mbar_init(&bars[i], 1);
             tc::fence_barrier_init();
         }
         __syncwarp();
     }
-    __device__ __forceinline__ bool full() const { return in_flight == slots; }
-    // the slot at the tail, once its copies have landed
-    __device__ __forceinline__ uint8_t* wait(int lane) {
-        if (ok) {
-            ok = __all_sync(0xffffffffu, wait_for(&bars[tail], phase));
-            if (!ok && lane == 0) atomicExch(&g_q4_status, SMOE_ETIMEOUT);
+    __device__ __forceinline__ bool full() const { return fetched - taken == kStages; }
+    // the next slot, once its copies have landed
+    __device__ __forceinline__ const uint8_t* wait(int lane) {
+        const uint32_t at = taken & 1, phase = (taken >> 1) & 1;
+        if (!__all_sync(0xffffffffu, tc::mbar_try_wait(&bars[at], phase))) {
+            if (!dead && !__all_sync(0xffffffffu, wait_for(&bars[at], phase))) {
+                dead = true;
+                if (lane == 0) atomicExch(&g_q4_status, SMOE_ETIMEOUT);
+            }
         }
-        return ptr + tail * slot_bytes;
+        return slots + at * slot_bytes;
     }
-    __device__ __forceinline__ void pop() {
-        if (!ok) return;  // (the slots not waited for are drained at the end)
-        --in_flight;
-        if (++tail == slots) tail = 0, phase ^= 1;
-    }
-    // lane 0 only for the copies; every lane keeps the cursor
-    __device__ __forceinline__ void push() {
-        ++in_flight;
-        if (++head == slots) head = 0;
+    // two copies of `bytes` into the next slot's halves (the whole warp calls, one lane issues)
+    __device__ __forceinline__ void fetch(const uint8_t* w0, const uint8_t* w1, uint32_t bytes, uint64_t policy) {
+        const uint32_t at = fetched & 1;
+        ++fetched;
+        if (elect_one()) {
+            uint64_t* bar = &bars[at];
+            const uint32_t dst = smem_addr(slots) + at * slot_bytes;
+            tc::mbar_arrive_expect_tx(bar, 2 * bytes);
+            bulk_load(dst, w0, bytes, bar, policy);
+            bulk_load(dst + slot_bytes / 2, w1, bytes, bar, policy);
+        }
     }
     // no copy may still be writing shared memory when the CTA leaves
     __device__ __forceinline__ void drain(int lane) {
-        ok = true;
-        while (in_flight > 0) {
-            if (!wait_for(&bars[tail], phase) && lane == 0) atomicExch(&g_q4_status, SMOE_ETIMEOUT);
-            pop();
-        }
+        for (uint32_t i = fetched < kStages ? 0 : fetched - kStages; i < fetched; ++i)
+            if (!wait_for(&bars[i & 1], (i >> 1) & 1) && lane == 0) atomicExch(&g_q4_status, SMOE_ETIMEOUT);
+    }
+};
+
+// Division of numbers from 0 to 2^31 - 1 by one that a kernel keeps
+struct Divisor {
+    uint32_t n, inverse;
+    __device__ __forceinline__ explicit Divisor(int by) : n(by), inverse(by > 1 ? 0xffffffffu / n : 0) {}
+    __device__ __forceinline__ int operator()(int a) const {
+        if (n == 1) return a;
+        uint32_t q = __umulhi(uint32_t(a), inverse);  // at most one too small: inverse is less than 1 below 2^32 / n
+        if (uint32_t(a) - q * n >= n) ++q;
+        return static_cast<int>(q);
     }
 };
 
@@ -242,10 +253,9 @@ __device__ __forceinline__ PairBlocks pair_blocks(uint8_t* mem, const uint32_t* 
 }
 
 constexpr int kMt = 2;      // strips whose tiles are multiplied together: gate and up, or two neighbours of one matrix
-constexpr int kStep = 2;    // tiles of a stage
-constexpr int kStages = 2;  // slots of a warp's ring
-constexpr int kCtas = 2;    // CTAs of an SM
-constexpr int kM = 8;       // rows of activations in a block
+constexpr int kStep = 2;  // tiles of a stage
+constexpr int kCtas = 2;  // CTAs of an SM
+constexpr int kM = 8;     // rows of activations in a block
 template <int G>
 __host__ __device__ constexpr int slot_bytes() {
     return kMt * kStep * tile_bytes<G>();
@@ -279,12 +289,12 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_product_kernel(const Produ
     uint64_t* bars = reinterpret_cast<uint64_t*>(table + pair_blocks_bytes(a.pairs, a.experts));
     red += team * a.team * 2 * kRedFloats;  // [job's parity][member][strip][row][column]
     Ring ring;
-    ring.init(smem + size_t(warp) * kStages * kSlot, bars + warp * kStages, kStages, kSlot, lane);
-    const uint64_t policy = tc::policy_evict_first();
+    ring.init(smem + size_t(warp) * kStages * kSlot, bars + warp * kStages, kSlot, lane);
+    // (weights of experts are read once; a layer's may be read again by its next block of tokens or its next call)
+    const uint64_t policy = a.hint ? tc::policy_evict_first() : policy_evict_normal();
 
     const int ntiles = static_cast<int>(tiles_of_cols(a.cols));
     const int tile0 = member * ntiles / a.team, tile1 = (member + 1) * ntiles / a.team;
-    const int steps = (tile1 - tile0 + kStep - 1) / kStep;
     const int64_t strip_bytes = int64_t(ntiles) * kTile;
     const int d_strips = static_cast<int>(strips_of_rows(a.d_rows)), r_strips = static_cast<int>(strips_of_rows(a.r_rows));
     const int d_wide = (d_strips + kWide - 1) / kWide, r_wide = (r_strips + kWide - 1) / kWide;
@@ -295,49 +305,43 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_product_kernel(const Produ
 
     // job -> strips (from kWide times the first) and block of rows; a strip's blocks are neighbours in time, so that the
     // second reads the strip from L2
+    const Divisor by_dense(max(1, d_blocks)), by_share(static_cast<int>(max(int64_t(1), a.share)));
+    Divisor by_blocks(1);
     auto place = [&](int j, int& strip, int& block) {
-        const int n = j < d_jobs ? d_blocks : blocks.n;
-        j = j < d_jobs ? j : j - d_jobs;
-        strip = j / n;
-        block = j - strip * n;
+        if (j < d_jobs) {
+            strip = by_dense(j);
+            block = j - strip * d_blocks;
+        } else {
+            j -= d_jobs;
+            strip = by_blocks(j);
+            block = j - strip * blocks.n;
+        }
     };
 
     // the copies' cursor: the next stage to fetch
-    int fetch_job = team_id, fetch_step = 0;
-    const uint8_t* fetch_w[kMt] = {};
+    int fetch_job = tile0 < tile1 ? team_id : 0x7fffffff, fetch_left = 0;
+    const uint8_t *fetch0 = nullptr, *fetch1 = nullptr;
     auto fetch = [&]() {  // (a slot is free)
-        if (fetch_job >= jobs || steps == 0 || !ring.ok) return;
-        if (fetch_step == 0) {
+        if (fetch_left == 0) {
+            if (fetch_job >= jobs || ring.dead) return;
             int strip, block;
             place(fetch_job, strip, block);
             const bool dense = fetch_job < d_jobs;
+            const int strips = dense ? d_strips : r_strips;
             const int64_t first = dense ? 0 : int64_t(blocks.expert[block]) * r_strips;
-#pragma unroll
-            for (int m = 0; m < kMt; ++m) {
-                const uint8_t* w = dense ? a.dw[GLU ? m : 0] : a.rw[GLU ? m : 0];
-                // (the last job of an odd number of strips takes its one strip twice)
-                const int s = GLU ? strip : min(2 * strip + m, (dense ? d_strips : r_strips) - 1);
-                fetch_w[m] = w + (first + s) * strip_bytes + int64_t(tile0) * kTile;
-            }
-        }
-        const uint32_t bytes = fetch_step + 1 < steps ? kStep * kTile : (tile1 - tile0 - fetch_step * kStep) * kTile;
-        if (elect_one()) {
-            uint64_t* bar = &ring.bars[ring.head];
-            tc::mbar_arrive_expect_tx(bar, bytes * kMt);
-#pragma unroll
-            for (int m = 0; m < kMt; ++m) {
-                const uint32_t dst = ring.base + ring.head * kSlot + m * kStep * kTile;
-                if (a.hint) bulk_load_hint(dst, fetch_w[m], bytes, bar, policy);
-                else bulk_load(dst, fetch_w[m], bytes, bar);
-            }
-        }
-        ring.push();
-#pragma unroll
-        for (int m = 0; m < kMt; ++m) fetch_w[m] += bytes;
-        if (++fetch_step == steps) {
-            fetch_step = 0;
+            const uint8_t* w0 = dense ? a.dw[0] : a.rw[0];
+            const uint8_t* w1 = !GLU ? w0 : dense ? a.dw[1] : a.rw[1];
+            fetch0 = w0 + (first + strip * kWide) * strip_bytes + tile0 * kTile;
+            // (the last job of an odd number of strips takes its one strip twice)
+            fetch1 = w1 + (first + (GLU ? strip : min(strip * 2 + 1, strips - 1))) * strip_bytes + tile0 * kTile;
+            fetch_left = tile1 - tile0;
             fetch_job += teams;
         }
+        const int n = min(kStep, fetch_left);
+        ring.fetch(fetch0, fetch1, n * kTile, policy);
+        fetch0 += n * kTile;
+        fetch1 += n * kTile;
+        fetch_left -= n;
     };
     if (!a.early) pdl_wait();
     // the dense part's weights, while the launch before still runs
@@ -346,14 +350,19 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_product_kernel(const Produ
     if (a.pairs > 0) {
         blocks = pair_blocks(table, a.idx, static_cast<int>(a.pairs), static_cast<int>(a.experts), kM, warp_sums);
         jobs = d_jobs + blocks.n * r_wide;
-        while (!ring.full() && fetch_job < jobs && steps > 0) fetch();
+        by_blocks = Divisor(max(1, blocks.n));
+        for (int i = 0; i < kStages; ++i)
+            if (!ring.full()) fetch();
         if (blockIdx.x == 0)
             for (int i = tid; i < a.n_zero; i += kThreads) a.zero[i] = 0;
     }
 
     const Ones<T> one;
-    const T* x = static_cast<const T*>(a.x);
-    const int col_runs = static_cast<int>(a.cols / 32);
+    const T* x = static_cast<const T*>(a.x) + 8 * t;
+    const int runs0 = static_cast<int>(a.cols / 32) - 4 * tile0;
+    // the thread's part of a job's results: a row, and every so many of its columns
+    constexpr int kOut = kWide * kRows;
+    const int out_r = lane & (kOut - 1), out_n = (member * 32 + lane) / kOut;
     int parity = 0;
     for (int job = team_id; job < jobs; job += teams, parity ^= 1) {
         const bool dense = job < d_jobs;
@@ -363,21 +372,21 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_product_kernel(const Produ
         const int count = dense ? static_cast<int>(min(int64_t(kM), a.d_tokens - start)) : blocks.count[block];
         // (columns past the count repeat the first row; their results are not written)
         const int at = g < count ? start + g : start;
-        const T* xp = x + (dense ? int64_t(at) : int64_t(blocks.list[at]) / a.share) * a.cols + 8 * t;
+        const T* xp = x + int64_t(dense ? at : by_share(blocks.list[at])) * a.cols + tile0 * kCols;
         float acc[kMt][4] = {};
         // (a tile's activations are loaded a tile ahead: their latency passes during the one before)
-        TileActs<T> x0(xp + tile0 * kCols, steps > 0 ? col_runs - 4 * tile0 : 0);
-        for (int tile = tile0; tile < tile1; tile += kStep) {
+        int left = tile1 - tile0, runs = runs0;
+        TileActs<T> x0(xp, left > 0 ? runs : 0);
+        for (; left > 0; left -= kStep, runs -= 4 * kStep, xp += kStep * kCols) {
             const uint8_t* slot = ring.wait(lane);
-            const bool more = tile + 1 < tile1;
-            const TileActs<T> x1(xp + (tile + 1) * kCols, more ? col_runs - 4 * (tile + 1) : 0);
+            const TileActs<T> x1(xp + kCols, left > 1 ? runs - 4 : 0);
             tile_mma<T, G>(slot, kStep * kTile, lane, x0, acc, one);
-            if (more) {
-                x0.load(xp + (tile + 2) * kCols, tile + 2 < tile1 ? col_runs - 4 * (tile + 2) : 0);
+            if (left > 1) {
+                x0.load(xp + 2 * kCols, left > 2 ? runs - 8 : 0);
                 tile_mma<T, G>(slot + kTile, kStep * kTile, lane, x1, acc, one);
             }
             __syncwarp();
-            ring.pop();
+            ++ring.taken;
             fetch();
         }
         // the team's sums, in the order of the column ranges (one barrier a job: the next job's sums have another place)
@@ -390,35 +399,37 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_product_kernel(const Produ
         if (a.team == 1) __syncwarp();
         else tc::named_barrier(1 + team, 32 * a.team);
         const int rows = static_cast<int>(dense ? a.d_rows : a.r_rows);
-        for (int i = member * 32 + lane; i < kWide * kRows * count; i += 32 * a.team) {
-            const int r = i & (kWide * kRows - 1), n = i / (kWide * kRows);
-            const int row = strip * kWide * kRows + r;
-            if (row >= rows) continue;
-            float v = 0.0f, u = 0.0f;
-            for (int w = 0; w < a.team; ++w) {
-                v += sums[(w * kMt * kRows + r) * kM + n];
-                if constexpr (GLU) u += sums[((w * kMt + 1) * kRows + r) * kM + n];
-            }
-            const int64_t to = dense ? start + n : blocks.list[start + n];
-            v *= unit<T>();
-            if constexpr (GLU) {
-                // silu(gate) up, times the row's share of the block's output: float32 up to the one rounding
-                v = v * sigmoid_f(v) * (u * unit<T>());
-                if (dense) {
-                    if (a.d_gate != nullptr) v *= sigmoid_f(to_f32(static_cast<const T*>(a.d_gate)[to]));
-                } else if (a.weights != nullptr) {
-                    v *= a.weights[to];
+        const int row = strip * kOut + out_r;
+        if (row < rows) {
+            T* out = static_cast<T*>(dense ? a.d_out : a.r_out) + row;
+            const float* from = sums + out_r * kM;
+            for (int n = out_n; n < count; n += 32 / kOut * a.team) {
+                float v = 0.0f, u = 0.0f;
+                for (int w = 0; w < a.team; ++w) {
+                    v += from[w * kRedFloats + n];
+                    if constexpr (GLU) u += from[w * kRedFloats + kRows * kM + n];
+                }
+                const int64_t to = dense ? start + n : blocks.list[start + n];
+                v *= unit<T>();
+                if constexpr (GLU) {
+                    // silu(gate) up, times the row's share of the block's output: float32 up to the one rounding
+                    v = v * sigmoid_f(v) * (u * unit<T>());
+                    if (dense) {
+                        if (a.d_gate != nullptr) v *= sigmoid_f(to_f32(static_cast<const T*>(a.d_gate)[to]));
+                    } else if (a.weights != nullptr) {
+                        v *= a.weights[to];
+                    }
+                }
+                const T first = from_f32<T>(v);
+                if (GLU && sizeof(T) == 2 && a.pieces) {
+                    out[2 * to * rows] = first;
+                    out[(2 * to + 1) * rows] = from_f32<T>(v - to_f32(first));
+                } else {
+                    out[to * rows] = first;
                 }
             }
-            T* out = static_cast<T*>(dense ? a.d_out : a.r_out);
-            const T first = from_f32<T>(v);
-            if (GLU && sizeof(T) == 2 && a.pieces) {
-                out[2 * to * rows + row] = first;
-                out[(2 * to + 1) * rows + row] = from_f32<T>(v - to_f32(first));
-            } else {
-                out[to * rows + row] = first;
-            }
         }
+        if (a.team == 1) __syncwarp();
     }
     pdl_release();
     ring.drain(lane);
@@ -464,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_down_kernel(const DownArgs
     uint8_t* table = reinterpret_cast<uint8_t*>(red + kWarps * tokens * kTokenStride);
     uint64_t* bars = reinterpret_cast<uint64_t*>(table + pair_blocks_bytes(pairs, a.experts));
     Ring ring;
-    ring.init(smem + size_t(warp) * kStages * kSlot, bars + warp * kStages, kStages, kSlot, lane);
+    ring.init(smem + size_t(warp) * kStages * kSlot, bars + warp * kStages, kSlot, lane);
     const uint64_t policy = tc::policy_evict_first();
     float* mine = red + warp * tokens * kTokenStride;
 
@@ -520,35 +531,26 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_down_kernel(const DownArgs
 
     int fetch_job = job_first, fetch_seg = -1;
     Cursor fc = job_first < job_last ? cursor_of(fetch_job) : Cursor{0, 0, 0, 0};
-    const uint8_t* fetch_w[kMt] = {};
+    const uint8_t *fetch0 = nullptr, *fetch1 = nullptr;
     auto fetch = [&]() {  // (a slot is free)
-        if (!ring.ok) return;
         while (fc.item >= fc.last) {
             if (fetch_job + 1 >= job_last) return;
             fc = cursor_of(++fetch_job);
             fetch_seg = -1;
         }
         if (fc.seg != fetch_seg) {
+            if (ring.dead) return;
             fetch_seg = fc.seg;
             const bool shared = fc.seg < sblocks;
             const int64_t strip_bytes = int64_t(shared ? stiles : ftiles) * kTile;
             const uint8_t* w = shared ? a.sw : a.w + int64_t(blocks.expert[fc.seg - sblocks]) * strips * strip_bytes;
-            w += int64_t(fc.tile) * kTile;
-            fetch_w[0] = w + (fetch_job * kMt) * strip_bytes;
-            fetch_w[1] = w + min(fetch_job * kMt + 1, strips - 1) * strip_bytes;
+            fetch0 = w + (fetch_job * kMt) * strip_bytes + fc.tile * kTile;
+            fetch1 = w + min(fetch_job * kMt + 1, strips - 1) * strip_bytes + fc.tile * kTile;
         }
         const int n = stage_of(fc);
-        const uint32_t bytes = n * kTile;
-        if (elect_one()) {
-            uint64_t* bar = &ring.bars[ring.head];
-            tc::mbar_arrive_expect_tx(bar, bytes * kMt);
-#pragma unroll
-            for (int m = 0; m < kMt; ++m)
-                bulk_load_hint(ring.base + ring.head * kSlot + m * kStep * kTile, fetch_w[m], bytes, bar, policy);
-        }
-        ring.push();
-#pragma unroll
-        for (int m = 0; m < kMt; ++m) fetch_w[m] += bytes;
+        ring.fetch(fetch0, fetch1, n * kTile, policy);
+        fetch0 += n * kTile;
+        fetch1 += n * kTile;
         advance(fc, n);
     };
     for (int i = 0; i < kStages; ++i) fetch();
@@ -581,7 +583,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_down_kernel(const DownArgs
             tile_mma<T, G>(slot, kStep * kTile, lane, x0, acc, one);
             if (n > 1) tile_mma<T, G>(slot + kTile, kStep * kTile, lane, x1, acc, one);
             __syncwarp();
-            ring.pop();
+            ++ring.taken;
             fetch();
             advance(c, n);
             if (c.seg != seg || c.item == c.last) {
