@@ -101,13 +101,39 @@ __device__ __forceinline__ uint64_t policy_evict_normal() {
     return p;
 }
 
+// Shared memory by its 32-bit addresses: a generic pointer would be two registers and two additions
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+    uint32_t v;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ void arrive_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(bytes) : "memory");
+}
+
 // Bulk copy of `bytes` (a multiple of 16, both addresses 16-byte aligned) of this GPU's memory into this CTA's
 // shared memory, completing on `bar`, with an L2 cache policy.
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar, uint64_t policy) {
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar, uint64_t policy) {
     asm volatile(
         "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;\n" ::"r"(
             dst),
-        "l"(src), "r"(bytes), "r"(smem_addr(bar)), "l"(policy)
+        "l"(src), "r"(bytes), "r"(bar), "l"(policy)
         : "memory");
 }
 
@@ -291,17 +317,15 @@ template <typename T> struct TileActs;
 template <>
 struct TileActs<__half> {
     Acts<__half> x[4];
-    __device__ __forceinline__ TileActs(const __half* p, int runs) { load(p, runs); }
+    __device__ __forceinline__ void load(const __half* p) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j].load(p + 32 * j);
+    }
     __device__ __forceinline__ void load(const __half* p, int runs) {
-        if (runs >= 4) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[j].load(p + 32 * j);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                x[j].zero();
-                if (j < runs) x[j].load(p + 32 * j);
-            }
+        for (int j = 0; j < 4; ++j) {
+            x[j].zero();
+            if (j < runs) x[j].load(p + 32 * j);
         }
     }
     __device__ __forceinline__ Acts<__half> run(int j) const { return x[j]; }
@@ -311,7 +335,7 @@ template <>
 struct TileActs<float> {
     const float* p;
     int runs;
-    __device__ __forceinline__ TileActs(const float* at, int n) : p(at), runs(n) {}
+    __device__ __forceinline__ void load(const float* at) { p = at, runs = 4; }
     __device__ __forceinline__ void load(const float* at, int n) { p = at, runs = n; }
     __device__ __forceinline__ Acts<float> run(int j) const {
         Acts<float> x;
@@ -321,21 +345,20 @@ struct TileActs<float> {
     }
 };
 
-// One tile of two strips (shared memory, `stride` bytes apart) times a block of 8 activation rows.
+// One tile of two strips (in shared memory at `tile`, `stride` bytes apart) times a block of 8 activation rows.
 template <typename T, int G>
-__device__ __forceinline__ void tile_mma(const uint8_t* tile, int stride, int lane, const TileActs<T>& x,
+__device__ __forceinline__ void tile_mma(uint32_t tile, int stride, int lane, const TileActs<T>& x,
                                          float (&acc)[2][4], const Ones<T>& one) {
     constexpr int kRuns = G / 32, kPairs = kCols / G;
     uint32_t wa[2][4], wb[2][4];
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-        const uint8_t* p = tile + m * stride + lane_chunk(lane);
-        const uint4 u = *reinterpret_cast<const uint4*>(p);
-        const uint4 v = *reinterpret_cast<const uint4*>(p + 512);
+        const uint4 u = lds128(tile + lane_chunk(lane) + m * stride);
+        const uint4 v = lds128(tile + lane_chunk(lane) + m * stride + 512);
         wa[m][0] = u.x, wa[m][1] = u.y, wa[m][2] = u.z, wa[m][3] = u.w;
         wb[m][0] = v.x, wb[m][1] = v.y, wb[m][2] = v.z, wb[m][3] = v.w;
     }
-    const uint8_t* pairs = tile + kCodeBytes + (lane >> 2) * kPairs * 4;
+    const uint32_t pairs = tile + kCodeBytes + (lane >> 2) * kPairs * 4;
 #pragma unroll
     for (int gi = 0; gi < kPairs; ++gi) {
         Sums<T, 2> s;
@@ -348,9 +371,8 @@ __device__ __forceinline__ void tile_mma(const uint8_t* tile, int stride, int la
         }
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-            const uint8_t* q = pairs + m * stride + 4 * gi;
-            group_end<T, 2>(acc[m], s, m, *reinterpret_cast<const uint32_t*>(q),
-                            *reinterpret_cast<const uint32_t*>(q + 8 * kPairs * 4));
+            const uint32_t q = pairs + m * stride + 4 * gi;
+            group_end<T, 2>(acc[m], s, m, lds32(q), lds32(q + 8 * kPairs * 4));
         }
     }
 }

@@ -41,16 +41,17 @@ inline int status_of(cudaError_t e, const char* what) {
     return -static_cast<int>(e);
 }
 
-// Warps that share a job's columns: the count with the least work for the busiest warp, a job's end taken as the work of
+// Warps that share a job's columns, as a power of two: the count with the least work for the busiest warp, a job's end taken as the work of
 // two tiles.
-inline int team_for(int64_t jobs, int64_t tiles) {
-    int best = 1;
+inline int team_log_for(int64_t jobs, int64_t tiles) {
+    int best = 0;
     int64_t least = 0;
-    for (int w = 1; w <= kWarps; w *= 2) {
+    for (int log = 0; (1 << log) <= kWarps; ++log) {
+        const int w = 1 << log;
         const int64_t teams = int64_t(kSms) * kCtas * kWarps / w;
         const int64_t work = (jobs + teams - 1) / teams * ((tiles + w - 1) / w + 2);
         if (w == 1 || work < least) {
-            best = w;
+            best = log;
             least = work;
         }
     }
@@ -60,11 +61,19 @@ inline int team_for(int64_t jobs, int64_t tiles) {
 template <typename T, int G, bool GLU>
 inline int launch_product(const ProductArgs& args, const Writes& w, cudaStream_t st) {
     ProductArgs a = args;
-    const int64_t wide = GLU ? 1 : 2;
-    const int64_t d_wide = (strips_of_rows(a.d_rows) + wide - 1) / wide, r_wide = (strips_of_rows(a.r_rows) + wide - 1) / wide;
-    const int64_t jobs = d_wide * ((a.d_tokens + kM - 1) / kM) + r_wide * std::min(a.pairs, a.experts + a.pairs / kM);
+    constexpr int kWide = GLU ? 1 : 2;
+    a.tiles = static_cast<int>(tiles_of_cols(a.cols));
+    a.runs = static_cast<int>(a.cols / 32);
+    a.d_strips = static_cast<int>(strips_of_rows(a.d_rows));
+    a.r_strips = static_cast<int>(strips_of_rows(a.r_rows));
+    a.d_wide = (a.d_strips + kWide - 1) / kWide;
+    a.r_wide = (a.r_strips + kWide - 1) / kWide;
+    a.d_blocks = static_cast<int>((a.d_tokens + kM - 1) / kM);
+    a.by_dense = Divisor(std::max(1, a.d_blocks));
+    a.by_share = Divisor(static_cast<int>(a.share));
+    const int64_t jobs = int64_t(a.d_wide) * a.d_blocks + a.r_wide * std::min(a.pairs, a.experts + a.pairs / kM);
     // (a dense matrix's by its shape alone: a token's sums are split alike alone and in a window)
-    a.team = team_for(a.pairs > 0 ? jobs : d_wide, tiles_of_cols(a.cols));
+    a.team_log = team_log_for(a.pairs > 0 ? jobs : a.d_wide, a.tiles);
     const size_t smem = product_smem<G>(a.pairs, a.experts);
     if (int e = max_smem(q4_product_kernel<T, G, GLU>, static_cast<int>(smem))) return status_of(static_cast<cudaError_t>(-e), "q4_product");
     // (a team's CTA of its own while there are slots for it: the teams spread evenly over the SMs)
@@ -86,7 +95,15 @@ inline int product(const ProductArgs& a, int group, const Writes& w, cudaStream_
 }
 
 template <typename T, int G>
-inline int launch_down(const DownArgs& a, const Writes& w, cudaStream_t st) {
+inline int launch_down(const DownArgs& args, const Writes& w, cudaStream_t st) {
+    DownArgs a = args;
+    a.stiles = static_cast<int>(tiles_of_cols(a.sffn));
+    a.ftiles = static_cast<int>(tiles_of_cols(a.ffn));
+    a.strips = static_cast<int>(strips_of_rows(a.rows));
+    a.jobs = (a.strips + kMt - 1) / kMt;
+    a.by_k = Divisor(static_cast<int>(a.k));
+    a.by_stiles = Divisor(std::max(1, a.stiles));
+    a.by_ftiles = Divisor(a.ftiles);
     const size_t smem = down_smem<G>(a.tokens, a.tokens * a.k, a.experts);
     if (int e = max_smem(q4_down_kernel<T, G>, static_cast<int>(smem))) return status_of(static_cast<cudaError_t>(-e), "q4_moe");
     return status_of(launch_pdl(w, q4_down_kernel<T, G>, dim3(kDownCtas), dim3(kThreads), smem, st, a), "q4_moe");

@@ -32,6 +32,19 @@ constexpr int kMaxPairs = 2048;
 // then not valid. smoe_q4_status reads and clears it. One per translation unit.
 static __device__ int g_q4_status = 0;
 
+// Division of numbers from 0 to 2^31 - 1 by one that a kernel keeps
+struct Divisor {
+    uint32_t n = 1, inverse = 0;
+    Divisor() = default;
+    __host__ __device__ __forceinline__ explicit Divisor(int by) : n(by), inverse(by > 1 ? 0xffffffffu / n : 0) {}
+    __device__ __forceinline__ int operator()(int a) const {
+        if (n == 1) return a;
+        uint32_t q = __umulhi(uint32_t(a), inverse);  // at most one too small: inverse is less than 1 below 2^32 / n
+        if (uint32_t(a) - q * n >= n) ++q;
+        return static_cast<int>(q);
+    }
+};
+
 struct ProductArgs {
     const void* x;  // (rows, cols), row stride cols
     int64_t cols;
@@ -49,7 +62,11 @@ struct ProductArgs {
     bool pieces;     // GLU, float16: a result as two rows, its float16 and what that leaves (rows 2 p and 2 p + 1 of out)
     uint32_t* zero;  // words to clear for the launch after (its counters)
     int n_zero;
-    int team;    // warps that share a job's columns
+    // what a warp would work out for itself first (the host's: a division is some 40 instructions of every warp's start)
+    int team_log;                         // log2 of the warps that share a job's columns
+    int tiles, runs;                      // of a row: 128-column tiles, 32-column runs
+    int d_strips, r_strips, d_wide, r_wide, d_blocks;  // strips, jobs of one block of rows, blocks of tokens
+    Divisor by_dense, by_share;           // by d_blocks, by share
     bool early;  // the weights may be read before pdl_wait()
     bool hint;   // weights evict-first in L2
 };
@@ -65,6 +82,8 @@ struct DownArgs {
     float* partial;      // [CTAs][2][tokens][32]
     uint32_t* counters;  // one a job, zero
     bool early;          // idx and the weights may be read before pdl_wait()
+    int stiles, ftiles, strips, jobs;
+    Divisor by_k, by_stiles, by_ftiles;
 };
 
 // ---- a warp's ring of bulk copies: two slots, the copies' and the reader's counts say which
@@ -72,62 +91,51 @@ struct DownArgs {
 constexpr int kStages = 2;  // slots
 
 struct Ring {
-    uint8_t* slots;
-    uint64_t* bars;
-    int slot_bytes;
+    uint32_t slots, bars;  // shared addresses
     uint32_t fetched = 0, taken = 0;
     bool dead = false;  // a wait gave up: what follows is read as it lies, nothing more is fetched
 
-    __device__ __forceinline__ void init(uint8_t* p, uint64_t* b, int bytes, int lane) {
-        slots = p;
-        bars = b;
-        slot_bytes = bytes;
+    __device__ __forceinline__ void init(uint8_t* p, uint64_t* b, int lane) {
+        slots = smem_addr(p);
+        bars = smem_addr(b);
         if (lane == 0) {
-            for (int i = 0; i < kStages; ++i) tc::mbar_init(&bars[i], 1);
+            for (int i = 0; i < kStages; ++i) tc::mbar_init(&b[i], 1);
             tc::fence_barrier_init();
         }
         __syncwarp();
     }
+    __device__ __forceinline__ uint64_t* barrier(uint32_t i) const {
+        return static_cast<uint64_t*>(__cvta_shared_to_generic(bars + 8 * i));
+    }
     __device__ __forceinline__ bool full() const { return fetched - taken == kStages; }
-    // the next slot, once its copies have landed
-    __device__ __forceinline__ const uint8_t* wait(int lane) {
+    // the next slot's shared address, once its copies have landed
+    template <int SLOT>
+    __device__ __forceinline__ uint32_t wait(int lane) {
         const uint32_t at = taken & 1, phase = (taken >> 1) & 1;
-        if (!__all_sync(0xffffffffu, tc::mbar_try_wait(&bars[at], phase))) {
-            if (!dead && !__all_sync(0xffffffffu, wait_for(&bars[at], phase))) {
+        if (!__all_sync(0xffffffffu, try_wait(bars + 8 * at, phase))) {
+            if (!dead && !__all_sync(0xffffffffu, wait_for(barrier(at), phase))) {
                 dead = true;
                 if (lane == 0) atomicExch(&g_q4_status, SMOE_ETIMEOUT);
             }
         }
-        return slots + at * slot_bytes;
+        return slots + at * SLOT;
     }
     // two copies of `bytes` into the next slot's halves (the whole warp calls, one lane issues)
+    template <int SLOT>
     __device__ __forceinline__ void fetch(const uint8_t* w0, const uint8_t* w1, uint32_t bytes, uint64_t policy) {
         const uint32_t at = fetched & 1;
         ++fetched;
         if (elect_one()) {
-            uint64_t* bar = &bars[at];
-            const uint32_t dst = smem_addr(slots) + at * slot_bytes;
-            tc::mbar_arrive_expect_tx(bar, 2 * bytes);
+            const uint32_t bar = bars + 8 * at, dst = slots + at * SLOT;
+            arrive_expect(bar, 2 * bytes);
             bulk_load(dst, w0, bytes, bar, policy);
-            bulk_load(dst + slot_bytes / 2, w1, bytes, bar, policy);
+            bulk_load(dst + SLOT / 2, w1, bytes, bar, policy);
         }
     }
     // no copy may still be writing shared memory when the CTA leaves
     __device__ __forceinline__ void drain(int lane) {
         for (uint32_t i = fetched < kStages ? 0 : fetched - kStages; i < fetched; ++i)
-            if (!wait_for(&bars[i & 1], (i >> 1) & 1) && lane == 0) atomicExch(&g_q4_status, SMOE_ETIMEOUT);
-    }
-};
-
-// Division of numbers from 0 to 2^31 - 1 by one that a kernel keeps
-struct Divisor {
-    uint32_t n, inverse;
-    __device__ __forceinline__ explicit Divisor(int by) : n(by), inverse(by > 1 ? 0xffffffffu / n : 0) {}
-    __device__ __forceinline__ int operator()(int a) const {
-        if (n == 1) return a;
-        uint32_t q = __umulhi(uint32_t(a), inverse);  // at most one too small: inverse is less than 1 below 2^32 / n
-        if (uint32_t(a) - q * n >= n) ++q;
-        return static_cast<int>(q);
+            if (!wait_for(barrier(i & 1), (i >> 1) & 1) && lane == 0) atomicExch(&g_q4_status, SMOE_ETIMEOUT);
     }
 };
 
@@ -262,6 +270,50 @@ __host__ __device__ constexpr int slot_bytes() {
 }
 constexpr int kRedFloats = kMt * kRows * kM;  // a warp's sums of one job
 
+// `left` tiles of two strips, as they come through the ring in stages of kStep and a last one of what is left, times a
+// block of activation rows: xp is this lane's place in its row at the first tile's first column, runs the row's 32-column
+// runs from there on. Pairs of whole tiles take a loop without any other condition (the conditions of a general one cost
+// 60 of its 250 instructions a tile), each tile's activations loaded during the tile before.
+template <typename T, int G, class Fetch>
+__device__ __forceinline__ void stream_tiles(Ring& ring, Fetch& fetch, const T* xp, int left, int runs, int lane,
+                                             float (&acc)[2][4], const Ones<T>& one) {
+    static_assert(kStep == 2, "a stage is a pair of tiles");
+    constexpr int kTile = tile_bytes<G>(), kStride = kStep * kTile;
+    int pairs = min(left, runs >> 2) >> 1;
+    left -= 2 * pairs;
+    if (pairs > 0) {
+        runs -= 8 * pairs;
+        TileActs<T> x0, x1;
+        x0.load(xp);
+#pragma unroll 1
+        do {
+            const uint32_t slot = ring.wait<2 * kStride>(lane);
+            x1.load(xp + kCols);
+            tile_mma<T, G>(slot, kStride, lane, x0, acc, one);
+            --pairs;
+            xp += 2 * kCols;
+            x0.load(pairs > 0 ? xp : xp - 2 * kCols);  // (after the last pair: any place of the row)
+            tile_mma<T, G>(slot + kTile, kStride, lane, x1, acc, one);
+            __syncwarp();
+            ++ring.taken;
+            fetch();
+        } while (pairs > 0);
+    }
+#pragma unroll 1
+    while (left > 0) {
+        const uint32_t slot = ring.wait<2 * kStride>(lane);
+#pragma unroll 1
+        for (int i = 0; i < kStep && left > 0; ++i, --left, xp += kCols, runs -= 4) {
+            TileActs<T> x;
+            x.load(xp, runs);
+            tile_mma<T, G>(slot + i * kTile, kStride, lane, x, acc, one);
+        }
+        __syncwarp();
+        ++ring.taken;
+        fetch();
+    }
+}
+
 // Shared memory: [ring slots, 8 warps][two jobs' partial sums, 8 warps][pair blocks][barriers]
 template <int G>
 __host__ __device__ constexpr size_t product_smem(int64_t pairs, int64_t experts) {
@@ -280,37 +332,32 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_product_kernel(const Produ
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int warp_sums[kWarps];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int team = warp / a.team, member = warp - team * a.team;
+    const int team_size = 1 << a.team_log, team = warp >> a.team_log, member = warp & (team_size - 1);
     // (teams of one CTA are far apart in the jobs' order: a few jobs spread over the SMs)
-    const int team_id = team * gridDim.x + blockIdx.x, teams = kWarps / a.team * gridDim.x;
+    const int team_id = team * gridDim.x + blockIdx.x, teams = (kWarps >> a.team_log) * gridDim.x;
 
     float* red = reinterpret_cast<float*>(smem + size_t(kWarps) * kStages * kSlot);
     uint8_t* table = reinterpret_cast<uint8_t*>(red + kWarps * 2 * kRedFloats);
     uint64_t* bars = reinterpret_cast<uint64_t*>(table + pair_blocks_bytes(a.pairs, a.experts));
-    red += team * a.team * 2 * kRedFloats;  // [job's parity][member][strip][row][column]
+    red += (team << a.team_log) * 2 * kRedFloats;  // [job's parity][member][strip][row][column]
     Ring ring;
-    ring.init(smem + size_t(warp) * kStages * kSlot, bars + warp * kStages, kSlot, lane);
+    ring.init(smem + size_t(warp) * kStages * kSlot, bars + warp * kStages, lane);
     // (weights of experts are read once; a layer's may be read again by its next block of tokens or its next call)
     const uint64_t policy = a.hint ? tc::policy_evict_first() : policy_evict_normal();
 
-    const int ntiles = static_cast<int>(tiles_of_cols(a.cols));
-    const int tile0 = member * ntiles / a.team, tile1 = (member + 1) * ntiles / a.team;
-    const int64_t strip_bytes = int64_t(ntiles) * kTile;
-    const int d_strips = static_cast<int>(strips_of_rows(a.d_rows)), r_strips = static_cast<int>(strips_of_rows(a.r_rows));
-    const int d_wide = (d_strips + kWide - 1) / kWide, r_wide = (r_strips + kWide - 1) / kWide;
-    const int d_blocks = static_cast<int>((a.d_tokens + kM - 1) / kM);
-    const int d_jobs = d_wide * d_blocks;
+    const int tile0 = (member * a.tiles) >> a.team_log, tile1 = ((member + 1) * a.tiles) >> a.team_log;
+    const int64_t strip_bytes = int64_t(a.tiles) * kTile;
+    const int d_jobs = a.d_wide * a.d_blocks;
     PairBlocks blocks{nullptr, nullptr, nullptr, nullptr, 0};
     int jobs = d_jobs;  // jobs known so far
 
     // job -> strips (from kWide times the first) and block of rows; a strip's blocks are neighbours in time, so that the
     // second reads the strip from L2
-    const Divisor by_dense(max(1, d_blocks)), by_share(static_cast<int>(max(int64_t(1), a.share)));
-    Divisor by_blocks(1);
+    Divisor by_blocks;
     auto place = [&](int j, int& strip, int& block) {
         if (j < d_jobs) {
-            strip = by_dense(j);
-            block = j - strip * d_blocks;
+            strip = a.by_dense(j);
+            block = j - strip * a.d_blocks;
         } else {
             j -= d_jobs;
             strip = by_blocks(j);
@@ -327,8 +374,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_product_kernel(const Produ
             int strip, block;
             place(fetch_job, strip, block);
             const bool dense = fetch_job < d_jobs;
-            const int strips = dense ? d_strips : r_strips;
-            const int64_t first = dense ? 0 : int64_t(blocks.expert[block]) * r_strips;
+            const int strips = dense ? a.d_strips : a.r_strips;
+            const int64_t first = dense ? 0 : int64_t(blocks.expert[block]) * a.r_strips;
             const uint8_t* w0 = dense ? a.dw[0] : a.rw[0];
             const uint8_t* w1 = !GLU ? w0 : dense ? a.dw[1] : a.rw[1];
             fetch0 = w0 + (first + strip * kWide) * strip_bytes + tile0 * kTile;
@@ -338,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_product_kernel(const Produ
             fetch_job += teams;
         }
         const int n = min(kStep, fetch_left);
-        ring.fetch(fetch0, fetch1, n * kTile, policy);
+        ring.template fetch<kSlot>(fetch0, fetch1, n * kTile, policy);
         fetch0 += n * kTile;
         fetch1 += n * kTile;
         fetch_left -= n;
@@ -349,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_product_kernel(const Produ
     pdl_wait();
     if (a.pairs > 0) {
         blocks = pair_blocks(table, a.idx, static_cast<int>(a.pairs), static_cast<int>(a.experts), kM, warp_sums);
-        jobs = d_jobs + blocks.n * r_wide;
+        jobs = d_jobs + blocks.n * a.r_wide;
         by_blocks = Divisor(max(1, blocks.n));
         for (int i = 0; i < kStages; ++i)
             if (!ring.full()) fetch();
@@ -359,7 +406,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_product_kernel(const Produ
 
     const Ones<T> one;
     const T* x = static_cast<const T*>(a.x) + 8 * t;
-    const int runs0 = static_cast<int>(a.cols / 32) - 4 * tile0;
+    const int runs0 = a.runs - 4 * tile0;
     // the thread's part of a job's results: a row, and every so many of its columns
     constexpr int kOut = kWide * kRows;
     const int out_r = lane & (kOut - 1), out_n = (member * 32 + lane) / kOut;
@@ -372,40 +419,26 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_product_kernel(const Produ
         const int count = dense ? static_cast<int>(min(int64_t(kM), a.d_tokens - start)) : blocks.count[block];
         // (columns past the count repeat the first row; their results are not written)
         const int at = g < count ? start + g : start;
-        const T* xp = x + int64_t(dense ? at : by_share(blocks.list[at])) * a.cols + tile0 * kCols;
+        const T* xp = x + int64_t(dense ? at : a.by_share(blocks.list[at])) * a.cols + tile0 * kCols;
         float acc[kMt][4] = {};
-        // (a tile's activations are loaded a tile ahead: their latency passes during the one before)
-        int left = tile1 - tile0, runs = runs0;
-        TileActs<T> x0(xp, left > 0 ? runs : 0);
-        for (; left > 0; left -= kStep, runs -= 4 * kStep, xp += kStep * kCols) {
-            const uint8_t* slot = ring.wait(lane);
-            const TileActs<T> x1(xp + kCols, left > 1 ? runs - 4 : 0);
-            tile_mma<T, G>(slot, kStep * kTile, lane, x0, acc, one);
-            if (left > 1) {
-                x0.load(xp + 2 * kCols, left > 2 ? runs - 8 : 0);
-                tile_mma<T, G>(slot + kTile, kStep * kTile, lane, x1, acc, one);
-            }
-            __syncwarp();
-            ++ring.taken;
-            fetch();
-        }
+        stream_tiles<T, G>(ring, fetch, xp, tile1 - tile0, runs0, lane, acc, one);
         // the team's sums, in the order of the column ranges (one barrier a job: the next job's sums have another place)
-        float* sums = red + parity * a.team * kRedFloats;
+        float* sums = red + ((parity * kRedFloats) << a.team_log);
 #pragma unroll
         for (int m = 0; m < kMt; ++m)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 sums[((member * kMt + m) * kRows + g + 8 * (i >> 1)) * kM + 2 * t + (i & 1)] = acc[m][i];
-        if (a.team == 1) __syncwarp();
-        else tc::named_barrier(1 + team, 32 * a.team);
+        if (team_size == 1) __syncwarp();
+        else tc::named_barrier(1 + team, 32 * team_size);
         const int rows = static_cast<int>(dense ? a.d_rows : a.r_rows);
         const int row = strip * kOut + out_r;
         if (row < rows) {
             T* out = static_cast<T*>(dense ? a.d_out : a.r_out) + row;
             const float* from = sums + out_r * kM;
-            for (int n = out_n; n < count; n += 32 / kOut * a.team) {
+            for (int n = out_n; n < count; n += 32 / kOut * team_size) {
                 float v = 0.0f, u = 0.0f;
-                for (int w = 0; w < a.team; ++w) {
+                for (int w = 0; w < team_size; ++w) {
                     v += from[w * kRedFloats + n];
                     if constexpr (GLU) u += from[w * kRedFloats + kRows * kM + n];
                 }
@@ -429,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_product_kernel(const Produ
                 }
             }
         }
-        if (a.team == 1) __syncwarp();
+        if (team_size == 1) __syncwarp();
     }
     pdl_release();
     ring.drain(lane);
@@ -467,22 +500,21 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_down_kernel(const DownArgs
     __shared__ int warp_sums[kWarps];
     __shared__ uint32_t arrived;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int strips = static_cast<int>(strips_of_rows(a.rows));
-    const int jobs = (strips + kMt - 1) / kMt;
+    const int strips = a.strips, jobs = a.jobs;
     const int tokens = static_cast<int>(a.tokens), k = static_cast<int>(a.k), pairs = tokens * k;
 
     float* red = reinterpret_cast<float*>(smem + size_t(kWarps) * kStages * kSlot);  // [warp][token][row]
     uint8_t* table = reinterpret_cast<uint8_t*>(red + kWarps * tokens * kTokenStride);
     uint64_t* bars = reinterpret_cast<uint64_t*>(table + pair_blocks_bytes(pairs, a.experts));
     Ring ring;
-    ring.init(smem + size_t(warp) * kStages * kSlot, bars + warp * kStages, kSlot, lane);
+    ring.init(smem + size_t(warp) * kStages * kSlot, bars + warp * kStages, lane);
     const uint64_t policy = tc::policy_evict_first();
     float* mine = red + warp * tokens * kTokenStride;
 
     if (!a.early) pdl_wait();
     const PairBlocks blocks = pair_blocks(table, a.idx, pairs, static_cast<int>(a.experts), kRowsIn, warp_sums);
     // segments of a job: the shared expert's blocks of tokens, then the pairs' blocks
-    const int stiles = static_cast<int>(tiles_of_cols(a.sffn)), ftiles = static_cast<int>(tiles_of_cols(a.ffn));
+    const int stiles = a.stiles, ftiles = a.ftiles;
     const int sblocks = stiles > 0 ? (tokens + kRowsIn - 1) / kRowsIn : 0;
     const int shared_items = sblocks * stiles;
     const int items = max(1, shared_items + blocks.n * ftiles);  // (a job without any tile still writes its zeros)
@@ -501,57 +533,55 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_down_kernel(const DownArgs
         i1 = p0 + (warp + 1) * n / kWarps;
         if (!any) i0 = i1 = 0;
     };
+    // a warp's place in a job: the tiles still to come, from tile `tile` of segment `seg` on
     struct Cursor {
-        int item, last, seg, tile;
+        int left, seg, tile;
     };
     auto cursor_of = [&](int job) {
-        Cursor c;
-        range_of(job, c.item, c.last);
-        if (c.item < shared_items) {
-            c.seg = c.item / stiles;
-            c.tile = c.item - c.seg * stiles;
+        int i0, i1;
+        range_of(job, i0, i1);
+        Cursor c{i1 - i0, 0, i0};
+        if (i0 < shared_items) {
+            c.seg = a.by_stiles(i0);
+            c.tile = i0 - c.seg * stiles;
         } else {
-            const int i = c.item - shared_items;
-            c.seg = i / ftiles;
-            c.tile = i - c.seg * ftiles;
+            i0 -= shared_items;
+            c.seg = a.by_ftiles(i0);
+            c.tile = i0 - c.seg * ftiles;
             c.seg += sblocks;
         }
         return c;
     };
-    auto tiles_in = [&](int seg) { return seg < sblocks ? stiles : ftiles; };
-    auto stage_of = [&](const Cursor& c) { return min(min(kStep, tiles_in(c.seg) - c.tile), c.last - c.item); };
-    auto advance = [&](Cursor& c, int n) {
-        c.item += n;
-        c.tile += n;
-        if (c.tile == tiles_in(c.seg)) {
-            c.tile = 0;
-            ++c.seg;
-        }
+    // its tiles of the segment it is in
+    auto tiles_of = [&](const Cursor& c) { return min(c.left, (c.seg < sblocks ? stiles : ftiles) - c.tile); };
+    auto next_segment = [&](Cursor& c, int n) {
+        c.left -= n;
+        c.tile = 0;
+        ++c.seg;
     };
 
-    int fetch_job = job_first, fetch_seg = -1;
-    Cursor fc = job_first < job_last ? cursor_of(fetch_job) : Cursor{0, 0, 0, 0};
+    int fetch_job = job_first, fetch_left = 0;
+    Cursor fc = job_first < job_last ? cursor_of(fetch_job) : Cursor{0, 0, 0};
     const uint8_t *fetch0 = nullptr, *fetch1 = nullptr;
     auto fetch = [&]() {  // (a slot is free)
-        while (fc.item >= fc.last) {
-            if (fetch_job + 1 >= job_last) return;
-            fc = cursor_of(++fetch_job);
-            fetch_seg = -1;
-        }
-        if (fc.seg != fetch_seg) {
-            if (ring.dead) return;
-            fetch_seg = fc.seg;
+        if (fetch_left == 0) {
+            while (fc.left == 0) {
+                if (fetch_job + 1 >= job_last || ring.dead) return;
+                fc = cursor_of(++fetch_job);
+            }
             const bool shared = fc.seg < sblocks;
             const int64_t strip_bytes = int64_t(shared ? stiles : ftiles) * kTile;
             const uint8_t* w = shared ? a.sw : a.w + int64_t(blocks.expert[fc.seg - sblocks]) * strips * strip_bytes;
             fetch0 = w + (fetch_job * kMt) * strip_bytes + fc.tile * kTile;
             fetch1 = w + min(fetch_job * kMt + 1, strips - 1) * strip_bytes + fc.tile * kTile;
+            fetch_left = tiles_of(fc);
+            next_segment(fc, fetch_left);
         }
-        const int n = stage_of(fc);
-        ring.fetch(fetch0, fetch1, n * kTile, policy);
+        const int n = min(kStep, fetch_left);
+        ring.template fetch<kSlot>(fetch0, fetch1, n * kTile, policy);
         fetch0 += n * kTile;
         fetch1 += n * kTile;
-        advance(fc, n);
+        fetch_left -= n;
     };
     for (int i = 0; i < kStages; ++i) fetch();
     pdl_wait();
@@ -560,69 +590,47 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_down_kernel(const DownArgs
     for (int job = job_first; job < job_last; ++job) {
         for (int i = lane; i < tokens * kTokenStride; i += 32) mine[i] = 0.0f;
         __syncwarp();
-        float acc[kMt][4] = {};
-        const T* xp = nullptr;
-        int count = 0, start = 0, runs = 0, seg = -1;
-        bool shared = false;
-        Cursor c = cursor_of(job);
-        while (c.item < c.last) {
-            if (c.seg != seg) {
-                seg = c.seg;
-                shared = seg < sblocks;
-                start = shared ? seg * kRowsIn : blocks.start[seg - sblocks];
-                count = shared ? min(kRowsIn, tokens - start) : blocks.count[seg - sblocks];
-                runs = static_cast<int>((shared ? a.sffn : a.ffn) / 32);
-                const int n = g % kRowsIn, at = n < count ? start + n : start;
-                xp = shared ? static_cast<const T*>(a.hs) + (at * kPieces + g / kRowsIn) * a.sffn + 8 * t
-                            : static_cast<const T*>(a.h) + (blocks.list[at] * kPieces + g / kRowsIn) * a.ffn + 8 * t;
-            }
-            const int n = stage_of(c);
-            const TileActs<T> x0(xp + c.tile * kCols, runs - 4 * c.tile);
-            const uint8_t* slot = ring.wait(lane);
-            const TileActs<T> x1(xp + (c.tile + 1) * kCols, n > 1 ? runs - 4 * (c.tile + 1) : 0);
-            tile_mma<T, G>(slot, kStep * kTile, lane, x0, acc, one);
-            if (n > 1) tile_mma<T, G>(slot + kTile, kStep * kTile, lane, x1, acc, one);
-            __syncwarp();
-            ++ring.taken;
-            fetch();
-            advance(c, n);
-            if (c.seg != seg || c.item == c.last) {
-                // the block's end: each column's sums to its token, this lane's columns 2 t and 2 t + 1 (with pieces,
-                // those of columns 2 t + 4 and 2 t + 5 added). A token that
-                // names an expert twice has two columns here, neighbours: column by column then.
-                if constexpr (kPieces == 2) {
-#pragma unroll
-                    for (int m = 0; m < kMt; ++m)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) acc[m][i] += __shfl_xor_sync(0xffffffffu, acc[m][i], 2);
-                }
-                auto add = [&](int h) {
-                    const int col = 2 * t + h;
-                    float* to = mine + (shared ? start + col : blocks.list[start + col] / k) * kTokenStride + g;
-#pragma unroll
-                    for (int m = 0; m < kMt; ++m) {
-                        to[m * kRows] += acc[m][h];
-                        to[m * kRows + 8] += acc[m][2 + h];
-                    }
-                };
-                const bool again = !shared && lane + 1 < count &&
-                                   blocks.list[start + lane] / k == blocks.list[start + lane + 1] / k;
-                if (__any_sync(0xffffffffu, again)) {
-                    for (int col = 0; col < count; ++col) {
-                        if (col == 2 * t) add(0);
-                        if (col == 2 * t + 1) add(1);
-                        __syncwarp();
-                    }
-                } else {
-                    if (2 * t < count) add(0);
-                    if (2 * t + 1 < count) add(1);
-                }
-                __syncwarp();
+        for (Cursor c = cursor_of(job); c.left > 0;) {
+            const bool shared = c.seg < sblocks;
+            const int start = shared ? c.seg * kRowsIn : blocks.start[c.seg - sblocks];
+            const int count = shared ? min(kRowsIn, tokens - start) : blocks.count[c.seg - sblocks];
+            const int64_t width = shared ? a.sffn : a.ffn;
+            const int row = g % kRowsIn, of = row < count ? start + row : start;
+            const T* xp = static_cast<const T*>(shared ? a.hs : a.h) +
+                          ((shared ? of : blocks.list[of]) * kPieces + g / kRowsIn) * width + c.tile * kCols + 8 * t;
+            const int n = tiles_of(c);
+            float acc[kMt][4] = {};
+            stream_tiles<T, G>(ring, fetch, xp, n, static_cast<int>(width / 32) - 4 * c.tile, lane, acc, one);
+            next_segment(c, n);
+            // each column's sums to its token, this lane's columns 2 t and 2 t + 1 (with pieces, those of columns 2 t + 4
+            // and 2 t + 5 added). A token that names an expert twice has two columns here, neighbours: column by column then.
+            if constexpr (kPieces == 2) {
 #pragma unroll
                 for (int m = 0; m < kMt; ++m)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[m][i] = 0.0f;
+                    for (int i = 0; i < 4; ++i) acc[m][i] += __shfl_xor_sync(0xffffffffu, acc[m][i], 2);
             }
+            auto token_of = [&](int col) { return shared ? start + col : a.by_k(blocks.list[start + col]); };
+            auto add = [&](int h) {
+                float* to = mine + token_of(2 * t + h) * kTokenStride + g;
+#pragma unroll
+                for (int m = 0; m < kMt; ++m) {
+                    to[m * kRows] += acc[m][h];
+                    to[m * kRows + 8] += acc[m][2 + h];
+                }
+            };
+            const bool again = !shared && lane + 1 < count && token_of(lane) == token_of(lane + 1);
+            if (__any_sync(0xffffffffu, again)) {
+                for (int col = 0; col < count; ++col) {
+                    if (col == 2 * t) add(0);
+                    if (col == 2 * t + 1) add(1);
+                    __syncwarp();
+                }
+            } else {
+                if (2 * t < count) add(0);
+                if (2 * t + 1 < count) add(1);
+            }
+            __syncwarp();
         }
         __syncthreads();
         const int at = job * items;
