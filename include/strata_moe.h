@@ -539,6 +539,14 @@ SMOE_API size_t smoe_q4_moe_workspace_size(int64_t tokens, int64_t k, int64_t hi
                                              int64_t shared_ffn);
 SMOE_API int smoe_q4_moe(const SmoeQ4Moe* m, void* workspace, size_t workspace_bytes, void* stream);
 
+/* smoe_route for a window of 1 to 64 float16 tokens with the router's sums on the tensor cores (exact products, float32
+ * sums in another order than smoe_route's): logits [tokens][experts], idx, weights [tokens][k], gate_out [tokens]
+ * float16 of gate_weight (both or neither). hidden a multiple of 32, experts <= 2048, k <= 32. `counter`: one word, zero
+ * before the first call and left zero; calls that may overlap need one each. */
+SMOE_API int smoe_route_window(const uint16_t* weight, const uint16_t* gate_weight, const uint16_t* x, int64_t tokens,
+                               int64_t experts, int64_t hidden, int64_t k, float* logits, uint32_t* idx, float* weights,
+                               uint16_t* gate_out, uint32_t* counter, void* stream);
+
 /* Whether a bounded wait of the 4-bit kernels gave up since the last clear (SMOE_ETIMEOUT; outputs since are not
  * valid). Synchronizes the device. */
 SMOE_API int smoe_q4_status(int* status, int clear);

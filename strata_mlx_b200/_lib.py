@@ -146,6 +146,7 @@ SIGNATURES = {
     "smoe_q4_product": (_i, [_c.POINTER(SmoeQ4Product), _p]),
     "smoe_q4_moe_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64]),
     "smoe_q4_moe": (_i, [_c.POINTER(SmoeQ4Moe), _p, _sz, _p]),
+    "smoe_route_window": (_i, [_p, _p, _p, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p]),
     "smoe_q4_status": (_i, [_c.POINTER(_i), _i]),
 }
 

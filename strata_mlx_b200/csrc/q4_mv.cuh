@@ -393,6 +393,10 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_product_kernel(const Produ
     if (!a.early) pdl_wait();
     // the dense part's weights, while the launch before still runs
     for (int i = 0; i < kStages; ++i) fetch();
+    // (and a first go at the pairs, whatever idx holds yet: nothing of it is used, but the code is in the cache when it
+    // counts, 1 us earlier)
+    if (a.pairs > 0)
+        pair_blocks(table, a.idx, static_cast<int>(a.pairs), static_cast<int>(a.experts), kM, warp_sums);
     pdl_wait();
     if (a.pairs > 0) {
         blocks = pair_blocks(table, a.idx, static_cast<int>(a.pairs), static_cast<int>(a.experts), kM, warp_sums);
@@ -483,6 +487,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_product_kernel(const Produ
 template <typename T>
 __host__ __device__ constexpr int down_rows() { return sizeof(T) == 2 ? kM / 2 : kM; }
 
+constexpr int kByJob = 32;  // tiles of a CTA up to which it keeps to one job
 constexpr int kTokenStride = kMt * kRows + 4;  // floats of a token's sums: rows 0, 8, .. of four tokens on 32 banks
 
 template <int G>
@@ -519,10 +524,22 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_down_kernel(const DownArgs
     const int shared_items = sblocks * stiles;
     const int items = max(1, shared_items + blocks.n * ftiles);  // (a job without any tile still writes its zeros)
     const bool any = shared_items + blocks.n > 0;
-    // a CTA's tiles of all jobs': an even share, at least a tile a warp (32 bits hold them: the host checks)
+    // a CTA's tiles of all jobs': an even share in a row, at least a tile a warp (32 bits hold them: the host checks); or
+    // with few tiles an even share of one job (a second job's end would cost the CTA more than the uneven load)
     const int all = jobs * items;
-    const int share = max(min(kWarps, all), (all + int(gridDim.x) - 1) / int(gridDim.x));
-    const int begin = min(all, int(blockIdx.x) * share), end = min(all, begin + share);
+    const int parts = int(gridDim.x) / jobs;  // CTAs of a job
+    const bool by_job = parts > 0 && items <= parts * kByJob;
+    const int share = by_job ? max(min(kWarps, items), (items + parts - 1) / parts)
+                             : max(min(kWarps, all), (all + int(gridDim.x) - 1) / int(gridDim.x));
+    int begin, end;
+    if (by_job) {
+        const int job = blockIdx.x / parts, part = blockIdx.x - job * parts;
+        begin = job < jobs ? job * items + min(items, part * share) : all;
+        end = job < jobs ? min(begin + share, (job + 1) * items) : all;
+    } else {
+        begin = min(all, int(blockIdx.x) * share);
+        end = min(all, begin + share);
+    }
     const int job_first = begin / items, job_last = begin < end ? (end + items - 1) / items : job_first;
 
     // a warp's tiles of a job
@@ -652,7 +669,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_down_kernel(const DownArgs
         }
         if (!whole) {
             // the CTAs of this job: those whose ranges meet it
-            const int c0 = at / share, c1 = (at + items - 1) / share;
+            const int c0 = by_job ? job * parts : at / share;
+            const int c1 = by_job ? c0 + (items - 1) / share : (at + items - 1) / share;
             __threadfence();
             __syncthreads();
             if (tid == 0) arrived = atomicAdd(&a.counters[job], 1u);
@@ -661,9 +679,17 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_down_kernel(const DownArgs
                 __threadfence();
                 for (int i = tid; i < values; i += kThreads) {
                     float sum = 0.0f;
-                    for (int cta = c0; cta <= c1; ++cta) {
-                        const int slot = cta * share >= at ? 0 : 1;  // (its range begins in this job, or before)
-                        sum += __ldcg(a.partial + (int64_t(cta) * 2 + slot) * values + i);
+                    for (int cta = c0; cta <= c1; cta += 8) {
+                        // (eight CTAs' sums in flight together, added in their order)
+                        float v[8];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const int from = 2 * min(cta + j, c1) + (by_job || (cta + j) * share >= at ? 0 : 1);
+                            v[j] = __ldcg(a.partial + int64_t(from) * values + i);  // (its range begins in this job, or before)
+                        }
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            if (cta + j <= c1) sum += v[j];
                     }
                     write(i, sum);
                 }

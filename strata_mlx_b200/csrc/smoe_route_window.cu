@@ -1,0 +1,176 @@
+// The route of a window of tokens (router product, top-k, softmax over the chosen, the shared expert's gate) with its
+// sums on the tensor cores, in one launch.
+//
+//   logits[t, e] = router[e] . x[t];  idx = the k largest, ties to the lower index;  weights = softmax of the chosen;
+//   gate_out[t] = gate_weight . x[t]
+//
+// A CTA takes 16 rows of the router (the shared gate's row is one more) and every token: 16 warps share the columns, each
+// m16n8k16 on its own (router rows the M side, tokens the N side, products exact, float32 sums), partial sums added in
+// the order of the columns. The last CTA to arrive takes the top-k, a warp a token. Bound by latency (the router is 2 to
+// 4 MB): the rows' first columns are loaded before the launch waits for the one before it. Next to a row's sums on CUDA
+// cores for eight tokens a CTA this reads the router once for up to 64 tokens.
+#include <algorithm>
+#include <string>
+
+#include "q4.cuh"
+#include "router_dev.cuh"
+
+namespace smoe {
+namespace {
+
+constexpr int kRwWarps = 16;
+constexpr int kRwThreads = 32 * kRwWarps;
+constexpr int kRwRows = 16;
+constexpr int kRwAhead = 5;  // runs of 32 columns a warp loads before it waits (hidden 2560: all of its own)
+constexpr int kRwTokens = 64;
+
+struct RouteWindow {
+    const __half* weight;
+    const __half* gate_weight;
+    const __half* x;
+    int tokens, experts, runs, k;  // runs: hidden / 32
+    int64_t hidden;
+    float* logits;
+    uint32_t* idx;
+    float* weights;
+    __half* gate_out;
+    uint32_t* counter;
+    bool early;  // the router may be read before pdl_wait()
+};
+
+constexpr int kRwStride = kRwRows + 4;  // floats of a token's sums: a warp's writes and reads are on different banks
+
+template <int NT>
+constexpr size_t route_window_smem() { return size_t(kRwWarps) * 8 * NT * kRwStride * 4; }
+
+template <int NT, int NV>
+__global__ void __launch_bounds__(kRwThreads, 1) route_window_kernel(const RouteWindow a) {
+    extern __shared__ __align__(16) float part[];  // [warp][token][row]
+    __shared__ bool last;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int row0 = blockIdx.x * kRwRows, rows = a.experts + (a.gate_weight != nullptr);
+    const int run0 = warp * a.runs / kRwWarps, run1 = (warp + 1) * a.runs / kRwWarps;
+    // this lane's rows g and g + 8 (rows past the last repeat it; their sums are not written), columns 8 t .. of a run
+    auto row_of = [&](int r) {
+        r = min(r, rows - 1);
+        return (r < a.experts ? a.weight + r * a.hidden : a.gate_weight) + 8 * t;
+    };
+    const __half *wa = row_of(row0 + g), *wb = row_of(row0 + g + 8);
+    uint4 ahead[kRwAhead][2];
+    if (!a.early) pdl_wait();
+#pragma unroll
+    for (int i = 0; i < kRwAhead; ++i) {
+        const int run = min(run0 + i, a.runs - 1);
+        ahead[i][0] = __ldg(reinterpret_cast<const uint4*>(wa + 32 * run));
+        ahead[i][1] = __ldg(reinterpret_cast<const uint4*>(wb + 32 * run));
+    }
+    pdl_wait();
+    pdl_release();
+    const __half* xp[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) xp[nt] = a.x + min(8 * nt + g, a.tokens - 1) * a.hidden + 8 * t;
+    float acc[NT][4] = {};
+    auto step = [&](const uint4& u, const uint4& v, int run) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const uint4 x = *reinterpret_cast<const uint4*>(xp[nt] + 32 * run);
+            q4::mma_f16<false>(acc[nt], u.x, v.x, u.y, v.y, x.x, x.y);
+            q4::mma_f16<false>(acc[nt], u.z, v.z, u.w, v.w, x.z, x.w);
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < kRwAhead; ++i)
+        if (run0 + i < run1) step(ahead[i][0], ahead[i][1], run0 + i);
+    for (int run = run0 + kRwAhead; run < run1; ++run)
+        step(__ldg(reinterpret_cast<const uint4*>(wa + 32 * run)), __ldg(reinterpret_cast<const uint4*>(wb + 32 * run)), run);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            part[(warp * 8 * NT + 8 * nt + 2 * t + (i & 1)) * kRwStride + g + 8 * (i >> 1)] = acc[nt][i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < kRwRows * a.tokens; i += kRwThreads) {
+        const int r = i & (kRwRows - 1), n = i / kRwRows, row = row0 + r;
+        float sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kRwWarps; ++w) sum += part[(w * 8 * NT + n) * kRwStride + r];
+        if (row < a.experts) a.logits[n * int64_t(a.experts) + row] = sum;
+        else if (row < rows) a.gate_out[n] = __float2half_rn(sum);
+    }
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) last = atomicAdd(a.counter, 1u) == gridDim.x - 1;
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    for (int n = warp; n < a.tokens; n += kRwWarps) {
+        const float* in = a.logits + n * int64_t(a.experts);
+        topk_row<NV>([&](int j) { return __ldcg(in + j); }, a.experts, a.k, a.idx + n * a.k, a.weights + n * a.k);
+        __syncwarp();
+    }
+    if (threadIdx.x == 0) *a.counter = 0u;
+}
+
+template <int NT>
+int launch(const RouteWindow& a, const Writes& w, cudaStream_t st) {
+    auto go = [&](auto kernel) {
+        const size_t smem = route_window_smem<NT>();
+        cudaError_t e = static_cast<cudaError_t>(-max_smem(kernel, static_cast<int>(smem)));
+        const int rows = a.experts + (a.gate_weight != nullptr);
+        if (e == cudaSuccess)
+            e = launch_pdl(w, kernel, dim3((rows + kRwRows - 1) / kRwRows), dim3(kRwThreads), smem, st, a);
+        if (e == cudaSuccess) return launch_status("route_window");
+        cudaGetLastError();
+        return fail(-static_cast<int>(e), std::string("route_window: ") + cudaGetErrorString(e));
+    };
+    if (a.experts <= 256) return go(route_window_kernel<NT, 8>);
+    if (a.experts <= 512) return go(route_window_kernel<NT, 16>);
+    if (a.experts <= 1024) return go(route_window_kernel<NT, 32>);
+    return go(route_window_kernel<NT, 64>);
+}
+
+}  // namespace
+}  // namespace smoe
+
+using namespace smoe;
+
+extern "C" int smoe_route_window(const uint16_t* weight, const uint16_t* gate_weight, const uint16_t* x, int64_t tokens,
+                                 int64_t experts, int64_t hidden, int64_t k, float* logits, uint32_t* idx, float* weights,
+                                 uint16_t* gate_out, uint32_t* counter, void* stream) {
+    if (tokens == 0) return SMOE_OK;
+    SMOE_REQUIRE(weight && x && logits && idx && weights && counter && tokens > 0 && experts > 0, SMOE_EARG,
+                 "route_window: null pointer or empty router");
+    SMOE_REQUIRE((gate_weight == nullptr) == (gate_out == nullptr), SMOE_EARG,
+                 "the shared gate's weight and output come together");
+    SMOE_REQUIRE(tokens <= kRwTokens, SMOE_ESHAPE, "route_window takes up to 64 tokens a call");
+    SMOE_REQUIRE(hidden > 0 && hidden % 32 == 0 && hidden < (int64_t(1) << 24), SMOE_ESHAPE,
+                 "route_window takes rows of a multiple of 32 values");
+    SMOE_REQUIRE(experts <= 2048, SMOE_ESHAPE, "route_window takes rows of 1 to 2048 logits");
+    SMOE_REQUIRE(k >= 1 && k <= experts && k <= 32, SMOE_ESHAPE, "route_window takes 1 <= k <= min(experts, 32)");
+    SMOE_REQUIRE(((reinterpret_cast<uintptr_t>(weight) | reinterpret_cast<uintptr_t>(x) |
+                   reinterpret_cast<uintptr_t>(gate_weight)) & 15) == 0,
+                 SMOE_EARG, "router weights and activations must be 16-byte aligned");
+    cudaStream_t st = as_stream(stream);
+    RouteWindow a = {};
+    a.weight = reinterpret_cast<const __half*>(weight);
+    a.gate_weight = reinterpret_cast<const __half*>(gate_weight);
+    a.x = reinterpret_cast<const __half*>(x);
+    a.tokens = static_cast<int>(tokens);
+    a.experts = static_cast<int>(experts);
+    a.runs = static_cast<int>(hidden / 32);
+    a.k = static_cast<int>(k);
+    a.hidden = hidden;
+    a.logits = logits;
+    a.idx = idx;
+    a.weights = weights;
+    a.gate_out = reinterpret_cast<__half*>(gate_out);
+    a.counter = counter;
+    a.early = pdl_early(st, weight, size_t(experts) * hidden * 2) && pdl_early(st, gate_weight, size_t(hidden) * 2);
+    Writes w;
+    w.add(logits, size_t(tokens) * experts * 4).add(idx, size_t(tokens) * k * 4).add(weights, size_t(tokens) * k * 4);
+    w.add(gate_out, size_t(tokens) * 2).add(counter, 4);
+    if (tokens <= 8) return launch<1>(a, w, st);
+    if (tokens <= 16) return launch<2>(a, w, st);
+    if (tokens <= 32) return launch<4>(a, w, st);
+    return launch<8>(a, w, st);
+}

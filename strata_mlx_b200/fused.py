@@ -220,6 +220,29 @@ def route(gate: "WindowLinear", shared_gate, x: torch.Tensor, k: int, local=None
     return out if local is None else out + (lidx.reshape(*lead, k),)
 
 
+def route_window(gate: "WindowLinear", shared_gate: "WindowLinear", x: torch.Tensor, k: int):
+    """`route` for up to 64 float16 tokens with the router's sums on the tensor cores (float32, in another order than
+    route's: the last bits of the logits may differ); (idx, w, g), or None where the kernel does not take x."""
+    tokens = x.numel() // gate.cols
+    if (x.dtype != torch.float16 or not 1 <= tokens <= 64 or gate.cols % 32 or gate.rows > 2048 or not gate.takes(x)
+            or not 1 <= k <= min(gate.rows, 32) or not shared_gate.takes(x) or shared_gate.rows != 1
+            or shared_gate.cols != gate.cols):
+        return None
+    _lib.require_cuda(gate.weight, x)
+    dev = x.device
+    x2 = affine._aligned(x)
+    wt, gw = gate.weight.contiguous(), shared_gate.weight.contiguous()
+    logits = torch.empty((tokens, gate.rows), dtype=torch.float32, device=dev)
+    idx = torch.empty((tokens, k), dtype=torch.uint32, device=dev)
+    w = torch.empty((tokens, k), dtype=torch.float32, device=dev)
+    g = torch.empty((tokens,), dtype=x.dtype, device=dev)
+    counter = _route_counters(4, False, dev)
+    _lib.call("smoe_route_window", _lib.ptr(wt), _lib.ptr(gw), _lib.ptr(x2), tokens, gate.rows, gate.cols, k,
+              _lib.ptr(logits), _lib.ptr(idx), _lib.ptr(w), _lib.ptr(g), _lib.ptr(counter), _lib.stream())
+    lead = x.shape[:-1]
+    return idx.reshape(*lead, k), w.reshape(*lead, k), g.reshape(*lead, 1)
+
+
 def launch_route(step) -> None:
     """Launch a deferred route (`route(..., defer=True)`) by itself."""
     if step.tokens:
@@ -265,6 +288,8 @@ class SparseMoeBlock:
         out = decode_layer(self, x)
         if out is not None:
             return out
+        if affine.moe_takes(self.switch_mlp, self.shared_expert):
+            return self._quantized(x)
         # the route goes into the gate / up launch of the decode products where they take it (FUSED_ROUTE)
         r = route(self.gate, self.shared_expert_gate, x, self.top_k, defer=FUSED_ROUTE)
         step = None
@@ -277,10 +302,6 @@ class SparseMoeBlock:
             idx, w = top_k_softmax(logits, self.top_k)
             g = self.shared_expert_gate(x).to(x.dtype)
         ys = None
-        if affine.moe_takes(self.switch_mlp, self.shared_expert):
-            if step is not None:
-                launch_route(step)
-            return affine.moe(self.switch_mlp, self.shared_expert, x, idx, w, g)
         if isinstance(self.switch_mlp, BlockSwitchGLU) and isinstance(self.shared_expert, BlockMLP):
             ys = decode_products(self.switch_mlp, self.shared_expert, x, idx, w, g, route_step=step)
         if ys is None and step is not None:
@@ -292,6 +313,18 @@ class SparseMoeBlock:
         if out is None:
             raise ValueError("the combine takes float16 or float32 activations")
         return out
+
+
+    def _quantized(self, x: torch.Tensor) -> torch.Tensor:
+        """The block on 4-bit experts: the route, then `affine.moe`."""
+        _lib.require_cuda(x)
+        with torch.cuda.device(x.device):
+            r = route_window(self.gate, self.shared_expert_gate, x, self.top_k)
+            if r is None:
+                r = route(self.gate, self.shared_expert_gate, x, self.top_k)
+            if r is None:
+                r = (*top_k_softmax(self.gate(x), self.top_k), self.shared_expert_gate(x).to(x.dtype))
+            return affine.moe(self.switch_mlp, self.shared_expert, x, *r)
 
 
 _Routed = SparseMoeBlock

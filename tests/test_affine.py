@@ -109,6 +109,17 @@ def test_the_moe_block_checks_its_workspace(lib):
     assert lib.smoe_q4_moe_workspace_size(0, 2, 128, 64, 64) == 0
 
 
+def test_the_route_of_a_window_checks_its_arguments(lib):
+    def call(w=A, gw=A, x=A, tokens=2, experts=8, hidden=64, k=2, g=A, counter=A):
+        return lib.smoe_route_window(w, gw, x, tokens, experts, hidden, k, A, A, A, g, counter, None)
+
+    assert call(tokens=0) == 0
+    assert call(tokens=65) == ESHAPE and call(hidden=48) == ESHAPE and call(experts=2049) == ESHAPE
+    assert call(k=9) == ESHAPE and call(k=0) == ESHAPE and call(experts=64, k=33) == ESHAPE
+    assert call(w=None) == EARG and call(counter=None) == EARG and call(g=None) == EARG and call(gw=None) == EARG
+    assert call(x=A + 8) == EARG and call(w=A + 2) == EARG and call(tokens=-1) == EARG
+
+
 def test_there_is_no_cpu_path():
     w = torch.zeros(4, 128)
     parts = torch.zeros(4, 16, dtype=torch.int32), torch.zeros(4, 2, dtype=torch.float16), torch.zeros(4, 2, dtype=torch.float16)

@@ -347,6 +347,40 @@ def test_the_experts_alone_are_their_definition(cuda, dtype):
     close(mlp(x), want, eh @ wd.abs().mT + sums(160, 32) * ((h.abs() + eh) @ md.mT) + last(want, dtype))
 
 
+@pytest.mark.parametrize("tokens, experts, hidden, k", [(1, 512, 2560, 10), (1, 1, 32, 1), (2, 33, 1056, 4), (8, 256, 4096, 8),
+                                                        (9, 15, 96, 15), (17, 300, 2048, 32), (33, 2048, 64, 3), (64, 511, 512, 10)])
+def test_the_route_of_a_window_is_its_definition(cuda, tokens, experts, hidden, k):
+    gen = gen_of(tokens + experts)
+    router = (hidden**-0.5 * torch.randn(experts, hidden, device=cuda, generator=gen)).half()
+    sgate = (hidden**-0.5 * torch.randn(1, hidden, device=cuda, generator=gen)).half()
+    x = torch.randn(tokens, hidden, device=cuda, generator=gen).half()
+    gate, shared = fused.WindowLinear(router), fused.WindowLinear(sgate)
+    # one addition for every column in the order of any sum, at most 2^-23 of the magnitudes each
+    logits, off = x.double() @ router.double().mT, hidden * 2.0**-23 * (x.double().abs() @ router.double().abs().mT)
+    for _ in range(3):  # (the counter is left as it was found)
+        idx, w, g = fused.route_window(gate, shared, x, k)
+        idx = idx.view(torch.int32).long()
+        chosen = logits.gather(1, idx)
+        slack = off.max()
+        assert (idx.sort(-1).values.diff(dim=-1) > 0).all() and (chosen.diff(dim=-1) <= 2 * slack).all()
+        left = logits.scatter(1, idx, -torch.inf).amax(-1)
+        assert (chosen.amin(-1) >= left - 2 * slack).all()
+        close(w, torch.softmax(chosen, -1), (2 * slack + 2.0**-20) * torch.softmax(chosen, -1) + 1e-30)
+        want = x.double() @ sgate.double().mT
+        close(g, want, hidden * 2.0**-23 * (x.double().abs() @ sgate.double().abs().mT) + last(want, F16))
+    assert fused.route_window(gate, shared, x.float(), k) is None
+    assert fused.route_window(gate, shared, x.expand(65, -1, -1).reshape(-1, hidden), k) is None
+
+
+def test_equal_logits_go_to_the_lower_index(cuda):
+    router = torch.ones(40, 64, dtype=F16, device=cuda)
+    router[7] = 0.5
+    x = torch.ones(3, 64, dtype=F16, device=cuda)
+    idx, w, _ = fused.route_window(fused.WindowLinear(router), fused.WindowLinear(router[:1]), x, 9)
+    assert idx.view(torch.int32).tolist() == [[0, 1, 2, 3, 4, 5, 6, 8, 9]] * 3
+    assert (w - 1 / 9).abs().max() < 2.0**-20
+
+
 def make_block(gen, experts, hidden, ffn, shared, group, k, from_floats=False):
     router = (hidden**-0.5 * torch.randn(experts, hidden, device="cuda", generator=gen)).half()
     sgate = (hidden**-0.5 * torch.randn(1, hidden, device="cuda", generator=gen)).half()
