@@ -541,11 +541,11 @@ SMOE_API int smoe_q4_moe(const SmoeQ4Moe* m, void* workspace, size_t workspace_b
 
 /* smoe_route for a window of 1 to 64 float16 tokens with the router's sums on the tensor cores (exact products, float32
  * sums in another order than smoe_route's): logits [tokens][experts], idx, weights [tokens][k], gate_out [tokens]
- * float16 of gate_weight (both or neither). hidden a multiple of 32, experts <= 2048, k <= 32. `counter`: one word, zero
- * before the first call and left zero; calls that may overlap need one each. */
+ * float16 of gate_weight (both or neither). hidden a multiple of 32, experts <= 2048, k <= 32. `counters`: a word for
+ * every eight tokens, zero before the first call and left zero; calls that may overlap need their own. */
 SMOE_API int smoe_route_window(const uint16_t* weight, const uint16_t* gate_weight, const uint16_t* x, int64_t tokens,
                                int64_t experts, int64_t hidden, int64_t k, float* logits, uint32_t* idx, float* weights,
-                               uint16_t* gate_out, uint32_t* counter, void* stream);
+                               uint16_t* gate_out, uint32_t* counters, void* stream);
 
 /* Whether a bounded wait of the 4-bit kernels gave up since the last clear (SMOE_ETIMEOUT; outputs since are not
  * valid). Synchronizes the device. */

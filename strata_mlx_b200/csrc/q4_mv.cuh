@@ -487,7 +487,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_product_kernel(const Produ
 template <typename T>
 __host__ __device__ constexpr int down_rows() { return sizeof(T) == 2 ? kM / 2 : kM; }
 
-constexpr int kByJob = 32;  // tiles of a CTA up to which it keeps to one job
+constexpr int kByJob = 64;  // tiles of a CTA up to which it keeps to one job
 constexpr int kTokenStride = kMt * kRows + 4;  // floats of a token's sums: rows 0, 8, .. of four tokens on 32 banks
 
 template <int G>

@@ -4,11 +4,11 @@
 //   logits[t, e] = router[e] . x[t];  idx = the k largest, ties to the lower index;  weights = softmax of the chosen;
 //   gate_out[t] = gate_weight . x[t]
 //
-// A CTA takes 16 rows of the router (the shared gate's row is one more) and every token: 16 warps share the columns, each
+// A CTA takes 16 rows of the router (the shared gate's row is one more) and eight tokens: 16 warps share the columns, each
 // m16n8k16 on its own (router rows the M side, tokens the N side, products exact, float32 sums), partial sums added in
-// the order of the columns. The last CTA to arrive takes the top-k, a warp a token. Bound by latency (the router is 2 to
-// 4 MB): the rows' first columns are loaded before the launch waits for the one before it. Next to a row's sums on CUDA
-// cores for eight tokens a CTA this reads the router once for up to 64 tokens.
+// the order of the columns. The last CTA of eight tokens to arrive takes their top-k, a warp a token. Bound by latency
+// (the router is 2 to 4 MB, read from L2 once for every eight tokens): the rows' first columns are loaded before the
+// launch waits for the one before it. All tokens in one CTA took 19 us at 32 tokens and 512 experts, eight 9 us.
 #include <algorithm>
 #include <string>
 
@@ -21,7 +21,8 @@ namespace {
 constexpr int kRwWarps = 16;
 constexpr int kRwThreads = 32 * kRwWarps;
 constexpr int kRwRows = 16;
-constexpr int kRwAhead = 5;  // runs of 32 columns a warp loads before it waits (hidden 2560: all of its own)
+constexpr int kRwAhead = 4;   // runs of 32 columns a warp loads before it waits
+constexpr int kRwWidth = 8;   // tokens of a CTA
 constexpr int kRwTokens = 64;
 
 struct RouteWindow {
@@ -34,21 +35,19 @@ struct RouteWindow {
     uint32_t* idx;
     float* weights;
     __half* gate_out;
-    uint32_t* counter;
+    uint32_t* counters;  // one for every eight tokens
     bool early;  // the router may be read before pdl_wait()
 };
 
 constexpr int kRwStride = kRwRows + 4;  // floats of a token's sums: a warp's writes and reads are on different banks
 
-template <int NT>
-constexpr size_t route_window_smem() { return size_t(kRwWarps) * 8 * NT * kRwStride * 4; }
-
-template <int NT, int NV>
-__global__ void __launch_bounds__(kRwThreads, 1) route_window_kernel(const RouteWindow a) {
-    extern __shared__ __align__(16) float part[];  // [warp][token][row]
+template <int NV>
+__global__ void __launch_bounds__(kRwThreads, NV <= 16 ? 2 : 1) route_window_kernel(const RouteWindow a) {
+    __shared__ float part[kRwWarps * kRwWidth * kRwStride];  // [warp][token][row]
     __shared__ bool last;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int row0 = blockIdx.x * kRwRows, rows = a.experts + (a.gate_weight != nullptr);
+    const int token0 = blockIdx.y * kRwWidth, tokens = min(kRwWidth, a.tokens - token0);
     const int run0 = warp * a.runs / kRwWarps, run1 = (warp + 1) * a.runs / kRwWarps;
     // this lane's rows g and g + 8 (rows past the last repeat it; their sums are not written), columns 8 t .. of a run
     auto row_of = [&](int r) {
@@ -66,17 +65,13 @@ __global__ void __launch_bounds__(kRwThreads, 1) route_window_kernel(const Route
     }
     pdl_wait();
     pdl_release();
-    const __half* xp[NT];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) xp[nt] = a.x + min(8 * nt + g, a.tokens - 1) * a.hidden + 8 * t;
-    float acc[NT][4] = {};
+    // (columns past the tokens repeat the first one; their sums are not written)
+    const __half* xp = a.x + (token0 + (g < tokens ? g : 0)) * a.hidden + 8 * t;
+    float acc[4] = {};
     auto step = [&](const uint4& u, const uint4& v, int run) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const uint4 x = *reinterpret_cast<const uint4*>(xp[nt] + 32 * run);
-            q4::mma_f16<false>(acc[nt], u.x, v.x, u.y, v.y, x.x, x.y);
-            q4::mma_f16<false>(acc[nt], u.z, v.z, u.w, v.w, x.z, x.w);
-        }
+        const uint4 x = *reinterpret_cast<const uint4*>(xp + 32 * run);
+        q4::mma_f16<false>(acc, u.x, v.x, u.y, v.y, x.x, x.y);
+        q4::mma_f16<false>(acc, u.z, v.z, u.w, v.w, x.z, x.w);
     };
 #pragma unroll
     for (int i = 0; i < kRwAhead; ++i)
@@ -84,49 +79,43 @@ __global__ void __launch_bounds__(kRwThreads, 1) route_window_kernel(const Route
     for (int run = run0 + kRwAhead; run < run1; ++run)
         step(__ldg(reinterpret_cast<const uint4*>(wa + 32 * run)), __ldg(reinterpret_cast<const uint4*>(wb + 32 * run)), run);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            part[(warp * 8 * NT + 8 * nt + 2 * t + (i & 1)) * kRwStride + g + 8 * (i >> 1)] = acc[nt][i];
+    for (int i = 0; i < 4; ++i) part[(warp * kRwWidth + 2 * t + (i & 1)) * kRwStride + g + 8 * (i >> 1)] = acc[i];
     __syncthreads();
-    for (int i = threadIdx.x; i < kRwRows * a.tokens; i += kRwThreads) {
-        const int r = i & (kRwRows - 1), n = i / kRwRows, row = row0 + r;
+    if (threadIdx.x < kRwRows * tokens) {
+        const int r = threadIdx.x & (kRwRows - 1), n = threadIdx.x / kRwRows, row = row0 + r;
         float sum = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kRwWarps; ++w) sum += part[(w * 8 * NT + n) * kRwStride + r];
-        if (row < a.experts) a.logits[n * int64_t(a.experts) + row] = sum;
-        else if (row < rows) a.gate_out[n] = __float2half_rn(sum);
+        for (int w = 0; w < kRwWarps; ++w) sum += part[(w * kRwWidth + n) * kRwStride + r];
+        if (row < a.experts) a.logits[(token0 + n) * int64_t(a.experts) + row] = sum;
+        else if (row < rows) a.gate_out[token0 + n] = __float2half_rn(sum);
     }
     __threadfence();
     __syncthreads();
-    if (threadIdx.x == 0) last = atomicAdd(a.counter, 1u) == gridDim.x - 1;
+    if (threadIdx.x == 0) last = atomicAdd(&a.counters[blockIdx.y], 1u) == gridDim.x - 1;
     __syncthreads();
     if (!last) return;
     __threadfence();
-    for (int n = warp; n < a.tokens; n += kRwWarps) {
+    if (warp < tokens) {
+        const int n = token0 + warp;
         const float* in = a.logits + n * int64_t(a.experts);
         topk_row<NV>([&](int j) { return __ldcg(in + j); }, a.experts, a.k, a.idx + n * a.k, a.weights + n * a.k);
-        __syncwarp();
     }
-    if (threadIdx.x == 0) *a.counter = 0u;
+    if (threadIdx.x == 0) a.counters[blockIdx.y] = 0u;
 }
 
-template <int NT>
 int launch(const RouteWindow& a, const Writes& w, cudaStream_t st) {
     auto go = [&](auto kernel) {
-        const size_t smem = route_window_smem<NT>();
-        cudaError_t e = static_cast<cudaError_t>(-max_smem(kernel, static_cast<int>(smem)));
         const int rows = a.experts + (a.gate_weight != nullptr);
-        if (e == cudaSuccess)
-            e = launch_pdl(w, kernel, dim3((rows + kRwRows - 1) / kRwRows), dim3(kRwThreads), smem, st, a);
+        const dim3 grid((rows + kRwRows - 1) / kRwRows, (a.tokens + kRwWidth - 1) / kRwWidth);
+        const cudaError_t e = launch_pdl(w, kernel, grid, dim3(kRwThreads), 0, st, a);
         if (e == cudaSuccess) return launch_status("route_window");
         cudaGetLastError();
         return fail(-static_cast<int>(e), std::string("route_window: ") + cudaGetErrorString(e));
     };
-    if (a.experts <= 256) return go(route_window_kernel<NT, 8>);
-    if (a.experts <= 512) return go(route_window_kernel<NT, 16>);
-    if (a.experts <= 1024) return go(route_window_kernel<NT, 32>);
-    return go(route_window_kernel<NT, 64>);
+    if (a.experts <= 256) return go(route_window_kernel<8>);
+    if (a.experts <= 512) return go(route_window_kernel<16>);
+    if (a.experts <= 1024) return go(route_window_kernel<32>);
+    return go(route_window_kernel<64>);
 }
 
 }  // namespace
@@ -136,9 +125,9 @@ using namespace smoe;
 
 extern "C" int smoe_route_window(const uint16_t* weight, const uint16_t* gate_weight, const uint16_t* x, int64_t tokens,
                                  int64_t experts, int64_t hidden, int64_t k, float* logits, uint32_t* idx, float* weights,
-                                 uint16_t* gate_out, uint32_t* counter, void* stream) {
+                                 uint16_t* gate_out, uint32_t* counters, void* stream) {
     if (tokens == 0) return SMOE_OK;
-    SMOE_REQUIRE(weight && x && logits && idx && weights && counter && tokens > 0 && experts > 0, SMOE_EARG,
+    SMOE_REQUIRE(weight && x && logits && idx && weights && counters && tokens > 0 && experts > 0, SMOE_EARG,
                  "route_window: null pointer or empty router");
     SMOE_REQUIRE((gate_weight == nullptr) == (gate_out == nullptr), SMOE_EARG,
                  "the shared gate's weight and output come together");
@@ -164,13 +153,10 @@ extern "C" int smoe_route_window(const uint16_t* weight, const uint16_t* gate_we
     a.idx = idx;
     a.weights = weights;
     a.gate_out = reinterpret_cast<__half*>(gate_out);
-    a.counter = counter;
+    a.counters = counters;
     a.early = pdl_early(st, weight, size_t(experts) * hidden * 2) && pdl_early(st, gate_weight, size_t(hidden) * 2);
     Writes w;
     w.add(logits, size_t(tokens) * experts * 4).add(idx, size_t(tokens) * k * 4).add(weights, size_t(tokens) * k * 4);
-    w.add(gate_out, size_t(tokens) * 2).add(counter, 4);
-    if (tokens <= 8) return launch<1>(a, w, st);
-    if (tokens <= 16) return launch<2>(a, w, st);
-    if (tokens <= 32) return launch<4>(a, w, st);
-    return launch<8>(a, w, st);
+    w.add(gate_out, size_t(tokens) * 2).add(counters, size_t(tokens + 7) / 8 * 4);
+    return launch(a, w, st);
 }

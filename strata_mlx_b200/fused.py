@@ -236,9 +236,9 @@ def route_window(gate: "WindowLinear", shared_gate: "WindowLinear", x: torch.Ten
     idx = torch.empty((tokens, k), dtype=torch.uint32, device=dev)
     w = torch.empty((tokens, k), dtype=torch.float32, device=dev)
     g = torch.empty((tokens,), dtype=x.dtype, device=dev)
-    counter = _route_counters(4, False, dev)
+    counters = _route_counters(32, False, dev)
     _lib.call("smoe_route_window", _lib.ptr(wt), _lib.ptr(gw), _lib.ptr(x2), tokens, gate.rows, gate.cols, k,
-              _lib.ptr(logits), _lib.ptr(idx), _lib.ptr(w), _lib.ptr(g), _lib.ptr(counter), _lib.stream())
+              _lib.ptr(logits), _lib.ptr(idx), _lib.ptr(w), _lib.ptr(g), _lib.ptr(counters), _lib.stream())
     lead = x.shape[:-1]
     return idx.reshape(*lead, k), w.reshape(*lead, k), g.reshape(*lead, 1)
 
