@@ -174,7 +174,7 @@ struct PairBlocks {
     int n;
 };
 __host__ __device__ constexpr size_t pair_blocks_bytes(int64_t pairs, int64_t experts) {
-    return pairs > 0 ? (size_t(experts) * 4 + size_t(pairs) * 10 + 15) & ~size_t(15) : 0;
+    return pairs > 0 ? (size_t(experts) * 4 + size_t(pairs) * 12 + 15) & ~size_t(15) : 0;
 }
 __device__ __forceinline__ PairBlocks pair_blocks(uint8_t* mem, const uint32_t* __restrict__ idx, int pairs, int experts,
                                                   int most, int* warp_sums) {
@@ -185,6 +185,7 @@ __device__ __forceinline__ PairBlocks pair_blocks(uint8_t* mem, const uint32_t* 
     b.expert = place + pairs;
     b.start = b.expert + pairs;
     b.count = b.start + pairs;
+    uint16_t* key = b.count + pairs;  // a pair's expert, or none
     const int tid = threadIdx.x;
     if (pairs <= 32) {
         // (a decode step's few pairs: one warp, one barrier)
@@ -212,16 +213,21 @@ __device__ __forceinline__ PairBlocks pair_blocks(uint8_t* mem, const uint32_t* 
         b.n = warp_sums[0];
         return b;
     }
+    constexpr uint16_t kNone = 0xffff;
     for (int e = tid; e < experts; e += kThreads) seen[e] = 0;
+    for (int p = tid; p < pairs; p += kThreads) {
+        const uint32_t e = idx[p];
+        key[p] = e < uint32_t(experts) ? uint16_t(e) : kNone;
+    }
     __syncthreads();
     if (tid < 32) {
         // places in pair order (one warp, 32 pairs at a time): every CTA must cut an expert's pairs into the same blocks
         for (int p0 = 0; p0 < pairs; p0 += 32) {
             const int p = p0 + tid;
-            const uint32_t e = p < pairs ? idx[p] : 0xffffffffu;
+            const uint32_t e = p < pairs ? key[p] : kNone;
             const uint32_t same = __match_any_sync(0xffffffffu, e);
             const int before = __popc(same & ((1u << tid) - 1));
-            if (e < uint32_t(experts)) {
+            if (e != kNone) {
                 const uint32_t n = seen[e];
                 place[p] = uint16_t(n + before);
                 __syncwarp(same);
@@ -252,10 +258,8 @@ __device__ __forceinline__ PairBlocks pair_blocks(uint8_t* mem, const uint32_t* 
         at += n;
     }
     __syncthreads();
-    for (int p = tid; p < pairs; p += kThreads) {
-        const uint32_t e = idx[p];
-        if (e < uint32_t(experts)) b.list[seen[e] + place[p]] = uint16_t(p);
-    }
+    for (int p = tid; p < pairs; p += kThreads)
+        if (key[p] != kNone) b.list[seen[key[p]] + place[p]] = uint16_t(p);
     __syncthreads();
     return b;
 }
@@ -393,10 +397,6 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_product_kernel(const Produ
     if (!a.early) pdl_wait();
     // the dense part's weights, while the launch before still runs
     for (int i = 0; i < kStages; ++i) fetch();
-    // (and a first go at the pairs, whatever idx holds yet: nothing of it is used, but the code is in the cache when it
-    // counts, 1 us earlier)
-    if (a.pairs > 0)
-        pair_blocks(table, a.idx, static_cast<int>(a.pairs), static_cast<int>(a.experts), kM, warp_sums);
     pdl_wait();
     if (a.pairs > 0) {
         blocks = pair_blocks(table, a.idx, static_cast<int>(a.pairs), static_cast<int>(a.experts), kM, warp_sums);
@@ -607,6 +607,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_down_kernel(const DownArgs
     for (int job = job_first; job < job_last; ++job) {
         for (int i = lane; i < tokens * kTokenStride; i += 32) mine[i] = 0.0f;
         __syncwarp();
+        float acc[kMt][4] = {};
         for (Cursor c = cursor_of(job); c.left > 0;) {
             const bool shared = c.seg < sblocks;
             const int start = shared ? c.seg * kRowsIn : blocks.start[c.seg - sblocks];
@@ -616,9 +617,9 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_down_kernel(const DownArgs
             const T* xp = static_cast<const T*>(shared ? a.hs : a.h) +
                           ((shared ? of : blocks.list[of]) * kPieces + g / kRowsIn) * width + c.tile * kCols + 8 * t;
             const int n = tiles_of(c);
-            float acc[kMt][4] = {};
             stream_tiles<T, G>(ring, fetch, xp, n, static_cast<int>(width / 32) - 4 * c.tile, lane, acc, one);
             next_segment(c, n);
+            if (tokens == 1 && c.left > 0) continue;  // (one token: one row of h a block, and all blocks one sum)
             // each column's sums to its token, this lane's columns 2 t and 2 t + 1 (with pieces, those of columns 2 t + 4
             // and 2 t + 5 added). A token that names an expert twice has two columns here, neighbours: column by column then.
             if constexpr (kPieces == 2) {
@@ -648,6 +649,10 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_down_kernel(const DownArgs
                 if (2 * t + 1 < count) add(1);
             }
             __syncwarp();
+#pragma unroll
+            for (int m = 0; m < kMt; ++m)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[m][i] = 0.0f;
         }
         __syncthreads();
         const int at = job * items;

@@ -1,9 +1,10 @@
 // 4-bit weights with group scales: floats to codes and back, the layout of the kernels, and the entry points of the
 // products and of a MoE block on them.
 //
-// The conversions are one pass over memory each: a thread holds eight columns (one code word), so a warp reads 512
-// bytes of float16 or 1 KB of float32 in 16-byte pieces and writes 128 bytes of codes; a group's extremes come from
-// the 4, 8 or 16 lanes that hold it by shuffles. Bound by HBM.
+// The conversions are one pass over memory each, bound by HBM: every access of a thread to floats is 16 bytes next to its
+// neighbours' (8 float16 weights and a 32-bit word of codes, or 4 float32 weights and half a word; float32 in two
+// pieces a thread, 32 bytes apart between neighbours, ran at 4.1 TB/s), four of them in flight. A group's extremes come
+// from the lanes that hold it by shuffles.
 #include <algorithm>
 #include <string>
 
@@ -25,107 +26,168 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
-__device__ __forceinline__ void load8(const __half* p, float (&f)[8]) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+// 16 bytes of floats, and the codes that go with them
+template <typename T> struct Piece;
+template <>
+struct Piece<__half> {
+    using Word = uint32_t;
+    static constexpr int kN = 8;
+    static __device__ __forceinline__ void load(const __half* p, float (&f)[8]) {
+        const uint4 v = *reinterpret_cast<const uint4*>(p);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 q = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-        f[2 * i] = q.x;
-        f[2 * i + 1] = q.y;
+        for (int i = 0; i < 4; ++i) {
+            const float2 q = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            f[2 * i] = q.x;
+            f[2 * i + 1] = q.y;
+        }
     }
-}
-__device__ __forceinline__ void load8(const float* p, float (&f)[8]) {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-}
-__device__ __forceinline__ void store8(__half* p, const float (&f)[8]) {
-    uint4 v;
-    v.x = tc::pack_half2(f[0], f[1]);
-    v.y = tc::pack_half2(f[2], f[3]);
-    v.z = tc::pack_half2(f[4], f[5]);
-    v.w = tc::pack_half2(f[6], f[7]);
-    *reinterpret_cast<uint4*>(p) = v;
-}
-__device__ __forceinline__ void store8(float* p, const float (&f)[8]) {
-    *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
-    *reinterpret_cast<float4*>(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
-}
+    static __device__ __forceinline__ void store(__half* p, const float (&f)[8]) {
+        *reinterpret_cast<uint4*>(p) = make_uint4(tc::pack_half2(f[0], f[1]), tc::pack_half2(f[2], f[3]),
+                                                  tc::pack_half2(f[4], f[5]), tc::pack_half2(f[6], f[7]));
+    }
+};
+template <>
+struct Piece<float> {
+    using Word = uint16_t;
+    static constexpr int kN = 4;
+    static __device__ __forceinline__ void load(const float* p, float (&f)[4]) {
+        const float4 v = *reinterpret_cast<const float4*>(p);
+        f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
+    }
+    static __device__ __forceinline__ void store(float* p, const float (&f)[4]) {
+        *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
+    }
+};
+constexpr int kConvPieces = 4;  // of a thread
+constexpr float kRound = 12582912.0f;  // 1.5 * 2^23
 
-// words = rows cols / 8. The arithmetic of each value is a chain of single IEEE float32 operations (difference,
-// quotient, rounding to even), so the codes are the formula's exactly.
+// pieces = rows cols / kN. The arithmetic of each value is a chain of single IEEE float32 operations (difference,
+// quotient, rounding to even), so the codes are the formula's exactly. A quotient is a product with the reciprocal
+// of 15 scales (clamped to 0 .. 1 for free, then times 15), within 15 x 4 x 2^-23 of the division's: only one that close to
+// the border of two codes is divided out (a division for every value was 106 us for 24576 x 4096 float32, bound by its instructions; the bytes are
+// 72 us).
 template <typename T, int G>
-__global__ void __launch_bounds__(kConvThreads) q4_quantize_kernel(const T* __restrict__ w, int64_t words,
-                                                                   uint32_t* __restrict__ codes,
+__global__ void __launch_bounds__(kConvThreads) q4_quantize_kernel(const T* __restrict__ w, int64_t pieces,
+                                                                   typename Piece<T>::Word* __restrict__ codes,
                                                                    __half* __restrict__ scales,
                                                                    __half* __restrict__ biases) {
-    const int64_t i = int64_t(blockIdx.x) * kConvThreads + threadIdx.x;
-    const bool in = i < words;
-    float f[8] = {};
-    if (in) load8(w + 8 * i, f);
-    float lo = f[0], hi = f[0];
+    constexpr int N = Piece<T>::kN, kLanes = G / N;  // lanes of a group
+    // (a warp's pieces are 32 apart: its scales and biases are one sector each)
+    const int lane = threadIdx.x & 31;
+    const int64_t i0 = (int64_t(blockIdx.x) * kConvThreads + (threadIdx.x & ~31)) * kConvPieces + lane;
+    float f[kConvPieces][N] = {};
 #pragma unroll
-    for (int j = 1; j < 8; ++j) {
-        lo = min_nan(lo, f[j]);
-        hi = max_nan(hi, f[j]);
-    }
-    // (a group's lanes are all in or all out: words is a multiple of G / 8)
+    for (int c = 0; c < kConvPieces; ++c)
+        if (i0 + c * 32 < pieces) Piece<T>::load(w + N * (i0 + c * 32), f[c]);
+    float lo[kConvPieces], hi[kConvPieces];
 #pragma unroll
-    for (int o = 1; o < G / 8; o <<= 1) {
-        lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    }
-    if (!in) return;
-    const __half sh = __float2half_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.0f)), bh = __float2half_rn(lo);
-    const float s = __half2float(sh), b = __half2float(bh);
-    uint32_t word = 0;
+    for (int c = 0; c < kConvPieces; ++c) {
+        lo[c] = hi[c] = f[c][0];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        float q = s > 0.0f ? rintf(__fdiv_rn(__fsub_rn(f[j], b), s)) : 0.0f;
-        q = fminf(fmaxf(q, 0.0f), 15.0f);  // (a NaN becomes code 0; its group's scale or bias is not finite either)
-        word |= static_cast<uint32_t>(q) << (4 * j);
+        for (int j = 1; j < N; ++j) {
+            lo[c] = min_nan(lo[c], f[c][j]);
+            hi[c] = max_nan(hi[c], f[c][j]);
+        }
+        // (a group's lanes are all in or all out: pieces is a multiple of kLanes)
+#pragma unroll
+        for (int o = 1; o < kLanes; o <<= 1) {
+            lo[c] = min_nan(lo[c], __shfl_xor_sync(0xffffffffu, lo[c], o));
+            hi[c] = max_nan(hi[c], __shfl_xor_sync(0xffffffffu, hi[c], o));
+        }
     }
-    codes[i] = word;
-    if (i % (G / 8) == 0) {
-        scales[i / (G / 8)] = sh;
-        biases[i / (G / 8)] = bh;
+    // a lane in four works out one piece's scale, bias and reciprocal for its group (kLanes is 4 or more): the divisions
+    static_assert(kConvPieces == 4, "one piece for each of four lanes");
+    const int own = lane & 3;
+    float l = lo[0], h = hi[0];
+#pragma unroll
+    for (int c = 1; c < kConvPieces; ++c) {
+        if (own == c) l = lo[c], h = hi[c];
+    }
+    const __half2 mine = __halves2half2(__float2half_rn(__fdiv_rn(__fsub_rn(h, l), 15.0f)), __float2half_rn(l));
+    const float my_inverse = __low2float(mine) > 0.0f ? __fdiv_rn(1.0f / 15.0f, __low2float(mine)) : 0.0f;
+#pragma unroll
+    for (int c = 0; c < kConvPieces; ++c) {
+        const int64_t i = i0 + c * 32;
+        const uint32_t both = __shfl_sync(0xffffffffu, *reinterpret_cast<const uint32_t*>(&mine), (lane & ~3) | c);
+        const float inverse = __shfl_sync(0xffffffffu, my_inverse, (lane & ~3) | c);
+        if (i >= pieces) continue;
+        const __half2 sb = *reinterpret_cast<const __half2*>(&both);
+        const float s = __low2float(sb), b = __high2float(sb);
+        // (the code is clamped before it is rounded, which is the same; adding kRound rounds to even into the sum's low bits,
+        // where rintf and a conversion would take a quarter-rate instruction each; a NaN becomes code 0, its group's scale
+        // or bias is not finite either)
+        uint32_t word = 0;
+        float worst = 0.0f;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const float v = __saturatef(__fsub_rn(f[c][j], b) * inverse);  // a fifteenth of the code
+            const float sum = fmaf(v, 15.0f, kRound);
+            worst = fmaxf(worst, fabsf(fmaf(v, 15.0f, kRound - sum)));
+            word += (__float_as_uint(sum) - __float_as_uint(kRound)) << (4 * j);
+        }
+        if (worst > 0.5f - 1e-5f) {
+            word = 0;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const float v = fminf(fmaxf(__fdiv_rn(__fsub_rn(f[c][j], b), s), 0.0f), 15.0f);
+                word += (__float_as_uint(__fadd_rn(v, kRound)) - __float_as_uint(kRound)) << (4 * j);
+            }
+        }
+        codes[i] = static_cast<typename Piece<T>::Word>(word);
+    }
+    const int64_t of = i0 + own * 32;
+    if ((lane & (kLanes - 1)) == own && of < pieces) {
+        scales[of / kLanes] = __low2half(mine);
+        biases[of / kLanes] = __high2half(mine);
     }
 }
 
-// w = code * scale + bias in float32 (two roundings), then to T. With `packed`, from the kernels' layout: word i of
-// the matrix's rows x cols / 8.
-template <typename T>
-__global__ void __launch_bounds__(kConvThreads) q4_dequant_kernel(const uint32_t* __restrict__ codes,
+// w = code * scale + bias in float32 (two roundings), then to T. PACKED: from the kernels' layout. group_log: log2 of a
+// group's columns.
+template <typename T, bool PACKED>
+__global__ void __launch_bounds__(kConvThreads) q4_dequant_kernel(const uint8_t* __restrict__ codes,
                                                                   const __half* __restrict__ scales,
-                                                                  const __half* __restrict__ biases,
-                                                                  const uint8_t* __restrict__ packed, int64_t words,
-                                                                  int64_t rows, int64_t cols, int group,
+                                                                  const __half* __restrict__ biases, int64_t pieces,
+                                                                  int64_t rows, int64_t cols, int group_log,
                                                                   T* __restrict__ out) {
-    const int64_t i = int64_t(blockIdx.x) * kConvThreads + threadIdx.x;
-    if (i >= words) return;
-    uint32_t word;
-    float s, b;
-    if (packed == nullptr) {
-        word = codes[i];
-        const int64_t at = i / (group / 8);
-        s = __half2float(scales[at]);
-        b = __half2float(biases[at]);
-    } else {
-        const int64_t per_row = cols / 8, all = i / per_row;
-        const int c = static_cast<int>(i - all * per_row) * 8;
-        const int64_t e = all / rows, r = all - e * rows;
-        const uint8_t* tile = packed + ((e * strips_of_rows(rows) + r / kRows) * tiles_of_cols(cols) + c / kCols) *
-                                           tile_bytes_of(group);
-        const int row = static_cast<int>(r % kRows), j = (c % kCols) / 32, t = (c % 32) / 8;
-        word = nibbles_out(*reinterpret_cast<const uint32_t*>(tile + chunk_at(row, t) + 4 * j));
-        const __half2 p = *reinterpret_cast<const __half2*>(tile + kCodeBytes + (row * (kCols / group) + (c % kCols) / group) * 4);
-        s = __low2float(p);
-        b = __high2float(p);
-    }
-    float f[8];
+    using Word = typename Piece<T>::Word;
+    constexpr int N = Piece<T>::kN;
+    const int64_t i0 = int64_t(blockIdx.x) * kConvThreads * kConvPieces + threadIdx.x;
+    uint32_t word[kConvPieces];
+    float s[kConvPieces], b[kConvPieces];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = __fadd_rn(__fmul_rn(static_cast<float>((word >> (4 * j)) & 15u), s), b);
-    store8(out + 8 * i, f);
+    for (int c = 0; c < kConvPieces; ++c) {
+        const int64_t i = i0 + c * kConvThreads;
+        if (i >= pieces) continue;
+        if constexpr (!PACKED) {
+            word[c] = reinterpret_cast<const Word*>(codes)[i];
+            const int64_t at = N * i >> group_log;
+            s[c] = __half2float(scales[at]);
+            b[c] = __half2float(biases[at]);
+        } else {
+            const int group = 1 << group_log;
+            const int64_t all = N * i / cols, e = all / rows, r = all - e * rows;
+            const int col = static_cast<int>(N * i - all * cols);
+            const uint8_t* tile = codes + ((e * strips_of_rows(rows) + r / kRows) * tiles_of_cols(cols) + col / kCols) *
+                                              tile_bytes_of(group);
+            const int row = static_cast<int>(r % kRows), j = (col % kCols) / 32, t = (col % 32) / 8;
+            word[c] = nibbles_out(*reinterpret_cast<const uint32_t*>(tile + chunk_at(row, t) + 4 * j)) >> (col % 8 * 4);
+            const __half2 p =
+                *reinterpret_cast<const __half2*>(tile + kCodeBytes + (row * (kCols / group) + (col % kCols) / group) * 4);
+            s[c] = __low2float(p);
+            b[c] = __high2float(p);
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < kConvPieces; ++c) {
+        const int64_t i = i0 + c * kConvThreads;
+        if (i >= pieces) continue;
+        float f[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) f[j] = __fadd_rn(__fmul_rn(static_cast<float>((word[c] >> (4 * j)) & 15u), s[c]), b[c]);
+        Piece<T>::store(out + N * i, f);
+    }
 }
 
 // One 32-bit word of the layout a thread: codes, or a (scale, bias) pair.
@@ -205,18 +267,19 @@ extern "C" int smoe_q4_quantize(const void* w, int dtype, int64_t rows, int64_t 
     if (rows == 0) return SMOE_OK;
     if (int s = check_matrix(rows, cols, group)) return s;
     SMOE_REQUIRE(w && codes && scales && biases && aligned16(w), SMOE_EARG, "q4_quantize: null or misaligned pointer");
-    const int64_t words = rows * (cols / 8);
+    const int64_t pieces = rows * cols / (dtype == SMOE_F16 ? 8 : 4);
     unsigned grid;
-    if (int s = conv_grid(words, &grid)) return s;
+    if (int s = conv_grid((pieces + kConvPieces - 1) / kConvPieces, &grid)) return s;
     cudaStream_t st = as_stream(stream);
     __half* sp = reinterpret_cast<__half*>(scales);
     __half* bp = reinterpret_cast<__half*>(biases);
     auto go = [&](auto xt) {
         using XT = decltype(xt);
         const XT* p = static_cast<const XT*>(w);
-        if (group == 32) q4_quantize_kernel<XT, 32><<<grid, kConvThreads, 0, st>>>(p, words, codes, sp, bp);
-        else if (group == 64) q4_quantize_kernel<XT, 64><<<grid, kConvThreads, 0, st>>>(p, words, codes, sp, bp);
-        else q4_quantize_kernel<XT, 128><<<grid, kConvThreads, 0, st>>>(p, words, codes, sp, bp);
+        auto* c = reinterpret_cast<typename Piece<XT>::Word*>(codes);
+        if (group == 32) q4_quantize_kernel<XT, 32><<<grid, kConvThreads, 0, st>>>(p, pieces, c, sp, bp);
+        else if (group == 64) q4_quantize_kernel<XT, 64><<<grid, kConvThreads, 0, st>>>(p, pieces, c, sp, bp);
+        else q4_quantize_kernel<XT, 128><<<grid, kConvThreads, 0, st>>>(p, pieces, c, sp, bp);
     };
     if (dtype == SMOE_F16) go(__half{});
     else if (dtype == SMOE_F32) go(float{});
@@ -232,20 +295,25 @@ static int dequant(const uint32_t* codes, const uint16_t* scales, const uint16_t
     SMOE_REQUIRE(experts > 0, SMOE_ESHAPE, "q4_dequant: a negative number of matrices");
     SMOE_REQUIRE((packed ? aligned16(packed) : codes && scales && biases) && out && aligned16(out), SMOE_EARG,
                  "q4_dequant: null or misaligned pointer");
-    const int64_t words = experts * rows * (cols / 8);
+    SMOE_REQUIRE(out_dtype == SMOE_F16 || out_dtype == SMOE_F32, SMOE_EDTYPE, "q4_dequant gives float16 or float32");
+    const int64_t pieces = experts * rows * cols / (out_dtype == SMOE_F16 ? 8 : 4);
     unsigned grid;
-    if (int s = conv_grid(words, &grid)) return s;
+    if (int s = conv_grid((pieces + kConvPieces - 1) / kConvPieces, &grid)) return s;
     cudaStream_t st = as_stream(stream);
     const __half* sp = reinterpret_cast<const __half*>(scales);
     const __half* bp = reinterpret_cast<const __half*>(biases);
-    if (out_dtype == SMOE_F16)
-        q4_dequant_kernel<__half><<<grid, kConvThreads, 0, st>>>(codes, sp, bp, packed, words, rows, cols, group,
-                                                               static_cast<__half*>(out));
-    else if (out_dtype == SMOE_F32)
-        q4_dequant_kernel<float><<<grid, kConvThreads, 0, st>>>(codes, sp, bp, packed, words, rows, cols, group,
-                                                              static_cast<float*>(out));
-    else
-        return fail(SMOE_EDTYPE, "q4_dequant gives float16 or float32");
+    const uint8_t* from = packed != nullptr ? packed : reinterpret_cast<const uint8_t*>(codes);
+    const int group_log = group == 32 ? 5 : group == 64 ? 6 : 7;
+    auto go = [&](auto kernel, auto* o) {
+        kernel<<<grid, kConvThreads, 0, st>>>(from, sp, bp, pieces, rows, cols, group_log, o);
+    };
+    if (out_dtype == SMOE_F16) {
+        __half* o = static_cast<__half*>(out);
+        packed ? go(q4_dequant_kernel<__half, true>, o) : go(q4_dequant_kernel<__half, false>, o);
+    } else {
+        float* o = static_cast<float*>(out);
+        packed ? go(q4_dequant_kernel<float, true>, o) : go(q4_dequant_kernel<float, false>, o);
+    }
     return launch_status("q4_dequant");
 }
 
