@@ -229,19 +229,18 @@ __global__ void __launch_bounds__(kGThreads, 1) q4_matmul_kernel(const GemmArgs 
             wait_for(&S.bfull[st % g.nb], (st / g.nb) & 1);
         }
     } else if (warp == kGDecoders) {
-        // ---------------- MMA (the converged warp issues, one elected lane)
-        const uint32_t idesc = tc::idesc_f16_f32(kGM, g.n);
-        Phase ap, bp, dp;
-        int count = 0;
-        for (int job = blockIdx.x; job < jobs && ok; job += gridDim.x, ++count, dp.next(nd)) {
-            if (count >= nd && !(ok = wait(&S.dfree[dp.slot], dp.phase ^ 1))) break;
-            tc::fence_after_sync();
-            const uint32_t d = tmem + uint32_t(g.n * dp.slot);
-            for (int s = 0; s < nk; ++s, ap.next(kGASlots), bp.next(g.nb)) {
-                if (!(ok = wait(&S.afull[ap.slot], ap.phase)) || !(ok = wait(&S.bfull[bp.slot], bp.phase))) break;
-                tc::fence_after_sync();
-                const uint64_t bd = tc::smem_desc_sw128(smem_addr(smem) + bp.slot * bslot);
-                if (elect_one()) {
+        // ---------------- MMA: one lane alone waits and issues
+        if (elect_one()) {
+            const uint32_t idesc = tc::idesc_f16_f32(kGM, g.n);
+            Phase ap, bp, dp;
+            int count = 0;
+            for (int job = blockIdx.x; job < jobs && ok; job += gridDim.x, ++count, dp.next(nd)) {
+                if (count >= nd && !(ok = wait_for(&S.dfree[dp.slot], dp.phase ^ 1))) break;
+                const uint32_t d = tmem + uint32_t(g.n * dp.slot);
+                for (int s = 0; s < nk; ++s, ap.next(kGASlots), bp.next(g.nb)) {
+                    if (!(ok = wait_for(&S.afull[ap.slot], ap.phase)) || !(ok = wait_for(&S.bfull[bp.slot], bp.phase))) break;
+                    tc::fence_after_sync();
+                    const uint64_t bd = tc::smem_desc_sw128(smem_addr(smem) + bp.slot * bslot);
 #pragma unroll
                     for (int k = 0; k < kCols / 16; ++k)
                         tc::mma_f16_ts(d, tmem + kGAColumn + 64u * ap.slot + 8u * k,
@@ -251,9 +250,10 @@ __global__ void __launch_bounds__(kGThreads, 1) q4_matmul_kernel(const GemmArgs 
                     tc::mma_commit(&S.bfree[bp.slot]);
                     if (s == nk - 1) tc::mma_commit(&S.dfull[dp.slot]);
                 }
-                __syncwarp();
             }
+            if (!ok) atomicExch(&g_q4_gemm_status, SMOE_ETIMEOUT);
         }
+        __syncwarp();
     } else {
         // ---------------- decoders and the end of a job: thread L of the four lane quarters is weight row L. A group of
         // eight warps takes every other stage, the two warps of a quarter two of the four chunks of the row's tile each
