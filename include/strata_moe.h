@@ -510,7 +510,9 @@ typedef struct SmoeQ4Product {
 } SmoeQ4Product;
 SMOE_API int smoe_q4_product(const SmoeQ4Product* p, void* stream);
 
-/* smoe_q4_product's dense part alone: out[t, r] = W[r, :] . x[t, :] for t < tokens (`nn.QuantizedLinear`). */
+/* smoe_q4_product's dense part alone: out[t, r] = W[r, :] . x[t, :] for t < tokens (`nn.QuantizedLinear`). More than 16
+ * float16 tokens may take the prompt's kernel, which rounds each weight to float16 once; up to 16 get the same bits each
+ * alone as together. */
 SMOE_API int smoe_q4_linear(const uint8_t* packed, int64_t rows, int64_t cols, int group, const void* x, int64_t tokens,
                             void* out, int dtype, void* stream);
 
@@ -519,9 +521,9 @@ SMOE_API int smoe_q4_linear(const uint8_t* packed, int64_t rows, int64_t cols, i
  *   out[t] = sum_j weights[t, j] down_e(silu(gate_e x) * up_e x) + sigmoid(shared_gate[t]) shared(x), e = idx[t, j]
  * gate, up: (experts, ffn, hidden) with groups of `group` columns, down: (experts, hidden, ffn) with `down_group`; the
  * shared expert's likewise with shared_ffn rows (0: none; shared_gate null: not gated). A choice idx >= experts adds
- * nothing. Sums and SwiGLU are float32; between the launches the SwiGLU times its weight is kept in 22 bits or
- * more. Workspace:
- * smoe_q4_moe_workspace_size() bytes, one for each call in flight. Replaces `_Routed.__call__` behind its router
+ * nothing. Sums and SwiGLU are float32; between the launches the SwiGLU times its weight is kept in 22 bits (down to
+ * 2^-25; float16 activations: within float16's range). Workspace: smoe_q4_moe_workspace_size() bytes, one for each call in
+ * flight. Replaces `_Routed.__call__` behind its router
  * (strata_mlx/fused.py:491-497). Weights as smoe_q4_product's. */
 typedef struct SmoeQ4Moe {
     int dtype;
@@ -547,8 +549,8 @@ SMOE_API int smoe_route_window(const uint16_t* weight, const uint16_t* gate_weig
                                int64_t experts, int64_t hidden, int64_t k, float* logits, uint32_t* idx, float* weights,
                                uint16_t* gate_out, uint32_t* counters, void* stream);
 
-/* Whether a bounded wait of the 4-bit kernels gave up since the last clear (SMOE_ETIMEOUT; outputs since are not
- * valid). Synchronizes the device. */
+/* Whether a bounded wait of the 4-bit kernels gave up on the current device since the last clear (SMOE_ETIMEOUT; outputs
+ * since are not valid). Synchronizes the device. */
 SMOE_API int smoe_q4_status(int* status, int clear);
 
 #ifdef __cplusplus

@@ -12,7 +12,8 @@ strata_mlx/mtp.py:34-75).
 
 A weight is code * scale + bias with a code of 4 bits, eight codes to a 32-bit word (weight 8 j + i in bits 4 i of
 word j), groups of 32, 64 or 128 columns. A layer lays its arrays out once for the kernels (libstrata_moe.so) and
-keeps that alone. Products are exact in each weight (codes are not rounded to floats first) with float32 sums.
+keeps that alone. Products are exact in each weight (codes are not rounded to floats first) with float32 sums; a layer's
+product of more than 16 float16 tokens may go by a kernel that rounds each weight to float16 once (as `dequantize` does).
 Activations are float16 or float32; tensors are torch CUDA tensors and there is no CPU path.
 """
 
@@ -57,7 +58,7 @@ def _check_parts(codes, scales, biases, group_size, bits=BITS):
     if scales.dtype != torch.float16 or biases.dtype != torch.float16:
         raise ValueError("scales and biases are float16")
     cs, ss = codes.shape, scales.shape
-    if len(cs) < 2 or ss != biases.shape or ss[:-1] != cs[:-1] or cs[-1] * 8 != ss[-1] * group_size:
+    if len(cs) < 1 or ss != biases.shape or ss[:-1] != cs[:-1] or cs[-1] * 8 != ss[-1] * group_size:
         raise ValueError(f"codes {tuple(cs)}, scales {tuple(ss)} and biases {tuple(biases.shape)} are no matrix in groups "
                          f"of {group_size}")
 
@@ -122,7 +123,10 @@ class _Packed:
             codes, scales, biases = codes.contiguous(), scales.contiguous(), biases.contiguous()
             _lib.call("smoe_q4_pack", _lib.ptr(codes), _lib.ptr(scales), _lib.ptr(biases), self.num_experts,
                       self.output_dims, self.input_dims, group_size, _lib.ptr(self.packed), _lib.stream())
-        self.data_ptr = self.packed.data_ptr()
+
+    @property
+    def data_ptr(self) -> int:
+        return self.packed.data_ptr()
 
     @property
     def nbytes(self) -> int:
@@ -148,7 +152,8 @@ class _Packed:
 
 class QuantizedLinear(_Packed):
     """One linear layer on 4-bit weights, used like `nn.Linear` without a bias: codes (out, in / 8), scales and biases
-    (out, in / group_size). x (..., in) -> (..., out) in x's type; a token gets the same bits alone as in a window."""
+    (out, in / group_size). x (..., in) -> (..., out) in x's type. A token gets the same bits
+    alone as in a window of up to 16 tokens; more float16 tokens take the prompt's kernel where that is the faster one."""
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor, group_size: int = 64):
         if codes.dim() != 2:
@@ -244,7 +249,7 @@ def _pairs_product(lin, lin2, x2, indices, share, weights=None):
             _check_pairs(idx, share)
             if x2.shape[0] * share != pairs:
                 raise ValueError("indices must hold the same number of experts for every row of x")
-        for p0, p1 in _pair_chunks(pairs, share):
+        for p0, p1 in _pair_chunks(pairs, share) if pairs else ():
             spec = _lib.SmoeQ4Product(dtype=code, group=lin.group_size, x=x2[p0 // share].data_ptr(), cols=lin.input_dims,
                                       stack=lin.data_ptr, stack2=lin2.data_ptr if lin2 is not None else None,
                                       rows=lin.output_dims, experts=lin.num_experts, idx=idx[p0:].data_ptr(),
@@ -319,8 +324,8 @@ def moe_takes(switch_mlp, shared) -> bool:
 def moe(switch_mlp: QuantizedSwitchGLU, shared: QuantizedMLP, x: torch.Tensor, indices: torch.Tensor, w: torch.Tensor,
         g: torch.Tensor) -> torch.Tensor:
     """sum_j w_j switch_mlp(x, indices)_j + sigmoid(g) shared(x) in two launches: x (..., hidden), indices and w (...,
-    k) with w float32, g (..., 1) in x's type. Sums are float32 and rounded to x's type once (the SwiGLU keeps 22 bits
-    or more between the launches). An index at or past the expert count adds nothing."""
+    k) with w float32, g (..., 1) in x's type. Sums are float32 and rounded to x's type once (the SwiGLU keeps 22 bits,
+    down to 2^-25, between the launches). An index at or past the expert count adds nothing."""
     if not moe_takes(switch_mlp, shared):
         raise ValueError("moe takes 4-bit experts of one hidden size, with one group size in gate / up and one in down")
     gate, down = switch_mlp.gate_proj, switch_mlp.down_proj
@@ -355,7 +360,8 @@ def moe(switch_mlp: QuantizedSwitchGLU, shared: QuantizedMLP, x: torch.Tensor, i
 
 
 def failed(clear: bool = False) -> bool:
-    """Whether a bounded wait of the 4-bit kernels gave up (outputs since are then not valid). Synchronizes."""
+    """Whether a bounded wait of the 4-bit kernels gave up on the current device (outputs since are then not valid).
+    Synchronizes."""
     status = ctypes.c_int(0)
     _lib.call("smoe_q4_status", ctypes.byref(status), int(clear))
     return status.value != 0

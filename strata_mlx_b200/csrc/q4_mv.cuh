@@ -8,8 +8,9 @@
 //                      block's down products and its combine, the pairs' weights already in h
 //
 // What bounds them: a weight is 4.5 bits (groups of 64) of HBM traffic and is used for at most a few rows, so the
-// floor is the weights' bytes; next to it stands the instruction issue (a tile of 16 x 128 weights is about 100 warp
-// instructions and 1152 bytes: 62 cycles of an SM at full bandwidth). So two strips of rows share each activation
+// floor is the weights' bytes; next to it stands the instruction issue (a tile of 16 x 128 weights is about 108 warp
+// instructions and 1088 bytes, 47 cycles of an SM at full bandwidth, and a job's ends are 580 instructions more). 64007 x 2560 with 5 tokens runs at 5.4 TB/s between its start and end (21.6 us), a block of 512 experts of
+// 640 x 2560 at 32 tokens in 162 us (4.0 TB/s, the ends of its 8-row blocks). So two strips of rows share each activation
 // operand, and nothing but a warp's own copies is waited for inside a job: every warp has a ring of bulk copies of its
 // own that runs ahead of the arithmetic across the ends of jobs, 16 warps a SM, 75 to 150 KB of a SM in flight (6.5
 // TB/s x 1 us of latency over 148 SMs asks for 44 KB).
@@ -276,8 +277,8 @@ constexpr int kRedFloats = kMt * kRows * kM;  // a warp's sums of one job
 
 // `left` tiles of two strips, as they come through the ring in stages of kStep and a last one of what is left, times a
 // block of activation rows: xp is this lane's place in its row at the first tile's first column, runs the row's 32-column
-// runs from there on. Pairs of whole tiles take a loop without any other condition (the conditions of a general one cost
-// 60 of its 250 instructions a tile), each tile's activations loaded during the tile before.
+// runs from there on. Pairs of whole tiles take a loop without any other condition (215 instructions a tile of both strips
+// with groups of 128, against 250 with the conditions of a general one), each tile's activations loaded during the tile before.
 template <typename T, int G, class Fetch>
 __device__ __forceinline__ void stream_tiles(Ring& ring, Fetch& fetch, const T* xp, int left, int runs, int lane,
                                              float (&acc)[2][4], const Ones<T>& one) {
@@ -382,9 +383,9 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_product_kernel(const Produ
             const int64_t first = dense ? 0 : int64_t(blocks.expert[block]) * a.r_strips;
             const uint8_t* w0 = dense ? a.dw[0] : a.rw[0];
             const uint8_t* w1 = !GLU ? w0 : dense ? a.dw[1] : a.rw[1];
-            fetch0 = w0 + (first + strip * kWide) * strip_bytes + tile0 * kTile;
+            fetch0 = w0 + (first + strip * kWide) * strip_bytes + int64_t(tile0) * kTile;
             // (the last job of an odd number of strips takes its one strip twice)
-            fetch1 = w1 + (first + (GLU ? strip : min(strip * 2 + 1, strips - 1))) * strip_bytes + tile0 * kTile;
+            fetch1 = w1 + (first + (GLU ? strip : min(strip * 2 + 1, strips - 1))) * strip_bytes + int64_t(tile0) * kTile;
             fetch_left = tile1 - tile0;
             fetch_job += teams;
         }
@@ -480,14 +481,16 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_product_kernel(const Produ
 // warp. A warp adds a block's sums into its own copy of the result in shared memory when the block ends, each row of h to
 // its token; a CTA adds its warps' in order, and the last CTA of a job to come adds the CTAs' in order.
 //
-// float16: h lies in two pieces of float16 (11 + 11 bits), because rounding it once would leave the block's result with
+// float16: h lies in two pieces of float16 (11 + 11 bits, down to 2^-25), because rounding it once would leave the block's result with
 // 1.4 times the error of its own rounding. A block is then four rows of h, their first pieces in columns 0 .. 3 of the
 // MMAs and their second in 4 .. 7: no more instructions than eight rows.
 
 template <typename T>
 __host__ __device__ constexpr int down_rows() { return sizeof(T) == 2 ? kM / 2 : kM; }
 
-constexpr int kByJob = 64;  // tiles of a CTA up to which it keeps to one job
+// Tiles of a CTA up to which it keeps to one job (whole blocks of 256 experts of 1536 x 4096: one token, 64 tiles, 43.9 us by
+// job and 45.8 in even ranges; five tokens, some 200 tiles, 107.8 and 106.9; 32 tokens of the 512-expert block 172.0 and 168.5)
+constexpr int kByJob = 64;
 constexpr int kTokenStride = kMt * kRows + 4;  // floats of a token's sums: rows 0, 8, .. of four tokens on 32 banks
 
 template <int G>
@@ -589,8 +592,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_down_kernel(const DownArgs
             const bool shared = fc.seg < sblocks;
             const int64_t strip_bytes = int64_t(shared ? stiles : ftiles) * kTile;
             const uint8_t* w = shared ? a.sw : a.w + int64_t(blocks.expert[fc.seg - sblocks]) * strips * strip_bytes;
-            fetch0 = w + (fetch_job * kMt) * strip_bytes + fc.tile * kTile;
-            fetch1 = w + min(fetch_job * kMt + 1, strips - 1) * strip_bytes + fc.tile * kTile;
+            fetch0 = w + (fetch_job * kMt) * strip_bytes + int64_t(fc.tile) * kTile;
+            fetch1 = w + min(fetch_job * kMt + 1, strips - 1) * strip_bytes + int64_t(fc.tile) * kTile;
             fetch_left = tiles_of(fc);
             next_segment(fc, fetch_left);
         }

@@ -65,8 +65,8 @@ constexpr float kRound = 12582912.0f;  // 1.5 * 2^23
 // pieces = rows cols / kN. The arithmetic of each value is a chain of single IEEE float32 operations (difference,
 // quotient, rounding to even), so the codes are the formula's exactly. A quotient is a product with the reciprocal
 // of 15 scales (clamped to 0 .. 1 for free, then times 15), within 15 x 4 x 2^-23 of the division's: only one that close to
-// the border of two codes is divided out (a division for every value was 106 us for 24576 x 4096 float32, bound by its instructions; the bytes are
-// 72 us).
+// the border of two codes is divided out (24576 x 4096 float32: 87 us, 5.4 TB/s, bound by the ALU still; 106 us with a division
+// for every value; the bytes alone are 72 us).
 template <typename T, int G>
 __global__ void __launch_bounds__(kConvThreads) q4_quantize_kernel(const T* __restrict__ w, int64_t pieces,
                                                                    typename Piece<T>::Word* __restrict__ codes,
@@ -226,6 +226,8 @@ static size_t stack_bytes(int64_t experts, int64_t rows, int64_t cols, int group
     return size_t(experts) * strips_of_rows(rows) * tiles_of_cols(cols) * tile_bytes_of(group);
 }
 constexpr int64_t kMost = int64_t(1) << 30;  // rows, columns and tokens of a matrix
+constexpr int64_t kMostWeights = int64_t(1) << 40;  // of a matrix, and matrices of a stack: products stay in 64 bits
+constexpr int64_t kMostExperts = int64_t(1) << 20;
 
 }  // namespace q4
 }  // namespace smoe
@@ -251,13 +253,15 @@ static int check_matrix(int64_t rows, int64_t cols, int group) {
     SMOE_REQUIRE(group_ok(group), SMOE_ESHAPE, "groups have 32, 64 or 128 columns, not " + std::to_string(group));
     SMOE_REQUIRE(rows > 0 && rows <= kMost && cols > 0 && cols <= kMost, SMOE_ESHAPE,
                  "a 4-bit matrix of " + std::to_string(rows) + " x " + std::to_string(cols));
+    SMOE_REQUIRE(rows <= kMostWeights / cols, SMOE_ESHAPE, "a 4-bit matrix of more than 2^40 weights");
     SMOE_REQUIRE(cols % group == 0, SMOE_ESHAPE,
                  std::to_string(cols) + " columns are no whole number of groups of " + std::to_string(group));
     return SMOE_OK;
 }
 
 extern "C" size_t smoe_q4_bytes(int64_t experts, int64_t rows, int64_t cols, int group) {
-    if (!group_ok(group) || experts < 0 || rows <= 0 || cols <= 0 || cols % group != 0) return 0;
+    if (!group_ok(group) || experts < 0 || experts > kMostExperts || rows <= 0 || cols <= 0 || cols % group != 0) return 0;
+    if (rows > kMost || cols > kMost || rows > kMostWeights / cols) return 0;
     return stack_bytes(experts, rows, cols, group);
 }
 
@@ -292,7 +296,7 @@ static int dequant(const uint32_t* codes, const uint16_t* scales, const uint16_t
                    int64_t experts, int64_t rows, int64_t cols, int group, void* out, int out_dtype, void* stream) {
     if (experts == 0 || rows == 0) return SMOE_OK;
     if (int s = check_matrix(rows, cols, group)) return s;
-    SMOE_REQUIRE(experts > 0, SMOE_ESHAPE, "q4_dequant: a negative number of matrices");
+    SMOE_REQUIRE(experts > 0 && experts <= kMostExperts, SMOE_ESHAPE, "q4_dequant: a stack holds 1 to 2^20 matrices");
     SMOE_REQUIRE((packed ? aligned16(packed) : codes && scales && biases) && out && aligned16(out), SMOE_EARG,
                  "q4_dequant: null or misaligned pointer");
     SMOE_REQUIRE(out_dtype == SMOE_F16 || out_dtype == SMOE_F32, SMOE_EDTYPE, "q4_dequant gives float16 or float32");
@@ -337,7 +341,7 @@ extern "C" int smoe_q4_pack(const uint32_t* codes, const uint16_t* scales, const
     Q4_TRY
     if (experts == 0) return SMOE_OK;
     if (int s = check_matrix(rows, cols, group)) return s;
-    SMOE_REQUIRE(experts > 0, SMOE_ESHAPE, "q4_pack: a negative number of matrices");
+    SMOE_REQUIRE(experts > 0 && experts <= kMostExperts, SMOE_ESHAPE, "q4_pack: a stack holds 1 to 2^20 matrices");
     SMOE_REQUIRE(codes && scales && biases && packed && aligned16(packed), SMOE_EARG,
                  "q4_pack: null or misaligned pointer");
     const size_t bytes = stack_bytes(experts, rows, cols, group);
@@ -526,7 +530,8 @@ extern "C" int smoe_q4_moe(const SmoeQ4Moe* m, void* workspace, size_t workspace
     p.share = m->k;
     p.weights = m->weights;
     p.out = h;
-    if (int s = q4_product(&p, p.dtype == SMOE_F16, counters, static_cast<int>(MoeSpace::n_counters(m->hidden)), stream)) return s;
+    if (int s = q4_product(&p, p.dtype == SMOE_F16, counters, static_cast<int>(MoeSpace::n_counters(m->hidden)), stream))
+        return s;
     DownArgs d = {};
     d.h = h;
     d.hs = m->shared_ffn > 0 ? hs : nullptr;
@@ -552,6 +557,7 @@ extern "C" int smoe_q4_moe(const SmoeQ4Moe* m, void* workspace, size_t workspace
 }
 
 extern "C" int smoe_q4_status(int* status, int clear) {
+    Q4_TRY
     SMOE_REQUIRE(status, SMOE_EARG, "q4_status: null pointer");
     *status = 0;
     cudaError_t e = cudaDeviceSynchronize();
@@ -562,4 +568,5 @@ extern "C" int smoe_q4_status(int* status, int clear) {
     }
     if (e != cudaSuccess) return fail(-static_cast<int>(e), std::string("q4_status: ") + cudaGetErrorString(e));
     return SMOE_OK;
+    Q4_CATCH("q4_status")
 }

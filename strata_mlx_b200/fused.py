@@ -231,7 +231,7 @@ def route_window(gate: "WindowLinear", shared_gate: "WindowLinear", x: torch.Ten
     _lib.require_cuda(gate.weight, x)
     dev = x.device
     x2 = affine._aligned(x)
-    wt, gw = gate.weight.contiguous(), shared_gate.weight.contiguous()
+    wt, gw = affine._aligned(gate.weight), affine._aligned(shared_gate.weight)
     logits = torch.empty((tokens, gate.rows), dtype=torch.float32, device=dev)
     idx = torch.empty((tokens, k), dtype=torch.uint32, device=dev)
     w = torch.empty((tokens, k), dtype=torch.float32, device=dev)

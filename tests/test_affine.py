@@ -27,12 +27,14 @@ def test_sizes_of_the_layout(lib):
     assert lib.smoe_q4_bytes(1, 16, 128, 128) == 1024 + 64
     assert lib.smoe_q4_bytes(1, 16, 128, 64) == 1024 + 128
     assert lib.smoe_q4_bytes(3, 17, 160, 32) == 3 * 2 * 2 * (1024 + 256)
-    for bad in ((1, 16, 100, 64), (1, 16, 128, 16), (1, 0, 128, 64), (-1, 16, 128, 64), (1, 16, 96, 64)):
+    for bad in ((1, 16, 100, 64), (1, 16, 128, 16), (1, 0, 128, 64), (-1, 16, 128, 64), (1, 16, 96, 64),
+                (1, 2**31, 128, 64), (1, 2**20, 2**21, 128), (2**20 + 1, 16, 128, 64)):
         assert lib.smoe_q4_bytes(*bad) == 0, bad
 
 
 @pytest.mark.parametrize("rows, cols, group, code", [(4, 128, 48, ESHAPE), (4, 100, 32, ESHAPE), (4, 96, 64, ESHAPE),
-                                                     (-1, 128, 64, ESHAPE), (4, 0, 64, ESHAPE)])
+                                                     (-1, 128, 64, ESHAPE), (4, 0, 64, ESHAPE),
+                                                     (2**20, 2**21, 128, ESHAPE), (4, 2**31, 32, ESHAPE)])
 def test_matrices_that_do_not_divide_are_refused(lib, rows, cols, group, code):
     assert lib.smoe_q4_quantize(A, 1, rows, cols, group, A, A, A, None) == code
     assert lib.smoe_q4_dequant(A, A, A, rows, cols, group, A, 1, None) == code
@@ -49,6 +51,8 @@ def test_pointers_and_types_are_checked(lib):
     assert lib.smoe_q4_dequant(A, A, None, 4, 128, 64, A, 1, None) == EARG
     assert lib.smoe_q4_dequant(A, A, A, 4, 128, 64, A, 2, None) == EDTYPE
     assert lib.smoe_q4_pack(A, A, A, -1, 4, 128, 64, A, None) == ESHAPE
+    assert lib.smoe_q4_pack(A, A, A, 2**20 + 1, 4, 128, 64, A, None) == ESHAPE
+    assert lib.smoe_q4_unpack(A, 2**20 + 1, 4, 128, 64, A, 1, None) == ESHAPE
     assert lib.smoe_q4_pack(A, A, A, 1, 4, 128, 64, None, None) == EARG
     assert lib.smoe_q4_unpack(None, 1, 4, 128, 64, A, 1, None) == EARG
     assert lib.smoe_q4_linear(A, 4, 128, 64, A + 4, 3, A, 1, None) == EARG  # activations off a 16-byte boundary

@@ -6,6 +6,7 @@ cores truncate), and a row of c columns in groups of G takes at most 4 c / 32 (t
 G (the group's end) + 40 (warps, CTAs) of them. A result in type t is rounded once more: eps(t) / 2 of its value (and half
 the least subnormal, 2^-25, in float16). The SwiGLU kept between the launches is rounded to t once."""
 
+import copy
 import ctypes
 
 import pytest
@@ -218,6 +219,36 @@ def test_a_layer_takes_views_leads_and_no_tokens(cuda):
     assert layer(x[0, 0, :256]).shape == (96,)
 
 
+@pytest.mark.parametrize("rows, cols, tokens, dtype", [(16, 2**21, 2, F16), (3, 2**21, 1, F32), (40, 2**20, 20, F16), (200000, 32, 1, F16),
+                                                       (200000, 32, 40, F16)])
+def test_long_rows_and_many_rows(cuda, rows, cols, tokens, dtype):
+    gen = gen_of(18)
+    p = parts(gen, (), rows, cols, 32)
+    x = torch.randn(tokens, cols, device=cuda, generator=gen).to(dtype)
+    want, off = product64(x, p, 32, dtype)
+    if tokens > 16:  # (weights rounded to float16)
+        off = off + x.double().abs() @ (floats64(p)[0].abs().mT * 2.0**-11 + 2.0**-25)
+    close(affine.QuantizedLinear(*p, group_size=32)(x), want, off)
+
+
+def test_a_copy_of_a_layer_has_weights_of_its_own(cuda):
+    gen = gen_of(19)
+    layer = affine.QuantizedLinear(*parts(gen, (), 48, 128, 64))
+    x = torch.randn(3, 128, device=cuda, generator=gen).half()
+    want = layer(x)
+    other = copy.deepcopy(layer)
+    layer.packed.zero_()
+    torch.cuda.synchronize()  # (a layer's weights are not to be written by the launch before its product)
+    assert torch.equal(other(x), want) and not layer(x).any()
+
+
+def test_one_row_of_floats(cuda):
+    w = torch.randn(128, device=cuda, generator=gen_of(21))
+    p = affine.quantize(w, 32)
+    assert [t.shape for t in p] == [(16,), (4,), (4,)]
+    assert torch.equal(affine.dequantize(*p, 32), affine.dequantize(*affine.quantize(w[None], 32), 32)[0])
+
+
 def test_what_is_not_finite_stays_in_its_token(cuda):
     gen = gen_of(13)
     layer = affine.QuantizedLinear(*parts(gen, (), 64, 256, 64), group_size=64)
@@ -263,6 +294,16 @@ def test_pairs_of_no_expert_are_left_as_they_were(cuda):
     want = stack(x[:, None, None], idx.clamp(0, 5))[:, :, 0].reshape(8, 33)
     out_of = torch.tensor([0, 1, 0, 0, 1, 1, 0, 0], dtype=torch.bool, device=cuda)
     assert (out[out_of] == 7).all() and torch.equal(out[~out_of], want[~out_of])
+
+
+def test_no_pairs(cuda):
+    gen = gen_of(22)
+    _, _, glu, _ = make_experts(gen, 4, 128, 64, 64, 64)
+    x = torch.randn(3, 128, device=cuda, generator=gen).half()
+    none = torch.zeros(3, 0, dtype=torch.int32, device=cuda)
+    assert glu(x, none).shape == (3, 0, 128) and glu(x[:0], none[:0]).shape == (0, 0, 128)
+    assert glu(x[:0], torch.zeros(0, 2, dtype=torch.int32, device=cuda)).shape == (0, 2, 128)
+    assert glu.gate_proj(x[:, None, None], none).shape == (3, 0, 1, 64)
 
 
 # ---- the experts and the block
@@ -325,6 +366,45 @@ def test_a_block_behind_its_route_is_its_definition(cuda, dtype, tokens, experts
         idx[:, 1] = idx[:, -1]
     idx[-1] = -1
     close(affine.moe(glu, mlp, x, idx, w, g), *moe64(x, r, s, idx, w, g, group, down_group, dtype))
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("tokens, shared", [(3, 0), (3, 96), (64, 0)])
+def test_a_block_without_a_shared_expert_or_its_gate(cuda, dtype, tokens, shared):
+    gen = gen_of(33)
+    hidden, ffn, experts, k, group = 160, 96, 2048, 32, 32
+    r, s, glu, mlp = make_experts(gen, experts, hidden, ffn, shared or 32, group)
+    x = torch.randn(tokens, hidden, device=cuda, generator=gen).to(dtype)
+    idx = torch.randint(0, experts, (tokens, k), dtype=torch.int32, device=cuda, generator=gen)
+    w = torch.rand(tokens, k, device=cuda, generator=gen)
+    out = torch.full((tokens, hidden), 7.0, dtype=dtype, device=cuda)
+    spec = _lib.SmoeQ4Moe(dtype=_lib.dtype_code(dtype), group=group, down_group=group, tokens=tokens, hidden=hidden,
+                          experts=experts, k=k, ffn=ffn, shared_ffn=shared, x=x.data_ptr(), idx=idx.data_ptr(),
+                          weights=w.data_ptr(), gate=glu.gate_proj.data_ptr, up=glu.up_proj.data_ptr,
+                          down=glu.down_proj.data_ptr, out=out.data_ptr())
+    if shared:
+        spec.sgate, spec.sup, spec.sdown = (p.data_ptr for p in (mlp.gate_proj, mlp.up_proj, mlp.down_proj))
+    nbytes = int(_lib.lib().smoe_q4_moe_workspace_size(tokens, k, hidden, ffn, shared))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=cuda)
+    _lib.call("smoe_q4_moe", ctypes.byref(spec), _lib.ptr(ws), nbytes, _lib.stream())
+    # (the gate of a shared expert that has none is 1; one that is not there has weights of zero)
+    want = moe64(x, r, s if shared else [[t * 0 for t in p] for p in s], idx, w, torch.full((tokens, 1), 40.0, device=cuda), group,
+                 group, dtype)
+    close(out, *want)
+
+
+def test_a_router_at_any_address(cuda):
+    gen = gen_of(35)
+    _, _, block, router, sgate = make_block(gen, 20, 256, 128, 192, 64, 4)
+    x = torch.randn(5, 256, device=cuda, generator=gen).half()
+    want = block(x)
+
+    def moved(t):
+        return torch.empty(t.numel() + 1, dtype=t.dtype, device=cuda)[1:].view(t.shape).copy_(t)
+
+    other = fused.SparseMoeBlock(moved(router), block.switch_mlp, block.shared_expert, moved(sgate), 4)
+    assert torch.equal(other(moved(x)), want)
+    assert torch.equal(other(torch.stack((x, x), -1)[..., 1]), want)
 
 
 @pytest.mark.parametrize("dtype", [F16, F32])
