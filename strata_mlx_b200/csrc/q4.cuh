@@ -374,6 +374,9 @@ __device__ __forceinline__ void tile_mma(uint32_t tile, int stride, int lane, co
             const uint32_t q = pairs + m * stride + 4 * gi;
             group_end<T, 2>(acc[m], s, m, lds32(q), lds32(q + 8 * kPairs * 4));
         }
+        // (four groups of a tile interleaved want more registers than there are: 64007 x 2560 at 5 tokens 32.2 us, with them
+        // kept apart 28.0)
+        if (G == 32 && gi + 1 < kPairs) __syncwarp();
     }
 }
 

@@ -278,7 +278,9 @@ constexpr int kRedFloats = kMt * kRows * kM;  // a warp's sums of one job
 // `left` tiles of two strips, as they come through the ring in stages of kStep and a last one of what is left, times a
 // block of activation rows: xp is this lane's place in its row at the first tile's first column, runs the row's 32-column
 // runs from there on. Pairs of whole tiles take a loop without any other condition (215 instructions a tile of both strips
-// with groups of 128, against 250 with the conditions of a general one), each tile's activations loaded during the tile before.
+// with groups of 128, against 250 with the conditions of a general one), each tile's activations loaded during the tile
+// before; with groups of 32, whose sums take the registers, a pair's second tile's between the two (64007 x 2560 at 5 tokens
+// 26.3 us, and 28.0 with the loads ahead).
 template <typename T, int G, class Fetch>
 __device__ __forceinline__ void stream_tiles(Ring& ring, Fetch& fetch, const T* xp, int left, int runs, int lane,
                                              float (&acc)[2][4], const Ones<T>& one) {
@@ -293,8 +295,9 @@ __device__ __forceinline__ void stream_tiles(Ring& ring, Fetch& fetch, const T* 
 #pragma unroll 1
         do {
             const uint32_t slot = ring.wait<2 * kStride>(lane);
-            x1.load(xp + kCols);
+            if constexpr (G != 32) x1.load(xp + kCols);
             tile_mma<T, G>(slot, kStride, lane, x0, acc, one);
+            if constexpr (G == 32) x1.load(xp + kCols);
             --pairs;
             xp += 2 * kCols;
             x0.load(pairs > 0 ? xp : xp - 2 * kCols);  // (after the last pair: any place of the row)
@@ -489,7 +492,7 @@ template <typename T>
 __host__ __device__ constexpr int down_rows() { return sizeof(T) == 2 ? kM / 2 : kM; }
 
 // Tiles of a CTA up to which it keeps to one job (whole blocks of 256 experts of 1536 x 4096: one token, 64 tiles, 43.9 us by
-// job and 45.8 in even ranges; five tokens, some 200 tiles, 107.8 and 106.9; 32 tokens of the 512-expert block 172.0 and 168.5)
+// job and 45.8 in even ranges; five tokens, some 250 tiles, 107.8 and 106.9; 32 tokens of the 512-expert block 172.0 and 168.5)
 constexpr int kByJob = 64;
 constexpr int kTokenStride = kMt * kRows + 4;  // floats of a token's sums: rows 0, 8, .. of four tokens on 32 banks
 
