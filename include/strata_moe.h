@@ -516,6 +516,19 @@ SMOE_API int smoe_q4_product(const SmoeQ4Product* p, void* stream);
 SMOE_API int smoe_q4_linear(const uint8_t* packed, int64_t rows, int64_t cols, int group, const void* x, int64_t tokens,
                             void* out, int dtype, void* stream);
 
+/* A stack's products of a prompt's many (token, expert) pairs, in the tiles of smoe_tiles_of (16 slots, each tile one
+ * expert's, an expert's tiles next to one another): out[slot_row[s], r] = W[tile_expert[s / 16]][r, :] . a[s, :] for every slot
+ * s, row s itself without slot_row; rows at or past out_rows are not written, nor are the slots of tiles that name no
+ * expert. a (tiles * 16, cols) float16, out float16 or float32 (`out_dtype`); a weight is rounded to float16 once, sums are
+ * float32. smoe_q4_tile_plan makes a plan (smoe_q4_tile_plan_size bytes, 16-byte aligned) from tile_expert[tiles], for any
+ * number of products on the same tiles. The prompt's form of `QuantizedSwitchLinear` (strata_mlx/mtp.py:34-75). */
+SMOE_API size_t smoe_q4_tile_plan_size(int64_t tiles);
+SMOE_API int smoe_q4_tile_plan(const uint32_t* tile_expert, int64_t tiles, int64_t experts, void* plan, size_t plan_bytes,
+                               void* stream);
+SMOE_API int smoe_q4_tile_matmul(const uint8_t* packed, int64_t experts, int64_t rows, int64_t cols, int group, const void* a,
+                                 int64_t tiles, const void* plan, const uint32_t* slot_row, int64_t out_rows, void* out,
+                                 int out_dtype, void* stream);
+
 /* A MoE block behind its route (smoe_route's idx, weights and gate_out) on packed 4-bit experts, for 1 to 64 tokens,
  * in two launches (gate, up and SwiGLU of the routed and the shared expert; down and the combine):
  *   out[t] = sum_j weights[t, j] down_e(silu(gate_e x) * up_e x) + sigmoid(shared_gate[t]) shared(x), e = idx[t, j]

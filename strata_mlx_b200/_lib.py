@@ -144,6 +144,9 @@ SIGNATURES = {
     "smoe_q4_unpack": (_i, [_p, _i64, _i64, _i64, _i, _p, _i, _p]),
     "smoe_q4_linear": (_i, [_p, _i64, _i64, _i, _p, _i64, _p, _i, _p]),
     "smoe_q4_product": (_i, [_c.POINTER(SmoeQ4Product), _p]),
+    "smoe_q4_tile_plan_size": (_sz, [_i64]),
+    "smoe_q4_tile_plan": (_i, [_p, _i64, _i64, _p, _sz, _p]),
+    "smoe_q4_tile_matmul": (_i, [_p, _i64, _i64, _i64, _i, _p, _i64, _p, _p, _i64, _p, _i, _p]),
     "smoe_q4_moe_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64]),
     "smoe_q4_moe": (_i, [_c.POINTER(SmoeQ4Moe), _p, _sz, _p]),
     "smoe_route_window": (_i, [_p, _p, _p, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p]),

@@ -22,12 +22,14 @@ import ctypes
 import torch
 
 from . import _lib
-from .blocks import _flat_idx
+from .blocks import TOKENS_TILE, _flat_idx, slot_rows, swiglu_to, tiles_of
 
 BITS = 4
 GROUPS = (32, 64, 128)
-MAX_PAIRS = 2048  # (token, expert) pairs of one launch; a longer call goes in several
-MOE_TOKENS = 64  # tokens that `moe` takes at once; a longer call goes in several
+MAX_PAIRS = 2048  # (token, expert) pairs of one streaming launch; a longer call goes by tiles, or in several launches
+TILE_PAIRS = 1 << 18  # pairs that go by tiles at once (what bounds the float32 gate and up of a long prompt)
+MOE_TOKENS = 64  # tokens that `moe` takes in its two launches
+COMBINE_TOKENS = 1 << 15  # tokens of a prompt that it takes at once
 
 
 def _check_group(group_size: int, bits: int = BITS) -> None:
@@ -182,10 +184,39 @@ class QuantizedLinear(_Packed):
         return out
 
 
-def _pair_chunks(pairs: int, share: int):
-    """Ranges of pairs, whole rows of `share`, that one launch takes."""
-    step = max(1, MAX_PAIRS // share) * share
+def _pair_chunks(pairs: int, share: int, most: int = MAX_PAIRS):
+    """Ranges of up to `most` pairs, whole rows of `share`."""
+    step = max(1, most // share) * share
     return [(p, min(p + step, pairs)) for p in range(0, pairs, step)]
+
+
+def _by_tiles(lin, dtype, pairs: int) -> bool:
+    """Whether a call's pairs go in tiles of one expert's, through the prompt's kernel (float16; tiles_of takes up to 1024
+    experts): when one streaming launch would not take them. The SwiGLU of 512 experts of 640 x 2560, ten a token: 192
+    tokens 389 us streamed and 619 by tiles, 256 tokens 763 and 639, 1180 tokens 3065 and 699; 256 of 1536 x 4096, eight a
+    token: 192 tokens 656 and 1036, 512 tokens 2086 and 1053, 1180 tokens 4790 and 1243."""
+    return dtype == torch.float16 and lin.num_experts <= 1024 and pairs > MAX_PAIRS
+
+
+class _Tiles:
+    """A call's pairs by expert: `row` the row of x in each slot, `slot_row` each slot's pair."""
+
+    def __init__(self, lin, indices: torch.Tensor, share: int):
+        self.lin, self.pairs = lin, indices.numel()
+        tile_expert, token, where = tiles_of(indices.reshape(-1, share), lin.num_experts)
+        self.row, self.count = token.view(torch.int32), tile_expert.numel()
+        self.slot_row = slot_rows(where, self.count * TOKENS_TILE)
+        nbytes = int(_lib.lib().smoe_q4_tile_plan_size(self.count))
+        self.plan = torch.empty(nbytes, dtype=torch.uint8, device=lin.device)
+        _lib.call("smoe_q4_tile_plan", _lib.ptr(tile_expert), self.count, lin.num_experts, _lib.ptr(self.plan), nbytes,
+                  _lib.stream())
+
+    def product(self, lin, a: torch.Tensor, out: torch.Tensor, in_pairs: bool) -> torch.Tensor:
+        """lin's products of the slots' rows `a`, into out's rows in the order of the slots or of the pairs."""
+        _lib.call("smoe_q4_tile_matmul", lin.data_ptr, lin.num_experts, lin.output_dims, lin.input_dims, lin.group_size,
+                  _lib.ptr(a), self.count, _lib.ptr(self.plan), _lib.ptr(self.slot_row) if in_pairs else None, out.shape[0],
+                  _lib.ptr(out), _lib.dtype_code(out.dtype), _lib.stream())
+        return out
 
 
 def _check_pairs(indices, k):
@@ -235,8 +266,9 @@ class QuantizedSwitchLinear(_Packed):
         return out.reshape(*ishape, 1, self.output_dims)
 
 
-def _pairs_product(lin, lin2, x2, indices, share, weights=None):
-    """(pairs, out): rows x2[p // share] through expert indices[p] of `lin`, or through gate `lin` and up `lin2`."""
+def _pairs_product(lin, lin2, x2, indices, share, zeros=False):
+    """(pairs, out): rows x2[p // share] through expert indices[p] of `lin`, or through gate `lin` and up `lin2`; zeros:
+    pairs of no expert get rows of zeros."""
     code = _lib.dtype_code(x2.dtype)
     if indices.device != lin.device:
         _lib.require_cuda(indices)
@@ -244,11 +276,16 @@ def _pairs_product(lin, lin2, x2, indices, share, weights=None):
     with torch.cuda.device(lin.device):
         idx = _flat_idx(indices)
         pairs = idx.numel()
-        out = torch.empty((pairs, lin.output_dims), dtype=x2.dtype, device=lin.device)
+        out = (torch.zeros if zeros else torch.empty)((pairs, lin.output_dims), dtype=x2.dtype, device=lin.device)
         if pairs:
             _check_pairs(idx, share)
             if x2.shape[0] * share != pairs:
                 raise ValueError("indices must hold the same number of experts for every row of x")
+        if lin2 is None and _by_tiles(lin, x2.dtype, pairs):
+            for p0, p1 in _pair_chunks(pairs, share, TILE_PAIRS):
+                tiles = _Tiles(lin, idx[p0:p1], share)
+                tiles.product(lin, x2[p0 // share : p1 // share].index_select(0, tiles.row), out[p0:p1], True)
+            return out
         for p0, p1 in _pair_chunks(pairs, share) if pairs else ():
             spec = _lib.SmoeQ4Product(dtype=code, group=lin.group_size, x=x2[p0 // share].data_ptr(), cols=lin.input_dims,
                                       stack=lin.data_ptr, stack2=lin2.data_ptr if lin2 is not None else None,
@@ -283,14 +320,32 @@ class QuantizedSwitchGLU:
     def __call__(self, x: torch.Tensor, indices: torch.Tensor) -> torch.Tensor:
         if indices.dim() < 1:
             raise ValueError("indices must hold k experts for every token of x")
-        h = _pairs_product(self.gate_proj, self.up_proj, self.gate_proj._rows(x).reshape(-1, x.shape[-1]), indices,
-                           indices.shape[-1])
-        out = _pairs_product(self.down_proj, None, h, indices, 1)
+        out = self._pairs(self.gate_proj._rows(x).reshape(-1, x.shape[-1]), indices)
         return out.reshape(*indices.shape, self.down_proj.output_dims)
+
+    def _pairs(self, x2: torch.Tensor, indices: torch.Tensor, zeros: bool = False) -> torch.Tensor:
+        """The experts' outputs (pairs, out); zeros: rows of zeros for pairs of no expert."""
+        gate, up, down = self.gate_proj, self.up_proj, self.down_proj
+        pairs, k = indices.numel(), indices.shape[-1]
+        if not _by_tiles(gate, x2.dtype, pairs) or indices.device != gate.device or x2.shape[0] * k != pairs or k > MAX_PAIRS:
+            h = _pairs_product(gate, up, x2, indices, k)
+            return _pairs_product(down, None, h, indices, 1, zeros)
+        # a prompt: gate and up in the order of the slots, the SwiGLU of their float32 sums rounded once
+        with torch.cuda.device(gate.device):
+            idx = _flat_idx(indices)
+            out = (torch.zeros if zeros else torch.empty)((pairs, down.output_dims), dtype=x2.dtype, device=gate.device)
+            for p0, p1 in _pair_chunks(pairs, k, TILE_PAIRS):
+                tiles = _Tiles(gate, idx[p0:p1], k)
+                a = x2[p0 // k : p1 // k].index_select(0, tiles.row)
+                g, u = (tiles.product(p, a, torch.empty((len(a), p.output_dims), dtype=torch.float32, device=a.device), False)
+                        for p in (gate, up))
+                tiles.product(down, swiglu_to(g, u, x2.dtype), out[p0:p1], True)
+        return out
 
 
 class QuantizedMLP:
-    """The shared expert on 4-bit weights: down(silu(gate x) * up x)."""
+    """The shared expert on 4-bit weights: down(silu(gate x) * up x). Gate, up and the SwiGLU are one launch; a long
+    float16 prompt's are the prompt's products and a SwiGLU, each rounded to float16."""
 
     def __init__(self, gate: QuantizedLinear, up: QuantizedLinear, down: QuantizedLinear):
         _check_glu(gate, up, down)
@@ -300,6 +355,10 @@ class QuantizedMLP:
         code = _lib.dtype_code(x.dtype)
         gate, up = self.gate_proj, self.up_proj
         x2 = gate._rows(x).reshape(-1, gate.input_dims)
+        if x.dtype == torch.float16 and self._apart(x2.shape[0]):
+            with torch.cuda.device(gate.device):
+                out = self.down_proj(swiglu_to(gate(x2), up(x2), x.dtype))
+            return out.reshape(*x.shape[:-1], self.down_proj.output_dims)
         with torch.cuda.device(gate.device):
             h = torch.empty((x2.shape[0], gate.output_dims), dtype=x.dtype, device=gate.device)
             if x2.shape[0]:
@@ -309,6 +368,13 @@ class QuantizedMLP:
                 _lib.call("smoe_q4_product", ctypes.byref(spec), _lib.stream())
             out = self.down_proj(h)
         return out.reshape(*x.shape[:-1], self.down_proj.output_dims)
+
+
+    def _apart(self, tokens: int) -> bool:
+        """Whether gate and up go by the prompt's kernel: the streaming launch takes 0.3 us and 0.25 ps a weight for every
+        8 tokens, 30 us of which are about the other's start (whole calls of 4096 x 4096: 48 tokens 51 us streamed and 58
+        apart, 96 tokens 78 and 57; of 640 x 2560: 256 tokens 31 and 33, 512 tokens 50 and 35)."""
+        return (tokens + 7) // 8 * (0.3 + 2.5e-7 * self.gate_proj.output_dims * self.gate_proj.input_dims) > 30
 
 
 def moe_takes(switch_mlp, shared) -> bool:
@@ -323,9 +389,10 @@ def moe_takes(switch_mlp, shared) -> bool:
 
 def moe(switch_mlp: QuantizedSwitchGLU, shared: QuantizedMLP, x: torch.Tensor, indices: torch.Tensor, w: torch.Tensor,
         g: torch.Tensor) -> torch.Tensor:
-    """sum_j w_j switch_mlp(x, indices)_j + sigmoid(g) shared(x) in two launches: x (..., hidden), indices and w (...,
-    k) with w float32, g (..., 1) in x's type. Sums are float32 and rounded to x's type once (the SwiGLU keeps 22 bits,
-    down to 2^-25, between the launches). An index at or past the expert count adds nothing."""
+    """sum_j w_j switch_mlp(x, indices)_j + sigmoid(g) shared(x): x (..., hidden), indices and w (..., k) with w float32,
+    g (..., 1) in x's type. Up to MOE_TOKENS tokens in two launches, sums float32 and rounded to x's type once (the SwiGLU
+    keeps 22 bits, down to 2^-25, between the launches); more tokens by switch_mlp, shared and the block's combine, each
+    rounded to x's type. An index at or past the expert count adds nothing."""
     if not moe_takes(switch_mlp, shared):
         raise ValueError("moe takes 4-bit experts of one hidden size, with one group size in gate / up and one in down")
     gate, down = switch_mlp.gate_proj, switch_mlp.down_proj
@@ -343,18 +410,24 @@ def moe(switch_mlp: QuantizedSwitchGLU, shared: QuantizedMLP, x: torch.Tensor, i
     with torch.cuda.device(gate.device):
         idx, w, g = _flat_idx(indices), w.contiguous(), g.contiguous()
         out = torch.empty((tokens, gate.input_dims), dtype=x.dtype, device=gate.device)
-        for t0 in range(0, tokens, MOE_TOKENS):
-            n = min(MOE_TOKENS, tokens - t0)
-            nbytes = int(_lib.lib().smoe_q4_moe_workspace_size(n, k, gate.input_dims, gate.output_dims,
+        if tokens > MOE_TOKENS:
+            # (512 experts of 640 x 2560, ten a token, 96 tokens: 384 us, in calls of 64 tokens 615)
+            idx = idx.reshape(tokens, k)
+            for t0 in range(0, tokens, COMBINE_TOKENS):
+                t1 = min(t0 + COMBINE_TOKENS, tokens)
+                y, s = switch_mlp._pairs(x2[t0:t1], idx[t0:t1], zeros=True), shared(x2[t0:t1])
+                _lib.call("smoe_combine", _lib.ptr(y), w.data_ptr() + 4 * t0 * k, g.data_ptr() + g.element_size() * t0,
+                          _lib.ptr(s), t1 - t0, k, gate.input_dims, out[t0:].data_ptr(), code, _lib.stream())
+        elif tokens:
+            nbytes = int(_lib.lib().smoe_q4_moe_workspace_size(tokens, k, gate.input_dims, gate.output_dims,
                                                                 sgate.output_dims))
             ws = torch.empty(nbytes, dtype=torch.uint8, device=gate.device)
             spec = _lib.SmoeQ4Moe(
-                dtype=code, group=gate.group_size, down_group=down.group_size, tokens=n, hidden=gate.input_dims,
-                experts=gate.num_experts, k=k, ffn=gate.output_dims, shared_ffn=sgate.output_dims, x=x2[t0:].data_ptr(),
-                idx=idx[t0 * k:].data_ptr(), weights=w.data_ptr() + 4 * t0 * k,
-                shared_gate=g.data_ptr() + g.element_size() * t0, gate=gate.data_ptr, up=switch_mlp.up_proj.data_ptr,
-                down=down.data_ptr, sgate=sgate.data_ptr, sup=shared.up_proj.data_ptr, sdown=sdown.data_ptr,
-                out=out[t0:].data_ptr())
+                dtype=code, group=gate.group_size, down_group=down.group_size, tokens=tokens, hidden=gate.input_dims,
+                experts=gate.num_experts, k=k, ffn=gate.output_dims, shared_ffn=sgate.output_dims, x=x2.data_ptr(),
+                idx=idx.data_ptr(), weights=w.data_ptr(), shared_gate=g.data_ptr(), gate=gate.data_ptr,
+                up=switch_mlp.up_proj.data_ptr, down=down.data_ptr, sgate=sgate.data_ptr, sup=shared.up_proj.data_ptr,
+                sdown=sdown.data_ptr, out=out.data_ptr())
             _lib.call("smoe_q4_moe", ctypes.byref(spec), _lib.ptr(ws), nbytes, _lib.stream())
     return out.reshape(x.shape)
 

@@ -19,6 +19,18 @@ int down_f32(const DownArgs& a, int group, const Writes& w, cudaStream_t st);
 // the dense part of `a` on the prompt's kernel (float16), and whether that is the faster one
 bool matmul_better(int64_t tokens, int64_t rows, int64_t cols);
 int matmul_f16(const ProductArgs& a, int group, const Writes& w, cudaStream_t st);
+// the prompt's kernel on a stack, its activations x in tiles of 16 slots, each one expert's
+struct TileArgs {
+    const uint8_t* w;
+    int64_t experts, rows, cols, tiles;
+    const void *x, *plan;
+    const uint32_t* slot_row;
+    int64_t out_rows;
+    void* out;
+    bool floats;
+};
+int tile_plan(const uint32_t* tile_expert, int64_t tiles, int64_t experts, void* plan, const Writes& w, cudaStream_t st);
+int tile_matmul(const TileArgs& p, int group, const Writes& w, cudaStream_t st);
 cudaError_t matmul_status(int* v, bool clear);
 cudaError_t product_status_f16(int* v, bool clear);
 cudaError_t product_status_f32(int* v, bool clear);

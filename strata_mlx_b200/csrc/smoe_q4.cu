@@ -448,6 +448,48 @@ extern "C" int smoe_q4_linear(const uint8_t* packed, int64_t rows, int64_t cols,
     Q4_CATCH("q4_linear")
 }
 
+extern "C" size_t smoe_q4_tile_plan_size(int64_t tiles) { return tiles > 0 ? size_t(tiles + 1) * 16 : 0; }
+
+static int check_tiles(int64_t tiles, int64_t experts) {
+    SMOE_REQUIRE(tiles > 0 && tiles <= (int64_t(1) << 24), SMOE_ESHAPE, "1 to 2^24 tiles a call");
+    SMOE_REQUIRE(experts > 0 && experts <= kMostExperts, SMOE_ESHAPE, "a stack holds 1 to 2^20 matrices");
+    return SMOE_OK;
+}
+
+extern "C" int smoe_q4_tile_plan(const uint32_t* tile_expert, int64_t tiles, int64_t experts, void* plan, size_t plan_bytes,
+                                 void* stream) {
+    Q4_TRY
+    if (tiles == 0) return SMOE_OK;
+    if (int s = check_tiles(tiles, experts)) return s;
+    SMOE_REQUIRE(tile_expert, SMOE_EARG, "q4_tile_plan: null pointer");
+    SMOE_REQUIRE(plan && aligned16(plan) && plan_bytes >= smoe_q4_tile_plan_size(tiles), SMOE_EWORKSPACE,
+                 "q4_tile_plan: plan missing, misaligned or too small");
+    Writes w;
+    w.add(plan, smoe_q4_tile_plan_size(tiles));
+    return tile_plan(tile_expert, tiles, experts, plan, w, as_stream(stream));
+    Q4_CATCH("q4_tile_plan")
+}
+
+extern "C" int smoe_q4_tile_matmul(const uint8_t* packed, int64_t experts, int64_t rows, int64_t cols, int group, const void* a,
+                                   int64_t tiles, const void* plan, const uint32_t* slot_row, int64_t out_rows, void* out,
+                                   int out_dtype, void* stream) {
+    Q4_TRY
+    if (tiles == 0 || out_rows == 0) return SMOE_OK;
+    if (int s = check_tiles(tiles, experts)) return s;
+    if (int s = check_matrix(rows, cols, group)) return s;
+    SMOE_REQUIRE(out_rows > 0, SMOE_EARG, "q4_tile_matmul: a negative count");
+    SMOE_REQUIRE(experts * strips_of_rows(rows) <= kMost && tiles * strips_of_rows(rows) <= kMost, SMOE_ESHAPE,
+                 "too many rows for one q4_tile_matmul call");
+    SMOE_REQUIRE(packed && a && plan && out && aligned16(packed) && aligned16(a) && aligned16(plan), SMOE_EARG,
+                 "q4_tile_matmul: null or misaligned pointer");
+    SMOE_REQUIRE(out_dtype == SMOE_F16 || out_dtype == SMOE_F32, SMOE_EDTYPE, "q4_tile_matmul gives float16 or float32");
+    Writes w;
+    w.add(out, size_t(out_rows) * rows * (out_dtype == SMOE_F16 ? 2 : 4));
+    const TileArgs p = {packed, experts, rows, cols, tiles, a, plan, slot_row, out_rows, out, out_dtype == SMOE_F32};
+    return tile_matmul(p, group, w, as_stream(stream));
+    Q4_CATCH("q4_tile_matmul")
+}
+
 // A call's workspace: the SwiGLU of the pairs and of the shared expert, the partial sums and the counters of the down
 // products' jobs.
 struct MoeSpace {

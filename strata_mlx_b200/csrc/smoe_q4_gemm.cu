@@ -52,6 +52,17 @@ struct GemmArgs {
     int mblocks;
     int nb, nr;   // activation and raw slots
     bool early;
+    // TILES: a stack, its activations in tiles of 16 slots of one expert's
+    const uint4* plan;  // word 0: .x blocks of slots; then each block's first slot, slots, expert
+    const uint32_t* slot_row;
+    int64_t out_rows;
+    int strips;  // of an expert
+    bool floats;
+};
+
+// A job's activation rows: the first and how many, and the first strip of its matrix
+struct GemmBlock {
+    int row0, n, strip0;
 };
 
 struct alignas(64) GemmMaps {
@@ -96,7 +107,9 @@ __device__ __forceinline__ void decode8(uint32_t word, __half2 s, __half2 b, uin
     }
 }
 
-template <int G>
+// TILES: the activations are tiles of 16 slots, each one expert's; a job is up to g.n slots of one expert (`plan`), its
+// MMAs as wide as it has slots, and slot s's row goes to row slot_row[s] of out.
+template <int G, bool TILES>
 __global__ void __launch_bounds__(kGThreads, 1) q4_matmul_kernel(const GemmArgs g, const __grid_constant__ GemmMaps maps) {
     constexpr int kTile = tile_bytes<G>();
     constexpr int kRaw = raw_slot_bytes<G>();
@@ -106,8 +119,15 @@ __global__ void __launch_bounds__(kGThreads, 1) q4_matmul_kernel(const GemmArgs 
     uint8_t* raw = smem + size_t(g.nb) * bslot;
     GemmSmem& S = *reinterpret_cast<GemmSmem*>(raw + g.nr * kRaw);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int jobs = g.nblocks * g.mblocks;
+    if constexpr (TILES) pdl_wait();  // (the plan is a launch's before)
+    const int jobs = (TILES ? static_cast<int>(__ldcg(g.plan).x) : g.nblocks) * g.mblocks;
     const int nk = static_cast<int>(tiles_of_cols(g.cols));
+    auto block_of = [&](int job) {
+        const int b = job / g.mblocks, strip = (job - b * g.mblocks) * kGStrips;
+        if constexpr (!TILES) return GemmBlock{b * g.n, g.n, strip};
+        const uint4 p = __ldcg(g.plan + 1 + b);
+        return GemmBlock{static_cast<int>(p.x), static_cast<int>(p.y), static_cast<int>(p.z) * g.strips + strip};
+    };
     const int nd = 2 * g.n <= int(kGAColumn) ? 2 : 1;
     if (smem_addr(smem) & 1023u) {  // the swizzled layout needs it
         if (threadIdx.x == 0) atomicExch(&g_q4_gemm_status, SMOE_EARG);
@@ -146,15 +166,28 @@ __global__ void __launch_bounds__(kGThreads, 1) q4_matmul_kernel(const GemmArgs 
     // columns c0, c0 + step, .. (eight tokens each) of a job's accumulator, this warp's 32 rows
     auto write_out = [&](int job, int slot, int c0, int step) {
         tc::fence_after_sync();
-        const int64_t r = int64_t(job % g.mblocks) * kGM + 32 * (warp & 3) + lane, tok0 = int64_t(job / g.mblocks) * g.n;
+        const GemmBlock b = block_of(job);
+        const int64_t r = int64_t(job % g.mblocks) * kGM + 32 * (warp & 3) + lane, tok0 = b.row0;
         const uint32_t from = tmem + (uint32_t(32 * (warp & 3)) << 16) + uint32_t(g.n * slot);
-        const int valid = static_cast<int>(min(int64_t(g.n), g.tokens - tok0));
+        const int valid = static_cast<int>(min(int64_t(b.n), g.tokens - tok0));
         __half* out = g.out + (tok0 + c0) * g.rows + r;
         for (int c = c0; c < valid; c += step, out += step * g.rows) {
             uint32_t v[8];
             tc::tmem_ld8(from + c, v);
             tc::tmem_wait_ld();
-            if (r < g.rows) {
+            if (TILES && r < g.rows) {
+                // (whole tiles: every slot is one of the plan's; eight loads of rows in flight together)
+                int64_t to[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) to[j] = g.slot_row ? int64_t(__ldcg(g.slot_row + tok0 + c + j)) : tok0 + c + j;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    if (to[j] >= g.out_rows) continue;
+                    const float f = __uint_as_float(v[j]);
+                    if (g.floats) reinterpret_cast<float*>(g.out)[to[j] * g.rows + r] = f;
+                    else g.out[to[j] * g.rows + r] = __float2half_rn(f);
+                }
+            } else if (r < g.rows) {
                 __half* to = out;
 #pragma unroll
                 for (int j = 0; j < 8; ++j, to += g.rows)
@@ -182,13 +215,13 @@ __global__ void __launch_bounds__(kGThreads, 1) q4_matmul_kernel(const GemmArgs 
         Phase rp;
         int stage = 0;
         for (int job = blockIdx.x; job < jobs && ok; job += gridDim.x) {
-            const int mb = job % g.mblocks;
+            const int strip0 = block_of(job).strip0;
             for (int s = 0; s < nk; ++s, ++stage, rp.next(g.nr)) {
                 if (stage >= g.nr && !(ok = wait(&S.rawfree[rp.slot], rp.phase ^ 1))) break;
                 if (lane == 0) {
                     // (strips past the last read as zeros: weights of zero)
                     tc::mbar_arrive_expect_tx(&S.rawfull[rp.slot], kRaw);
-                    tc::tma_load_2d(smem_addr(raw) + rp.slot * kRaw, &maps.w, s * (kTile / 8), mb * kGStrips,
+                    tc::tma_load_2d(smem_addr(raw) + rp.slot * kRaw, &maps.w, s * (kTile / 8), strip0,
                                     &S.rawfull[rp.slot]);
                 }
                 __syncwarp();
@@ -205,20 +238,20 @@ __global__ void __launch_bounds__(kGThreads, 1) q4_matmul_kernel(const GemmArgs 
         Phase bp;
         int stage = 0;
         for (int job = blockIdx.x; job < jobs && ok; job += gridDim.x) {
-            const int tok0 = job / g.mblocks * g.n;
+            const GemmBlock b = block_of(job);
             for (int s = 0; s < nk; ++s, ++stage, bp.next(g.nb)) {
                 if (stage >= g.nb && !(ok = wait(&S.bfree[bp.slot], bp.phase ^ 1))) break;
                 if (lane == 0) {
                     const uint32_t dst = smem_addr(smem) + bp.slot * bslot;
-                    tc::mbar_arrive_expect_tx(&S.bfull[bp.slot], static_cast<uint32_t>(bslot));
+                    tc::mbar_arrive_expect_tx(&S.bfull[bp.slot], static_cast<uint32_t>(b_slot_bytes(b.n)));
                     int done = 0;
-                    for (int left = g.n; left > 0;) {
-                        const int b = left >= 128 ? 3 : left >= 64 ? 2 : left >= 32 ? 1 : 0;
+                    for (int left = b.n; left > 0;) {
+                        const int m = left >= 128 ? 3 : left >= 64 ? 2 : left >= 32 ? 1 : 0;
                         for (int h = 0; h < 2; ++h)
-                            tc::tma_load_2d(dst + h * g.n * 128 + done * 128, &maps.a[b], s * kCols + 64 * h, tok0 + done,
+                            tc::tma_load_2d(dst + h * g.n * 128 + done * 128, &maps.a[m], s * kCols + 64 * h, b.row0 + done,
                                             &S.bfull[bp.slot]);
-                        done += 16 << b;
-                        left -= 16 << b;
+                        done += 16 << m;
+                        left -= 16 << m;
                     }
                 }
                 __syncwarp();
@@ -231,12 +264,11 @@ __global__ void __launch_bounds__(kGThreads, 1) q4_matmul_kernel(const GemmArgs 
     } else if (warp == kGDecoders) {
         // ---------------- MMA: one lane alone waits and issues
         if (elect_one()) {
-            const uint32_t idesc = tc::idesc_f16_f32(kGM, g.n);
             Phase ap, bp, dp;
             int count = 0;
             for (int job = blockIdx.x; job < jobs && ok; job += gridDim.x, ++count, dp.next(nd)) {
                 if (count >= nd && !(ok = wait_for(&S.dfree[dp.slot], dp.phase ^ 1))) break;
-                const uint32_t d = tmem + uint32_t(g.n * dp.slot);
+                const uint32_t d = tmem + uint32_t(g.n * dp.slot), idesc = tc::idesc_f16_f32(kGM, block_of(job).n);
                 for (int s = 0; s < nk; ++s, ap.next(kGASlots), bp.next(g.nb)) {
                     if (!(ok = wait_for(&S.afull[ap.slot], ap.phase)) || !(ok = wait_for(&S.bfull[bp.slot], bp.phase))) break;
                     tc::fence_after_sync();
@@ -358,7 +390,7 @@ bool matmul_better(int64_t tokens, int64_t rows, int64_t cols) {
     return time_of(tokens, rows, cols, tokens_of_job(tokens, rows, cols)) < stream;
 }
 
-template <int G>
+template <int G, bool TILES>
 static int launch_gemm(GemmArgs a, const GemmMaps& maps, const Writes& w, cudaStream_t st) {
     // (the copies' latency is what the rings hide: a stage of weights is 9 KB and some 0.2 us of work, so as many as fit
     // beside three stages of activations, then more of those)
@@ -369,10 +401,44 @@ static int launch_gemm(GemmArgs a, const GemmMaps& maps, const Writes& w, cudaSt
     while (a.nr > 4 && gemm_smem<G>(a.n, a.nb, a.nr) > kGSmemLimit) a.nr -= 2;
     while (a.nb < kGMaxB && gemm_smem<G>(a.n, a.nb + 1, a.nr) <= kGSmemLimit) ++a.nb;
     const size_t smem = gemm_smem<G>(a.n, a.nb, a.nr);
-    if (int e = max_smem(q4_matmul_kernel<G>, static_cast<int>(smem))) return status_of(static_cast<cudaError_t>(-e), "q4_matmul");
+    if (int e = max_smem(q4_matmul_kernel<G, TILES>, static_cast<int>(smem)))
+        return status_of(static_cast<cudaError_t>(-e), "q4_matmul");
     const int64_t jobs = int64_t(a.nblocks) * a.mblocks;
-    return status_of(launch_pdl(w, q4_matmul_kernel<G>, dim3(static_cast<unsigned>(std::min<int64_t>(jobs, kSms))),
+    return status_of(launch_pdl(w, q4_matmul_kernel<G, TILES>, dim3(static_cast<unsigned>(std::min<int64_t>(jobs, kSms))),
                                 dim3(kGThreads), smem, st, a, maps), "q4_matmul");
+}
+
+// Tensor maps of `strips` strips of weights and of `tokens` rows of activations, and the launch
+template <bool TILES>
+static int encode_and_launch(GemmArgs& a, int group, int64_t strips, const void* x, const Writes& w, cudaStream_t st) {
+    EncodeTiledFn encode = encoder();
+    if (!encode) return fail(SMOE_EARG, "q4_matmul: cuTensorMapEncodeTiled is not available");
+    GemmMaps maps;
+    const cuuint32_t one[2] = {1, 1};
+    {
+        const int64_t tile = tile_bytes_of(group), strip_bytes = tiles_of_cols(a.cols) * tile;
+        const cuuint64_t dims[2] = {static_cast<cuuint64_t>(strip_bytes / 8), static_cast<cuuint64_t>(strips)};
+        const cuuint64_t strides[1] = {static_cast<cuuint64_t>(strip_bytes)};
+        const cuuint32_t box[2] = {static_cast<cuuint32_t>(tile / 8), kGStrips};
+        const CUresult r = encode(&maps.w, CU_TENSOR_MAP_DATA_TYPE_INT64, 2, const_cast<uint8_t*>(a.w), dims, strides, box, one,
+                                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (r != CUDA_SUCCESS) return fail(SMOE_EARG, "q4_matmul: weight tensor map rejected (" + std::to_string(int(r)) + ")");
+    }
+    for (int b = 0; b < 4; ++b) {
+        // (rows past the tokens and columns past the last read as zeros)
+        const cuuint64_t dims[2] = {static_cast<cuuint64_t>(a.cols), static_cast<cuuint64_t>(a.tokens)};
+        const cuuint64_t strides[1] = {static_cast<cuuint64_t>(a.cols) * 2};
+        const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(16 << b)};
+        const CUresult r = encode(&maps.a[b], CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(x), dims, strides, box, one,
+                                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (r != CUDA_SUCCESS)
+            return fail(SMOE_EARG, "q4_matmul: activation tensor map rejected (" + std::to_string(int(r)) + ")");
+    }
+    if (group == 32) return launch_gemm<32, TILES>(a, maps, w, st);
+    if (group == 64) return launch_gemm<64, TILES>(a, maps, w, st);
+    return launch_gemm<128, TILES>(a, maps, w, st);
 }
 
 int matmul_f16(const ProductArgs& p, int group, const Writes& w, cudaStream_t st) {
@@ -386,35 +452,85 @@ int matmul_f16(const ProductArgs& p, int group, const Writes& w, cudaStream_t st
     a.mblocks = static_cast<int>((p.d_rows + kGM - 1) / kGM);
     a.n = tokens_of_job(p.d_tokens, p.d_rows, p.cols);
     a.nblocks = static_cast<int>((p.d_tokens + a.n - 1) / a.n);
-    EncodeTiledFn encode = encoder();
-    if (!encode) return fail(SMOE_EARG, "q4_product: cuTensorMapEncodeTiled is not available");
-    GemmMaps maps;
-    const cuuint32_t one[2] = {1, 1};
-    {
-        const int64_t tile = tile_bytes_of(group), strip_bytes = tiles_of_cols(p.cols) * tile;
-        const cuuint64_t dims[2] = {static_cast<cuuint64_t>(strip_bytes / 8), static_cast<cuuint64_t>(strips_of_rows(p.d_rows))};
-        const cuuint64_t strides[1] = {static_cast<cuuint64_t>(strip_bytes)};
-        const cuuint32_t box[2] = {static_cast<cuuint32_t>(tile / 8), kGStrips};
-        const CUresult r = encode(&maps.w, CU_TENSOR_MAP_DATA_TYPE_INT64, 2, const_cast<uint8_t*>(p.dw[0]), dims, strides, box,
-                                  one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
-                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-        if (r != CUDA_SUCCESS)
-            return fail(SMOE_EARG, "q4_product: weight tensor map rejected (" + std::to_string(int(r)) + ")");
+    return encode_and_launch<false>(a, group, strips_of_rows(p.d_rows), p.x, w, st);
+}
+
+// ---- a stack's products of many pairs, in tiles of 16 slots of one expert's (smoe_tiles_of)
+
+// Slots of a job: a stage's decoding takes as long as the MMAs of 100 tokens, so blocks of few slots cost no more, and
+// two accumulators fit.
+constexpr int kTileSlots = 128;
+constexpr int kPlanThreads = 1024;
+constexpr int kSlots = 16;  // of a tile
+
+// Runs of one expert's tiles cut into blocks of up to kTileSlots slots, in their order: one CTA, 1024 tiles at a time.
+__global__ void __launch_bounds__(kPlanThreads) q4_plan_kernel(const uint32_t* __restrict__ tile_expert, int tiles,
+                                                               uint32_t experts, uint4* __restrict__ plan) {
+    constexpr int kMost = kTileSlots / kSlots;
+    __shared__ int starts[kPlanThreads / 32], counts[kPlanThreads / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    pdl_wait();
+    int run = 0, blocks = 0;  // the last run's first tile, and the blocks, of the tiles before
+    for (int t0 = 0; t0 < tiles; t0 += kPlanThreads) {
+        const int t = t0 + static_cast<int>(threadIdx.x);
+        const uint32_t e = t < tiles ? tile_expert[t] : experts;
+        const bool in = e < experts, first = in && (t == 0 || tile_expert[t - 1] != e);
+        int start = first ? t : 0;  // this tile's run's first tile: the largest one up to here
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, start, o);
+            if (lane >= o) start = max(start, u);
+        }
+        if (lane == 31) starts[warp] = start;
+        __syncthreads();
+        int latest = run;
+        for (int w = 0; w < kPlanThreads / 32; ++w) {
+            if (w < warp) start = max(start, starts[w]);
+            latest = max(latest, starts[w]);
+        }
+        start = max(start, run);
+        const bool lead = in && (t - start) % kMost == 0;
+        const uint32_t leads = __ballot_sync(0xffffffffu, lead);
+        if (lane == 0) counts[warp] = __popc(leads);
+        __syncthreads();
+        int at = blocks + __popc(leads & ((1u << lane) - 1));
+        for (int w = 0; w < kPlanThreads / 32; ++w) {
+            if (w < warp) at += counts[w];
+            blocks += counts[w];
+        }
+        if (lead) {
+            int n = 1;
+            while (n < kMost && t + n < tiles && tile_expert[t + n] == e) ++n;
+            plan[1 + at] = make_uint4(uint32_t(t) * kSlots, uint32_t(n) * kSlots, e, 0);
+        }
+        run = latest;
+        __syncthreads();
     }
-    for (int b = 0; b < 4; ++b) {
-        // (rows past the tokens and columns past the last read as zeros)
-        const cuuint64_t dims[2] = {static_cast<cuuint64_t>(p.cols), static_cast<cuuint64_t>(p.d_tokens)};
-        const cuuint64_t strides[1] = {static_cast<cuuint64_t>(p.cols) * 2};
-        const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(16 << b)};
-        const CUresult r = encode(&maps.a[b], CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(p.x), dims, strides, box,
-                                  one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-        if (r != CUDA_SUCCESS)
-            return fail(SMOE_EARG, "q4_product: activation tensor map rejected (" + std::to_string(int(r)) + ")");
-    }
-    if (group == 32) return launch_gemm<32>(a, maps, w, st);
-    if (group == 64) return launch_gemm<64>(a, maps, w, st);
-    return launch_gemm<128>(a, maps, w, st);
+    if (threadIdx.x == 0) plan[0] = make_uint4(uint32_t(blocks), 0, 0, 0);
+    pdl_release();
+}
+
+int tile_plan(const uint32_t* tile_expert, int64_t tiles, int64_t experts, void* plan, const Writes& w, cudaStream_t st) {
+    return status_of(launch_pdl(w, q4_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, tile_expert, static_cast<int>(tiles),
+                                static_cast<uint32_t>(experts), static_cast<uint4*>(plan)), "q4_tile_plan");
+}
+
+int tile_matmul(const TileArgs& p, int group, const Writes& w, cudaStream_t st) {
+    GemmArgs a = {};
+    a.w = p.w;
+    a.out = static_cast<__half*>(p.out);
+    a.rows = p.rows;
+    a.cols = p.cols;
+    a.tokens = p.tiles * kSlots;
+    a.mblocks = static_cast<int>((p.rows + kGM - 1) / kGM);
+    a.n = kTileSlots;
+    a.nblocks = static_cast<int>(p.tiles);  // (at most)
+    a.plan = static_cast<const uint4*>(p.plan);
+    a.slot_row = p.slot_row;
+    a.out_rows = p.out_rows;
+    a.strips = static_cast<int>(strips_of_rows(p.rows));
+    a.floats = p.floats;
+    return encode_and_launch<true>(a, group, p.experts * strips_of_rows(p.rows), p.x, w, st);
 }
 
 cudaError_t matmul_status(int* v, bool clear) {

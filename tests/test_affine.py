@@ -64,6 +64,24 @@ def test_pointers_and_types_are_checked(lib):
     assert lib.smoe_q4_moe(None, None, 0, None) == EARG
 
 
+def test_tile_products_check_their_arguments(lib):
+    def plan(te=A, tiles=3, experts=4, plan=A, nbytes=64):
+        return lib.smoe_q4_tile_plan(te, tiles, experts, plan, nbytes, None)
+
+    def product(w=A, experts=4, rows=16, cols=128, group=64, a=A, tiles=3, plan=A, slot=A, out_rows=9, out=A, dtype=1):
+        return lib.smoe_q4_tile_matmul(w, experts, rows, cols, group, a, tiles, plan, slot, out_rows, out, dtype, None)
+
+    assert lib.smoe_q4_tile_plan_size(3) == 64 and lib.smoe_q4_tile_plan_size(0) == 0
+    assert plan(tiles=0) == 0 and product(tiles=0) == 0 and product(out_rows=0) == 0
+    assert plan(te=None) == EARG and plan(tiles=-1) == ESHAPE and plan(experts=0) == ESHAPE and plan(tiles=2**24 + 1) == ESHAPE
+    assert plan(plan=None) == EWORKSPACE and plan(nbytes=63) == EWORKSPACE and plan(plan=A + 8) == EWORKSPACE
+    for bad in (dict(w=None), dict(a=None), dict(plan=None), dict(out=None), dict(w=A + 8), dict(a=A + 2), dict(out_rows=-1)):
+        assert product(**bad) == EARG, bad
+    for bad in (dict(tiles=-1), dict(experts=0), dict(cols=96), dict(group=16), dict(rows=0), dict(tiles=2**24, rows=2**20)):
+        assert product(**bad) == ESHAPE, bad
+    assert product(dtype=3) == EDTYPE
+
+
 def test_empty_calls_do_nothing(lib):
     assert lib.smoe_q4_quantize(A, 1, 0, 128, 64, A, A, A, None) == 0
     assert lib.smoe_q4_linear(A, 4, 128, 64, A, 0, A, 1, None) == 0

@@ -60,9 +60,14 @@ def product64(x, p, group, dtype=None):
     return (y, off if dtype is None else off + last(y, dtype))
 
 
-def glu64(x, gate, up, group, dtype, share=None):
-    """silu(gate x) up x (times share) in float64, and its tolerance once rounded to dtype (a block keeps more of it)."""
+def glu64(x, gate, up, group, dtype, share=None, rounded=False, apart=False):
+    """silu(gate x) up x (times share) in float64, and its tolerance once rounded to dtype (a block keeps more of it);
+    rounded: of products whose weights are rounded to float16; apart: that are rounded to float16 themselves."""
     (g, eg), (u, eu) = product64(x, gate, group), product64(x, up, group)
+    if rounded:
+        eg, eu = (e + x.double().abs() @ last(floats64(p)[0], F16).mT for e, p in ((eg, gate), (eu, up)))
+    if apart:
+        eg, eu = eg + last(g, F16), eu + last(u, F16)
     a = g * torch.sigmoid(g)
     h, off = a * u, 1.1 * eg * u.abs() + a.abs() * eu + 1.1 * eg * eu
     off = off + (a * u).abs() * 2.0**-20  # float32 exp, quotient and products
@@ -164,10 +169,10 @@ def test_a_layer_is_its_definition(cuda, rows, cols, group, tokens, dtype):
     close(got, *layer64(x, p, group, dtype))
 
 
-def layer64(x, p, group, dtype):
+def layer64(x, p, group, dtype, rounded=False):
     """More than 16 float16 tokens may multiply weights rounded to float16: half a step of each, or of a subnormal."""
     y, off = product64(x, p, group, dtype)
-    if dtype == F16 and x.shape[0] > 16:
+    if dtype == F16 and (rounded or x.shape[0] > 16):
         off = off + x.double().abs() @ last(floats64(p)[0], F16).mT
     return y, off
 
@@ -277,7 +282,11 @@ def test_pair_products_are_their_definition(cuda, dtype, tokens, k, experts):
     assert got.shape == (tokens, k, 1, rows)
     for e in range(experts):
         t, j = (idx == e).nonzero(as_tuple=True)
-        close(got[t, j, 0], *product64(x[t, 0, 0], [a[e] for a in p], group, dtype))
+        one = [a[e] for a in p]
+        want, off = product64(x[t, 0, 0], one, group, dtype)
+        if dtype == F16 and tokens * k > affine.MAX_PAIRS:  # (by tiles: half a step of each weight, rounded to float16)
+            off = off + x[t, 0, 0].double().abs() @ last(floats64(one)[0], F16).mT
+        close(got[t, j, 0], want, off)
     each = stack(x.expand(tokens, k, 1, cols), idx)  # a row of its own for every pair
     close(each.double(), got.double(), last(got.double(), dtype) * 2 + sums(cols, group) * 8)
 
@@ -294,6 +303,67 @@ def test_pairs_of_no_expert_are_left_as_they_were(cuda):
     want = stack(x[:, None, None], idx.clamp(0, 5))[:, :, 0].reshape(8, 33)
     out_of = torch.tensor([0, 1, 0, 0, 1, 1, 0, 0], dtype=torch.bool, device=cuda)
     assert (out[out_of] == 7).all() and torch.equal(out[~out_of], want[~out_of])
+
+
+@pytest.fixture
+def by_tiles(monkeypatch):
+    """Every float16 call of pairs by the tiles of a prompt."""
+    monkeypatch.setattr(affine, "_by_tiles", lambda lin, dtype, pairs: dtype == F16 and pairs > 0)
+
+
+TILES = [(1, 1, 1, 40, 32, 32), (5, 3, 4, 16, 128, 64), (40, 2, 3, 129, 160, 32), (30, 32, 40, 250, 384, 128), (700, 3, 7, 600, 96, 32),
+         (2000, 1, 2, 24, 2176, 64), (300, 8, 1024, 33, 64, 64), (1180, 8, 256, 130, 128, 64)]
+
+
+@pytest.mark.parametrize("tokens, k, experts, rows, cols, group", TILES)
+def test_pair_products_by_tiles_are_their_definition(cuda, by_tiles, tokens, k, experts, rows, cols, group):
+    gen = gen_of(tokens + rows)
+    p = parts(gen, (experts,), rows, cols, group)
+    stack = affine.QuantizedSwitchLinear(*p, group_size=group)
+    idx = torch.randint(0, experts, (tokens, k), dtype=torch.int32, device=cuda, generator=gen)
+    x = torch.randn(tokens, 1, 1, cols, device=cuda, generator=gen).half()
+    got = stack(x, idx)
+    assert got.shape == (tokens, k, 1, rows)
+    for e in range(experts):
+        t, j = (idx == e).nonzero(as_tuple=True)
+        if len(t):
+            close(got[t, j, 0], *layer64(x[t, 0, 0], [a[e] for a in p], group, F16, rounded=True))
+    assert torch.equal(stack(x.expand(tokens, k, 1, cols), idx), got) and torch.equal(stack(x, idx), got)
+    assert not affine.failed()
+
+
+@pytest.mark.parametrize("tokens, k, experts, hidden, ffn, group, down_group", [(9, 2, 3, 96, 64, 32, 64), (200, 6, 17, 320, 160, 32, 32),
+                                                                               (700, 4, 5, 256, 384, 128, 64)])
+def test_experts_by_tiles_are_their_definition(cuda, by_tiles, tokens, k, experts, hidden, ffn, group, down_group):
+    gen = gen_of(tokens)
+    r, _, glu, _ = make_experts(gen, experts, hidden, ffn, 128, group, down_group)
+    x = torch.randn(tokens, hidden, device=cuda, generator=gen).half()
+    idx = torch.rand(tokens, experts, device=cuda, generator=gen).argsort(-1)[:, :k] if k <= experts else torch.randint(
+        0, experts, (tokens, k), device=cuda, generator=gen)
+    idx[3, 1], idx[5] = experts, -1  # pairs of no expert
+    y = glu(x, idx)
+    for e in range(experts):
+        t, j = (idx == e).nonzero(as_tuple=True)
+        gate, up, down = ([a[e] for a in p] for p in r)
+        h, eh = glu64(x[t], gate, up, group, F16, rounded=True)
+        want, off = layer64(h, down, down_group, F16, rounded=True)
+        close(y[t, j], want, off + eh @ floats64(down)[0].abs().mT * 1.01)
+
+
+def test_pairs_of_no_expert_by_tiles_are_left_as_they_were(cuda):
+    gen = gen_of(24)
+    stack = affine.QuantizedSwitchLinear(*parts(gen, (6,), 33, 64, 64), group_size=64)
+    x = torch.randn(4, 64, device=cuda, generator=gen).half()
+    idx = torch.tensor([[0, 6], [5, 5], [7, -1], [2, 1]], dtype=torch.int32, device=cuda)
+    want = stack(x[:, None, None], idx.clamp(0, 5))[:, :, 0].reshape(8, 33)
+    tiles = affine._Tiles(stack, idx.reshape(-1), 2)
+    a = x.index_select(0, tiles.row)
+    for dtype in (F16, F32):
+        out = tiles.product(stack, a, torch.full((8, 33), 7.0, dtype=dtype, device=cuda), True)
+        out_of = torch.tensor([0, 1, 0, 0, 1, 1, 0, 0], dtype=torch.bool, device=cuda)
+        assert (out[out_of] == 7).all() and (out[~out_of] - want[~out_of].to(dtype)).abs().max() < 0.02
+        none = affine._Tiles(stack, torch.full((8,), 9, dtype=torch.int32, device=cuda), 2)
+        assert (none.product(stack, a[: none.count * 16], torch.full((8, 33), 7.0, dtype=dtype, device=cuda), True) == 7).all()
 
 
 def test_no_pairs(cuda):
@@ -321,17 +391,26 @@ def make_experts(gen, experts, hidden, ffn, shared, group, down_group=None):
     return r, s, glu, mlp
 
 
-def moe64(x, r, s, idx, w, g, group, down_group, dtype):
-    """The block behind its route in float64 and its tolerance; idx past the experts adds nothing."""
+def moe64(x, r, s, idx, w, g, group, down_group, dtype, rounded=False):
+    """The block behind its route in float64 and its tolerance; idx past the experts adds nothing. Past 64 tokens the
+    experts' outputs, the shared expert's, its gate (and their product) and the sum of the experts' are rounded to dtype
+    each: three half steps of every term at most (in float32 the sum's k additions and products besides). rounded: float16
+    weights, and the shared expert's gate and up, too."""
     tokens, hidden = x.shape
     out, off = torch.zeros(tokens, hidden, dtype=torch.float64, device=x.device), torch.zeros(tokens, hidden, dtype=torch.float64, device=x.device)
 
     def add(t, mats, share, members):
-        h, eh = glu64(x[t], mats[0], mats[1], group, dtype, share[:, None])
+        h, eh = glu64(x[t], mats[0], mats[1], group, dtype, share[:, None], rounded, rounded)
         wd, md = floats64(mats[2])
         n = sums(wd.shape[-1] * members, down_group)  # (one sum over every expert's columns)
         out.index_add_(0, t, h @ wd.mT)
         off.index_add_(0, t, eh @ wd.abs().mT + n * ((h.abs() + eh) @ md.mT))
+        if rounded:
+            off.index_add_(0, t, (h.abs() + eh) @ last(wd, F16).mT)
+        if tokens > 64:
+            y = h @ wd.mT
+            each = y.abs() * torch.finfo(dtype).eps / 2 + (2.0**-25 if dtype == F16 else 0)
+            off.index_add_(0, t, 1.01 * each * (3 if dtype == F16 else 2 * members + 3))
 
     members = idx.shape[1] + 1
     for e in range(r[0][0].shape[0]):
@@ -495,7 +574,7 @@ def test_floats_made_4_bit_and_run_as_a_block(cuda, dtype, tokens):
 def test_a_graph_replays_the_eager_bits(cuda):
     gen = gen_of(43)
     _, _, block, _, _ = make_block(gen, 40, 256, 128, 192, 64, 5)
-    for tokens in (1, 5, 20):
+    for tokens in (1, 5, 20, 500):
         xs = [torch.randn(tokens, 256, device=cuda, generator=gen).half() for _ in range(3)]
         eager = [block(x).clone() for x in xs]
         step = fused.GraphedBlock(block, tokens, 256, F16, cuda)
@@ -503,6 +582,40 @@ def test_a_graph_replays_the_eager_bits(cuda):
             for x, want in zip(xs, eager):
                 assert torch.equal(step(x), want)
     assert not affine.failed()
+
+
+@pytest.mark.parametrize("tokens, experts, k, hidden, ffn, shared, group", [(700, 20, 4, 256, 192, 1120, 32), (260, 12, 10, 1024, 64, 2048, 64)])
+def test_a_prompt_through_the_experts_and_their_combine(cuda, tokens, experts, k, hidden, ffn, shared, group):
+    gen = gen_of(tokens)
+    r, s, glu, mlp = make_experts(gen, experts, hidden, ffn, shared, group)
+    assert tokens * k > affine.MAX_PAIRS and mlp._apart(tokens) == (tokens == 700)
+    x = torch.randn(tokens, hidden, device=cuda, generator=gen).half()
+    idx = torch.rand(tokens, experts, device=cuda, generator=gen).argsort(-1)[:, :k].to(torch.int32)
+    w = torch.softmax(torch.randn(tokens, k, device=cuda, generator=gen), -1)
+    g = torch.randn(tokens, 1, device=cuda, generator=gen).half()
+    idx[::7, 0], idx[11] = experts, -1  # choices of no expert
+    close(affine.moe(glu, mlp, x, idx, w, g), *moe64(x, r, s, idx, w, g, group, group, F16, rounded=True))
+    assert not affine.failed()
+
+
+def test_a_prompt_in_several_parts(cuda, monkeypatch):
+    gen = gen_of(46)
+    _, _, block, _, _ = make_block(gen, 40, 256, 128, 192, 64, 5)
+    x = torch.randn(900, 256, device=cuda, generator=gen).half()
+    idx = torch.randint(0, 40, (900, 5), dtype=torch.int32, device=cuda, generator=gen)
+    up = block.switch_mlp.up_proj
+    want = block(x), up(x[:, None, None], idx)
+    monkeypatch.setattr(affine, "TILE_PAIRS", 1111)
+    assert torch.equal(block(x), want[0]) and torch.equal(up(x[:, None, None], idx), want[1])
+    # (a part's calls are those of a prompt of its length, whose kernels may be others)
+    w, g = torch.rand(900, 5, device=cuda, generator=gen), torch.randn(900, 1, device=cuda, generator=gen).half()
+
+    def moe(a, b):
+        return affine.moe(block.switch_mlp, block.shared_expert, x[a:b], idx[a:b], w[a:b], g[a:b])
+
+    parts_of = torch.cat((moe(0, 500), moe(500, 900)))
+    monkeypatch.setattr(affine, "COMBINE_TOKENS", 500)
+    assert torch.equal(moe(0, 900), parts_of)
 
 
 def test_two_graphs_and_an_eager_call_at_once(cuda):
