@@ -3,17 +3,18 @@
 // out[t, r] = sum_c w[r, c] x[t, c], the weights w = code scale + bias rounded once to float16 (the activations' type)
 // and float32 sums. 128 weight rows are the M side of a tcgen05 MMA (8 strips), up to 256 tokens the N side, so a row is
 // decoded once for that many tokens. What bounds it: the tensor pipe (2 rows cols tokens flops at 4,096 multiply-adds a
-// cycle of an SM) and beside it the decoding's issue, 17 instructions for 8 weights: a stage of 128 x 128 weights takes
-// 272 issue slots a scheduler, its MMAs 4 cycles a token. From about 70 tokens a job on the tensor pipe is the longer.
+// cycle of an SM) and beside it the decoding, 17 instructions for 8 weights: a stage of 128 x 128 weights takes 272
+// issue slots a scheduler, and with its hand-offs 0.38 us; its MMAs take 2.8 ns a token, so from about 140 tokens a job the
+// tensor pipe is the longer. 4096 x 4096 at 1180 tokens: 36 us, 1100 TFLOP/s.
 //
 // Per CTA (persistent over jobs = (block of tokens, 128 rows)), warp-specialized, every hand-off an mbarrier:
 //   warp 17   weights: a stage is one tile of each of the 8 strips, one TMA box (a copy a strip took the warp 120 cycles
 //             each to issue, more than the stage's work) into a ring of up to 10 slots
-//   warp 18   activations: the tokens' 128 columns by TMA (boxes of 128 / 64 / 32 / 16 rows x 64 columns, 128-byte
-//             swizzle) into a ring of its own
-//   warps 0-15 decoders, two groups on every other stage: a thread reads half of its row's 128 columns, (q | 0x6400) - 1024 makes a pair of codes
-//             float16 exactly, one fused multiply-add with the group's scale and bias rounds it to the weight; stored to
-//             its TMEM lane of an A slot
+//   warp 18   activations: the tokens' 128 columns by TMA into a ring of its own, two boxes of all the job's rows x 64
+//             columns (128-byte swizzle)
+//   warps 0-15 decoders, two groups on every other stage: a thread reads half of its row's 128 columns, (q | 0x6400) - 1024
+//             makes a pair of codes float16 exactly, one fused multiply-add with the group's scale and bias rounds it to
+//             the weight; stored to its TMEM lane of an A slot
 //   warp 16   MMA: A from TMEM, B from shared memory, 8 MMAs of K = 16 a stage; commits free the slots.
 //   warps 19-22 read a job's sums back and write them out while the next job runs (jobs of up to 160 tokens have two
 //             accumulators); a CTA's last job is the decoders'
@@ -65,9 +66,15 @@ struct GemmBlock {
     int row0, n, strip0;
 };
 
+// Slots of a job of TILES: a stage's decoding takes as long as the MMAs of 140 tokens, and two accumulators fit (the SwiGLU
+// of 256 experts of 1536 x 4096, 128 tokens each: 1709 us, in jobs of 128 slots 2029; 37 tokens each: 1079 and 1055).
+constexpr int kTileSlots = 160;
+constexpr int kSlots = 16;  // of a tile
+
+template <bool TILES>
 struct alignas(64) GemmMaps {
-    CUtensorMap w;     // strips of the matrix as rows of 8-byte words, in boxes of a tile of 8 strips
-    CUtensorMap a[4];  // boxes of 16, 32, 64, 128 rows x 64 columns
+    CUtensorMap w;  // strips of the matrix as rows of 8-byte words, in boxes of a tile of 8 strips
+    CUtensorMap a[TILES ? kTileSlots / kSlots : 1];  // boxes of a job's rows x 64 columns; TILES: of 16, 32, .. rows
 };
 
 struct GemmSmem {
@@ -110,7 +117,7 @@ __device__ __forceinline__ void decode8(uint32_t word, __half2 s, __half2 b, uin
 // TILES: the activations are tiles of 16 slots, each one expert's; a job is up to g.n slots of one expert (`plan`), its
 // MMAs as wide as it has slots, and slot s's row goes to row slot_row[s] of out.
 template <int G, bool TILES>
-__global__ void __launch_bounds__(kGThreads, 1) q4_matmul_kernel(const GemmArgs g, const __grid_constant__ GemmMaps maps) {
+__global__ void __launch_bounds__(kGThreads, 1) q4_matmul_kernel(const GemmArgs g, const __grid_constant__ GemmMaps<TILES> maps) {
     constexpr int kTile = tile_bytes<G>();
     constexpr int kRaw = raw_slot_bytes<G>();
     extern __shared__ __align__(1024) uint8_t gsmem[];
@@ -244,15 +251,9 @@ __global__ void __launch_bounds__(kGThreads, 1) q4_matmul_kernel(const GemmArgs 
                 if (lane == 0) {
                     const uint32_t dst = smem_addr(smem) + bp.slot * bslot;
                     tc::mbar_arrive_expect_tx(&S.bfull[bp.slot], static_cast<uint32_t>(b_slot_bytes(b.n)));
-                    int done = 0;
-                    for (int left = b.n; left > 0;) {
-                        const int m = left >= 128 ? 3 : left >= 64 ? 2 : left >= 32 ? 1 : 0;
-                        for (int h = 0; h < 2; ++h)
-                            tc::tma_load_2d(dst + h * g.n * 128 + done * 128, &maps.a[m], s * kCols + 64 * h, b.row0 + done,
-                                            &S.bfull[bp.slot]);
-                        done += 16 << m;
-                        left -= 16 << m;
-                    }
+                    for (int h = 0; h < 2; ++h)
+                        tc::tma_load_2d(dst + h * g.n * 128, &maps.a[TILES ? b.n / kSlots - 1 : 0], s * kCols + 64 * h, b.row0,
+                                        &S.bfull[bp.slot]);
                 }
                 __syncwarp();
             }
@@ -366,11 +367,12 @@ static EncodeTiledFn encoder() {
 }
 
 // Microseconds of the prompt's kernel with jobs of n tokens, as measured: a start, and for every round of jobs over the SMs
-// a stage's 0.45 us (its hand-offs and decoding) or 4.5 ns a token (its MMAs), whichever is longer, and 1 us at its ends.
-// (64007 x 2560: 48 us at 33 tokens; 4096 x 4096: 17 us at 33, 40 us at 1180; 1024 x 1024: 6.5 us at 33.)
+// a stage's 0.38 us (its hand-offs and decoding) or 2.8 ns a token (its MMAs), whichever is longer, and 1 us at its ends.
+// (4096 x 4096, 128 tokens, one round: 17.5 us with jobs of 32 to 96 tokens, 18.2 of 160, 24.6 of 256; 1180 tokens: 36.9
+// in jobs of 144, two rounds, 52.8 of 96, three, 51.0 of 256; 1536 x 4096, 4096 tokens: 39.3 of 176, 48.5 of 112, 53.2 of 256.)
 static double time_of(int64_t tokens, int64_t rows, int64_t cols, int n) {
     const int64_t jobs = (tokens + n - 1) / n * ((rows + kGM - 1) / kGM);
-    const double stage = std::max(0.45, 0.0045 * n);
+    const double stage = std::max(0.38, 0.0028 * n);
     return 4.0 + double((jobs + kSms - 1) / kSms) * (double(tiles_of_cols(cols)) * stage + 1.0);
 }
 
@@ -391,7 +393,7 @@ bool matmul_better(int64_t tokens, int64_t rows, int64_t cols) {
 }
 
 template <int G, bool TILES>
-static int launch_gemm(GemmArgs a, const GemmMaps& maps, const Writes& w, cudaStream_t st) {
+static int launch_gemm(GemmArgs a, const GemmMaps<TILES>& maps, const Writes& w, cudaStream_t st) {
     // (the copies' latency is what the rings hide: a stage of weights is 9 KB and some 0.2 us of work, so as many as fit
     // beside three stages of activations, then more of those)
     a.nr = kGMaxRaw;
@@ -413,7 +415,7 @@ template <bool TILES>
 static int encode_and_launch(GemmArgs& a, int group, int64_t strips, const void* x, const Writes& w, cudaStream_t st) {
     EncodeTiledFn encode = encoder();
     if (!encode) return fail(SMOE_EARG, "q4_matmul: cuTensorMapEncodeTiled is not available");
-    GemmMaps maps;
+    GemmMaps<TILES> maps;
     const cuuint32_t one[2] = {1, 1};
     {
         const int64_t tile = tile_bytes_of(group), strip_bytes = tiles_of_cols(a.cols) * tile;
@@ -425,11 +427,11 @@ static int encode_and_launch(GemmArgs& a, int group, int64_t strips, const void*
                                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
         if (r != CUDA_SUCCESS) return fail(SMOE_EARG, "q4_matmul: weight tensor map rejected (" + std::to_string(int(r)) + ")");
     }
-    for (int b = 0; b < 4; ++b) {
+    for (int b = 0; b < int(sizeof(maps.a) / sizeof(maps.a[0])); ++b) {
         // (rows past the tokens and columns past the last read as zeros)
         const cuuint64_t dims[2] = {static_cast<cuuint64_t>(a.cols), static_cast<cuuint64_t>(a.tokens)};
         const cuuint64_t strides[1] = {static_cast<cuuint64_t>(a.cols) * 2};
-        const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(16 << b)};
+        const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(TILES ? kSlots * (b + 1) : a.n)};
         const CUresult r = encode(&maps.a[b], CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(x), dims, strides, box, one,
                                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -457,11 +459,7 @@ int matmul_f16(const ProductArgs& p, int group, const Writes& w, cudaStream_t st
 
 // ---- a stack's products of many pairs, in tiles of 16 slots of one expert's (smoe_tiles_of)
 
-// Slots of a job: a stage's decoding takes as long as the MMAs of 100 tokens, so blocks of few slots cost no more, and
-// two accumulators fit.
-constexpr int kTileSlots = 128;
 constexpr int kPlanThreads = 1024;
-constexpr int kSlots = 16;  // of a tile
 
 // Runs of one expert's tiles cut into blocks of up to kTileSlots slots, in their order: one CTA, 1024 tiles at a time.
 __global__ void __launch_bounds__(kPlanThreads) q4_plan_kernel(const uint32_t* __restrict__ tile_expert, int tiles,
