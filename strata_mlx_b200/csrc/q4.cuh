@@ -25,7 +25,10 @@
 // the end of the row. Products are exact and sums are float32: the result is the formula's but for float32 rounding.
 // The bias takes sum x over the group, from the same B operands times a matrix of 2^-24.
 // Float32 activations are three bfloat16 pieces (8 + 8 + 8 bits: the whole float32), each through the same MMAs;
-// codes become bfloat16 by (q | 0x4300) - 128, exact too.
+// codes become bfloat16 by (q | 0x4300) - 136, exact too: q - 8, with bias + 8 scale in the bias's place. A group's weights
+// lie on both sides of zero mostly, q scale and bias are then numbers of one size that nearly cancel, and their float32 sums
+// lose more than those of q - 8 do (a block of 64 experts, 2048 wide, is 1.03e-6 of its result off with q, 7.4e-7 with
+// q - 8, and 2.7e-7 with sums of their own for the activations' small pieces).
 #pragma once
 
 #include <cuda_bf16.h>
@@ -194,7 +197,7 @@ struct Codes<float> {
     uint32_t lo[4], hi[4];
     static __device__ __forceinline__ uint32_t code(uint32_t w) {
         const uint32_t b = (w & 0x000f000fu) | 0x43004300u;  // 128 + q
-        const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&b), __float2bfloat162_rn(128.0f));
+        const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&b), __float2bfloat162_rn(136.0f));
         return *reinterpret_cast<const uint32_t*>(&r);
     }
     __device__ __forceinline__ Codes(uint32_t u, uint32_t v) {
@@ -242,10 +245,11 @@ struct Ones {
 };
 
 // The sums of one group of columns of MT strips times a block of 8 activation rows: codes in lo and hi (float16: hi
-// holds 16 times its sum, both 2^-24 times theirs; float32: lo alone), the activations alone in on (times 2^-24 too).
+// holds 16 times its sum, both 2^-24 times theirs; float32: the activations' first pieces in lo, the others in hi), the
+// activations alone in on (times 2^-24 too).
 template <typename T, int MT>
 struct Sums {
-    float lo[MT][4], hi[MT][4], on[4], on2[4];  // (on2: half of the activations, to halve the chain of MMAs)
+    float lo[MT][4], hi[MT][4], on[4], on2[4];  // (on2: float16: half of the activations, to halve the chain of MMAs; float32: the small pieces)
 };
 
 template <bool FIRST, int MT>
@@ -275,21 +279,23 @@ __device__ __forceinline__ void run_mma(const Codes<float> (&a)[MT], const Acts<
                                         const Ones<float>& one) {
     float f[8] = {__uint_as_float(x.v.x), __uint_as_float(x.v.y), __uint_as_float(x.v.z), __uint_as_float(x.v.w),
                   __uint_as_float(x.w.x), __uint_as_float(x.w.y), __uint_as_float(x.w.z), __uint_as_float(x.w.w)};
-    auto piece = [&](auto first) {
+    // (the tensor core cuts its sums off, always towards zero: the small pieces have sums of their own, so that the large
+    // ones are cut two times a run and not six)
+    auto piece = [&](auto first, float (&sum)[MT][4], float (&on)[4]) {
         constexpr bool kFirst = decltype(first)::value;
         const uint32_t b0 = bf16_pair(f[0], f[1]), b1 = bf16_pair(f[2], f[3]);
         const uint32_t c0 = bf16_pair(f[4], f[5]), c1 = bf16_pair(f[6], f[7]);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-            mma_bf16<kFirst>(s.lo[m], a[m].lo[0], a[m].lo[1], a[m].lo[2], a[m].lo[3], b0, b1);
-            mma_bf16<false>(s.lo[m], a[m].hi[0], a[m].hi[1], a[m].hi[2], a[m].hi[3], c0, c1);
+            mma_bf16<kFirst>(sum[m], a[m].lo[0], a[m].lo[1], a[m].lo[2], a[m].lo[3], b0, b1);
+            mma_bf16<false>(sum[m], a[m].hi[0], a[m].hi[1], a[m].hi[2], a[m].hi[3], c0, c1);
         }
-        mma_bf16<kFirst>(s.on, one.v[0], one.v[1], one.v[2], one.v[3], b0, b1);
-        mma_bf16<kFirst>(s.on2, one.v[0], one.v[1], one.v[2], one.v[3], c0, c1);
+        mma_bf16<kFirst>(on, one.v[0], one.v[1], one.v[2], one.v[3], b0, b1);
+        mma_bf16<false>(on, one.v[0], one.v[1], one.v[2], one.v[3], c0, c1);
     };
-    piece(std::integral_constant<bool, FIRST>{});
-    piece(std::false_type{});
-    piece(std::false_type{});
+    piece(std::integral_constant<bool, FIRST>{}, s.lo, s.on);
+    piece(std::integral_constant<bool, FIRST>{}, s.hi, s.on2);
+    piece(std::false_type{}, s.hi, s.on2);
 }
 
 // What a row's sum is to be multiplied by in the end (the codes' 2^-24)
@@ -302,10 +308,11 @@ __device__ __forceinline__ void group_end(float (&acc)[4], const Sums<T, MT>& s,
     const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&sb0));
     const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&sb1));
     const float on[2] = {s.on[0] + s.on2[0], s.on[1] + s.on2[1]};  // (the same for both rows)
+    const float b[2] = {sizeof(T) == 2 ? p.y : fmaf(8.0f, p.x, p.y), sizeof(T) == 2 ? r.y : fmaf(8.0f, r.x, r.y)};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float q = sizeof(T) == 2 ? fmaf(s.hi[m][i], 0.0625f, s.lo[m][i]) : s.lo[m][i];
-        acc[i] = fmaf(q, i < 2 ? p.x : r.x, fmaf(on[i & 1], i < 2 ? p.y : r.y, acc[i]));
+        const float q = fmaf(s.hi[m][i], sizeof(T) == 2 ? 0.0625f : 1.0f, s.lo[m][i]);
+        acc[i] = fmaf(q, i < 2 ? p.x : r.x, fmaf(on[i & 1], b[i >> 1], acc[i]));
     }
 }
 
