@@ -19,8 +19,8 @@
 //
 // Arithmetic. A run of 32 columns is two m16n8k16 MMAs, rows the M side, activation rows the N side. The order of
 // columns inside an MMA is free as long as A and B agree, so lane (g, t)'s word goes in as it lies: columns 0 .. 3 to
-// one MMA, 4 .. 7 to the other (so that B's register pairs are halves of a 16-byte load). With float16 activations a nibble needs no conversion at all: (word &
-// 0x000f000f) is a pair of float16 subnormals q * 2^-24, exact in the tensor core, and (word & 0x00f000f0) a pair of 16
+// one MMA, 4 .. 7 to the other (so that B's register pairs are halves of a 16-byte load). With float16 activations a nibble
+// needs no conversion at all: (word & 0x000f000f) is a pair of float16 subnormals q * 2^-24, exact in the tensor core, and (word & 0x00f000f0) a pair of 16
 // q * 2^-24; the two MMAs keep sums of their own, joined as lo + hi / 16 at the end of the group, and the 2^24 comes at
 // the end of the row. Products are exact and sums are float32: the result is the formula's but for float32 rounding.
 // The bias takes sum x over the group, from the same B operands times a matrix of 2^-24.
@@ -249,7 +249,8 @@ struct Ones {
 // activations alone in on (times 2^-24 too).
 template <typename T, int MT>
 struct Sums {
-    float lo[MT][4], hi[MT][4], on[4], on2[4];  // (on2: float16: half of the activations, to halve the chain of MMAs; float32: the small pieces)
+    // (on2: float16: half of the activations, to halve the chain of MMAs; float32: their small pieces)
+    float lo[MT][4], hi[MT][4], on[4], on2[4];
 };
 
 template <bool FIRST, int MT>

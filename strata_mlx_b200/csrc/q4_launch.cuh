@@ -53,8 +53,8 @@ inline int status_of(cudaError_t e, const char* what) {
     return -static_cast<int>(e);
 }
 
-// Warps that share a job's columns, as a power of two: the count with the least work for the busiest warp, a job's end taken as the work of
-// two tiles.
+// Warps that share a job's columns, as a power of two: the count with the least work for the busiest warp, a job's end
+// taken as the work of two tiles.
 inline int team_log_for(int64_t jobs, int64_t tiles) {
     int best = 0;
     int64_t least = 0;
@@ -87,7 +87,8 @@ inline int launch_product(const ProductArgs& args, const Writes& w, cudaStream_t
     // (a dense matrix's by its shape alone: a token's sums are split alike alone and in a window)
     a.team_log = team_log_for(a.pairs > 0 ? jobs : a.d_wide, a.tiles);
     const size_t smem = product_smem<G>(a.pairs, a.experts);
-    if (int e = max_smem(q4_product_kernel<T, G, GLU>, static_cast<int>(smem))) return status_of(static_cast<cudaError_t>(-e), "q4_product");
+    if (int e = max_smem(q4_product_kernel<T, G, GLU>, static_cast<int>(smem)))
+        return status_of(static_cast<cudaError_t>(-e), "q4_product");
     // (a team's CTA of its own while there are slots for it: the teams spread evenly over the SMs)
     const int64_t ctas = std::min<int64_t>(jobs, kSms * kCtas);
     return status_of(launch_pdl(w, q4_product_kernel<T, G, GLU>, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), smem,

@@ -7,13 +7,13 @@
 //   q4_down_kernel     out[t, r] = sum over t's pairs of Wdown[e][r, :] . h[pair, :] + Wshared[r, :] . hs[t, :]: a MoE
 //                      block's down products and its combine, the pairs' weights already in h
 //
-// What bounds them: a weight is 4.5 bits (groups of 64) of HBM traffic and is used for at most a few rows, so the
-// floor is the weights' bytes; next to it stands the instruction issue (a tile of 16 x 128 weights is about 108 warp
-// instructions and 1088 bytes, 47 cycles of an SM at full bandwidth, and a job's ends are 580 instructions more). 64007 x 2560 with 5 tokens runs at 5.4 TB/s between its start and end (21.6 us), a block of 512 experts of
-// 640 x 2560 at 32 tokens in 162 us (4.0 TB/s, the ends of its 8-row blocks). So two strips of rows share each activation
-// operand, and nothing but a warp's own copies is waited for inside a job: every warp has a ring of bulk copies of its
-// own that runs ahead of the arithmetic across the ends of jobs, 16 warps a SM, 75 to 150 KB of a SM in flight (6.5
-// TB/s x 1 us of latency over 148 SMs asks for 44 KB).
+// What bounds them: a weight is 4.5 bits (groups of 64) of HBM traffic and is used for at most a few rows, so the floor is the
+// weights' bytes; next to it stands the instruction issue (a tile of 16 x 128 weights is about 108 warp instructions and
+// 1088 bytes, 47 cycles of an SM at full bandwidth, and a job's ends are 580 instructions more). So two strips of rows share
+// each activation operand, and nothing but a warp's own copies is waited for inside a job: every warp has a ring of bulk
+// copies of its own that runs ahead of the arithmetic across the ends of jobs, 16 warps a SM, 75 to 150 KB of a SM in flight
+// (6.5 TB/s x 1 us of latency over 148 SMs asks for 44 KB). 64007 x 2560 at 5 tokens: 20.4 us, 5.4 TB/s between its start and
+// its end; a block of 512 experts of 640 x 2560 at 32 tokens 168 us, 632 MB, the ends of its blocks of rows.
 //
 // A job of the product kernel is two strips of 16 rows (gate's and up's, or two neighbours) times one block of up to 8
 // activation rows of one expert; its columns are split over a team of 1 to 8 warps of a CTA, the partial sums added in
@@ -484,8 +484,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_product_kernel(const Produ
 // warp. A warp adds a block's sums into its own copy of the result in shared memory when the block ends, each row of h to
 // its token; a CTA adds its warps' in order, and the last CTA of a job to come adds the CTAs' in order.
 //
-// float16: h lies in two pieces of float16 (11 + 11 bits, down to 2^-25), because rounding it once would leave the block's result with
-// 1.4 times the error of its own rounding. A block is then four rows of h, their first pieces in columns 0 .. 3 of the
+// float16: h lies in two pieces of float16 (11 + 11 bits, down to 2^-25), because rounding it once would leave the block's
+// result with 1.4 times the error of its own rounding. A block is then four rows of h, their first pieces in columns 0 .. 3 of the
 // MMAs and their second in 4 .. 7: no more instructions than eight rows.
 
 template <typename T>

@@ -383,9 +383,9 @@ static int tokens_of_job(int64_t tokens, int64_t rows, int64_t cols) {
     return best;
 }
 
-// The streaming kernel takes 3 us, and for every 8 tokens 0.3 us and 0.125 ps a weight (64007 x 2560: 27 us at 8 tokens, 48
-// at 16, 67 at 24; 4096 x 4096: 6, 8 and 13; 1024 x 1024: 18 at 256); up to 16 tokens are always its (a verify window's token then has the bits it has
-// alone).
+// The streaming kernel takes 3 us, and for every 8 tokens 0.3 us and 0.125 ps a weight (64007 x 2560: 22 us at 5 tokens, 42
+// at 12, where the prompt's takes 39 at 24; 4096 x 4096: 8 us at 16 and 11 at 24, the prompt's 16.7 at 48); up to 16 tokens
+// are always its (a verify window's token then has the bits it has alone).
 bool matmul_better(int64_t tokens, int64_t rows, int64_t cols) {
     if (tokens <= 16) return false;
     const double stream = 3.0 + double((tokens + 7) / 8) * (0.3 + double(rows) * double(cols) * 1.25e-7);
