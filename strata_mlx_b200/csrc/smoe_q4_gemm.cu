@@ -3,9 +3,9 @@
 // out[t, r] = sum_c w[r, c] x[t, c], the weights w = code scale + bias rounded once to float16 (the activations' type)
 // and float32 sums. 128 weight rows are the M side of a tcgen05 MMA (8 strips), up to 256 tokens the N side, so a row is
 // decoded once for that many tokens. What bounds it: the tensor pipe (2 rows cols tokens flops at 4,096 multiply-adds a
-// cycle of an SM) and beside it the decoding, 17 instructions for 8 weights: a stage of 128 x 128 weights takes 272
-// issue slots a scheduler, and with its hand-offs 0.38 us; its MMAs take 2.8 ns a token, so from about 140 tokens a job the
-// tensor pipe is the longer. 4096 x 4096 at 1180 tokens: 36 us, 1100 TFLOP/s.
+// cycle of an SM) and beside it the decoding, 15 instructions for 8 weights: a stage of 128 x 128 weights takes 240
+// issue slots a scheduler, and with its hand-offs 0.35 us; its MMAs take 2.8 ns a token, so from about 130 tokens a job the
+// tensor pipe is the longer. 4096 x 4096 at 1180 tokens: 34.7 us, 1141 TFLOP/s.
 //
 // Per CTA (persistent over jobs = (block of tokens, 128 rows)), warp-specialized, every hand-off an mbarrier:
 //   warp 17   weights: a stage is one tile of each of the 8 strips, one TMA box (a copy a strip took the warp 120 cycles
@@ -66,7 +66,7 @@ struct GemmBlock {
     int row0, n, strip0;
 };
 
-// Slots of a job of TILES: a stage's decoding takes as long as the MMAs of 140 tokens, and two accumulators fit (the SwiGLU
+// Slots of a job of TILES: a stage's decoding takes as long as the MMAs of 130 tokens, and two accumulators fit (the SwiGLU
 // of 256 experts of 1536 x 4096, 128 tokens each: 1709 us, in jobs of 128 slots 2029; 37 tokens each: 1079 and 1055).
 constexpr int kTileSlots = 160;
 constexpr int kSlots = 16;  // of a tile
@@ -106,10 +106,13 @@ struct Phase {
 // Eight codes of the layout's word as weights: w[i] = columns 2 i, 2 i + 1
 __device__ __forceinline__ void decode8(uint32_t word, __half2 s, __half2 b, uint32_t* out) {
     const __half2 base = __half2half2(__ushort_as_half(0x6400));  // 1024
+    const __half2 sixteenth = __half2half2(__ushort_as_half(0x2c00)), off = __half2half2(__ushort_as_half(0xd400));  // 1/16, -64
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const uint32_t v = ((word >> (4 * i)) & 0x000f000fu) | 0x64006400u;
-        const __half2 w = __hfma2(__hsub2(*reinterpret_cast<const __half2*>(&v), base), s, b);
+        // (a code in the upper nibble is 1024 + 16 q as it lies, and a sixteenth of that less 64 is q: no shift)
+        const uint32_t v = ((word >> (i >= 2 ? 8 : 0)) & (i & 1 ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u;
+        const __half2 h = *reinterpret_cast<const __half2*>(&v), q = i & 1 ? __hfma2(h, sixteenth, off) : __hsub2(h, base);
+        const __half2 w = __hfma2(q, s, b);
         out[(i >> 1) + 2 * (i & 1)] = *reinterpret_cast<const uint32_t*>(&w);  // nibbles i and i + 4 of the word
     }
 }
@@ -367,12 +370,13 @@ static EncodeTiledFn encoder() {
 }
 
 // Microseconds of the prompt's kernel with jobs of n tokens, as measured: a start, and for every round of jobs over the SMs
-// a stage's 0.38 us (its hand-offs and decoding) or 2.8 ns a token (its MMAs), whichever is longer, and 1 us at its ends.
-// (4096 x 4096, 128 tokens, one round: 17.5 us with jobs of 32 to 96 tokens, 18.2 of 160, 24.6 of 256; 1180 tokens: 36.9
-// in jobs of 144, two rounds, 52.8 of 96, three, 51.0 of 256; 1536 x 4096, 4096 tokens: 39.3 of 176, 48.5 of 112, 53.2 of 256.)
+// a stage's 0.35 us (its hand-offs and decoding) or 2.8 ns a token (its MMAs), whichever is longer, and 1 us at its ends.
+// (With a stage of 0.38 us: 4096 x 4096, 128 tokens, one round: 17.5 us with jobs of 32 to 96 tokens, 18.2 of 160, 24.6 of
+// 256; 1180 tokens: 36.9 in jobs of 144, two rounds, 52.8 of 96, three, 51.0 of 256; 1536 x 4096, 4096 tokens: 39.3 of 176,
+// 48.5 of 112, 53.2 of 256.)
 static double time_of(int64_t tokens, int64_t rows, int64_t cols, int n) {
     const int64_t jobs = (tokens + n - 1) / n * ((rows + kGM - 1) / kGM);
-    const double stage = std::max(0.38, 0.0028 * n);
+    const double stage = std::max(0.35, 0.0028 * n);
     return 4.0 + double((jobs + kSms - 1) / kSms) * (double(tiles_of_cols(cols)) * stage + 1.0);
 }
 
@@ -384,7 +388,7 @@ static int tokens_of_job(int64_t tokens, int64_t rows, int64_t cols) {
 }
 
 // The streaming kernel takes 3 us, and for every 8 tokens 0.3 us and 0.125 ps a weight (64007 x 2560: 22 us at 5 tokens, 42
-// at 12, where the prompt's takes 39 at 24; 4096 x 4096: 8 us at 16 and 11 at 24, the prompt's 16.7 at 48); up to 16 tokens
+// at 12, where the prompt's takes 39 at 24; 4096 x 4096: 8 us at 16 and 11 at 24, the prompt's 15.8 at 48); up to 16 tokens
 // are always its (a verify window's token then has the bits it has alone).
 bool matmul_better(int64_t tokens, int64_t rows, int64_t cols) {
     if (tokens <= 16) return false;
