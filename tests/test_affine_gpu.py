@@ -312,7 +312,7 @@ def by_tiles(monkeypatch):
 
 
 TILES = [(1, 1, 1, 40, 32, 32), (5, 3, 4, 16, 128, 64), (40, 2, 3, 129, 160, 32), (30, 32, 40, 250, 384, 128), (700, 3, 7, 600, 96, 32),
-         (2000, 1, 2, 24, 2176, 64), (300, 8, 1024, 33, 64, 64), (1180, 8, 256, 130, 128, 64)]
+         (2000, 1, 2, 24, 2176, 64), (300, 8, 1024, 33, 64, 64), (1180, 8, 256, 130, 128, 64), (9000, 2, 3, 16, 32, 32)]
 
 
 @pytest.mark.parametrize("tokens, k, experts, rows, cols, group", TILES)
@@ -364,6 +364,19 @@ def test_pairs_of_no_expert_by_tiles_are_left_as_they_were(cuda):
         assert (out[out_of] == 7).all() and (out[~out_of] - want[~out_of].to(dtype)).abs().max() < 0.02
         none = affine._Tiles(stack, torch.full((8,), 9, dtype=torch.int32, device=cuda), 2)
         assert (none.product(stack, a[: none.count * 16], torch.full((8, 33), 7.0, dtype=dtype, device=cuda), True) == 7).all()
+
+
+def test_what_is_not_finite_stays_in_its_pairs_by_tiles(cuda, by_tiles):
+    gen = gen_of(25)
+    _, _, glu, _ = make_experts(gen, 5, 160, 96, 64, 32)
+    x = torch.randn(40, 160, device=cuda, generator=gen).half()
+    idx = torch.randint(0, 5, (40, 3), dtype=torch.int32, device=cuda, generator=gen)
+    want = glu(x, idx)
+    x[0, 5], x[17, 159] = float("nan"), float("inf")  # (token 0's row stands in the slots without a pair, too)
+    got = glu(x, idx)
+    hit = torch.zeros(40, dtype=torch.bool, device=cuda)
+    hit[[0, 17]] = True
+    assert not torch.isfinite(got[hit]).any() and torch.equal(got[~hit], want[~hit])
 
 
 def test_no_pairs(cuda):
