@@ -193,8 +193,8 @@ def _pair_chunks(pairs: int, share: int, most: int = MAX_PAIRS):
 def _by_tiles(lin, dtype, pairs: int) -> bool:
     """Whether a call's pairs go in tiles of one expert's, through the prompt's kernel (float16; tiles_of takes up to 1024
     experts): when one streaming launch would not take them. The SwiGLU of 512 experts of 640 x 2560, ten a token: 192
-    tokens 389 us streamed and 619 by tiles, 256 tokens 763 and 639, 1180 tokens 3065 and 699; 256 of 1536 x 4096, eight a
-    token: 192 tokens 656 and 1036, 512 tokens 2086 and 1053, 1180 tokens 4790 and 1243."""
+    tokens 395 us streamed and 571 by tiles, 256 tokens 757 and 580, 1180 tokens 3087 and 679; 256 of 1536 x 4096, eight a
+    token: 192 tokens 662 and 938, 512 tokens 2087 and 963, 1180 tokens 4812 and 1031."""
     return dtype == torch.float16 and lin.num_experts <= 1024 and pairs > MAX_PAIRS
 
 
@@ -372,8 +372,8 @@ class QuantizedMLP:
 
     def _apart(self, tokens: int) -> bool:
         """Whether gate and up go by the prompt's kernel: the streaming launch takes 0.3 us and 0.25 ps a weight for every
-        8 tokens, 30 us of which are about the other's start (whole calls of 4096 x 4096: 48 tokens 51 us streamed and 58
-        apart, 96 tokens 78 and 57; of 640 x 2560: 256 tokens 31 and 33, 512 tokens 50 and 35)."""
+        8 tokens, 30 us of which are about the other's start (whole calls of 4096 x 4096: 48 tokens 48 us streamed and 49
+        apart, 96 tokens 78 and 50; of 640 x 2560: 128 tokens 21 and 27, 512 tokens 50 and 31)."""
         return (tokens + 7) // 8 * (0.3 + 2.5e-7 * self.gate_proj.output_dims * self.gate_proj.input_dims) > 30
 
 
