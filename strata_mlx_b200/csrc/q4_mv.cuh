@@ -625,7 +625,9 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_down_kernel(const DownArgs
             const int n = tiles_of(c);
             stream_tiles<T, G>(ring, fetch, xp, n, static_cast<int>(width / 32) - 4 * c.tile, lane, acc, one);
             next_segment(c, n);
-            if (tokens == 1 && c.left > 0) continue;  // (one token: one row of h a block, and all blocks one sum)
+            // (one token: blocks of one row of h in a row are one sum. An expert that the token names twice has a block of more
+            // rows: the sums before it end here, whose other columns hold copies, and so do its own.)
+            if (tokens == 1 && c.left > 0 && count == 1 && (c.seg < sblocks || blocks.count[c.seg - sblocks] == 1)) continue;
             // each column's sums to its token, this lane's columns 2 t and 2 t + 1 (with pieces, those of columns 2 t + 4
             // and 2 t + 5 added). A token that names an expert twice has two columns here, neighbours: column by column then.
             if constexpr (kPieces == 2) {

@@ -1,0 +1,97 @@
+"""Calls of the 4-bit layers at the edges of what they allow, against their definition in 64 bits. The tolerances are those
+derived in test_affine_gpu.py: the worst case of every rounding, which is a large part of the result where its terms cancel.
+Weights and activations here are positive, so that nothing cancels and a tolerance is a small fraction of the result."""
+
+import ctypes
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+from strata_mlx_b200 import _lib, affine, fused  # noqa: E402
+from test_affine_gpu import F16, F32, MOE, close, gen_of, moe64  # noqa: E402
+
+
+def positive(gen, lead, rows, cols, group):
+    """Codes over all 16 values, scales and biases of a matrix of weights from 0.005 to 0.05."""
+    codes = torch.randint(-(2**31), 2**31, (*lead, rows, cols // 8), dtype=torch.int32, device="cuda", generator=gen)
+    shape = (*lead, rows, cols // group)
+    scales = 0.001 * (1 + torch.rand(shape, device="cuda", generator=gen))
+    biases = 0.005 + 0.01 * torch.rand(shape, device="cuda", generator=gen)
+    return codes, scales.half(), biases.half()
+
+
+def positive_rows(gen, tokens, cols, dtype):
+    """Activations that such a matrix takes to about 1.5."""
+    return (150 / cols * (0.05 + torch.rand(tokens, cols, device="cuda", generator=gen))).to(dtype)
+
+
+def positive_experts(gen, experts, hidden, ffn, shared, group, down_group):
+    r = [positive(gen, (experts,), *d, n) for *d, n in ((ffn, hidden, group), (ffn, hidden, group), (hidden, ffn, down_group))]
+    s = [positive(gen, (), *d, n) for *d, n in ((shared, hidden, group), (shared, hidden, group), (hidden, shared, down_group))]
+    gs = (group, group, down_group)
+    return (r, s, affine.QuantizedSwitchGLU(*(affine.QuantizedSwitchLinear(*p, group_size=n) for p, n in zip(r, gs))),
+            affine.QuantizedMLP(*(affine.QuantizedLinear(*p, group_size=n) for p, n in zip(s, gs))))
+
+
+def near(got, want, off):
+    assert (off <= 0.01 * want).all()
+    close(got, want, off)
+
+
+def block_behind_route(glu, mlp, x, idx, w, g):
+    """smoe_q4_moe of one call; mlp None: without a shared expert."""
+    gate, down = glu.gate_proj, glu.down_proj
+    (tokens, hidden), k, shared = x.shape, idx.shape[1], mlp.gate_proj.output_dims if mlp else 0
+    out = torch.full((tokens, hidden), 7.0, dtype=x.dtype, device=x.device)
+    spec = _lib.SmoeQ4Moe(dtype=_lib.dtype_code(x.dtype), group=gate.group_size, down_group=down.group_size, tokens=tokens,
+                          hidden=hidden, experts=gate.num_experts, k=k, ffn=gate.output_dims, shared_ffn=shared,
+                          x=x.data_ptr(), idx=idx.data_ptr(), weights=w.data_ptr(), shared_gate=g.data_ptr(),
+                          gate=gate.data_ptr, up=glu.up_proj.data_ptr, down=down.data_ptr, out=out.data_ptr())
+    if mlp:
+        spec.sgate, spec.sup, spec.sdown = (p.data_ptr for p in (mlp.gate_proj, mlp.up_proj, mlp.down_proj))
+    nbytes = int(_lib.lib().smoe_q4_moe_workspace_size(tokens, k, hidden, gate.output_dims, shared))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    _lib.call("smoe_q4_moe", ctypes.byref(spec), _lib.ptr(ws), nbytes, _lib.stream())
+    return out
+
+
+# the choices of one token among 12 experts: an expert twice or more, next to and apart from itself, before, between and
+# after single ones, beside choices of no expert, more often than a block of rows holds, and all distinct
+CHOICES = [[3, 3], [3, 3, 5], [5, 3, 3], [1, 5, 5, 9], [3, 9, 3], [9, 0, 9, 0], [4, 4, 4], [11, 4, 2, 4, 4, 0], [6, -1, 6, 12, 2],
+           [7] * 9 + [2], [0] + [7] * 5 + [11], [2, 1, 0] * 10 + [1, 1], [10, 3, 8, 1], [-1, 12]]
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("hidden, ffn, shared, group, down_group", [(2560, 640, 640, 64, 64), (4096, 1536, 4096, 64, 64),
+                                                                    (96, 32, 64, 32, 32), (256, 384, 128, 128, 64)])
+def test_one_token_that_names_an_expert_twice(cuda, dtype, hidden, ffn, shared, group, down_group):
+    gen = gen_of(hidden + ffn)
+    r, s, glu, mlp = positive_experts(gen, 12, hidden, ffn, shared, group, down_group)
+    none = [[t * 0 for t in p] for p in s]
+    for choice in CHOICES:
+        x = positive_rows(gen, 1, hidden, dtype)
+        idx = torch.tensor([choice], dtype=torch.int32, device=cuda)
+        w = 0.05 + torch.rand(1, len(choice), device=cuda, generator=gen)
+        g = torch.randn(1, 1, device=cuda, generator=gen).to(dtype)
+        near(affine.moe(glu, mlp, x, idx, w, g), *moe64(x, r, s, idx, w, g, group, down_group, dtype))
+        want, off = moe64(x, r, none, idx, w, g, group, down_group, dtype)
+        alone = block_behind_route(glu, None, x, idx, w, g)
+        if choice == [-1, 12]:
+            assert not alone.any()
+        else:
+            near(alone, want, off)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("tokens, experts, k, hidden, ffn, shared, group, down_group", MOE)
+def test_a_block_of_positive_weights(cuda, dtype, tokens, experts, k, hidden, ffn, shared, group, down_group):
+    gen = gen_of(tokens + ffn)
+    r, s, glu, mlp = positive_experts(gen, experts, hidden, ffn, shared, group, down_group)
+    x = positive_rows(gen, tokens, hidden, dtype)
+    w = 0.05 + torch.rand(tokens, k, device=cuda, generator=gen)
+    g = torch.randn(tokens, 1, device=cuda, generator=gen).to(dtype)
+    idx = torch.randint(0, experts, (tokens, k), dtype=torch.int32, device=cuda, generator=gen)  # repeats among them
+    near(affine.moe(glu, mlp, x, idx, w, g), *moe64(x, r, s, idx, w, g, group, down_group, dtype))
+    idx[::2, 0] = experts
+    near(affine.moe(glu, mlp, x, idx, w, g), *moe64(x, r, s, idx, w, g, group, down_group, dtype))
