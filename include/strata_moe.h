@@ -533,7 +533,7 @@ SMOE_API int smoe_q4_tile_matmul(const uint8_t* packed, int64_t experts, int64_t
  * in two launches (gate, up and SwiGLU of the routed and the shared expert; down and the combine):
  *   out[t] = sum_j weights[t, j] down_e(silu(gate_e x) * up_e x) + sigmoid(shared_gate[t]) shared(x), e = idx[t, j]
  * gate, up: (experts, ffn, hidden) with groups of `group` columns, down: (experts, hidden, ffn) with `down_group`; the
- * shared expert's likewise with shared_ffn rows (0: none; shared_gate null: not gated). A choice idx >= experts adds
+ * shared expert's likewise with shared_ffn rows (0: none; shared_gate and shared_gate32 null: not gated). A choice idx >= experts adds
  * nothing. Sums and SwiGLU are float32; between the launches the SwiGLU times its weight is kept in 22 bits (down to
  * 2^-25; float16 activations: within float16's range). Workspace: smoe_q4_moe_workspace_size() bytes, one for each call in
  * flight. Replaces `_Routed.__call__` behind its router
@@ -549,6 +549,7 @@ typedef struct SmoeQ4Moe {
     const uint8_t *gate, *up, *down;
     const uint8_t *sgate, *sup, *sdown;
     void* out;
+    const float* shared_gate32;  /* the gate in float32, in shared_gate's place where given (no rounding of it) */
 } SmoeQ4Moe;
 SMOE_API size_t smoe_q4_moe_workspace_size(int64_t tokens, int64_t k, int64_t hidden, int64_t ffn,
                                              int64_t shared_ffn);
@@ -561,6 +562,11 @@ SMOE_API int smoe_q4_moe(const SmoeQ4Moe* m, void* workspace, size_t workspace_b
 SMOE_API int smoe_route_window(const uint16_t* weight, const uint16_t* gate_weight, const uint16_t* x, int64_t tokens,
                                int64_t experts, int64_t hidden, int64_t k, float* logits, uint32_t* idx, float* weights,
                                uint16_t* gate_out, uint32_t* counters, void* stream);
+
+/* smoe_route_window with gate_out in float32 (smoe_q4_moe's shared_gate32). */
+SMOE_API int smoe_route_window_f32(const uint16_t* weight, const uint16_t* gate_weight, const uint16_t* x, int64_t tokens,
+                                   int64_t experts, int64_t hidden, int64_t k, float* logits, uint32_t* idx, float* weights,
+                                   float* gate_out, uint32_t* counters, void* stream);
 
 /* Whether a bounded wait of the 4-bit kernels gave up on the current device since the last clear (SMOE_ETIMEOUT; outputs
  * since are not valid). Synchronizes the device. */

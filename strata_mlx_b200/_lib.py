@@ -74,7 +74,7 @@ class SmoeQ4Moe(ctypes.Structure):
     _fields_ = [("dtype", _i), ("group", _i), ("down_group", _i), ("tokens", _i64), ("hidden", _i64), ("experts", _i64),
                 ("k", _i64), ("ffn", _i64), ("shared_ffn", _i64), ("x", _p), ("idx", _p), ("weights", _p),
                 ("shared_gate", _p), ("gate", _p), ("up", _p), ("down", _p), ("sgate", _p), ("sup", _p), ("sdown", _p),
-                ("out", _p)]
+                ("out", _p), ("shared_gate32", _p)]
 
 
 # name -> (restype, argtypes): the declarations of include/strata_moe.h
@@ -150,6 +150,7 @@ SIGNATURES = {
     "smoe_q4_moe_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64]),
     "smoe_q4_moe": (_i, [_c.POINTER(SmoeQ4Moe), _p, _sz, _p]),
     "smoe_route_window": (_i, [_p, _p, _p, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p]),
+    "smoe_route_window_f32": (_i, [_p, _p, _p, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p]),
     "smoe_q4_status": (_i, [_c.POINTER(_i), _i]),
 }
 

@@ -395,6 +395,13 @@ def moe(switch_mlp: QuantizedSwitchGLU, shared: QuantizedMLP, x: torch.Tensor, i
     rounded to x's type. An index at or past the expert count adds nothing."""
     if not moe_takes(switch_mlp, shared):
         raise ValueError("moe takes 4-bit experts of one hidden size, with one group size in gate / up and one in down")
+    if g.dtype != x.dtype:
+        raise ValueError("gate values are of the activations' type")
+    return _moe(switch_mlp, shared, x, indices, w, g)
+
+
+def _moe(switch_mlp, shared, x, indices, w, g):
+    """`moe` for experts that it takes; g in x's type or, up to MOE_TOKENS tokens, in float32."""
     gate, down = switch_mlp.gate_proj, switch_mlp.down_proj
     sgate, sdown = shared.gate_proj, shared.down_proj
     code = _lib.dtype_code(x.dtype)
@@ -405,7 +412,7 @@ def moe(switch_mlp: QuantizedSwitchGLU, shared: QuantizedMLP, x: torch.Tensor, i
     tokens, k = x2.shape[0], indices.shape[-1] if indices.dim() else 0
     if indices.numel() != tokens * k or w.numel() != tokens * k or g.numel() != tokens or not 1 <= k <= 32:
         raise ValueError("moe takes 1 to 32 experts and weights and one gate value for every token")
-    if w.dtype != torch.float32 or g.dtype != x.dtype:
+    if w.dtype != torch.float32 or (g.dtype != x.dtype and (g.dtype != torch.float32 or tokens > MOE_TOKENS)):
         raise ValueError("weights are float32 and gate values of the activations' type")
     with torch.cuda.device(gate.device):
         idx, w, g = _flat_idx(indices), w.contiguous(), g.contiguous()
@@ -425,9 +432,13 @@ def moe(switch_mlp: QuantizedSwitchGLU, shared: QuantizedMLP, x: torch.Tensor, i
             spec = _lib.SmoeQ4Moe(
                 dtype=code, group=gate.group_size, down_group=down.group_size, tokens=tokens, hidden=gate.input_dims,
                 experts=gate.num_experts, k=k, ffn=gate.output_dims, shared_ffn=sgate.output_dims, x=x2.data_ptr(),
-                idx=idx.data_ptr(), weights=w.data_ptr(), shared_gate=g.data_ptr(), gate=gate.data_ptr,
+                idx=idx.data_ptr(), weights=w.data_ptr(), gate=gate.data_ptr,
                 up=switch_mlp.up_proj.data_ptr, down=down.data_ptr, sgate=sgate.data_ptr, sup=shared.up_proj.data_ptr,
                 sdown=sdown.data_ptr, out=out.data_ptr())
+            if g.dtype == x.dtype:
+                spec.shared_gate = g.data_ptr()
+            else:
+                spec.shared_gate32 = g.data_ptr()
             _lib.call("smoe_q4_moe", ctypes.byref(spec), _lib.ptr(ws), nbytes, _lib.stream())
     return out.reshape(x.shape)
 

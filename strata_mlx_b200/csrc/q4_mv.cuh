@@ -54,6 +54,7 @@ struct ProductArgs {
     void* d_out;
     int64_t d_rows, d_tokens;
     const void* d_gate;  // GLU: the row's result times sigmoid of this (one a token), or null
+    const float* d_gate32;  // the same in float32, in d_gate's place
     // routed part: pair p takes row p / share of x through expert idx[p] of a stack
     const uint8_t* rw[2];
     void* r_out;
@@ -456,7 +457,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_product_kernel(const Produ
                     // silu(gate) up, times the row's share of the block's output: float32 up to the one rounding
                     v = v * sigmoid_f(v) * (u * unit<T>());
                     if (dense) {
-                        if (a.d_gate != nullptr) v *= sigmoid_f(to_f32(static_cast<const T*>(a.d_gate)[to]));
+                        if (a.d_gate32 != nullptr) v *= sigmoid_f(a.d_gate32[to]);
+                        else if (a.d_gate != nullptr) v *= sigmoid_f(to_f32(static_cast<const T*>(a.d_gate)[to]));
                     } else if (a.weights != nullptr) {
                         v *= a.weights[to];
                     }

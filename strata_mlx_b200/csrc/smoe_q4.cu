@@ -356,9 +356,9 @@ extern "C" int smoe_q4_pack(const uint32_t* codes, const uint16_t* scales, const
     Q4_CATCH("q4_pack")
 }
 
-// pieces: results as two rows of float16 each (q4_mv.cuh); `zero`: words that the launch clears besides, for the launch
-// after it
-static int q4_product(const SmoeQ4Product* p, bool pieces, uint32_t* zero, int n_zero, void* stream) {
+// pieces: results as two rows of float16 each (q4_mv.cuh); gate32: the dense gate in float32; `zero`: words that the launch
+// clears besides, for the launch after it
+static int q4_product(const SmoeQ4Product* p, bool pieces, const float* gate32, uint32_t* zero, int n_zero, void* stream) {
     SMOE_REQUIRE(p, SMOE_EARG, "q4_product: null pointer");
     SMOE_REQUIRE(p->dtype == SMOE_F16 || p->dtype == SMOE_F32, SMOE_EDTYPE,
                  "q4_product takes float16 or float32 activations");
@@ -388,6 +388,7 @@ static int q4_product(const SmoeQ4Product* p, bool pieces, uint32_t* zero, int n
         a.d_rows = p->dense_rows;
         a.d_tokens = p->dense_tokens;
         a.d_gate = p->dense_gate;
+        a.d_gate32 = gate32;
         w.add(p->dense_out, size_t(p->dense_tokens) * p->dense_rows * item * (pieces ? 2 : 1));
         const size_t bytes = stack_bytes(1, p->dense_rows, p->cols, p->group);
         a.early = a.early && pdl_early(st, p->dense, bytes) && (!p->dense2 || pdl_early(st, p->dense2, bytes));
@@ -428,7 +429,7 @@ static int q4_product(const SmoeQ4Product* p, bool pieces, uint32_t* zero, int n
 
 extern "C" int smoe_q4_product(const SmoeQ4Product* p, void* stream) {
     Q4_TRY
-    return q4_product(p, false, nullptr, 0, stream);
+    return q4_product(p, false, nullptr, nullptr, 0, stream);
     Q4_CATCH("q4_product")
 }
 
@@ -444,7 +445,7 @@ extern "C" int smoe_q4_linear(const uint8_t* packed, int64_t rows, int64_t cols,
     p.dense_rows = rows;
     p.dense_tokens = tokens;
     p.dense_out = out;
-    return q4_product(&p, false, nullptr, 0, stream);
+    return q4_product(&p, false, nullptr, nullptr, 0, stream);
     Q4_CATCH("q4_linear")
 }
 
@@ -572,7 +573,8 @@ extern "C" int smoe_q4_moe(const SmoeQ4Moe* m, void* workspace, size_t workspace
     p.share = m->k;
     p.weights = m->weights;
     p.out = h;
-    if (int s = q4_product(&p, p.dtype == SMOE_F16, counters, static_cast<int>(MoeSpace::n_counters(m->hidden)), stream))
+    if (int s = q4_product(&p, p.dtype == SMOE_F16, m->shared_gate32, counters,
+                           static_cast<int>(MoeSpace::n_counters(m->hidden)), stream))
         return s;
     DownArgs d = {};
     d.h = h;

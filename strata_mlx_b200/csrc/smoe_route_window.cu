@@ -2,7 +2,7 @@
 // sums on the tensor cores, in one launch.
 //
 //   logits[t, e] = router[e] . x[t];  idx = the k largest, ties to the lower index;  weights = softmax of the chosen;
-//   gate_out[t] = gate_weight . x[t]
+//   gate_out[t] = gate_weight . x[t], in float32 or rounded to float16
 //
 // A CTA takes 16 rows of the router (the shared gate's row is one more) and eight tokens: 16 warps share the columns, each
 // m16n8k16 on its own (router rows the M side, tokens the N side, products exact, float32 sums), partial sums added in
@@ -35,7 +35,8 @@ struct RouteWindow {
     float* logits;
     uint32_t* idx;
     float* weights;
-    __half* gate_out;
+    void* gate_out;
+    bool gate32;  // gate_out is float32
     uint32_t* counters;  // one for every eight tokens
     bool early;  // the router may be read before pdl_wait()
 };
@@ -88,7 +89,8 @@ __global__ void __launch_bounds__(kRwThreads, NV <= 16 ? 2 : 1) route_window_ker
 #pragma unroll
         for (int w = 0; w < kRwWarps; ++w) sum += part[(w * kRwWidth + n) * kRwStride + r];
         if (row < a.experts) a.logits[(token0 + n) * int64_t(a.experts) + row] = sum;
-        else if (row < rows) a.gate_out[token0 + n] = __float2half_rn(sum);
+        else if (row < rows && a.gate32) static_cast<float*>(a.gate_out)[token0 + n] = sum;
+        else if (row < rows) static_cast<__half*>(a.gate_out)[token0 + n] = __float2half_rn(sum);
     }
     __threadfence();
     __syncthreads();
@@ -119,14 +121,9 @@ int launch(const RouteWindow& a, const Writes& w, cudaStream_t st) {
     return go(route_window_kernel<64>);
 }
 
-}  // namespace
-}  // namespace smoe
-
-using namespace smoe;
-
-extern "C" int smoe_route_window(const uint16_t* weight, const uint16_t* gate_weight, const uint16_t* x, int64_t tokens,
-                                 int64_t experts, int64_t hidden, int64_t k, float* logits, uint32_t* idx, float* weights,
-                                 uint16_t* gate_out, uint32_t* counters, void* stream) try {
+int route_window(const uint16_t* weight, const uint16_t* gate_weight, const uint16_t* x, int64_t tokens, int64_t experts,
+                 int64_t hidden, int64_t k, float* logits, uint32_t* idx, float* weights, void* gate_out, bool gate32,
+                 uint32_t* counters, void* stream) {
     if (tokens == 0) return SMOE_OK;
     SMOE_REQUIRE(weight && x && logits && idx && weights && counters && tokens > 0 && experts > 0, SMOE_EARG,
                  "route_window: null pointer or empty router");
@@ -153,13 +150,35 @@ extern "C" int smoe_route_window(const uint16_t* weight, const uint16_t* gate_we
     a.logits = logits;
     a.idx = idx;
     a.weights = weights;
-    a.gate_out = reinterpret_cast<__half*>(gate_out);
+    a.gate_out = gate_out;
+    a.gate32 = gate32;
     a.counters = counters;
     a.early = pdl_early(st, weight, size_t(experts) * hidden * 2) && pdl_early(st, gate_weight, size_t(hidden) * 2);
     Writes w;
     w.add(logits, size_t(tokens) * experts * 4).add(idx, size_t(tokens) * k * 4).add(weights, size_t(tokens) * k * 4);
-    w.add(gate_out, size_t(tokens) * 2).add(counters, size_t(tokens + 7) / 8 * 4);
+    w.add(gate_out, size_t(tokens) * (gate32 ? 4 : 2)).add(counters, size_t(tokens + 7) / 8 * 4);
     return launch(a, w, st);
+}
+
+}  // namespace
+}  // namespace smoe
+
+using namespace smoe;
+
+extern "C" int smoe_route_window(const uint16_t* weight, const uint16_t* gate_weight, const uint16_t* x, int64_t tokens,
+                                 int64_t experts, int64_t hidden, int64_t k, float* logits, uint32_t* idx, float* weights,
+                                 uint16_t* gate_out, uint32_t* counters, void* stream) try {
+    return route_window(weight, gate_weight, x, tokens, experts, hidden, k, logits, idx, weights, gate_out, false, counters,
+                        stream);
+} catch (...) {
+    return fail(SMOE_EARG, "route_window: the host is out of memory");
+}
+
+extern "C" int smoe_route_window_f32(const uint16_t* weight, const uint16_t* gate_weight, const uint16_t* x, int64_t tokens,
+                                     int64_t experts, int64_t hidden, int64_t k, float* logits, uint32_t* idx, float* weights,
+                                     float* gate_out, uint32_t* counters, void* stream) try {
+    return route_window(weight, gate_weight, x, tokens, experts, hidden, k, logits, idx, weights, gate_out, true, counters,
+                        stream);
 } catch (...) {
     return fail(SMOE_EARG, "route_window: the host is out of memory");
 }

@@ -220,13 +220,14 @@ def route(gate: "WindowLinear", shared_gate, x: torch.Tensor, k: int, local=None
     return out if local is None else out + (lidx.reshape(*lead, k),)
 
 
-def route_window(gate: "WindowLinear", shared_gate: "WindowLinear", x: torch.Tensor, k: int):
+def route_window(gate: "WindowLinear", shared_gate: "WindowLinear", x: torch.Tensor, k: int, gate_dtype=None):
     """`route` for up to 64 float16 tokens with the router's sums on the tensor cores (float32, in another order than
-    route's: the last bits of the logits may differ); (idx, w, g), or None where the kernel does not take x."""
+    route's: the last bits of the logits may differ); (idx, w, g), or None where the kernel does not take x. g is float32 as
+    it was summed with gate_dtype=torch.float32, else rounded to x's type."""
     tokens = x.numel() // gate.cols
     if (x.dtype != torch.float16 or not 1 <= tokens <= 64 or gate.cols % 32 or gate.rows > 2048 or not gate.takes(x)
             or not 1 <= k <= min(gate.rows, 32) or not shared_gate.takes(x) or shared_gate.rows != 1
-            or shared_gate.cols != gate.cols):
+            or shared_gate.cols != gate.cols or gate_dtype not in (None, torch.float16, torch.float32)):
         return None
     _lib.require_cuda(gate.weight, x)
     dev = x.device
@@ -235,9 +236,9 @@ def route_window(gate: "WindowLinear", shared_gate: "WindowLinear", x: torch.Ten
     logits = torch.empty((tokens, gate.rows), dtype=torch.float32, device=dev)
     idx = torch.empty((tokens, k), dtype=torch.uint32, device=dev)
     w = torch.empty((tokens, k), dtype=torch.float32, device=dev)
-    g = torch.empty((tokens,), dtype=x.dtype, device=dev)
+    g = torch.empty((tokens,), dtype=gate_dtype or x.dtype, device=dev)
     counters = _route_counters(32, False, dev)
-    _lib.call("smoe_route_window", _lib.ptr(wt), _lib.ptr(gw), _lib.ptr(x2), tokens, gate.rows, gate.cols, k,
+    _lib.call("smoe_route_window_f32" if g.dtype == torch.float32 else "smoe_route_window", _lib.ptr(wt), _lib.ptr(gw), _lib.ptr(x2), tokens, gate.rows, gate.cols, k,
               _lib.ptr(logits), _lib.ptr(idx), _lib.ptr(w), _lib.ptr(g), _lib.ptr(counters), _lib.stream())
     lead = x.shape[:-1]
     return idx.reshape(*lead, k), w.reshape(*lead, k), g.reshape(*lead, 1)
@@ -316,15 +317,16 @@ class SparseMoeBlock:
 
 
     def _quantized(self, x: torch.Tensor) -> torch.Tensor:
-        """The block on 4-bit experts: the route, then `affine.moe`."""
+        """The block on 4-bit experts: the route, then `affine.moe`; up to 64 float16 tokens keep the shared gate in float32
+        between the two (rounded to float16 it was all of the block's error beside its output's rounding)."""
         _lib.require_cuda(x)
         with torch.cuda.device(x.device):
-            r = route_window(self.gate, self.shared_expert_gate, x, self.top_k)
+            r = route_window(self.gate, self.shared_expert_gate, x, self.top_k, torch.float32)
             if r is None:
                 r = route(self.gate, self.shared_expert_gate, x, self.top_k)
             if r is None:
                 r = (*top_k_softmax(self.gate(x), self.top_k), self.shared_expert_gate(x).to(x.dtype))
-            return affine.moe(self.switch_mlp, self.shared_expert, x, *r)
+            return affine._moe(self.switch_mlp, self.shared_expert, x, *r)
 
 
 _Routed = SparseMoeBlock
