@@ -80,6 +80,7 @@ struct alignas(64) GemmMaps {
 struct GemmSmem {
     uint64_t rawfull[kGMaxRaw], rawfree[kGMaxRaw], bfull[kGMaxB], bfree[kGMaxB];
     uint64_t afull[kGASlots], afree[kGASlots], dfull[2], dfree[2];
+    uint64_t done;  // the CTA's last job's sums: used once
     uint32_t tmem_base;
 };
 
@@ -160,6 +161,7 @@ __global__ void __launch_bounds__(kGThreads, 1) q4_matmul_kernel(const GemmArgs 
             tc::mbar_init(&S.dfull[i], 1);
             tc::mbar_init(&S.dfree[i], kGEnders);
         }
+        tc::mbar_init(&S.done, 1);
         tc::fence_barrier_init();
     }
     if (warp == kGDecoders) {
@@ -284,7 +286,7 @@ __global__ void __launch_bounds__(kGThreads, 1) q4_matmul_kernel(const GemmArgs 
                                        (s > 0 || k > 0) ? 1u : 0u);
                     tc::mma_commit(&S.afree[ap.slot]);
                     tc::mma_commit(&S.bfree[bp.slot]);
-                    if (s == nk - 1) tc::mma_commit(&S.dfull[dp.slot]);
+                    if (s == nk - 1) tc::mma_commit(job + int(gridDim.x) < jobs ? &S.dfull[dp.slot] : &S.done);
                 }
             }
             if (!ok) atomicExch(&g_q4_gemm_status, SMOE_ETIMEOUT);
@@ -299,7 +301,7 @@ __global__ void __launch_bounds__(kGThreads, 1) q4_matmul_kernel(const GemmArgs 
         const uint32_t lanes = tmem + (uint32_t(32 * (warp & 3)) << 16);
         const uint8_t* mine = raw + (L / kRows) * kTile;
         const uint8_t *at0 = mine + chunk_at(row, 2 * pair), *at1 = mine + chunk_at(row, 2 * pair + 1);
-        Phase rp, ap, dp, last;
+        Phase rp, ap, dp;
         int stage = 0;
         for (int job = blockIdx.x; job < jobs && ok; job += gridDim.x, dp.next(nd)) {
             for (int s = 0; s < nk; ++s, ++stage, rp.next(g.nr), ap.next(kGASlots)) {
@@ -330,12 +332,11 @@ __global__ void __launch_bounds__(kGThreads, 1) q4_matmul_kernel(const GemmArgs 
                     tc::mbar_arrive(&S.rawfree[rp.slot]);
                 }
             }
-            // (a CTA's last job is written out by its decoders, who have nothing else left. They see every job's sums
-            // complete, one job late, which costs nothing: a wait two phases behind its barrier would return at once)
-            if (ok && job != int(blockIdx.x)) ok = wait(&S.dfull[last.slot], last.phase);
-            last = dp;
+            // A CTA's last job is written out by its decoders, who have nothing else left, behind a barrier of its own that
+            // completes once. (At a job's barrier a decoder held up for the length of its last eight MMAs could meet the phase of
+            // the next job but one on that accumulator, which without its own decoding never completes.)
             if (!ok || job + int(gridDim.x) < jobs) continue;
-            if (!(ok = wait(&S.dfull[dp.slot], dp.phase))) break;
+            if (!(ok = wait(&S.done, 0))) break;
             pdl_wait();  // before an output
             write_out(job, dp.slot, 8 * (warp >> 2), 8 * (kGDecoders / 4));
         }

@@ -9,7 +9,7 @@ import pytest
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 from strata_mlx_b200 import _lib, affine, fused  # noqa: E402
-from test_affine_gpu import F16, F32, MOE, close, gen_of, moe64  # noqa: E402
+from test_affine_gpu import F16, F32, MOE, close, gen_of, layer64, moe64  # noqa: E402
 
 
 def positive(gen, lead, rows, cols, group):
@@ -120,3 +120,18 @@ def test_the_shared_gate_is_not_rounded_between_the_route_and_the_block(cuda, to
     got = fused.SparseMoeBlock(router, glu, mlp, sgate, 2)(x)
     assert got.dtype == F16
     close(got, want, off)
+
+
+@pytest.mark.parametrize("rows, cols, tokens, group", [(1536, 4096, 4096, 64), (4096, 1024, 2048, 128), (9000, 128, 1500, 64),
+                                                       (6000, 32, 2311, 32), (128 * 150, 256, 300, 32)])
+def test_prompts_with_one_accumulator_or_one_stage_a_job(cuda, rows, cols, tokens, group):
+    # several jobs a CTA on one accumulator (more than 160 tokens a job), and jobs that one group of decoders decodes alone
+    gen = gen_of(rows + cols)
+    p = positive(gen, (), rows, cols, group)
+    layer = affine.QuantizedLinear(*p, group_size=group)
+    x = positive_rows(gen, tokens, cols, F16)
+    want = layer(x)
+    near(want, *layer64(x, p, group, F16))
+    for _ in range(20):
+        assert torch.equal(layer(x), want)
+    assert not affine.failed()
