@@ -14,18 +14,22 @@
 // A row's 16 code words of a tile: word j of chunk t (four chunks of 16 bytes) holds the codes of columns 32 j + 8 t ..
 // + 7, so that lane (g, t) of a warp (g = lane / 4, t = lane % 4) has its columns of all four 32-column runs in one
 // 16-byte read. Chunk t of row r lies at place t ^ (r / 2 % 4): eight rows' chunks t are on eight different bank groups
-// (a thread a row reads so in the prompt's product). In a word, columns 0 .. 7 lie in nibbles 0, 4, 2, 6, 1, 5, 3, 7: the
-// nibbles under one mask, 16 bits apart, are neighbouring columns.
+// (a thread a row reads so in the prompt's product). In a word, columns 0 .. 7 lie in nibbles 0, 4, 2, 6, 1, 5, 3, 7, the whole
+// rotated left by two bits: the nibbles under one mask, 16 bits apart, are neighbouring columns, and nibbles 0 and 1 lie in bits
+// 2 .. 5 and 6 .. 9 of a half word.
 //
 // Arithmetic. A run of 32 columns is two m16n8k16 MMAs, rows the M side, activation rows the N side. The order of
 // columns inside an MMA is free as long as A and B agree, so lane (g, t)'s word goes in as it lies: columns 0 .. 3 to
 // one MMA, 4 .. 7 to the other (so that B's register pairs are halves of a 16-byte load). With float16 activations a nibble
-// needs no conversion at all: (word & 0x000f000f) is a pair of float16 subnormals q * 2^-24, exact in the tensor core, and (word & 0x00f000f0) a pair of 16
-// q * 2^-24; the two MMAs keep sums of their own, joined as lo + hi / 16 at the end of the group, and the 2^24 comes at
-// the end of the row. Products are exact and sums are float32: the result is the formula's but for float32 rounding.
-// The bias takes sum x over the group, from the same B operands times a matrix of 2^-24.
+// needs no conversion at all: (word & 0x003c003c) is a pair of float16 subnormals q * 2^-22, exact in the tensor core, and
+// (word & 0x03c003c0) a pair of 16 q * 2^-22; the two MMAs keep sums of their own, joined as lo + hi / 16 at the end of the group,
+// and the 2^22 comes at the end of the row. The bias takes sum x over the group, from the same B operands times a matrix of
+// 2^-14. Products are exact and sums are float32, which the tensor core adds with a fixed number of bits below its operands'
+// exponents: a subnormal counts there as 2^-14, so codes lie as high in the mantissa as two to a half word allow and the matrix
+// of ones is the least normal number. (With codes in bits 0 .. 7 and ones of 2^-24 4.8 % of a
+// 640 x 2560 layer's results were rounded to the wrong neighbour, now 0.1 %, and of a block of 512 experts 23 %, now 0.4 %.)
 // Float32 activations are three bfloat16 pieces (8 + 8 + 8 bits: the whole float32), each through the same MMAs;
-// codes become bfloat16 by (q | 0x4300) - 136, exact too: q - 8, with bias + 8 scale in the bias's place. A group's weights
+// codes become bfloat16 by (4 q | 0x4200) - 40, exact too: q - 8, with bias + 8 scale in the bias's place. A group's weights
 // lie on both sides of zero mostly, q scale and bias are then numbers of one size that nearly cancel, and their float32 sums
 // lose more than those of q - 8 do (a block of 64 experts, 2048 wide, is 1.03e-6 of its result off with q, 7.4e-7 with
 // q - 8, and 2.7e-7 with sums of their own for the activations' small pieces).
@@ -61,15 +65,25 @@ __host__ __device__ constexpr int chunk_at(int row, int t) { return row * 64 + (
 __device__ __forceinline__ int lane_chunk(int lane) { return chunk_at(lane >> 2, lane & 3); }
 // The nibble of a word that holds its column i
 __host__ __device__ constexpr int nibble_of(int i) { return (i >> 2) + 2 * ((i >> 1) & 1) + 4 * (i & 1); }
+__device__ __forceinline__ uint32_t turn(uint32_t w, int right) { return __funnelshift_r(w, w, right); }
+// turn(w, 8). (Written as a permutation of bytes: a funnel shift costs the kernels registers, 64007 x 2560 at 5 tokens 24.7 us
+// against 21.9.)
+__device__ __forceinline__ uint32_t turn8(uint32_t w) {
+    uint32_t r;
+    asm("prmt.b32 %0, %1, %1, 0x0321;" : "=r"(r) : "r"(w));
+    return r;
+}
+constexpr uint32_t kLow = 0x003c003cu, kHigh = 0x03c003c0u;  // nibbles 0 and 4, 1 and 5 (turned by 8: 2 and 6, 3 and 7)
 // A word of eight codes, weight i in bits 4 i, in the layout's order of nibbles, and back
 __device__ __forceinline__ uint32_t nibbles_in(uint32_t w) {
     uint32_t r = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) r |= ((w >> (4 * i)) & 15u) << (4 * nibble_of(i));
-    return r;
+    return (r << 2) | (r >> 30);
 }
 __device__ __forceinline__ uint32_t nibbles_out(uint32_t w) {
     uint32_t r = 0;
+    w = turn(w, 2);
 #pragma unroll
     for (int i = 0; i < 8; ++i) r |= ((w >> (4 * nibble_of(i))) & 15u) << (4 * i);
     return r;
@@ -178,26 +192,26 @@ template <>
 struct Codes<__half> {
     uint32_t lo[4], hi[4];  // hi holds 16 q
     __device__ __forceinline__ Codes(uint32_t u, uint32_t v) {
-        lo[0] = u & 0x000f000fu;
-        hi[0] = u & 0x00f000f0u;
-        lo[1] = v & 0x000f000fu;
-        hi[1] = v & 0x00f000f0u;
-        u >>= 8;
-        v >>= 8;
-        lo[2] = u & 0x000f000fu;
-        hi[2] = u & 0x00f000f0u;
-        lo[3] = v & 0x000f000fu;
-        hi[3] = v & 0x00f000f0u;
+        lo[0] = u & kLow;
+        hi[0] = u & kHigh;
+        lo[1] = v & kLow;
+        hi[1] = v & kHigh;
+        u = turn8(u);
+        v = turn8(v);
+        lo[2] = u & kLow;
+        hi[2] = u & kHigh;
+        lo[3] = v & kLow;
+        hi[3] = v & kHigh;
     }
-    static constexpr uint32_t kOne = 0x00010001u;  // 2^-24, as the codes
+    static constexpr uint32_t kOne = 0x04000400u;  // 2^-14: 256 times a code's unit
 };
 
 template <>
 struct Codes<float> {
     uint32_t lo[4], hi[4];
     static __device__ __forceinline__ uint32_t code(uint32_t w) {
-        const uint32_t b = (w & 0x000f000fu) | 0x43004300u;  // 128 + q
-        const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&b), __float2bfloat162_rn(136.0f));
+        const uint32_t b = (w & kLow) | 0x42004200u;  // 32 + q
+        const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&b), __float2bfloat162_rn(40.0f));
         return *reinterpret_cast<const uint32_t*>(&r);
     }
     __device__ __forceinline__ Codes(uint32_t u, uint32_t v) {
@@ -206,9 +220,9 @@ struct Codes<float> {
         lo[1] = code(v);
         hi[1] = code(v >> 4);
         lo[2] = code(u >> 8);
-        hi[2] = code(u >> 12);
+        hi[2] = code(turn(u, 12));
         lo[3] = code(v >> 8);
-        hi[3] = code(v >> 12);
+        hi[3] = code(turn(v, 12));
     }
     static constexpr uint32_t kOne = 0x3f803f80u;
 };
@@ -233,7 +247,7 @@ struct Acts<float> {
     }
 };
 
-// The matrix of ones (times 2^-24 for float16) as an A operand. Made by volatile moves: a constant would be moved into the
+// The matrix of ones (times 2^-14 for float16) as an A operand. Made by volatile moves: a constant would be moved into the
 // operand's four registers again for every MMA.
 template <typename T>
 struct Ones {
@@ -245,8 +259,8 @@ struct Ones {
 };
 
 // The sums of one group of columns of MT strips times a block of 8 activation rows: codes in lo and hi (float16: hi
-// holds 16 times its sum, both 2^-24 times theirs; float32: the activations' first pieces in lo, the others in hi), the
-// activations alone in on (times 2^-24 too).
+// holds 16 times its sum, both 2^-22 times theirs; float32: the activations' first pieces in lo, the others in hi), the
+// activations alone in on (float16: times 2^-14).
 template <typename T, int MT>
 struct Sums {
     // (on2: float16: half of the activations, to halve the chain of MMAs; float32: their small pieces)
@@ -299,16 +313,17 @@ __device__ __forceinline__ void run_mma(const Codes<float> (&a)[MT], const Acts<
     piece(std::false_type{}, s.hi, s.on2);
 }
 
-// What a row's sum is to be multiplied by in the end (the codes' 2^-24)
+// What a row's sum is to be multiplied by in the end (the codes' 2^-22)
 template <typename T>
-__host__ __device__ constexpr float unit() { return sizeof(T) == 2 ? 16777216.0f : 1.0f; }
+__host__ __device__ constexpr float unit() { return sizeof(T) == 2 ? 4194304.0f : 1.0f; }
 
 // The end of a group: acc += scale (lo + hi) + bias on, rows g (values 0, 1) and g + 8 (values 2, 3).
 template <typename T, int MT>
 __device__ __forceinline__ void group_end(float (&acc)[4], const Sums<T, MT>& s, int m, uint32_t sb0, uint32_t sb1) {
     const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&sb0));
     const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&sb1));
-    const float on[2] = {s.on[0] + s.on2[0], s.on[1] + s.on2[1]};  // (the same for both rows)
+    constexpr float kOnes = sizeof(T) == 2 ? 1.0f / 256.0f : 1.0f;  // a code's unit in that of the ones
+    const float on[2] = {(s.on[0] + s.on2[0]) * kOnes, (s.on[1] + s.on2[1]) * kOnes};  // (the same for both rows)
     const float b[2] = {sizeof(T) == 2 ? p.y : fmaf(8.0f, p.x, p.y), sizeof(T) == 2 ? r.y : fmaf(8.0f, r.x, r.y)};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {

@@ -12,9 +12,9 @@
 //             each to issue, more than the stage's work) into a ring of up to 10 slots
 //   warp 18   activations: the tokens' 128 columns by TMA into a ring of its own, two boxes of all the job's rows x 64
 //             columns (128-byte swizzle)
-//   warps 0-15 decoders, two groups on every other stage: a thread reads half of its row's 128 columns, (q | 0x6400) - 1024
-//             makes a pair of codes float16 exactly, one fused multiply-add with the group's scale and bias rounds it to
-//             the weight; stored to its TMEM lane of an A slot
+//   warps 0-15 decoders, two groups on every other stage: a thread reads half of its row's 128 columns, a mask and one
+//             multiply-add make a pair of codes float16 exactly, another with the group's scale and bias rounds it to the
+//             weight; stored to its TMEM lane of an A slot
 //   warp 16   MMA: A from TMEM, B from shared memory, 8 MMAs of K = 16 a stage; commits free the slots.
 //   warps 19-22 read a job's sums back and write them out while the next job runs (jobs of up to 160 tokens have two
 //             accumulators); a CTA's last job is the decoders'
@@ -106,13 +106,14 @@ struct Phase {
 
 // Eight codes of the layout's word as weights: w[i] = columns 2 i, 2 i + 1
 __device__ __forceinline__ void decode8(uint32_t word, __half2 s, __half2 b, uint32_t* out) {
-    const __half2 base = __half2half2(__ushort_as_half(0x6400));  // 1024
-    const __half2 sixteenth = __half2half2(__ushort_as_half(0x2c00)), off = __half2half2(__ushort_as_half(0xd400));  // 1/16, -64
+    auto pair = [](uint16_t bits) { return __half2half2(__ushort_as_half(bits)); };
+    const __half2 unit[2] = {pair(0x3400), pair(0x2400)}, off[2] = {pair(0xdc00), pair(0xcc00)};  // 1/4 and -256, 1/64 and -16
+    const uint32_t turned = turn8(word);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        // (a code in the upper nibble is 1024 + 16 q as it lies, and a sixteenth of that less 64 is q: no shift)
-        const uint32_t v = ((word >> (i >= 2 ? 8 : 0)) & (i & 1 ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u;
-        const __half2 h = *reinterpret_cast<const __half2*>(&v), q = i & 1 ? __hfma2(h, sixteenth, off) : __hsub2(h, base);
+        // (with 1024's exponent a code as it lies is 1024 + 4 q or 1024 + 64 q; a quarter less 256, a 64th less 16 is q: exact)
+        const uint32_t v = ((i >= 2 ? turned : word) & (i & 1 ? kHigh : kLow)) | 0x64006400u;
+        const __half2 h = *reinterpret_cast<const __half2*>(&v), q = __hfma2(h, unit[i & 1], off[i & 1]);
         const __half2 w = __hfma2(q, s, b);
         out[(i >> 1) + 2 * (i & 1)] = *reinterpret_cast<const uint32_t*>(&w);  // nibbles i and i + 4 of the word
     }

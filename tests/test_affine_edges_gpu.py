@@ -9,7 +9,7 @@ import pytest
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 from strata_mlx_b200 import _lib, affine, fused  # noqa: E402
-from test_affine_gpu import F16, F32, MOE, close, gen_of, layer64, moe64  # noqa: E402
+from test_affine_gpu import F16, F32, MOE, close, floats64, gen_of, last, layer64, moe64  # noqa: E402
 
 
 def positive(gen, lead, rows, cols, group):
@@ -135,3 +135,32 @@ def test_prompts_with_one_accumulator_or_one_stage_a_job(cuda, rows, cols, token
     for _ in range(20):
         assert torch.equal(layer(x), want)
     assert not affine.failed()
+
+
+@pytest.mark.parametrize("cols, group", [(256, 64), (1024, 32), (512, 128)])
+def test_small_terms_beside_large_ones_that_cancel(cuda, cols, group):
+    # In every 32 columns a pair of +-32768 with equal codes in each half of the columns of an MMA step: their terms cancel
+    # exactly, and what is left are terms of 0.125 to 0.875. A step of float32 sums cuts its 16 products and the sum so far at
+    # 2^-23 of the largest at the worst: of 15 x 32768 in the codes' sums, of 32768 in the activations' (which the bias
+    # multiplies). So a step of 16 columns adds at most 17 x 2^-23 (15 scale + |bias|) x 32768, and the group's end and the
+    # sums of groups, all of them small, 2^-20 of the terms left.
+    gen = gen_of(49)
+    rows, tokens = 64, 4
+    codes = torch.randint(0, 16, (rows, cols), device=cuda, generator=gen)
+    x = (torch.randint(1, 8, (tokens, cols), device=cuda, generator=gen) / 8).half()
+    for c in range(0, cols, 32):
+        for at in (c, c + 4):
+            codes[:, at + 1] = codes[:, at]
+            x[:, at], x[:, at + 1] = 32768, -32768
+    words = sum(codes.reshape(rows, -1, 8)[..., i] << (4 * i) for i in range(8))
+    words = (words - ((words >> 31) << 32)).to(torch.int32)
+    scales = (0.001 * (1 + torch.rand(rows, cols // group, device=cuda, generator=gen))).half()
+    biases = (-7.5 * scales.float()).half()
+    p = words, scales, biases
+    w, mag = floats64(p)
+    want = x.double() @ w.mT
+    left = x.double().where(x.abs() < 1, 0.0)
+    step = (15 * scales.double() + biases.double().abs()).sum(-1) * group / 16 * 17 * 32768 * 2.0**-23
+    off = step + 2.0**-20 * (left @ mag.mT) + last(want, F16)
+    assert (off < 0.05 * (left @ mag.mT)).all()
+    close(affine.QuantizedLinear(*p, group_size=group)(x), want, off)
