@@ -369,12 +369,11 @@ class QuantizedMLP:
             out = self.down_proj(h)
         return out.reshape(*x.shape[:-1], self.down_proj.output_dims)
 
-
     def _apart(self, tokens: int) -> bool:
-        """Whether gate and up go by the prompt's kernel: the streaming launch takes 0.3 us and 0.25 ps a weight for every
+        """Whether gate and up go by the prompt's kernel, for more than a window's 16 tokens: the streaming launch takes 0.3 us and 0.25 ps a weight for every
         8 tokens, 30 us of which are about the other's start (whole calls of 4096 x 4096: 48 tokens 48 us streamed and 49
         apart, 96 tokens 78 and 50; of 640 x 2560: 128 tokens 21 and 27, 512 tokens 50 and 31)."""
-        return (tokens + 7) // 8 * (0.3 + 2.5e-7 * self.gate_proj.output_dims * self.gate_proj.input_dims) > 30
+        return tokens > 16 and (tokens + 7) // 8 * (0.3 + 2.5e-7 * self.gate_proj.output_dims * self.gate_proj.input_dims) > 30
 
 
 def moe_takes(switch_mlp, shared) -> bool:

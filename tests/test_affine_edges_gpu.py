@@ -9,7 +9,7 @@ import pytest
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 from strata_mlx_b200 import _lib, affine, fused  # noqa: E402
-from test_affine_gpu import F16, F32, MOE, close, floats64, gen_of, last, layer64, moe64  # noqa: E402
+from test_affine_gpu import F16, F32, MOE, close, floats64, gen_of, glu64, last, layer64, moe64, product64  # noqa: E402
 
 
 def positive(gen, lead, rows, cols, group):
@@ -164,3 +164,19 @@ def test_small_terms_beside_large_ones_that_cancel(cuda, cols, group):
     off = step + 2.0**-20 * (left @ mag.mT) + last(want, F16)
     assert (off < 0.05 * (left @ mag.mT)).all()
     close(affine.QuantizedLinear(*p, group_size=group)(x), want, off)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_a_wide_shared_expert_in_windows(cuda, dtype):
+    # (9 and more tokens of 59 million weights are where the cost of gate and up in one launch passes that of a prompt's)
+    gen = gen_of(50)
+    hidden, ffn, group = 8192, 7680, 128
+    s = [positive(gen, (), *d, group) for d in ((ffn, hidden), (ffn, hidden), (hidden, ffn))]
+    mlp = affine.QuantizedMLP(*(affine.QuantizedLinear(*p, group_size=group) for p in s))
+    x = positive_rows(gen, 16, hidden, dtype)
+    each = torch.cat([mlp(x[i : i + 1]) for i in range(16)])
+    for tokens in (2, 8, 9, 16):
+        assert torch.equal(mlp(x[:tokens]), each[:tokens])
+    h, eh = glu64(x, s[0], s[1], group, dtype)
+    want, off = product64(h, s[2], group, dtype)
+    near(each, want, off + eh @ floats64(s[2])[0].mT)
