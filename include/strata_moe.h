@@ -516,6 +516,13 @@ SMOE_API int smoe_q4_product(const SmoeQ4Product* p, void* stream);
 SMOE_API int smoe_q4_linear(const uint8_t* packed, int64_t rows, int64_t cols, int group, const void* x, int64_t tokens,
                             void* out, int dtype, void* stream);
 
+/* The prompt's kernel by itself: smoe_q4_linear's product of float16 activations, each weight rounded to float16 once, sums
+ * float32, out float16 or float32 (`out_dtype`). smoe_q4_is_prompt: whether smoe_q4_linear takes that kernel for so many float16
+ * tokens (1 or 0). */
+SMOE_API int smoe_q4_prompt(const uint8_t* packed, int64_t rows, int64_t cols, int group, const void* x, int64_t tokens, void* out,
+                            int out_dtype, void* stream);
+SMOE_API int smoe_q4_is_prompt(int64_t tokens, int64_t rows, int64_t cols);
+
 /* A stack's products of a prompt's many (token, expert) pairs, in the tiles of smoe_tiles_of (16 slots, each tile one
  * expert's, an expert's tiles next to one another): out[slot_row[s], r] = W[tile_expert[s / 16]][r, :] . a[s, :] for every slot
  * s, row s itself without slot_row; rows at or past out_rows are not written, nor are the slots of tiles that name no

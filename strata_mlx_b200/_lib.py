@@ -143,6 +143,8 @@ SIGNATURES = {
     "smoe_q4_pack": (_i, [_p, _p, _p, _i64, _i64, _i64, _i, _p, _p]),
     "smoe_q4_unpack": (_i, [_p, _i64, _i64, _i64, _i, _p, _i, _p]),
     "smoe_q4_linear": (_i, [_p, _i64, _i64, _i, _p, _i64, _p, _i, _p]),
+    "smoe_q4_prompt": (_i, [_p, _i64, _i64, _i, _p, _i64, _p, _i, _p]),
+    "smoe_q4_is_prompt": (_i, [_i64, _i64, _i64]),
     "smoe_q4_product": (_i, [_c.POINTER(SmoeQ4Product), _p]),
     "smoe_q4_tile_plan_size": (_sz, [_i64]),
     "smoe_q4_tile_plan": (_i, [_p, _i64, _i64, _p, _sz, _p]),
@@ -162,7 +164,7 @@ KERNELS_PER_CALL = {"smoe_tiles_of": 2, "smoe_tiles_of_noalloc": 2, "smoe_tile_m
                     "smoe_ep_exchange_alloc": 0, "smoe_ep_exchange_open": 0, "smoe_ep_exchange_close": 0,
                     "smoe_ep_exchange_free": 0, "smoe_ep_exchange_status": 0, "smoe_decode_layer_status": 0, "smoe_decode_layer_wait_test": 0,
                     "smoe_matvec_status": 0, "smoe_matvec_wait_test": 0, "smoe_hyper_connection": 3,
-                    "smoe_q4_moe": 2, "smoe_q4_status": 0}
+                    "smoe_q4_moe": 2, "smoe_q4_status": 0, "smoe_q4_is_prompt": 0}
 launches = 0
 
 

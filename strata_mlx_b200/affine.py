@@ -183,6 +183,13 @@ class QuantizedLinear(_Packed):
                       x2.data_ptr(), tokens, out.data_ptr(), code, _lib.raw_stream(self.device.index))
         return out
 
+    def _prompt(self, x2: torch.Tensor) -> torch.Tensor:
+        """(tokens, out) in float32 of float16 rows x2, by the prompt's kernel, on the current device."""
+        out = torch.empty((x2.shape[0], self.output_dims), dtype=torch.float32, device=self.device)
+        _lib.call("smoe_q4_prompt", self.data_ptr, self.output_dims, self.input_dims, self.group_size, x2.data_ptr(),
+                  x2.shape[0], out.data_ptr(), _lib.F32, _lib.raw_stream(self.device.index))
+        return out
+
 
 def _pair_chunks(pairs: int, share: int, most: int = MAX_PAIRS):
     """Ranges of up to `most` pairs, whole rows of `share`."""
@@ -345,7 +352,7 @@ class QuantizedSwitchGLU:
 
 class QuantizedMLP:
     """The shared expert on 4-bit weights: down(silu(gate x) * up x). Gate, up and the SwiGLU are one launch; a long
-    float16 prompt's are the prompt's products and a SwiGLU, each rounded to float16."""
+    float16 prompt's are the prompt's products in float32 and a SwiGLU. Either rounds the SwiGLU to x's type once."""
 
     def __init__(self, gate: QuantizedLinear, up: QuantizedLinear, down: QuantizedLinear):
         _check_glu(gate, up, down)
@@ -357,7 +364,7 @@ class QuantizedMLP:
         x2 = gate._rows(x).reshape(-1, gate.input_dims)
         if x.dtype == torch.float16 and self._apart(x2.shape[0]):
             with torch.cuda.device(gate.device):
-                out = self.down_proj(swiglu_to(gate(x2), up(x2), x.dtype))
+                out = self.down_proj(swiglu_to(gate._prompt(x2), up._prompt(x2), x.dtype))
             return out.reshape(*x.shape[:-1], self.down_proj.output_dims)
         with torch.cuda.device(gate.device):
             h = torch.empty((x2.shape[0], gate.output_dims), dtype=x.dtype, device=gate.device)
@@ -372,8 +379,11 @@ class QuantizedMLP:
     def _apart(self, tokens: int) -> bool:
         """Whether gate and up go by the prompt's kernel, for more than a window's 16 tokens: the streaming launch takes 0.3 us and 0.25 ps a weight for every
         8 tokens, 30 us of which are about the other's start (whole calls of 4096 x 4096: 48 tokens 48 us streamed and 49
-        apart, 96 tokens 78 and 50; of 640 x 2560: 128 tokens 21 and 27, 512 tokens 50 and 31)."""
-        return tokens > 16 and (tokens + 7) // 8 * (0.3 + 2.5e-7 * self.gate_proj.output_dims * self.gate_proj.input_dims) > 30
+        apart, 96 tokens 78 and 50; of 640 x 2560: 128 tokens 21 and 27, 512 tokens 50 and 31). (A few long rows may be better
+        streamed all the same.)"""
+        rows, cols = self.gate_proj.output_dims, self.gate_proj.input_dims
+        return (tokens > 16 and (tokens + 7) // 8 * (0.3 + 2.5e-7 * rows * cols) > 30
+                and bool(_lib.lib().smoe_q4_is_prompt(tokens, rows, cols)))
 
 
 def moe_takes(switch_mlp, shared) -> bool:

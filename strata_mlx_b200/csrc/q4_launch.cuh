@@ -16,9 +16,9 @@ int product_f16(const ProductArgs& a, int group, const Writes& w, cudaStream_t s
 int product_f32(const ProductArgs& a, int group, const Writes& w, cudaStream_t st);
 int down_f16(const DownArgs& a, int group, const Writes& w, cudaStream_t st);
 int down_f32(const DownArgs& a, int group, const Writes& w, cudaStream_t st);
-// the dense part of `a` on the prompt's kernel (float16), and whether that is the faster one
+// the dense part of `a` on the prompt's kernel (float16, floats: with float32 results), and whether that is the faster one
 bool matmul_better(int64_t tokens, int64_t rows, int64_t cols);
-int matmul_f16(const ProductArgs& a, int group, const Writes& w, cudaStream_t st);
+int matmul_f16(const ProductArgs& a, int group, bool floats, const Writes& w, cudaStream_t st);
 // the prompt's kernel on a stack, its activations x in tiles of 16 slots, each one expert's
 struct TileArgs {
     const uint8_t* w;

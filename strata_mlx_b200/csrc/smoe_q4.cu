@@ -356,6 +356,24 @@ extern "C" int smoe_q4_pack(const uint32_t* codes, const uint16_t* scales, const
     Q4_CATCH("q4_pack")
 }
 
+// A product's dense part as the kernels take it. item: bytes of a result
+static int dense_part(const uint8_t* dense, const uint8_t* dense2, int64_t rows, int64_t cols, int group, int64_t tokens,
+                      void* out, size_t item, ProductArgs& a, Writes& w, cudaStream_t st) {
+    if (int s = check_matrix(rows, cols, group)) return s;
+    SMOE_REQUIRE(dense && out && aligned16(dense) && aligned16(dense2), SMOE_EARG, "q4_product: null or misaligned pointer");
+    SMOE_REQUIRE(tokens <= kMost && strips_of_rows(rows) * ((tokens + 7) / 8) <= kMost, SMOE_ESHAPE,
+                 "too many tokens for one q4_product call");
+    a.dw[0] = dense;
+    a.dw[1] = dense2;
+    a.d_out = out;
+    a.d_rows = rows;
+    a.d_tokens = tokens;
+    w.add(out, size_t(tokens) * rows * item);
+    const size_t bytes = stack_bytes(1, rows, cols, group);
+    a.early = a.early && pdl_early(st, dense, bytes) && (!dense2 || pdl_early(st, dense2, bytes));
+    return SMOE_OK;
+}
+
 // pieces: results as two rows of float16 each (q4_mv.cuh); gate32: the dense gate in float32; `zero`: words that the launch
 // clears besides, for the launch after it
 static int q4_product(const SmoeQ4Product* p, bool pieces, const float* gate32, uint32_t* zero, int n_zero, void* stream) {
@@ -376,22 +394,12 @@ static int q4_product(const SmoeQ4Product* p, bool pieces, const float* gate32, 
     a.share = 1;
     const bool glu = (p->dense_tokens > 0 ? p->dense2 : p->stack2) != nullptr;
     if (p->dense_tokens > 0) {
-        if (int s = check_matrix(p->dense_rows, p->cols, p->group)) return s;
-        SMOE_REQUIRE(p->dense && p->dense_out && aligned16(p->dense) && aligned16(p->dense2), SMOE_EARG,
-                     "q4_product: null or misaligned pointer");
         SMOE_REQUIRE(p->dense_gate == nullptr || glu, SMOE_EARG, "q4_product: a gate needs gate and up matrices");
-        SMOE_REQUIRE(p->dense_tokens <= kMost && strips_of_rows(p->dense_rows) * ((p->dense_tokens + 7) / 8) <= kMost,
-                     SMOE_ESHAPE, "too many tokens for one q4_product call");
-        a.dw[0] = p->dense;
-        a.dw[1] = p->dense2;
-        a.d_out = p->dense_out;
-        a.d_rows = p->dense_rows;
-        a.d_tokens = p->dense_tokens;
+        if (int s = dense_part(p->dense, p->dense2, p->dense_rows, p->cols, p->group, p->dense_tokens, p->dense_out,
+                               item * (pieces ? 2 : 1), a, w, st))
+            return s;
         a.d_gate = p->dense_gate;
         a.d_gate32 = gate32;
-        w.add(p->dense_out, size_t(p->dense_tokens) * p->dense_rows * item * (pieces ? 2 : 1));
-        const size_t bytes = stack_bytes(1, p->dense_rows, p->cols, p->group);
-        a.early = a.early && pdl_early(st, p->dense, bytes) && (!p->dense2 || pdl_early(st, p->dense2, bytes));
     }
     if (p->pairs > 0) {
         if (int s = check_matrix(p->rows, p->cols, p->group)) return s;
@@ -419,7 +427,7 @@ static int q4_product(const SmoeQ4Product* p, bool pieces, const float* gate32, 
         a.early = a.early && pdl_early(st, p->stack, bytes) && (!p->stack2 || pdl_early(st, p->stack2, bytes));
     }
     if (p->dtype == SMOE_F16 && p->pairs == 0 && !glu && matmul_better(p->dense_tokens, p->dense_rows, p->cols))
-        return matmul_f16(a, p->group, w, st);
+        return matmul_f16(a, p->group, false, w, st);
     a.pieces = pieces;
     a.zero = zero;
     a.n_zero = n_zero;
@@ -447,6 +455,28 @@ extern "C" int smoe_q4_linear(const uint8_t* packed, int64_t rows, int64_t cols,
     p.dense_out = out;
     return q4_product(&p, false, nullptr, nullptr, 0, stream);
     Q4_CATCH("q4_linear")
+}
+
+extern "C" int smoe_q4_is_prompt(int64_t tokens, int64_t rows, int64_t cols) {
+    return rows > 0 && cols > 0 && rows <= kMost && cols <= kMost && tokens <= kMost && matmul_better(tokens, rows, cols);
+}
+
+extern "C" int smoe_q4_prompt(const uint8_t* packed, int64_t rows, int64_t cols, int group, const void* x, int64_t tokens,
+                              void* out, int out_dtype, void* stream) {
+    Q4_TRY
+    SMOE_REQUIRE(out_dtype == SMOE_F16 || out_dtype == SMOE_F32, SMOE_EDTYPE, "q4_prompt gives float16 or float32");
+    SMOE_REQUIRE(tokens >= 0, SMOE_EARG, "q4_prompt: a negative count");
+    if (tokens == 0) return SMOE_OK;
+    SMOE_REQUIRE(x && aligned16(x), SMOE_EARG, "q4_prompt: activations must be 16-byte aligned");
+    ProductArgs a = {};
+    Writes w;
+    cudaStream_t st = as_stream(stream);
+    a.early = true;
+    a.x = x;
+    a.cols = cols;
+    if (int s = dense_part(packed, nullptr, rows, cols, group, tokens, out, out_dtype == SMOE_F16 ? 2 : 4, a, w, st)) return s;
+    return matmul_f16(a, group, out_dtype == SMOE_F32, w, st);
+    Q4_CATCH("q4_prompt")
 }
 
 extern "C" size_t smoe_q4_tile_plan_size(int64_t tiles) { return tiles > 0 ? size_t(tiles + 1) * 16 : 0; }

@@ -58,7 +58,7 @@ struct GemmArgs {
     const uint32_t* slot_row;
     int64_t out_rows;
     int strips;  // of an expert
-    bool floats;
+    bool floats;  // out is float32
 };
 
 // A job's activation rows: the first and how many, and the first strip of its matrix
@@ -183,8 +183,8 @@ __global__ void __launch_bounds__(kGThreads, 1) q4_matmul_kernel(const GemmArgs 
         const int64_t r = int64_t(job % g.mblocks) * kGM + 32 * (warp & 3) + lane, tok0 = b.row0;
         const uint32_t from = tmem + (uint32_t(32 * (warp & 3)) << 16) + uint32_t(g.n * slot);
         const int valid = static_cast<int>(min(int64_t(b.n), g.tokens - tok0));
-        __half* out = g.out + (tok0 + c0) * g.rows + r;
-        for (int c = c0; c < valid; c += step, out += step * g.rows) {
+        int64_t at = (tok0 + c0) * g.rows + r;
+        for (int c = c0; c < valid; c += step, at += step * g.rows) {
             uint32_t v[8];
             tc::tmem_ld8(from + c, v);
             tc::tmem_wait_ld();
@@ -201,10 +201,17 @@ __global__ void __launch_bounds__(kGThreads, 1) q4_matmul_kernel(const GemmArgs 
                     else g.out[to[j] * g.rows + r] = __float2half_rn(f);
                 }
             } else if (r < g.rows) {
-                __half* to = out;
+                if (g.floats) {
+                    float* to = reinterpret_cast<float*>(g.out) + at;
 #pragma unroll
-                for (int j = 0; j < 8; ++j, to += g.rows)
-                    if (c + j < valid) *to = __float2half_rn(__uint_as_float(v[j]));
+                    for (int j = 0; j < 8; ++j, to += g.rows)
+                        if (c + j < valid) *to = __uint_as_float(v[j]);
+                } else {
+                    __half* to = g.out + at;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j, to += g.rows)
+                        if (c + j < valid) *to = __float2half_rn(__uint_as_float(v[j]));
+                }
             }
             __syncwarp();
         }
@@ -449,7 +456,7 @@ static int encode_and_launch(GemmArgs& a, int group, int64_t strips, const void*
     return launch_gemm<128, TILES>(a, maps, w, st);
 }
 
-int matmul_f16(const ProductArgs& p, int group, const Writes& w, cudaStream_t st) {
+int matmul_f16(const ProductArgs& p, int group, bool floats, const Writes& w, cudaStream_t st) {
     GemmArgs a = {};
     a.w = p.dw[0];
     a.out = static_cast<__half*>(p.d_out);
@@ -457,6 +464,7 @@ int matmul_f16(const ProductArgs& p, int group, const Writes& w, cudaStream_t st
     a.cols = p.cols;
     a.tokens = p.d_tokens;
     a.early = p.early;
+    a.floats = floats;
     a.mblocks = static_cast<int>((p.d_rows + kGM - 1) / kGM);
     a.n = tokens_of_job(p.d_tokens, p.d_rows, p.cols);
     a.nblocks = static_cast<int>((p.d_tokens + a.n - 1) / a.n);

@@ -180,3 +180,31 @@ def test_a_wide_shared_expert_in_windows(cuda, dtype):
     h, eh = glu64(x, s[0], s[1], group, dtype)
     want, off = product64(h, s[2], group, dtype)
     near(each, want, off + eh @ floats64(s[2])[0].mT)
+
+
+@pytest.mark.parametrize("ffn, tokens", [(4096, 500), (640, 2900)])
+def test_gate_and_up_of_a_long_prompt_are_not_rounded_before_their_product(cuda, ffn, tokens):
+    # gate rows of one negative value each take an activation row of one value to -11 .. -9, where float16 has steps of 2^-7
+    # and silu follows them nearly in full (0.4 % at the most); up rows of one value to 480 .. 560; down is the identity.
+    # Every weight is a float16 and every sum of 256 equal terms is off by 2^-24 a step at most, 2^-14 of itself in all by the
+    # tensor core's 17 cuts a step of 16; silu's slope here is less than 12 times its value to one of the gate's.
+    hidden, group = 256, 64
+    gen = gen_of(51)
+
+    def rows_of(values, rows, cols):
+        codes = torch.zeros(rows, cols // 8, dtype=torch.int32, device=cuda)
+        return codes, torch.zeros(rows, cols // group, dtype=F16, device=cuda), values.half()[:, None].expand(-1, cols // group).contiguous()
+
+    gate = rows_of(-(9 + 2 * torch.rand(ffn, device=cuda, generator=gen)) / 256, ffn, hidden)
+    up = rows_of((480 + 80 * torch.rand(ffn, device=cuda, generator=gen)) / 256, ffn, hidden)
+    down = torch.zeros(hidden, ffn // 8, dtype=torch.int32, device=cuda)
+    r = torch.arange(hidden, device=cuda)
+    down[r, r // 8] = (1 << (4 * (r % 8))).to(torch.int32)
+    down = down, torch.ones(hidden, ffn // group, dtype=F16, device=cuda), torch.zeros(hidden, ffn // group, dtype=F16, device=cuda)
+    mlp = affine.QuantizedMLP(*(affine.QuantizedLinear(*p, group_size=group) for p in (gate, up, down)))
+    assert mlp._apart(tokens)
+    x = (1 + 0.03 * torch.rand(tokens, 1, device=cuda, generator=gen)).half().expand(-1, hidden)
+    g, u = (x.double() @ floats64(p)[0].mT for p in (gate, up))
+    want = (g * torch.sigmoid(g) * u)[:, :hidden]
+    close(mlp(x), want, 2 * last(want, F16) + 13 * 2.0**-14 * want.abs())
+    assert not affine.failed()
