@@ -170,6 +170,16 @@ def decode_layer_failed(x: torch.Tensor, block: "SparseMoeBlock") -> bool:
     return flag.value != 0
 
 
+def _check_route(gate: "WindowLinear", shared_gate, x: torch.Tensor) -> None:
+    """Refuse what a route's launch would read at a wrong place: activations of another width, weights on another device."""
+    if x.dim() < 1 or x.shape[-1] != gate.cols:
+        raise ValueError(f"activations {tuple(x.shape)} do not end in {gate.cols}")
+    device, w, s = x.device, gate.weight, None if shared_gate is None else shared_gate.weight
+    if device.type != "cuda" or w.device != device or (s is not None and s.device != device):
+        _lib.require_cuda(w, x, s)
+        raise ValueError(f"a router on device {w.device}, activations on {device}")
+
+
 def route(gate: "WindowLinear", shared_gate, x: torch.Tensor, k: int, local=None, defer: bool = False):
     """The start of the MoE block in one launch: (idx, w, g) = (top_k_softmax(gate(x), k),
     shared_gate(x).to(x.dtype)) with the same sums and choice as those calls (strata_mlx/fused.py:487-491).
@@ -184,7 +194,7 @@ def route(gate: "WindowLinear", shared_gate, x: torch.Tensor, k: int, local=None
         return None
     if shared_gate is not None and (not shared_gate.takes(x) or shared_gate.rows != 1 or shared_gate.cols != gate.cols):
         return None
-    _lib.require_cuda(gate.weight, x)
+    _check_route(gate, shared_gate, x)
     tokens = x.numel() // gate.cols
     x2 = x.reshape(tokens, gate.cols).contiguous()
     dev = x.device
@@ -229,7 +239,7 @@ def route_window(gate: "WindowLinear", shared_gate: "WindowLinear", x: torch.Ten
             or not 1 <= k <= min(gate.rows, 32) or not shared_gate.takes(x) or shared_gate.rows != 1
             or shared_gate.cols != gate.cols or gate_dtype not in (None, torch.float16, torch.float32)):
         return None
-    _lib.require_cuda(gate.weight, x)
+    _check_route(gate, shared_gate, x)
     dev = x.device
     x2 = affine._aligned(x)
     wt, gw = affine._aligned(gate.weight), affine._aligned(shared_gate.weight)

@@ -208,3 +208,38 @@ def test_gate_and_up_of_a_long_prompt_are_not_rounded_before_their_product(cuda,
     want = (g * torch.sigmoid(g) * u)[:, :hidden]
     close(mlp(x), want, 2 * last(want, F16) + 13 * 2.0**-14 * want.abs())
     assert not affine.failed()
+
+
+def small_block(gen, router_on="cuda", gate_on="cuda"):
+    _, _, glu, mlp = positive_experts(gen, 8, 64, 64, 64, 32, 32)
+    router = torch.randn(8, 64, device="cuda", generator=gen).half()
+    sgate = torch.randn(1, 64, device="cuda", generator=gen).half()
+    return fused.SparseMoeBlock(router.to(router_on), glu, mlp, sgate.to(gate_on), 2)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("tokens", [1, 70])
+def test_a_block_refuses_weights_of_the_route_on_another_device(cuda, dtype, tokens):
+    gen = gen_of(52)
+    x = torch.randn(tokens, 64, device=cuda, generator=gen).to(dtype)
+    assert small_block(gen)(x).shape == x.shape
+    for where in (dict(router_on="cpu"), dict(gate_on="cpu")):
+        block = small_block(gen, **where)
+        with pytest.raises(ValueError, match="CUDA|device"):
+            block(x)
+        for route in (fused.route, fused.route_window):
+            if route is fused.route or (dtype == F16 and tokens <= 64):
+                with pytest.raises(ValueError, match="CUDA|device"):
+                    route(block.gate, block.shared_expert_gate, x, 2)
+
+
+def test_a_route_refuses_activations_of_another_width(cuda):
+    gen = gen_of(53)
+    block = small_block(gen)
+    for shape in ((1, 96), (2, 32), (1, 127)):
+        x = torch.randn(*shape, device=cuda, generator=gen).half()
+        for route in (fused.route_window, fused.route):
+            with pytest.raises(ValueError, match="64"):
+                route(block.gate, block.shared_expert_gate, x, 2)
+        with pytest.raises(ValueError, match="64"):
+            block(x)
