@@ -92,15 +92,16 @@ def _route_counters(nbytes: int, defer: bool, device) -> torch.Tensor:
     """The zeroed counters of one route call; the kernels leave them zero. Eager calls of one stream run one after
     another and share theirs; a captured call gets words of its own, because two graphs that hold one may run at once."""
     words = nbytes // 4
-    if device not in _COUNTER_POOL and not torch.cuda.is_current_stream_capturing():
-        _COUNTER_POOL[device] = [torch.zeros(1 << 18, dtype=torch.int32, device=device), 0]
+    pool = _COUNTER_POOL.get(device)
     if torch.cuda.is_current_stream_capturing():
-        pool = _COUNTER_POOL.get(device)
         if pool is None or pool[1] + words > pool[0].numel():
             return torch.zeros(words, dtype=torch.int32, device=device)  # (a memset in the graph)
         at, pool[1] = pool[1], pool[1] + (words + 15) // 16 * 16
         return pool[0][at : at + words]
-    key = (str(device), nbytes, defer, torch.cuda.current_stream(device).cuda_stream)
+    if pool is None:
+        _COUNTER_POOL[device] = [torch.zeros(1 << 18, dtype=torch.int32, device=device), 0]
+        torch.cuda.current_stream(device).synchronize()  # (once: graphs use them on any stream)
+    key = (device, nbytes, defer, _lib.raw_stream(device.index))
     counters = _COUNTERS.get(key)
     if counters is None:
         counters = _COUNTERS[key] = torch.zeros(words, dtype=torch.int32, device=device)

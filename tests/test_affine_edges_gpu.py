@@ -243,3 +243,42 @@ def test_a_route_refuses_activations_of_another_width(cuda):
                 route(block.gate, block.shared_expert_gate, x, 2)
         with pytest.raises(ValueError, match="64"):
             block(x)
+
+
+def test_counters_for_captured_routes_are_zero_before_any_stream_can_use_them(cuda, monkeypatch):
+    # (a first call on a busy stream makes them; a graph that is captured and replayed on another stream does not wait for it)
+    block = small_block(gen_of(54))
+    x = torch.randn(3, 64, device=cuda, generator=gen_of(55)).half()
+    want = block(x)
+    monkeypatch.setattr(fused, "_COUNTER_POOL", {})
+    busy, other = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(busy):
+        used = torch.ones(1 << 18, dtype=torch.int32, device=cuda)  # memory of their size that held something else
+        assert used.any()  # (and the kernels loaded)
+        torch.cuda.synchronize()
+        del used
+        torch.cuda._sleep(200_000_000)  # a tenth of a second
+        assert not busy.query()
+        block(x)
+        seen = next(iter(fused._COUNTER_POOL.values()))[0]
+    with torch.cuda.stream(other):
+        assert not seen.any()
+        assert torch.equal(block(x), want)
+    torch.cuda.synchronize()
+
+
+def test_eager_routes_on_several_streams_have_counters_of_their_own(cuda):
+    gen = gen_of(56)
+    block = small_block(gen)
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    xs = [torch.randn(t, 64, device=cuda, generator=gen).half() for t in (1, 9, 33, 64)]
+    want = [block(x) for x in xs]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got = []
+        for st, x in zip(streams, xs):
+            with torch.cuda.stream(st):
+                got.append(block(x))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
