@@ -579,6 +579,11 @@ SMOE_API int smoe_route_window_f32(const uint16_t* weight, const uint16_t* gate_
  * since are not valid). Synchronizes the device. */
 SMOE_API int smoe_q4_status(int* status, int clear);
 
+/* For tests of those waits: while `withhold` is not 0, the products, blocks and prompts on 4-bit weights that this process
+ * launches have one copy each that never counts as landed, so that the wait for it runs out (a second or two a launch) and the
+ * status is set; their outputs are not valid. */
+SMOE_API int smoe_q4_wait_test(int withhold);
+
 #ifdef __cplusplus
 }
 #endif

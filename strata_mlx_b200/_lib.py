@@ -154,6 +154,7 @@ SIGNATURES = {
     "smoe_route_window": (_i, [_p, _p, _p, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p]),
     "smoe_route_window_f32": (_i, [_p, _p, _p, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p]),
     "smoe_q4_status": (_i, [_c.POINTER(_i), _i]),
+    "smoe_q4_wait_test": (_i, [_i]),
 }
 
 _lib = None
@@ -164,7 +165,8 @@ KERNELS_PER_CALL = {"smoe_tiles_of": 2, "smoe_tiles_of_noalloc": 2, "smoe_tile_m
                     "smoe_ep_exchange_alloc": 0, "smoe_ep_exchange_open": 0, "smoe_ep_exchange_close": 0,
                     "smoe_ep_exchange_free": 0, "smoe_ep_exchange_status": 0, "smoe_decode_layer_status": 0, "smoe_decode_layer_wait_test": 0,
                     "smoe_matvec_status": 0, "smoe_matvec_wait_test": 0, "smoe_hyper_connection": 3,
-                    "smoe_q4_moe": 2, "smoe_q4_status": 0, "smoe_q4_is_prompt": 0}
+                    "smoe_q4_moe": 2, "smoe_q4_status": 0, "smoe_q4_is_prompt": 0,
+                    "smoe_q4_wait_test": 0}
 launches = 0
 
 

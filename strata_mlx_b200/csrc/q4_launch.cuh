@@ -31,6 +31,7 @@ struct TileArgs {
 };
 int tile_plan(const uint32_t* tile_expert, int64_t tiles, int64_t experts, void* plan, const Writes& w, cudaStream_t st);
 int tile_matmul(const TileArgs& p, int group, const Writes& w, cudaStream_t st);
+int wait_test();  // what smoe_q4_wait_test was last given, 0 or 1
 cudaError_t matmul_status(int* v, bool clear);
 cudaError_t product_status_f16(int* v, bool clear);
 cudaError_t product_status_f32(int* v, bool clear);
@@ -73,6 +74,7 @@ inline int team_log_for(int64_t jobs, int64_t tiles) {
 template <typename T, int G, bool GLU>
 inline int launch_product(const ProductArgs& args, const Writes& w, cudaStream_t st) {
     ProductArgs a = args;
+    a.withhold = wait_test();
     constexpr int kWide = GLU ? 1 : 2;
     a.tiles = static_cast<int>(tiles_of_cols(a.cols));
     a.runs = static_cast<int>(a.cols / 32);
@@ -110,6 +112,7 @@ inline int product(const ProductArgs& a, int group, const Writes& w, cudaStream_
 template <typename T, int G>
 inline int launch_down(const DownArgs& args, const Writes& w, cudaStream_t st) {
     DownArgs a = args;
+    a.withhold = wait_test();
     a.stiles = static_cast<int>(tiles_of_cols(a.sffn));
     a.ftiles = static_cast<int>(tiles_of_cols(a.ffn));
     a.strips = static_cast<int>(strips_of_rows(a.rows));

@@ -71,6 +71,7 @@ struct ProductArgs {
     Divisor by_dense, by_share;           // by d_blocks, by share
     bool early;  // the weights may be read before pdl_wait()
     bool hint;   // weights evict-first in L2
+    int withhold;  // a test's: 1, CTA 0's first copy never counts as landed
 };
 
 struct DownArgs {
@@ -84,6 +85,7 @@ struct DownArgs {
     float* partial;      // [CTAs][2][tokens][32]
     uint32_t* counters;  // one a job, zero
     bool early;          // idx and the weights may be read before pdl_wait()
+    int withhold;        // as ProductArgs'
     int stiles, ftiles, strips, jobs;
     Divisor by_k, by_stiles, by_ftiles;
 };
@@ -95,13 +97,15 @@ constexpr int kStages = 2;  // slots
 struct Ring {
     uint32_t slots, bars;  // shared addresses
     uint32_t fetched = 0, taken = 0;
-    bool dead = false;  // a wait gave up: what follows is read as it lies, nothing more is fetched
+    int left = 0;  // tiles still to be fetched of the run of tiles that the copies' cursor is in
+    bool dead = false;  // a wait gave up: what follows is read as it lies, nothing more is fetched (a phase may be open)
 
-    __device__ __forceinline__ void init(uint8_t* p, uint64_t* b, int lane) {
+    // withhold: arrivals that the first slot's barrier waits for and that never come
+    __device__ __forceinline__ void init(uint8_t* p, uint64_t* b, int lane, int withhold) {
         slots = smem_addr(p);
         bars = smem_addr(b);
         if (lane == 0) {
-            for (int i = 0; i < kStages; ++i) tc::mbar_init(&b[i], 1);
+            for (int i = 0; i < kStages; ++i) tc::mbar_init(&b[i], i == 0 ? 1 + withhold : 1);
             tc::fence_barrier_init();
         }
         __syncwarp();
@@ -117,6 +121,7 @@ struct Ring {
         if (!__all_sync(0xffffffffu, try_wait(bars + 8 * at, phase))) {
             if (!dead && !__all_sync(0xffffffffu, wait_for(barrier(at), phase))) {
                 dead = true;
+                left = 0;  // (the next fetch looks for another run of tiles, and at this)
                 if (lane == 0) atomicExch(&g_q4_status, SMOE_ETIMEOUT);
             }
         }
@@ -350,7 +355,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_product_kernel(const Produ
     uint64_t* bars = reinterpret_cast<uint64_t*>(table + pair_blocks_bytes(a.pairs, a.experts));
     red += (team << a.team_log) * 2 * kRedFloats;  // [job's parity][member][strip][row][column]
     Ring ring;
-    ring.init(smem + size_t(warp) * kStages * kSlot, bars + warp * kStages, lane);
+    ring.init(smem + size_t(warp) * kStages * kSlot, bars + warp * kStages, lane, blockIdx.x == 0 && warp == 0 ? a.withhold : 0);
     // (weights of experts are read once; a layer's may be read again by its next block of tokens or its next call)
     const uint64_t policy = a.hint ? tc::policy_evict_first() : policy_evict_normal();
 
@@ -375,10 +380,10 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_product_kernel(const Produ
     };
 
     // the copies' cursor: the next stage to fetch
-    int fetch_job = tile0 < tile1 ? team_id : 0x7fffffff, fetch_left = 0;
+    int fetch_job = tile0 < tile1 ? team_id : 0x7fffffff;
     const uint8_t *fetch0 = nullptr, *fetch1 = nullptr;
     auto fetch = [&]() {  // (a slot is free)
-        if (fetch_left == 0) {
+        if (ring.left == 0) {
             if (fetch_job >= jobs || ring.dead) return;
             int strip, block;
             place(fetch_job, strip, block);
@@ -390,14 +395,14 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_product_kernel(const Produ
             fetch0 = w0 + (first + strip * kWide) * strip_bytes + int64_t(tile0) * kTile;
             // (the last job of an odd number of strips takes its one strip twice)
             fetch1 = w1 + (first + (GLU ? strip : min(strip * 2 + 1, strips - 1))) * strip_bytes + int64_t(tile0) * kTile;
-            fetch_left = tile1 - tile0;
+            ring.left = tile1 - tile0;
             fetch_job += teams;
         }
-        const int n = min(kStep, fetch_left);
+        const int n = min(kStep, ring.left);
         ring.template fetch<kSlot>(fetch0, fetch1, n * kTile, policy);
         fetch0 += n * kTile;
         fetch1 += n * kTile;
-        fetch_left -= n;
+        ring.left -= n;
     };
     if (!a.early) pdl_wait();
     // the dense part's weights, while the launch before still runs
@@ -520,7 +525,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_down_kernel(const DownArgs
     uint8_t* table = reinterpret_cast<uint8_t*>(red + kWarps * tokens * kTokenStride);
     uint64_t* bars = reinterpret_cast<uint64_t*>(table + pair_blocks_bytes(pairs, a.experts));
     Ring ring;
-    ring.init(smem + size_t(warp) * kStages * kSlot, bars + warp * kStages, lane);
+    ring.init(smem + size_t(warp) * kStages * kSlot, bars + warp * kStages, lane, blockIdx.x == 0 && warp == 0 ? a.withhold : 0);
     const uint64_t policy = tc::policy_evict_first();
     float* mine = red + warp * tokens * kTokenStride;
 
@@ -585,13 +590,14 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_down_kernel(const DownArgs
         ++c.seg;
     };
 
-    int fetch_job = job_first, fetch_left = 0;
+    int fetch_job = job_first;
     Cursor fc = job_first < job_last ? cursor_of(fetch_job) : Cursor{0, 0, 0};
     const uint8_t *fetch0 = nullptr, *fetch1 = nullptr;
     auto fetch = [&]() {  // (a slot is free)
-        if (fetch_left == 0) {
+        if (ring.left == 0) {
+            if (ring.dead) return;
             while (fc.left == 0) {
-                if (fetch_job + 1 >= job_last || ring.dead) return;
+                if (fetch_job + 1 >= job_last) return;
                 fc = cursor_of(++fetch_job);
             }
             const bool shared = fc.seg < sblocks;
@@ -599,14 +605,14 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_down_kernel(const DownArgs
             const uint8_t* w = shared ? a.sw : a.w + int64_t(blocks.expert[fc.seg - sblocks]) * strips * strip_bytes;
             fetch0 = w + (fetch_job * kMt) * strip_bytes + int64_t(fc.tile) * kTile;
             fetch1 = w + min(fetch_job * kMt + 1, strips - 1) * strip_bytes + int64_t(fc.tile) * kTile;
-            fetch_left = tiles_of(fc);
-            next_segment(fc, fetch_left);
+            ring.left = tiles_of(fc);
+            next_segment(fc, ring.left);
         }
-        const int n = min(kStep, fetch_left);
+        const int n = min(kStep, ring.left);
         ring.template fetch<kSlot>(fetch0, fetch1, n * kTile, policy);
         fetch0 += n * kTile;
         fetch1 += n * kTile;
-        fetch_left -= n;
+        ring.left -= n;
     };
     for (int i = 0; i < kStages; ++i) fetch();
     pdl_wait();

@@ -6,6 +6,7 @@
 // pieces a thread, 32 bytes apart between neighbours, ran at 4.1 TB/s), four of them in flight. A group's extremes come
 // from the lanes that hold it by shuffles.
 #include <algorithm>
+#include <atomic>
 #include <string>
 
 #include "q4_launch.cuh"
@@ -228,6 +229,9 @@ static size_t stack_bytes(int64_t experts, int64_t rows, int64_t cols, int group
 constexpr int64_t kMost = int64_t(1) << 30;  // rows, columns and tokens of a matrix
 constexpr int64_t kMostWeights = int64_t(1) << 40;  // of a matrix, and matrices of a stack: products stay in 64 bits
 constexpr int64_t kMostExperts = int64_t(1) << 20;
+
+static std::atomic<int> g_wait_test{0};
+int wait_test() { return g_wait_test.load(); }
 
 }  // namespace q4
 }  // namespace smoe
@@ -628,6 +632,11 @@ extern "C" int smoe_q4_moe(const SmoeQ4Moe* m, void* workspace, size_t workspace
     w.add(m->out, size_t(m->tokens) * m->hidden * (m->dtype == SMOE_F16 ? 2 : 4));
     return m->dtype == SMOE_F16 ? down_f16(d, m->down_group, w, st) : down_f32(d, m->down_group, w, st);
     Q4_CATCH("q4_moe")
+}
+
+extern "C" int smoe_q4_wait_test(int withhold) {
+    g_wait_test = withhold != 0;
+    return SMOE_OK;
 }
 
 extern "C" int smoe_q4_status(int* status, int clear) {

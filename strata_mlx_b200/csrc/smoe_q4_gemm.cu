@@ -53,6 +53,7 @@ struct GemmArgs {
     int mblocks;
     int nb, nr;   // activation and raw slots
     bool early;
+    int withhold;  // a test's: 1, CTA 0's first copy of weights never counts as landed
     // TILES: a stack, its activations in tiles of 16 slots of one expert's
     const uint4* plan;  // word 0: .x blocks of slots; then each block's first slot, slots, expert
     const uint32_t* slot_row;
@@ -147,7 +148,7 @@ __global__ void __launch_bounds__(kGThreads, 1) q4_matmul_kernel(const GemmArgs 
     }
     if (threadIdx.x == 0) {
         for (int i = 0; i < g.nr; ++i) {
-            tc::mbar_init(&S.rawfull[i], 1);
+            tc::mbar_init(&S.rawfull[i], i == 0 && blockIdx.x == 0 ? 1 + g.withhold : 1);
             tc::mbar_init(&S.rawfree[i], kGGroup);
         }
         for (int i = 0; i < g.nb; ++i) {
@@ -416,6 +417,7 @@ static int launch_gemm(GemmArgs a, const GemmMaps<TILES>& maps, const Writes& w,
     while (a.nr > 4 && gemm_smem<G>(a.n, a.nb, a.nr) > kGSmemLimit) a.nr -= 2;
     while (a.nb < kGMaxB && gemm_smem<G>(a.n, a.nb + 1, a.nr) <= kGSmemLimit) ++a.nb;
     const size_t smem = gemm_smem<G>(a.n, a.nb, a.nr);
+    a.withhold = wait_test();
     if (int e = max_smem(q4_matmul_kernel<G, TILES>, static_cast<int>(smem)))
         return status_of(static_cast<cudaError_t>(-e), "q4_matmul");
     const int64_t jobs = int64_t(a.nblocks) * a.mblocks;

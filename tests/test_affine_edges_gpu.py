@@ -282,3 +282,36 @@ def test_eager_routes_on_several_streams_have_counters_of_their_own(cuda):
         torch.cuda.synchronize()
         for a, b in zip(got, want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("call", ["layer", "block", "prompt", "experts"])
+def test_a_wait_that_runs_out_is_a_status_the_host_reads(cuda, call, dtype):
+    # one copy of each launch never counts as landed; the launch ends, the status says so, and the next call is right again
+    if dtype == F32 and call in ("prompt", "experts"):
+        pytest.skip("float16 alone has a prompt's kernel")
+    gen = gen_of(57)
+    tokens, hidden = {"layer": 5, "block": 3, "prompt": 700, "experts": 1100}[call], 512
+    _, s, glu, mlp = positive_experts(gen, 6, hidden, 256, 384, 64, 64)
+    x = positive_rows(gen, tokens, hidden, dtype)
+    idx = torch.randint(0, 6, (tokens, 2), dtype=torch.int32, device=cuda, generator=gen)
+    w, g = torch.rand(tokens, 2, device=cuda, generator=gen), torch.randn(tokens, 1, device=cuda, generator=gen).to(dtype)
+    wide = affine.QuantizedLinear(*positive(gen, (), 40, 16384, 64))  # (more copies to come behind the one that is missed)
+    wide_x = positive_rows(gen, tokens, 16384, dtype)
+
+    def run():
+        if call == "block":
+            return affine.moe(glu, mlp, x, idx, w, g)
+        return glu(x, idx) if call == "experts" else mlp.gate_proj(x) if call == "prompt" else wide(wide_x)
+
+    affine.failed(clear=True)
+    want = run()
+    assert not affine.failed()
+    try:
+        _lib.call("smoe_q4_wait_test", 1)
+        run()
+        assert affine.failed(clear=True)
+    finally:
+        _lib.call("smoe_q4_wait_test", 0)
+    assert not affine.failed()
+    assert torch.equal(run(), want) and not affine.failed()
