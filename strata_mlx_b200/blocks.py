@@ -420,10 +420,10 @@ def matvec_glu(lin, idx: torch.Tensor, gate: torch.Tensor, up: torch.Tensor):
     # (the kernel takes the pairs in as many launches as their activations need)
     fused = gate.dtype == torch.float16 and lin.kind in FUSED_GLU and lin.input_dims % FUSED_GLU_COLS == 0
     if not fused and gate.dtype == torch.float16 and lin.input_dims % MMA_MATVEC.get(lin.kind, 1 << 30) == 0:
-        h = swiglu(gate.reshape(pairs, -1), up.reshape(pairs, -1))
+        h = swiglu(gate.reshape(pairs, lin.input_dims), up.reshape(pairs, lin.input_dims))
         return _matvec(lin, h, idx, 1, gate.dtype)
-    gate = gate.reshape(pairs, -1).contiguous()
-    up = up.reshape(pairs, -1).contiguous()
+    gate = gate.reshape(pairs, lin.input_dims).contiguous()
+    up = up.reshape(pairs, lin.input_dims).contiguous()
     out = torch.empty((pairs, lin.output_dims), dtype=gate.dtype, device=gate.device)
     if pairs:
         _lib.call("smoe_matvec_glu", _kind(lin.kind), _lib.ptr(lin.blocks), lin.num_experts, lin.output_dims,

@@ -4,11 +4,14 @@ Weights and activations here are positive, so that nothing cancels and a toleran
 
 import ctypes
 
+import numpy as np
 import pytest
+
+from oracle import quants as Q
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
-from strata_mlx_b200 import _lib, affine, fused  # noqa: E402
+from strata_mlx_b200 import _lib, affine, blocks, fused  # noqa: E402
 from test_affine_gpu import F16, F32, MOE, close, floats64, gen_of, glu64, last, layer64, moe64, product64  # noqa: E402
 
 
@@ -315,3 +318,64 @@ def test_a_wait_that_runs_out_is_a_status_the_host_reads(cuda, call, dtype):
         _lib.call("smoe_q4_wait_test", 0)
     assert not affine.failed()
     assert torch.equal(run(), want) and not affine.failed()
+
+
+@pytest.mark.parametrize("tokens", [0, 1, 5, 70, 600])
+@pytest.mark.parametrize("which", ["shared", "routed"])
+def test_a_block_of_gguf_experts_beside_4_bit_ones(cuda, which, tokens):
+    # the shared expert 4-bit and the routed experts GGUF blocks (the reference's own mixture), and the other way round: the
+    # blocks' part is taken as it comes, the 4-bit part by its definition, the combine's roundings counted one by one
+    gen = gen_of(58)
+    hidden, ffn, experts, k, group = 256, 512, 6, 2, 32
+    rng = np.random.default_rng(5)
+
+    def stack(*shape):
+        data = Q.random_blocks("Q8_0", int(np.prod(shape)) // 32, rng, normal=0.001).reshape(-1)
+        return torch.from_numpy(data).to(cuda), "Q8_0", shape
+
+    r, s, glu, mlp = positive_experts(gen, experts, hidden, ffn, ffn, group, group)
+    if which == "shared":
+        glu = blocks.BlockSwitchGLU(*(blocks.BlockSwitchLinear(*stack(experts, *d)) for d in ((ffn, hidden), (ffn, hidden), (hidden, ffn))))
+    else:
+        mlp = blocks.BlockMLP(*(blocks.BlockLinear(*stack(*d)) for d in ((ffn, hidden), (ffn, hidden), (hidden, ffn))))
+    router, sgate = (torch.randn(n, hidden, device=cuda, generator=gen).half() for n in (experts, 1))
+    block = fused.SparseMoeBlock(router, glu, mlp, sgate, k)
+    x = positive_rows(gen, tokens, hidden, F16)
+    got = block(x)
+    assert got.shape == x.shape and got.dtype == F16
+    if not tokens:
+        return
+    idx, w, g = fused.route(block.gate, block.shared_expert_gate, x, k)
+    idx, share, eps = idx.view(torch.int32).long(), torch.sigmoid(g.double()), 2.0**-11
+    if which == "shared":
+        y, ey = glu(x, idx.to(torch.int32)).double(), 0
+        h, eh = glu64(x, s[0], s[1], group, F16, rounded=True)
+        sh, es = product64(h, s[2], group, F16)
+        es = es + (eh + eps * h) @ floats64(s[2])[0].mT
+    else:
+        sh, es = mlp(x).double(), 0
+        y, ey = torch.zeros(2, tokens, k, hidden, dtype=torch.float64, device=cuda)
+        for e in range(experts):
+            t, j = (idx == e).nonzero(as_tuple=True)
+            gate, up, down = ([a[e] for a in p] for p in r)
+            h, eh = glu64(x[t], gate, up, group, F16, rounded=True)
+            y[t, j], ey[t, j] = product64(h, down, group, F16)
+            ey[t, j] += (eh + eps * h) @ floats64(down)[0].mT
+    sums = (y * w.double()[..., None]).sum(1)
+    want = sums + share * sh
+    off = (1.01 * ey * w.double()[..., None]).sum(1) if which == "routed" else 0
+    off = off + 2 * eps * sums.abs() + share * (1.01 * es + 4 * eps * sh.abs()) + eps * want.abs() + 2.0**-23
+    close(got, want, off)
+
+
+def test_a_4_bit_block_as_a_step_with_its_copies(cuda):
+    gen = gen_of(59)
+    block = small_block(gen)
+    for tokens in (1, 17):
+        x = torch.randn(tokens, 64, device=cuda, generator=gen).half()
+        want = block(x)
+        step = fused.GraphedBlock(block, tokens, 64, F16, cuda, host_io=True)
+        for _ in range(2):
+            out = step(x.cpu())
+            step.ready.synchronize()
+            assert torch.equal(out, want.cpu())
