@@ -12,7 +12,7 @@ from oracle import quants as Q
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 from strata_mlx_b200 import _lib, affine, blocks, fused  # noqa: E402
-from test_affine_gpu import F16, F32, MOE, close, floats64, gen_of, glu64, last, layer64, moe64, product64  # noqa: E402
+from test_affine_gpu import F16, F32, MOE, SHAPES, close, floats64, gen_of, glu64, last, layer64, moe64, parts, product64  # noqa: E402
 
 
 def positive(gen, lead, rows, cols, group):
@@ -379,3 +379,61 @@ def test_a_4_bit_block_as_a_step_with_its_copies(cuda):
             out = step(x.cpu())
             step.ready.synchronize()
             assert torch.equal(out, want.cpu())
+
+
+def alone(w, mag, dtype, rounded=False):
+    """How far a weight may be that an activation of one brings out alone: the group's two terms in float32, its rounding."""
+    return mag * 2.0**-22 + last(w, dtype) * (2 if rounded else 1)
+
+
+@pytest.mark.parametrize("rows, cols, group", [(15, 96, 32), (16, 64, 64), (33, 160, 32), (129, 384, 128), (300, 1056, 32), (70, 2560, 64)])
+@pytest.mark.parametrize("tokens", [1, 7, 16, 24, 200])
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_every_weight_of_a_layer_alone(cuda, rows, cols, group, tokens, dtype):
+    gen = gen_of(60 + tokens)
+    p = parts(gen, (), rows, cols, group)
+    layer = affine.QuantizedLinear(*p, group_size=group)
+    w, mag = floats64(p)
+    eye = torch.eye(cols, dtype=dtype, device=cuda)
+    got = torch.cat([layer(eye[c : c + tokens]) for c in range(0, cols, tokens)]).T
+    close(got, w, alone(w, mag, dtype, tokens > 16))
+
+
+@pytest.mark.parametrize("experts, rows, cols, group", [(3, 33, 160, 32), (5, 130, 256, 64), (2, 16, 384, 128)])
+@pytest.mark.parametrize("dtype, tiles", [(F16, False), (F16, True), (F32, False)])
+def test_every_weight_of_a_stack_alone(cuda, experts, rows, cols, group, dtype, tiles, monkeypatch):
+    gen = gen_of(61)
+    p = parts(gen, (experts,), rows, cols, group)
+    stack = affine.QuantizedSwitchLinear(*p, group_size=group)
+    monkeypatch.setattr(affine, "_by_tiles", lambda lin, dt, pairs: tiles)
+    w, mag = floats64(p)
+    idx = torch.stack([torch.randperm(experts, device=cuda, generator=gen) for _ in range(cols)]).to(torch.int32)
+    got = stack(torch.eye(cols, dtype=dtype, device=cuda)[:, None, None], idx)[:, :, 0]  # (cols, experts, rows)
+    want, mag = (t.permute(2, 0, 1).gather(1, idx.long()[..., None].expand(-1, -1, rows)) for t in (w, mag))
+    close(got, want, alone(want, mag, dtype, tiles))
+
+
+@pytest.mark.parametrize("rows, cols, group", SHAPES)
+@pytest.mark.parametrize("tokens", [1, 5, 8, 13, 16, 17, 48, 700])
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_a_layer_of_positive_weights(cuda, rows, cols, group, tokens, dtype):
+    gen = gen_of(rows + cols + tokens)
+    p = positive(gen, (), rows, cols, group)
+    x = positive_rows(gen, tokens, cols, dtype)
+    near(affine.QuantizedLinear(*p, group_size=group)(x), *layer64(x, p, group, dtype))
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("tokens, k, experts, hidden, ffn, shared, group, down_group",
+                         [(300, 8, 17, 320, 160, 96, 32, 32), (700, 4, 5, 256, 384, 640, 128, 64), (260, 10, 12, 1024, 64, 2048, 64, 64),
+                          (70, 32, 64, 96, 64, 64, 32, 64), (2100, 1, 1, 64, 128, 64, 64, 64), (1100, 3, 1500, 64, 32, 32, 32, 32)])
+def test_a_prompt_of_positive_weights(cuda, dtype, tokens, k, experts, hidden, ffn, shared, group, down_group):
+    gen = gen_of(tokens + k)
+    r, s, glu, mlp = positive_experts(gen, experts, hidden, ffn, shared, group, down_group)
+    x = positive_rows(gen, tokens, hidden, dtype)
+    w = 0.05 + torch.rand(tokens, k, device=cuda, generator=gen)
+    g = torch.randn(tokens, 1, device=cuda, generator=gen).to(dtype)
+    idx = torch.randint(0, experts, (tokens, k), dtype=torch.int32, device=cuda, generator=gen)
+    idx[::5, 0], idx[7] = experts, -1
+    near(affine.moe(glu, mlp, x, idx, w, g), *moe64(x, r, s, idx, w, g, group, down_group, dtype, rounded=dtype == F16))
+    assert not affine.failed()
