@@ -313,22 +313,27 @@ __device__ __forceinline__ void run_mma(const Codes<float> (&a)[MT], const Acts<
     piece(std::false_type{}, s.hi, s.on2);
 }
 
-// What a row's sum is to be multiplied by in the end (the codes' 2^-22)
+// The unit of the ones in that of a code (float16's 2^-14 and 2^-22). The end of a group divides its sum of activations by it, or,
+// with groups of 32, multiplies its scale (64007 x 2560 at 5 tokens: groups of 32 28.7 us and 26.6; groups of 64 in a block of
+// 256 experts at 5 tokens 118.8 us and 120.3)
 template <typename T>
-__host__ __device__ constexpr float unit() { return sizeof(T) == 2 ? 4194304.0f : 1.0f; }
+__host__ __device__ constexpr float ones() { return sizeof(T) == 2 ? 256.0f : 1.0f; }
+// What a row's sum is to be multiplied by in the end
+template <typename T, int G>
+__host__ __device__ constexpr float unit() { return sizeof(T) != 2 ? 1.0f : G == 32 ? 16384.0f : 4194304.0f; }
 
 // The end of a group: acc += scale (lo + hi) + bias on, rows g (values 0, 1) and g + 8 (values 2, 3).
-template <typename T, int MT>
+template <typename T, int G, int MT>
 __device__ __forceinline__ void group_end(float (&acc)[4], const Sums<T, MT>& s, int m, uint32_t sb0, uint32_t sb1) {
     const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&sb0));
     const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&sb1));
-    constexpr float kOnes = sizeof(T) == 2 ? 1.0f / 256.0f : 1.0f;  // a code's unit in that of the ones
-    const float on[2] = {(s.on[0] + s.on2[0]) * kOnes, (s.on[1] + s.on2[1]) * kOnes};  // (the same for both rows)
+    constexpr float kOn = G == 32 ? 1.0f : 1.0f / ones<T>(), kScale = G == 32 ? ones<T>() : 1.0f;
+    const float on[2] = {(s.on[0] + s.on2[0]) * kOn, (s.on[1] + s.on2[1]) * kOn};  // (the same for both rows)
     const float b[2] = {sizeof(T) == 2 ? p.y : fmaf(8.0f, p.x, p.y), sizeof(T) == 2 ? r.y : fmaf(8.0f, r.x, r.y)};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float q = fmaf(s.hi[m][i], sizeof(T) == 2 ? 0.0625f : 1.0f, s.lo[m][i]);
-        acc[i] = fmaf(q, i < 2 ? p.x : r.x, fmaf(on[i & 1], b[i >> 1], acc[i]));
+        acc[i] = fmaf(q, (i < 2 ? p.x : r.x) * kScale, fmaf(on[i & 1], b[i >> 1], acc[i]));
     }
 }
 
@@ -395,7 +400,7 @@ __device__ __forceinline__ void tile_mma(uint32_t tile, int stride, int lane, co
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
             const uint32_t q = pairs + m * stride + 4 * gi;
-            group_end<T, 2>(acc[m], s, m, lds32(q), lds32(q + 8 * kPairs * 4));
+            group_end<T, G, 2>(acc[m], s, m, lds32(q), lds32(q + 8 * kPairs * 4));
         }
         // (four groups of a tile interleaved want more registers than there are: 64007 x 2560 at 5 tokens 32.2 us, with them
         // kept apart 28.0)

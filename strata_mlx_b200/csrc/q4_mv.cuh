@@ -94,11 +94,15 @@ struct DownArgs {
 
 constexpr int kStages = 2;  // slots
 
+// LOOK: how the copies stop once a wait gave up (a barrier's phase may then be open): each looks at `dead` first, or the wait
+// ends the run of tiles that is being fetched and the next run's first copy looks. (64007 x 2560 at 5 tokens: float32, groups of
+// 32, 63.7 us and 68.7; float16, groups of 64, 24.7 and 22.4.)
+template <bool LOOK>
 struct Ring {
     uint32_t slots, bars;  // shared addresses
     uint32_t fetched = 0, taken = 0;
     int left = 0;  // tiles still to be fetched of the run of tiles that the copies' cursor is in
-    bool dead = false;  // a wait gave up: what follows is read as it lies, nothing more is fetched (a phase may be open)
+    bool dead = false;  // a wait gave up: what follows is read as it lies, nothing more is fetched
 
     // withhold: arrivals that the first slot's barrier waits for and that never come
     __device__ __forceinline__ void init(uint8_t* p, uint64_t* b, int lane, int withhold) {
@@ -121,7 +125,7 @@ struct Ring {
         if (!__all_sync(0xffffffffu, try_wait(bars + 8 * at, phase))) {
             if (!dead && !__all_sync(0xffffffffu, wait_for(barrier(at), phase))) {
                 dead = true;
-                left = 0;  // (the next fetch looks for another run of tiles, and at this)
+                if constexpr (!LOOK) left = 0;
                 if (lane == 0) atomicExch(&g_q4_status, SMOE_ETIMEOUT);
             }
         }
@@ -130,6 +134,7 @@ struct Ring {
     // two copies of `bytes` into the next slot's halves (the whole warp calls, one lane issues)
     template <int SLOT>
     __device__ __forceinline__ void fetch(const uint8_t* w0, const uint8_t* w1, uint32_t bytes, uint64_t policy) {
+        if (LOOK && dead) return;
         const uint32_t at = fetched & 1;
         ++fetched;
         if (elect_one()) {
@@ -145,6 +150,9 @@ struct Ring {
             if (!wait_for(barrier(i & 1), (i >> 1) & 1) && lane == 0) atomicExch(&g_q4_status, SMOE_ETIMEOUT);
     }
 };
+
+template <typename T>
+using RingOf = Ring<sizeof(T) == 4>;
 
 __device__ __forceinline__ int warp_incl_sum(int v, int lane) {
 #pragma unroll
@@ -288,7 +296,7 @@ constexpr int kRedFloats = kMt * kRows * kM;  // a warp's sums of one job
 // before; with groups of 32, whose sums take the registers, a pair's second tile's between the two (64007 x 2560 at 5 tokens
 // 26.3 us, and 28.0 with the loads ahead).
 template <typename T, int G, class Fetch>
-__device__ __forceinline__ void stream_tiles(Ring& ring, Fetch& fetch, const T* xp, int left, int runs, int lane,
+__device__ __forceinline__ void stream_tiles(RingOf<T>& ring, Fetch& fetch, const T* xp, int left, int runs, int lane,
                                              float (&acc)[2][4], const Ones<T>& one) {
     static_assert(kStep == 2, "a stage is a pair of tiles");
     constexpr int kTile = tile_bytes<G>(), kStride = kStep * kTile;
@@ -354,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_product_kernel(const Produ
     uint8_t* table = reinterpret_cast<uint8_t*>(red + kWarps * 2 * kRedFloats);
     uint64_t* bars = reinterpret_cast<uint64_t*>(table + pair_blocks_bytes(a.pairs, a.experts));
     red += (team << a.team_log) * 2 * kRedFloats;  // [job's parity][member][strip][row][column]
-    Ring ring;
+    RingOf<T> ring;
     ring.init(smem + size_t(warp) * kStages * kSlot, bars + warp * kStages, lane, blockIdx.x == 0 && warp == 0 ? a.withhold : 0);
     // (weights of experts are read once; a layer's may be read again by its next block of tokens or its next call)
     const uint64_t policy = a.hint ? tc::policy_evict_first() : policy_evict_normal();
@@ -457,10 +465,10 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_product_kernel(const Produ
                     if constexpr (GLU) u += from[w * kRedFloats + kRows * kM + n];
                 }
                 const int64_t to = dense ? start + n : blocks.list[start + n];
-                v *= unit<T>();
+                v *= unit<T, G>();
                 if constexpr (GLU) {
                     // silu(gate) up, times the row's share of the block's output: float32 up to the one rounding
-                    v = v * sigmoid_f(v) * (u * unit<T>());
+                    v = v * sigmoid_f(v) * (u * unit<T, G>());
                     if (dense) {
                         if (a.d_gate32 != nullptr) v *= sigmoid_f(a.d_gate32[to]);
                         else if (a.d_gate != nullptr) v *= sigmoid_f(to_f32(static_cast<const T*>(a.d_gate)[to]));
@@ -524,7 +532,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_down_kernel(const DownArgs
     float* red = reinterpret_cast<float*>(smem + size_t(kWarps) * kStages * kSlot);  // [warp][token][row]
     uint8_t* table = reinterpret_cast<uint8_t*>(red + kWarps * tokens * kTokenStride);
     uint64_t* bars = reinterpret_cast<uint64_t*>(table + pair_blocks_bytes(pairs, a.experts));
-    Ring ring;
+    RingOf<T> ring;
     ring.init(smem + size_t(warp) * kStages * kSlot, bars + warp * kStages, lane, blockIdx.x == 0 && warp == 0 ? a.withhold : 0);
     const uint64_t policy = tc::policy_evict_first();
     float* mine = red + warp * tokens * kTokenStride;
@@ -676,7 +684,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) q4_down_kernel(const DownArgs
         const int values = kMt * kRows * tokens;
         auto write = [&](int i, float sum) {
             const int64_t row = int64_t(job) * kMt * kRows + (i & (kMt * kRows - 1));
-            if (row < a.rows) static_cast<T*>(a.out)[i / (kMt * kRows) * a.rows + row] = from_f32<T>(sum * unit<T>());
+            if (row < a.rows) static_cast<T*>(a.out)[i / (kMt * kRows) * a.rows + row] = from_f32<T>(sum * unit<T, G>());
         };
         // (a job that a CTA shares is the first or the last of its range)
         float* part = a.partial + (int64_t(blockIdx.x) * 2 + (job == job_first ? 0 : 1)) * values;
