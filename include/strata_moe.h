@@ -491,7 +491,10 @@ SMOE_API int smoe_q4_unpack(const uint8_t* packed, int64_t experts, int64_t rows
  * sigmoid(dense_gate[t]) (`dtype`) or weights[p] (float32) where given, rounded once. Both parts in one call are both
  * of one kind. Pairs with idx[p] >= experts are left out (their rows of out stay as they were). Up to 2048 pairs and
  * experts; x 16-byte aligned, its rows cols apart. The weights may be read while the launch before on the stream still
- * runs: they must not be written by it (smoe_q4_pack excepted). */
+ * runs: they must not be written by it (smoe_q4_pack excepted). Weights are exact, but for one case: a dense part alone, without
+ * a second matrix, of more than 16 float16 tokens may take the prompt's kernel (smoe_q4_is_prompt says when), which rounds each
+ * weight to float16 once, so that one beyond float16's range is infinite there. Outside of that kernel a row of x that holds an
+ * infinity gives NaN where the products' own sum may be an infinity (codes of 0 and the biases' sum meet it too). */
 typedef struct SmoeQ4Product {
     int dtype;
     int group;
@@ -510,9 +513,8 @@ typedef struct SmoeQ4Product {
 } SmoeQ4Product;
 SMOE_API int smoe_q4_product(const SmoeQ4Product* p, void* stream);
 
-/* smoe_q4_product's dense part alone: out[t, r] = W[r, :] . x[t, :] for t < tokens (`nn.QuantizedLinear`). More than 16
- * float16 tokens may take the prompt's kernel, which rounds each weight to float16 once; up to 16 get the same bits each
- * alone as together. */
+/* smoe_q4_product's dense part alone: out[t, r] = W[r, :] . x[t, :] for t < tokens (`nn.QuantizedLinear`), by the prompt's kernel
+ * where that one says so; up to 16 tokens get the same bits each alone as together. */
 SMOE_API int smoe_q4_linear(const uint8_t* packed, int64_t rows, int64_t cols, int group, const void* x, int64_t tokens,
                             void* out, int dtype, void* stream);
 
@@ -541,8 +543,9 @@ SMOE_API int smoe_q4_tile_matmul(const uint8_t* packed, int64_t experts, int64_t
  *   out[t] = sum_j weights[t, j] down_e(silu(gate_e x) * up_e x) + sigmoid(shared_gate[t]) shared(x), e = idx[t, j]
  * gate, up: (experts, ffn, hidden) with groups of `group` columns, down: (experts, hidden, ffn) with `down_group`; the
  * shared expert's likewise with shared_ffn rows (0: none; shared_gate and shared_gate32 null: not gated). A choice idx >= experts adds
- * nothing. Sums and SwiGLU are float32; between the launches the SwiGLU times its weight is kept in 22 bits (down to
- * 2^-25; float16 activations: within float16's range). Workspace: smoe_q4_moe_workspace_size() bytes, one for each call in
+ * nothing; a token may name an expert more than once. Sums and SwiGLU are float32; between the launches the SwiGLU times its
+ * weight is kept in 22 bits (float16 activations: down to 2^-25, and one beyond 65504 makes its token's result NaN). The order
+ * of a token's sums goes by all tokens of the call: its last bits may differ alone and in a window. Workspace: smoe_q4_moe_workspace_size() bytes, one for each call in
  * flight. Replaces `_Routed.__call__` behind its router
  * (strata_mlx/fused.py:491-497). Weights as smoe_q4_product's. */
 typedef struct SmoeQ4Moe {

@@ -13,8 +13,11 @@ strata_mlx/mtp.py:34-75).
 A weight is code * scale + bias with a code of 4 bits, eight codes to a 32-bit word (weight 8 j + i in bits 4 i of
 word j), groups of 32, 64 or 128 columns. A layer lays its arrays out once for the kernels (libstrata_moe.so) and
 keeps that alone. Products are exact in each weight (codes are not rounded to floats first) with float32 sums; a layer's
-product of more than 16 float16 tokens may go by a kernel that rounds each weight to float16 once (as `dequantize` does).
-Activations are float16 or float32; tensors are torch CUDA tensors and there is no CPU path.
+product of more than 16 float16 tokens, and experts' of more than MAX_PAIRS float16 pairs, may go by a kernel that rounds each
+weight to float16 once (as `dequantize` does: a weight beyond float16's range is infinite there). Activations that are not finite
+make their token's results not finite, NaN also where the definition has an infinity. Float32 has no kernel for prompts: a layer's
+weights are read and decoded again for every 8 tokens. Activations are float16 or float32; tensors are torch CUDA tensors and
+there is no CPU path.
 """
 
 import ctypes
@@ -69,7 +72,8 @@ def quantize(w: torch.Tensor, group_size: int = 64, bits: int = BITS):
     """Float weights (..., rows, cols) as (codes int32 (..., rows, cols / 8), scales, biases float16 (..., rows,
     cols / group_size)). Of each group, bias is the least value and scale a fifteenth of the range, both rounded to
     float16; a code is (w - bias) / scale rounded to even within 0 .. 15 (0 where the scale is 0). Values beyond
-    float16's range or not finite give groups that are not finite."""
+    float16's range or not finite give groups that are not finite. (MLX's quantize of the same arguments fits scale and bias in
+    a way of its own: arrays made there and here stand for the same weights within a step, but are not equal.)"""
     _check_group(group_size, bits)
     _lib.require_cuda(w)
     if w.dim() < 1 or w.shape[-1] == 0 or w.shape[-1] % group_size:
@@ -318,7 +322,8 @@ def _check_glu(gate, up, down):
 
 class QuantizedSwitchGLU:
     """The routed experts of one layer on 4-bit weights: x (..., in) and indices (..., k) -> (..., k, out), each
-    down(silu(gate x) * up x); gate and up in one launch that forms the SwiGLU."""
+    down(silu(gate x) * up x); gate and up in one launch that forms the SwiGLU, a prompt's by tiles and a SwiGLU of float32.
+    Rows of pairs of no expert are not written."""
 
     def __init__(self, gate: QuantizedSwitchLinear, up: QuantizedSwitchLinear, down: QuantizedSwitchLinear):
         _check_glu(gate, up, down)
@@ -399,9 +404,10 @@ def moe_takes(switch_mlp, shared) -> bool:
 def moe(switch_mlp: QuantizedSwitchGLU, shared: QuantizedMLP, x: torch.Tensor, indices: torch.Tensor, w: torch.Tensor,
         g: torch.Tensor) -> torch.Tensor:
     """sum_j w_j switch_mlp(x, indices)_j + sigmoid(g) shared(x): x (..., hidden), indices and w (..., k) with w float32,
-    g (..., 1) in x's type. Up to MOE_TOKENS tokens in two launches, sums float32 and rounded to x's type once (the SwiGLU
-    keeps 22 bits, down to 2^-25, between the launches); more tokens by switch_mlp, shared and the block's combine, each
-    rounded to x's type. An index at or past the expert count adds nothing."""
+    g (..., 1) in x's type. Up to MOE_TOKENS tokens in two launches, sums float32 and rounded to x's type once (the SwiGLU times
+    its weight keeps 22 bits between the launches, for float16 down to 2^-25; one beyond 65504 makes its token's result NaN);
+    more tokens by switch_mlp, shared and the block's combine, each rounded to x's type. An index at or past the expert count
+    adds nothing. A token's last bits may differ alone and in a window."""
     if not moe_takes(switch_mlp, shared):
         raise ValueError("moe takes 4-bit experts of one hidden size, with one group size in gate / up and one in down")
     if g.dtype != x.dtype:

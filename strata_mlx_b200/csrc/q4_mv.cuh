@@ -12,8 +12,9 @@
 // 1088 bytes, 47 cycles of an SM at full bandwidth, and a job's ends are 580 instructions more). So two strips of rows share
 // each activation operand, and nothing but a warp's own copies is waited for inside a job: every warp has a ring of bulk
 // copies of its own that runs ahead of the arithmetic across the ends of jobs, 16 warps a SM, 75 to 150 KB of a SM in flight
-// (6.5 TB/s x 1 us of latency over 148 SMs asks for 44 KB). 64007 x 2560 at 5 tokens: 20.4 us, 5.4 TB/s between its start and
-// its end; a block of 512 experts of 640 x 2560 at 32 tokens 168 us, 632 MB, the ends of its blocks of rows.
+// (6.5 TB/s x 1 us of latency over 148 SMs asks for 44 KB). 64007 x 2560 at 5 tokens: 20.6 us, 4.2 TB/s, a
+// start and an end of about 5 us and uneven shares (2001 jobs over 2368 warps, one or none each: the busiest has 1.18 times the
+// mean); a block of 512 experts of 640 x 2560 at 32 tokens 170 us, 632 MB, the ends of its blocks of rows.
 //
 // A job of the product kernel is two strips of 16 rows (gate's and up's, or two neighbours) times one block of up to 8
 // activation rows of one expert; its columns are split over a team of 1 to 8 warps of a CTA, the partial sums added in

@@ -4,8 +4,9 @@
 // and float32 sums. 128 weight rows are the M side of a tcgen05 MMA (8 strips), up to 256 tokens the N side, so a row is
 // decoded once for that many tokens. What bounds it: the tensor pipe (2 rows cols tokens flops at 4,096 multiply-adds a
 // cycle of an SM) and beside it the decoding, 15 instructions for 8 weights: a stage of 128 x 128 weights takes 240
-// issue slots a scheduler, and with its hand-offs 0.35 us; its MMAs take 2.8 ns a token, so from about 130 tokens a job the
-// tensor pipe is the longer. 4096 x 4096 at 1180 tokens: 34.7 us, 1141 TFLOP/s.
+// issue slots a scheduler (0.13 us), but 0.35 us, because a group of decoders waits, loads, waits, decodes, stores and hands over
+// strictly in turn and there are two groups; its MMAs take 2.8 ns a token, so from about 130 tokens a job the tensor pipe is the
+// longer. 4096 x 4096 at 1180 tokens: 34.0 us, 1164 TFLOP/s.
 //
 // Per CTA (persistent over jobs = (block of tokens, 128 rows)), warp-specialized, every hand-off an mbarrier:
 //   warp 17   weights: a stage is one tile of each of the 8 strips, one TMA box (a copy a strip took the warp 120 cycles
@@ -381,9 +382,8 @@ static EncodeTiledFn encoder() {
 
 // Microseconds of the prompt's kernel with jobs of n tokens, as measured: a start, and for every round of jobs over the SMs
 // a stage's 0.35 us (its hand-offs and decoding) or 2.8 ns a token (its MMAs), whichever is longer, and 1 us at its ends.
-// (With a stage of 0.38 us: 4096 x 4096, 128 tokens, one round: 17.5 us with jobs of 32 to 96 tokens, 18.2 of 160, 24.6 of
-// 256; 1180 tokens: 36.9 in jobs of 144, two rounds, 52.8 of 96, three, 51.0 of 256; 1536 x 4096, 4096 tokens: 39.3 of 176,
-// 48.5 of 112, 53.2 of 256.)
+// (4096 x 4096: 33 to 128 tokens, one round, 16.1 us, and 16.2 by this; 1180 tokens in jobs of 144, two rounds, 34.0 and 31.8;
+// 1536 x 4096, 4096 tokens in jobs of 176, 38.6 and 37.5.)
 static double time_of(int64_t tokens, int64_t rows, int64_t cols, int n) {
     const int64_t jobs = (tokens + n - 1) / n * ((rows + kGM - 1) / kGM);
     const double stage = std::max(0.35, 0.0028 * n);
@@ -398,7 +398,7 @@ static int tokens_of_job(int64_t tokens, int64_t rows, int64_t cols) {
 }
 
 // The streaming kernel takes 3 us, and for every 8 tokens 0.3 us and 0.125 ps a weight (64007 x 2560: 22 us at 5 tokens, 42
-// at 12, where the prompt's takes 39 at 24; 4096 x 4096: 8 us at 16 and 11 at 24, the prompt's 15.8 at 48); up to 16 tokens
+// at 12, where the prompt's takes 39 at 24; 4096 x 4096: 8 us at 16 and 11 at 24, the prompt's 16.0 at 48); up to 16 tokens
 // are always its (a verify window's token then has the bits it has alone).
 bool matmul_better(int64_t tokens, int64_t rows, int64_t cols) {
     if (tokens <= 16) return false;
@@ -408,7 +408,7 @@ bool matmul_better(int64_t tokens, int64_t rows, int64_t cols) {
 
 template <int G, bool TILES>
 static int launch_gemm(GemmArgs a, const GemmMaps<TILES>& maps, const Writes& w, cudaStream_t st) {
-    // (the copies' latency is what the rings hide: a stage of weights is 9 KB and some 0.2 us of work, so as many as fit
+    // (the copies' latency is what the rings hide: a stage of weights is 9 KB and 0.35 us of work or more, so as many as fit
     // beside three stages of activations, then more of those)
     a.nr = kGMaxRaw;
     a.nb = 3;

@@ -287,7 +287,9 @@ class SparseMoeBlock:
 
     gate: WindowLinear or float16 weight (experts, hidden); switch_mlp: BlockSwitchGLU; shared_expert:
     BlockMLP; shared_expert_gate: float16 weight (1, hidden). With the 4-bit experts of `affine` (QuantizedSwitchGLU,
-    QuantizedMLP) everything behind the route is two launches (`affine.moe`), its sums float32 to the end."""
+    QuantizedMLP) everything behind the route is two launches up to 64 tokens (`affine.moe`), its sums float32 to the end; a
+    token's last bits may then differ alone and in a window, and the logits' between 64 float16 tokens (`route_window`) and more
+    (`route`)."""
 
     def __init__(self, gate, switch_mlp, shared_expert, shared_expert_gate, top_k: int):
         self.gate = gate if isinstance(gate, WindowLinear) else WindowLinear(gate)
