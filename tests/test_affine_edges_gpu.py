@@ -437,3 +437,33 @@ def test_a_prompt_of_positive_weights(cuda, dtype, tokens, k, experts, hidden, f
     idx[::5, 0], idx[7] = experts, -1
     near(affine.moe(glu, mlp, x, idx, w, g), *moe64(x, r, s, idx, w, g, group, down_group, dtype, rounded=dtype == F16))
     assert not affine.failed()
+
+
+@pytest.mark.parametrize("rows, cols, group", [(1, 32, 32), (130, 96, 32), (300, 1024, 128), (1000, 320, 64)])
+@pytest.mark.parametrize("tokens", [1, 7, 16, 33, 161, 600])
+def test_the_prompts_kernel_at_any_count_in_both_types(cuda, rows, cols, group, tokens):
+    gen = gen_of(rows + tokens)
+    p = positive(gen, (), rows, cols, group)
+    layer = affine.QuantizedLinear(*p, group_size=group)
+    x = positive_rows(gen, tokens, cols, F16)
+    want, off = product64(x, p, group)
+    off = off + x.double() @ last(floats64(p)[0], F16).mT
+    got = layer._prompt(x)
+    assert got.dtype == F32
+    near(got, want, off + last(want, F32))
+    half = torch.full((tokens + 1, rows), 7.0, dtype=F16, device=cuda)
+    _lib.call("smoe_q4_prompt", layer.data_ptr, rows, cols, group, x.data_ptr(), tokens, half.data_ptr(), _lib.F16, _lib.stream())
+    assert torch.equal(half[:-1], got.half()) and (half[-1] == 7).all()
+
+
+def test_a_windows_route_with_a_gate_of_either_type(cuda):
+    gen = gen_of(62)
+    block = small_block(gen)
+    for tokens in (1, 8, 13, 64):
+        x = torch.randn(tokens, 64, device=cuda, generator=gen).half()
+        idx, w, g = fused.route_window(block.gate, block.shared_expert_gate, x, 2)
+        idx32, w32, g32 = fused.route_window(block.gate, block.shared_expert_gate, x, 2, torch.float32)
+        assert torch.equal(idx, idx32) and torch.equal(w, w32) and g.dtype == F16 and torch.equal(g32.half(), g)
+        want = x.double() @ block.shared_expert_gate.weight.double().mT
+        close(g32, want, 64 * 2.0**-23 * (x.double().abs() @ block.shared_expert_gate.weight.double().abs().mT))
+    assert fused.route_window(block.gate, block.shared_expert_gate, x, 2, torch.bfloat16) is None
