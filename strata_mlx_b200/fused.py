@@ -249,8 +249,9 @@ def route_window(gate: "WindowLinear", shared_gate: "WindowLinear", x: torch.Ten
     w = torch.empty((tokens, k), dtype=torch.float32, device=dev)
     g = torch.empty((tokens,), dtype=gate_dtype or x.dtype, device=dev)
     counters = _route_counters(32, False, dev)
-    _lib.call("smoe_route_window_f32" if g.dtype == torch.float32 else "smoe_route_window", _lib.ptr(wt), _lib.ptr(gw), _lib.ptr(x2), tokens, gate.rows, gate.cols, k,
-              _lib.ptr(logits), _lib.ptr(idx), _lib.ptr(w), _lib.ptr(g), _lib.ptr(counters), _lib.stream())
+    _lib.call("smoe_route_window_f32" if g.dtype == torch.float32 else "smoe_route_window", _lib.ptr(wt), _lib.ptr(gw),
+              _lib.ptr(x2), tokens, gate.rows, gate.cols, k, _lib.ptr(logits), _lib.ptr(idx), _lib.ptr(w), _lib.ptr(g),
+              _lib.ptr(counters), _lib.stream())
     lead = x.shape[:-1]
     return idx.reshape(*lead, k), w.reshape(*lead, k), g.reshape(*lead, 1)
 
@@ -331,7 +332,8 @@ class SparseMoeBlock:
 
     def _quantized(self, x: torch.Tensor) -> torch.Tensor:
         """The block on 4-bit experts: the route, then `affine.moe`; up to 64 float16 tokens keep the shared gate in float32
-        between the two (rounded to float16 it was all of the block's error beside its output's rounding)."""
+        between the two (sigmoid follows the last bits of a gate far from 0: rounded to float16, one of -9.3 left the shared
+        expert's part 0.3 % off)."""
         _lib.require_cuda(x)
         with torch.cuda.device(x.device):
             r = route_window(self.gate, self.shared_expert_gate, x, self.top_k, torch.float32)

@@ -467,3 +467,26 @@ def test_a_windows_route_with_a_gate_of_either_type(cuda):
         want = x.double() @ block.shared_expert_gate.weight.double().mT
         close(g32, want, 64 * 2.0**-23 * (x.double().abs() @ block.shared_expert_gate.weight.double().abs().mT))
     assert fused.route_window(block.gate, block.shared_expert_gate, x, 2, torch.bfloat16) is None
+
+
+def test_prompts_blocks_and_a_graph_on_several_streams(cuda):
+    gen = gen_of(63)
+    _, s, glu, mlp = positive_experts(gen, 9, 512, 256, 1024, 64, 64)
+    router, sgate = (torch.randn(n, 512, device=cuda, generator=gen).half() for n in (9, 1))
+    block = fused.SparseMoeBlock(router, glu, mlp, sgate, 3)
+    xs = [positive_rows(gen, t, 512, F16) for t in (900, 64, 1000, 800)]
+    idx = torch.randint(0, 9, (900, 3), dtype=torch.int32, device=cuda, generator=gen)
+    step = fused.GraphedBlock(block, 800, 512, F16, cuda)
+    calls = [lambda x: glu(x, idx), block, mlp.gate_proj, step]
+    want = [call(x).clone() for call, x in zip(calls, xs)]
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    for _ in range(30):
+        got = []
+        for st, call, x in zip(streams, calls, xs):
+            with torch.cuda.stream(st):
+                got.append(call(x))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+    assert not affine.failed()
